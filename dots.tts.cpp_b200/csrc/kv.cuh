@@ -1,0 +1,170 @@
+// The paged K/V cache: page layout, device metadata and the row codec shared by
+// its kernels (kv_cache.cu: rows and pages; kv_attend.cu: attention).
+//
+// Pool: [page][layer][kv head] segments; a segment holds P token rows as
+//   K rows [P][RB] | V rows [P][RB] | K scales [P][SB] | V scales [P][SB]
+// with RB = 2 D bytes (bf16) or D / 2 (int4), SB = 0 or D / 16 (one half per 32
+// values).  All parts are multiples of 16 bytes (P is 16, 32, 64 or 128).
+//
+// Row codec, int4: for every 32 consecutive values x (bf16) of a row
+//   s = clamp(bf16(max|x| / 7), 2^-14, 9344),  c = clamp(rint(x / s), -7, 7),
+// value = c s.  s has 8 significant bits and lies in half's normal range, c has
+// 3, so s and every value are exact in half.  A group with a non-finite member
+// gets s = NaN.  Nibbles hold c + 8.
+//
+// Order of the bytes inside a row, chosen for the fragments of the attention
+// kernel's m16n8k16 products (a quad lane t = lane % 4, a row lane g = lane / 4):
+//   int4 K: the word of dims 32 j + 8 t .. + 7 is word j of unit t (D / 8 bytes a
+//           unit), so lane t takes its part of all groups j with one load;
+//   int4 V: words in order; D = 128: 32-byte halves swapped in rows with bit 1 set;
+//   bf16:   16-byte units (8 dims) XORed with a function of the row.
+// The swaps make the loads of the attention kernel free of bank conflicts.
+#pragma once
+#include "common.cuh"
+#include <cuda_fp16.h>
+
+namespace dtts {
+
+constexpr int kKvGroup = 32;
+constexpr float kKvScaleMin = 6.103515625e-05f;   // 2^-14
+constexpr float kKvScaleMax = 9344.f;             // 146 * 64: 8 bits, and 7 * 9344 < 65504
+
+struct KvGeom {
+    int L, H, D, P, lgP, i4;
+    int RB, SB;                       // bytes of a row, of its scales
+    long long seg, page_stride;       // bytes of a (page, layer, head) segment, of a page
+    int n_pages, max_seqs, max_pages; // pool pages, table rows, pages of a table row
+};
+
+// Device metadata (ints): the current batch, then the page tables.
+//   seq, start, cnt, len, pos [max_seqs] each: table row of batch entry b, its
+//   first row among the batch's rows, its new tokens, its length with them, and
+//   the position of its first new token; tables [max_seqs + 1][max_pages] (the
+//   last row is the scratch table of a compaction).
+struct KvMeta {
+    const int *seq, *start, *cnt, *len, *pos, *table;
+};
+
+__host__ __device__ inline long long kv_seg_off(const KvGeom &g, int page, int layer, int head) {
+    return (long long)page * g.page_stride + ((long long)layer * g.H + head) * g.seg;
+}
+
+// XOR of the 16-byte unit index inside row r (r: row within the page or tile)
+__host__ __device__ constexpr int kv_swz_k(bool i4, int r) { return i4 ? 0 : (r & 1) << 2; }
+__host__ __device__ constexpr int kv_swz_v(bool i4, int D, int r) {
+    if (i4) return D == 128 ? ((r >> 1) & 1) << 1 : 0;
+    return D == 128 ? (((r >> 1) & 1) | (((r >> 2) & 1) << 2)) : ((((r >> 1) & 1) << 1) | (((r >> 2) & 1) << 2));
+}
+// byte offset of the int4 word that holds dims 8 w .. 8 w + 7 of row r
+__host__ __device__ constexpr int kv_word_k(int D, int w) { return (w & 3) * (D / 8) + (w >> 2) * 4; }
+__host__ __device__ constexpr int kv_word_v(int D, int w, int r) {
+    return (((w >> 2) ^ kv_swz_v(true, D, r)) << 4) + (w & 3) * 4;
+}
+
+// b with start[b] <= row < start[b] + cnt[b] among n entries (starts ascend; entries may be empty)
+DTTS_DEV int kv_find_entry(const int *start, int n, int row) {
+    int lo = 0, hi = n - 1;
+    while (lo < hi) {   // last b with start[b] <= row
+        const int mid = (lo + hi + 1) >> 1;
+        if (start[mid] <= row) lo = mid; else hi = mid - 1;
+    }
+    return lo;
+}
+
+// Quantises 8 bf16 values (a quarter of a group whose four lanes are neighbours)
+// to one word of nibbles; returns the group's scale through s16.  All lanes of
+// the warp take part.
+DTTS_DEV uint32_t kv_encode8(const float (&x)[8], __half *s16) {
+    float a = 0.f;
+    int bad = 0;
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        const float m = fabsf(x[i]);
+        bad |= !(m <= 3.402823466e38f);   // fmaxf drops NaN
+        a = fmaxf(a, m);
+    }
+#pragma unroll
+    for (int o = 1; o < 4; o <<= 1) {
+        a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, o));
+        bad |= __shfl_xor_sync(0xffffffffu, bad, o);
+    }
+    float s = __bfloat162float(__float2bfloat16_rn(__fdiv_rn(a, 7.0f)));
+    s = fminf(fmaxf(s, kKvScaleMin), kKvScaleMax);
+    *s16 = bad ? __ushort_as_half(0x7e00) : __float2half_rn(s);
+    uint32_t w = 0;
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        // IEEE division: x / s is on a rounding border only when the quotient is exact
+        const float c = fminf(fmaxf(rintf(__fdiv_rn(x[i], s)), -7.f), 7.f);
+        w |= (uint32_t)((bad ? 0 : (int)c) + 8) << (4 * i);
+    }
+    return w;
+}
+
+DTTS_DEV float kv_nibble(uint32_t w, int i) { return (float)((int)((w >> (4 * i)) & 15u) - 8); }
+
+// dims 8 w .. 8 w + 7 of row r of a segment (r within the page), as floats
+DTTS_DEV void kv_load8(const KvGeom &g, const uint8_t *seg, bool is_v, int r, int w, float (&x)[8]) {
+    if (g.i4) {
+        const uint8_t *row = seg + (is_v ? g.P * g.RB : 0) + r * g.RB;
+        const uint32_t q = *reinterpret_cast<const uint32_t *>(row + (is_v ? kv_word_v(g.D, w, r) : kv_word_k(g.D, w)));
+        const float s = __half2float(*reinterpret_cast<const __half *>(
+            seg + 2 * g.P * g.RB + (is_v ? g.P * g.SB : 0) + r * g.SB + (w >> 2) * 2));
+#pragma unroll
+        for (int i = 0; i < 8; i++) x[i] = kv_nibble(q, i) * s;
+    } else {
+        const int u = w ^ (is_v ? kv_swz_v(false, g.D, r) : kv_swz_k(false, r));
+        const uint4 q = *reinterpret_cast<const uint4 *>(seg + (is_v ? g.P * g.RB : 0) + r * g.RB + u * 16);
+        const uint32_t e[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            x[2 * i] = __uint_as_float(e[i] << 16);
+            x[2 * i + 1] = __uint_as_float(e[i] & 0xffff0000u);
+        }
+    }
+}
+
+// Stores 8 bf16 values (packed in q) as dims 8 w .. of row r; all lanes of the
+// warp call it, four neighbouring lanes hold one group; on: this lane stores.
+DTTS_DEV void kv_store8(const KvGeom &g, uint8_t *seg, bool is_v, int r, int w, uint4 q, bool on) {
+    if (g.i4) {
+        const uint32_t e[4] = {q.x, q.y, q.z, q.w};
+        float x[8];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            x[2 * i] = __uint_as_float(e[i] << 16);
+            x[2 * i + 1] = __uint_as_float(e[i] & 0xffff0000u);
+        }
+        __half s;
+        const uint32_t c = kv_encode8(x, &s);
+        if (!on) return;
+        uint8_t *row = seg + (is_v ? g.P * g.RB : 0) + r * g.RB;
+        *reinterpret_cast<uint32_t *>(row + (is_v ? kv_word_v(g.D, w, r) : kv_word_k(g.D, w))) = c;
+        if ((w & 3) == 0)
+            *reinterpret_cast<__half *>(seg + 2 * g.P * g.RB + (is_v ? g.P * g.SB : 0) + r * g.SB + (w >> 2) * 2) = s;
+    } else if (on) {
+        const int u = w ^ (is_v ? kv_swz_v(false, g.D, r) : kv_swz_k(false, r));
+        *reinterpret_cast<uint4 *>(seg + (is_v ? g.P * g.RB : 0) + r * g.RB + u * 16) = q;
+    }
+}
+
+// ---------------------------------------------------------------- attention
+struct KvAttendArgs {
+    KvGeom g;
+    KvMeta m;
+    const uint8_t *pool;     // + the layer's offset
+    const bf16 *q;
+    bf16 *out;
+    long long q_row, q_head, o_row, o_head;   // strides in elements
+    int n_seq, G, total_rows;                 // batch entries, query heads per kv head, rows of q / out
+    float scale_log2;                         // scale * log2(e)
+    int window, sinks;
+    int splits, tiles_per_split;              // parts of a long key range, key tiles a part should hold
+    float *ws;                                // partial results
+    int *cnt;                                 // arrivals per split unit, zero between calls
+    int *err;
+};
+// rows (new tokens x query heads per kv head) that the few-row kernel takes
+constexpr int kKvFewRows = 16;
+
+}  // namespace dtts

@@ -1,0 +1,785 @@
+// The paged K/V cache (dtts_kv_*): page tables and reference counts on the host,
+// rows in a pool of pages on the device.  A sequence is a list of pages; forks
+// share pages and copy the last, partly filled one when they grow.  The kernels
+// here store and read rows, copy the rows of a shared page, gather kept rows and
+// apply metadata updates that travel in kernel parameters (no host buffer has to
+// outlive a call).
+#include "kv_host.h"
+
+#include <algorithm>
+#include <cmath>
+#include <cstring>
+#include <memory>
+#include <new>
+
+using namespace dtts;
+
+namespace dtts {
+cudaError_t kv_attend_prepare();
+cudaError_t launch_kv_attend(const KvAttendArgs &a, bool many, int rows_or_tiles, cudaStream_t s);
+int kv_key_tile(const KvGeom &g, bool many);
+}  // namespace dtts
+
+namespace {
+
+constexpr int kWsFloats = 9 * 1024 * 1024;     // 36 MB of partial results
+constexpr int kMaxUnits = 1 << 16;             // split units with an arrival counter
+
+// ---------------------------------------------------------------- metadata
+constexpr int kPokes = 500;
+struct Pokes {
+    int n;
+    int index[kPokes], value[kPokes];
+};
+__global__ void kv_poke_kernel(int *__restrict__ meta, const __grid_constant__ Pokes p) {
+    pdl_wait();
+    pdl_trigger();
+    for (int i = threadIdx.x; i < p.n; i += blockDim.x) meta[p.index[i]] = p.value[i];
+}
+
+constexpr int kPuts = 1000;
+struct Puts {
+    int n;
+    int value[kPuts];
+};
+__global__ void kv_put_kernel(int *__restrict__ dst, const __grid_constant__ Puts p) {
+    pdl_wait();
+    pdl_trigger();
+    for (int i = threadIdx.x; i < p.n; i += blockDim.x) dst[i] = p.value[i];
+}
+
+constexpr int kForks = 900;
+struct Forks {
+    int n, src, pages;
+    int dst[kForks];
+};
+// one block per new table row
+__global__ void kv_fork_tables_kernel(int *__restrict__ table, int max_pages, const __grid_constant__ Forks f) {
+    pdl_wait();
+    pdl_trigger();
+    for (int i = threadIdx.x; i < f.pages; i += blockDim.x)
+        table[(long long)f.dst[blockIdx.x] * max_pages + i] = table[(long long)f.src * max_pages + i];
+}
+
+// ---------------------------------------------------------------- rows
+// A lane handles 8 dims of K or of V; D / 4 lanes take one (row, head): K by the
+// first half of them, V by the second.  The rows' places come from the batch.
+// Bound by memory: 4 D bytes read and 2 (RB + SB) written a row and head.
+__global__ void __launch_bounds__(256) kv_write_kernel(const __grid_constant__ KvGeom g, const __grid_constant__ KvMeta m,
+                                                       uint8_t *__restrict__ pool, int n_seq, int rows,
+                                                       const bf16 *__restrict__ k, const bf16 *__restrict__ v,
+                                                       long long k_row, long long k_head, long long v_row,
+                                                       long long v_head) {
+    pdl_wait();
+    pdl_trigger();
+    const int lpr = g.D / 4;   // lanes a (row, head): 32 or 16
+    const long long id = ((long long)blockIdx.x * blockDim.x + threadIdx.x) / lpr;
+    const int l = threadIdx.x % lpr, w = l % (lpr / 2);
+    const bool is_v = l >= lpr / 2;
+    bool on = id < (long long)rows * g.H;
+    const int row = on ? (int)(id / g.H) : 0, head = on ? (int)(id % g.H) : 0;
+    const int b = kv_find_entry(m.start, n_seq, row);
+    const int off = row - m.start[b];
+    on = on && off < m.cnt[b];
+    const int tok = on ? m.len[b] - m.cnt[b] + off : 0;
+    const int page = on ? m.table[(long long)m.seq[b] * g.max_pages + (tok >> g.lgP)] : -1;
+    on = on && page >= 0 && page < g.n_pages;
+    uint4 q = make_uint4(0u, 0u, 0u, 0u);
+    if (on)
+        q = is_v ? *reinterpret_cast<const uint4 *>(v + row * v_row + head * v_head + 8 * w)
+                 : *reinterpret_cast<const uint4 *>(k + row * k_row + head * k_head + 8 * w);
+    kv_store8(g, pool + kv_seg_off(g, on ? page : 0, 0, head), is_v, tok & (g.P - 1), w, q, on);
+}
+
+// Rows [first, first + count) of the listed sequences, for n_layers layers, as
+// [layer][row][head][D] fp32 or bf16.  Same lane split as the write.
+constexpr int kReads = 320;
+struct Reads {
+    int n, rows, n_layers;            // entries, rows a layer (of all entries of the call)
+    int seq[kReads], first[kReads], start[kReads + 1];   // start: first output row, start[n]: end
+};
+template <bool F32>
+__global__ void __launch_bounds__(256) kv_read_kernel(const __grid_constant__ KvGeom g, const int *__restrict__ table,
+                                                      const uint8_t *__restrict__ pool, const __grid_constant__ Reads r,
+                                                      void *__restrict__ k, void *__restrict__ v) {
+    pdl_wait();
+    pdl_trigger();
+    const int lpr = g.D / 4;
+    const long long id = ((long long)blockIdx.x * blockDim.x + threadIdx.x) / lpr;
+    const int l = threadIdx.x % lpr, w = l % (lpr / 2), n_rows = r.start[r.n] - r.start[0];
+    const bool is_v = l >= lpr / 2;
+    if (id >= (long long)n_rows * g.H) return;
+    const int row = r.start[0] + (int)(id / g.H), head = (int)(id % g.H), layer = blockIdx.y;
+    const int e = kv_find_entry(r.start, r.n, row);
+    const int tok = r.first[e] + row - r.start[e];
+    const int page = table[(long long)r.seq[e] * g.max_pages + (tok >> g.lgP)];
+    if (page < 0 || page >= g.n_pages) return;
+    float x[8];
+    kv_load8(g, pool + kv_seg_off(g, page, layer, head), is_v, tok & (g.P - 1), w, x);
+    const long long at = (((long long)layer * r.rows + row) * g.H + head) * g.D + 8 * w;
+    void *dst = is_v ? v : k;
+    if (F32) {
+        float4 *o = reinterpret_cast<float4 *>(static_cast<float *>(dst) + at);
+        o[0] = make_float4(x[0], x[1], x[2], x[3]);
+        o[1] = make_float4(x[4], x[5], x[6], x[7]);
+    } else {
+        *reinterpret_cast<uint4 *>(static_cast<bf16 *>(dst) + at) =
+            make_uint4(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), pack_bf16x2(x[4], x[5]), pack_bf16x2(x[6], x[7]));
+    }
+}
+
+// The first `rows` rows of pages src to pages dst, all layers and heads: four
+// contiguous runs a segment (K, V and their scales), copied in 16-byte units
+// (a scale run is rounded up, inside its part).
+constexpr int kCopies = 320;
+struct Copies {
+    int n;
+    int src[kCopies], dst[kCopies], rows[kCopies];
+};
+__global__ void __launch_bounds__(256) kv_copy_pages_kernel(const __grid_constant__ KvGeom g, uint8_t *__restrict__ pool,
+                                                            const __grid_constant__ Copies c) {
+    pdl_wait();
+    pdl_trigger();
+    const int e = blockIdx.y, n = c.rows[e];
+    const uint8_t *src = pool + (long long)c.src[e] * g.page_stride + (long long)blockIdx.x * g.seg;
+    uint8_t *dst = pool + (long long)c.dst[e] * g.page_stride + (long long)blockIdx.x * g.seg;
+    const int ur = n * g.RB / 16, us = (n * g.SB + 15) / 16;
+    for (int i = threadIdx.x; i < 2 * (ur + us); i += blockDim.x) {
+        int off;
+        if (i < 2 * ur)
+            off = (i < ur ? 0 : g.P * g.RB - ur * 16) + i * 16;
+        else {
+            const int j = i - 2 * ur;
+            off = 2 * g.P * g.RB + (j < us ? 0 : g.P * g.SB - us * 16) + j * 16;
+        }
+        *reinterpret_cast<uint4 *>(dst + off) = *reinterpret_cast<const uint4 *>(src + off);
+    }
+}
+
+// Rows keep[j] of table row src to rows j0 + j of table row dst (j < n), all
+// layers and heads.  A thread moves one 16-byte unit; units change their place
+// within the row as the row's number does.  Then the scales, a row at a time.
+__global__ void __launch_bounds__(256) kv_gather_kernel(const __grid_constant__ KvGeom g, const int *__restrict__ table,
+                                                        uint8_t *__restrict__ pool, const int *__restrict__ keep, int n,
+                                                        int j0, int src, int dst) {
+    pdl_wait();
+    pdl_trigger();
+    const int u_row = g.RB / 16, per = 2 * u_row + (g.i4 ? 2 : 0);   // units of K, of V; scales of K, of V
+    const long long base = (long long)blockIdx.y * g.seg;            // (layer, head)
+    for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < (long long)n * per;
+         i += (long long)gridDim.x * blockDim.x) {
+        const int j = (int)(i / per), u = (int)(i % per);
+        const int a = keep[j], b = j0 + j;
+        const int pa = table[(long long)src * g.max_pages + (a >> g.lgP)];
+        const int pb = table[(long long)dst * g.max_pages + (b >> g.lgP)];
+        if (pa < 0 || pa >= g.n_pages || pb < 0 || pb >= g.n_pages) continue;
+        const uint8_t *sa = pool + (long long)pa * g.page_stride + base;
+        uint8_t *sb = pool + (long long)pb * g.page_stride + base;
+        const int ra = a & (g.P - 1), rb = b & (g.P - 1);
+        if (u < 2 * u_row) {
+            const bool is_v = u >= u_row;
+            const int w = is_v ? u - u_row : u, part = is_v ? g.P * g.RB : 0;
+            const int ua = w ^ (is_v ? kv_swz_v(g.i4, g.D, ra) : kv_swz_k(g.i4, ra));
+            const int ub = w ^ (is_v ? kv_swz_v(g.i4, g.D, rb) : kv_swz_k(g.i4, rb));
+            *reinterpret_cast<uint4 *>(sb + part + rb * g.RB + ub * 16) =
+                *reinterpret_cast<const uint4 *>(sa + part + ra * g.RB + ua * 16);
+        } else {
+            const int part = 2 * g.P * g.RB + (u - 2 * u_row) * g.P * g.SB;
+            if (g.SB == 8)
+                *reinterpret_cast<uint2 *>(sb + part + rb * 8) = *reinterpret_cast<const uint2 *>(sa + part + ra * 8);
+            else
+                *reinterpret_cast<uint32_t *>(sb + part + rb * 4) = *reinterpret_cast<const uint32_t *>(sa + part + ra * 4);
+        }
+    }
+}
+
+bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+bool seq_ok(const dtts_kv *kv, int s) { return s >= 0 && s < kv->g.max_seqs && kv->seqs[s].open; }
+
+}  // namespace
+
+dtts_kv::~dtts_kv() {
+    mem.free_all();
+    if (handoff) cudaEventDestroy(handoff);
+    if (own_stream) cudaStreamDestroy(own_stream);
+}
+
+KvMeta dtts_kv::kv_meta() const {
+    KvMeta m;
+    m.seq = meta;
+    m.start = meta + g.max_seqs;
+    m.cnt = meta + 2 * g.max_seqs;
+    m.len = meta + 3 * g.max_seqs;
+    m.pos = meta + 4 * g.max_seqs;
+    m.table = meta + 5 * g.max_seqs;
+    return m;
+}
+
+int dtts_kv::flush() {
+    for (size_t i = 0; i < pokes.size(); i += kPokes) {
+        Pokes p;
+        p.n = (int)std::min<size_t>(kPokes, pokes.size() - i);
+        for (int j = 0; j < p.n; j++) {
+            p.index[j] = pokes[i + j];
+            p.value[j] = meta_h[pokes[i + j]];   // an index listed twice gets its last value both times
+        }
+        DTTS_CUDA(launch_k(kLaunchPdl, kv_poke_kernel, dim3(1), dim3(256), 0, stream, meta, p));
+    }
+    pokes.clear();
+    return DTTS_OK;
+}
+
+void dtts_kv::drop_batch() {
+    b_seq.clear();
+    b_cnt.clear();
+    b_len.clear();
+    b_rows = 0;
+    b_id++;
+}
+
+int dtts_kv::not_capturing(const char *what) const {
+    cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
+    DTTS_CUDA(cudaStreamIsCapturing(stream, &st));
+    DTTS_CHECK(st == cudaStreamCaptureStatusNone, DTTS_ERR_UNSUPPORTED,
+               "%s changes the cache's tables and cannot be captured into a graph", what);
+    return DTTS_OK;
+}
+
+// Grows the sequences and makes them the current batch.  Nothing changes unless
+// everything fits.
+int dtts_kv::extend(int n_seq, const int *sq, const int *n_new) {
+    int st = not_capturing("extend");
+    if (st) return st;
+    std::vector<int> listed(sq, sq + n_seq);
+    std::sort(listed.begin(), listed.end());
+    DTTS_CHECK(std::adjacent_find(listed.begin(), listed.end()) == listed.end(), DTTS_ERR_ARG,
+               "a sequence is listed twice");
+    long long need = 0, rows = 0;
+    std::vector<int> lowered;   // shared tail pages counted as copied
+    for (int b = 0; b < n_seq; b++) {
+        const Seq &s = seqs[sq[b]];
+        const long long len = (long long)s.len + n_new[b];
+        if (len > max_tokens || (long long)s.pos + n_new[b] > INT32_MAX) {
+            for (int p : lowered) refs[p]++;
+            set_error("sequence %d would hold %lld tokens (limit %lld)", sq[b], len, max_tokens);
+            return DTTS_ERR_ARG;
+        }
+        rows += n_new[b];
+        need += (len + g.P - 1) / g.P - (long long)s.pages.size();
+        if (n_new[b] > 0 && (s.len & (g.P - 1)) && refs[s.pages.back()] > 1) {
+            need++;
+            refs[s.pages.back()]--;
+            lowered.push_back(s.pages.back());
+        }
+    }
+    for (int p : lowered) refs[p]++;
+    DTTS_CHECK(rows <= INT32_MAX / 2, DTTS_ERR_ARG, "%lld new rows in one batch", rows);
+    DTTS_CHECK(need <= (long long)free_pages.size(), DTTS_ERR_OOM, "%lld pages needed, %zu free", need,
+               free_pages.size());
+    Copies c;
+    c.n = 0;
+    std::vector<Copies> copies;
+    b_seq.assign(sq, sq + n_seq);
+    b_cnt.assign(n_new, n_new + n_seq);
+    b_len.resize(n_seq);
+    b_rows = (int)rows;
+    b_id++;
+    int start = 0;
+    for (int b = 0; b < n_seq; b++) {
+        Seq &s = seqs[sq[b]];
+        if (n_new[b] > 0 && (s.len & (g.P - 1)) && refs[s.pages.back()] > 1) {
+            const int from = s.pages.back(), to = take_page();
+            refs[from]--;   // shared: never the last user here
+            s.pages.back() = to;
+            poke(table_at(sq[b], (int)s.pages.size() - 1), to);
+            c.src[c.n] = from;
+            c.dst[c.n] = to;
+            c.rows[c.n] = s.len & (g.P - 1);
+            if (++c.n == kCopies) { copies.push_back(c); c.n = 0; }
+        }
+        const int pos = s.pos;
+        s.len += n_new[b];
+        s.pos += n_new[b];
+        while ((long long)s.pages.size() * g.P < s.len) {
+            s.pages.push_back(take_page());
+            poke(table_at(sq[b], (int)s.pages.size() - 1), s.pages.back());
+        }
+        b_len[b] = s.len;
+        poke(b, sq[b]);
+        poke(g.max_seqs + b, start);
+        poke(2 * g.max_seqs + b, n_new[b]);
+        poke(3 * g.max_seqs + b, s.len);
+        poke(4 * g.max_seqs + b, pos);
+        start += n_new[b];
+    }
+    // entries behind the batch hold no rows (a graph captured for a larger batch finds nothing to do there)
+    for (int b = n_seq; b < g.max_seqs; b++) {
+        poke(g.max_seqs + b, start);
+        poke(2 * g.max_seqs + b, 0);
+    }
+    if (c.n) copies.push_back(c);
+    for (const Copies &cc : copies)
+        DTTS_CUDA(launch_k(kLaunchPdl, kv_copy_pages_kernel, dim3(g.L * g.H, cc.n), dim3(256), 0, stream, g, pool, cc));
+    return flush();
+}
+
+extern "C" {
+
+int dtts_kv_create(const dtts_kv_config *c, int device, dtts_kv **out) try {
+    DTTS_CHECK(c && out, DTTS_ERR_ARG, "null argument");
+    *out = nullptr;
+    DTTS_CHECK(c->dtype == DTTS_DTYPE_BF16 || c->dtype == DTTS_DTYPE_INT4, DTTS_ERR_UNSUPPORTED, "dtype %d", c->dtype);
+    DTTS_CHECK(c->head_dim == 64 || c->head_dim == 128, DTTS_ERR_UNSUPPORTED, "head_dim %d (64 or 128)", c->head_dim);
+    DTTS_CHECK(c->page_tokens == 16 || c->page_tokens == 32 || c->page_tokens == 64 || c->page_tokens == 128,
+               DTTS_ERR_UNSUPPORTED, "page_tokens %d (16, 32, 64 or 128)", c->page_tokens);
+    DTTS_CHECK(c->n_layers >= 1 && c->n_layers <= 1024 && c->n_kv_heads >= 1 && c->n_kv_heads <= 256, DTTS_ERR_ARG,
+               "bad geometry: %d layers, %d heads", c->n_layers, c->n_kv_heads);
+    DTTS_CHECK((long long)c->n_layers * c->n_kv_heads <= 65535, DTTS_ERR_ARG, "%d layers of %d heads (65535 in all)",
+               c->n_layers, c->n_kv_heads);
+    DTTS_CHECK(c->n_pages >= 1 && c->max_seqs >= 1 && c->max_seqs <= 65535 && c->max_tokens >= 1 &&
+                   c->max_tokens <= (1 << 24),
+               DTTS_ERR_ARG, "bad capacity: %d pages, %d sequences of %d tokens", c->n_pages, c->max_seqs, c->max_tokens);
+    const int P = c->page_tokens;
+    const long long max_pages = ((long long)c->max_tokens + P - 1) / P;
+    const long long ints = 5ll * c->max_seqs + (long long)(c->max_seqs + 1) * max_pages;
+    DTTS_CHECK(ints <= INT32_MAX, DTTS_ERR_ARG, "page tables of %d sequences of %d tokens", c->max_seqs, c->max_tokens);
+    int nsm = 0, st = check_device(device, &nsm);
+    if (st) return st;
+    DeviceGuard dg(device);
+    std::unique_ptr<dtts_kv> kv(new dtts_kv());
+    kv->device = device;
+    kv->num_sms = nsm;
+    kv->max_tokens = c->max_tokens;
+    KvGeom &g = kv->g;
+    g.L = c->n_layers; g.H = c->n_kv_heads; g.D = c->head_dim; g.P = P;
+    g.lgP = P == 16 ? 4 : P == 32 ? 5 : P == 64 ? 6 : 7;
+    g.i4 = c->dtype == DTTS_DTYPE_INT4;
+    g.RB = g.i4 ? g.D / 2 : g.D * 2;
+    g.SB = g.i4 ? g.D / kKvGroup * 2 : 0;
+    g.seg = 2ll * P * (g.RB + g.SB);
+    g.page_stride = g.seg * g.L * g.H;
+    g.n_pages = c->n_pages; g.max_seqs = c->max_seqs; g.max_pages = (int)max_pages;
+    DTTS_CUDA(cudaStreamCreateWithFlags(&kv->own_stream, cudaStreamNonBlocking));
+    kv->stream = kv->own_stream;
+    DTTS_CUDA(cudaEventCreateWithFlags(&kv->handoff, cudaEventDisableTiming));
+    DTTS_CUDA(kv_attend_prepare());
+    const size_t pool_bytes = (size_t)g.page_stride * g.n_pages;
+    kv->pool = (uint8_t *)kv->mem.alloc(pool_bytes);
+    kv->meta = (int *)kv->mem.alloc((size_t)ints * 4);
+    kv->keep = (int *)kv->mem.alloc((size_t)c->max_tokens * 4);
+    kv->cnt = (int *)kv->mem.alloc((size_t)kMaxUnits * 4);
+    kv->d_err = (int *)kv->mem.alloc(4);
+    kv->ws = (float *)kv->mem.alloc((size_t)kWsFloats * 4);
+    if (!kv->pool || !kv->meta || !kv->keep || !kv->cnt || !kv->d_err || !kv->ws) {
+        cudaGetLastError();   // a failed cudaMalloc must not surface in a later call
+        set_error("K/V cache allocation failed (%zu MB of pages)", pool_bytes >> 20);
+        return DTTS_ERR_OOM;
+    }
+    kv->meta_h.assign((size_t)ints, 0);
+    DTTS_CUDA(cudaMemsetAsync(kv->pool, 0, pool_bytes, kv->stream));
+    DTTS_CUDA(cudaMemsetAsync(kv->meta, 0, (size_t)ints * 4, kv->stream));
+    DTTS_CUDA(cudaMemsetAsync(kv->cnt, 0, (size_t)kMaxUnits * 4, kv->stream));
+    DTTS_CUDA(cudaMemsetAsync(kv->d_err, 0, 4, kv->stream));
+    DTTS_CUDA(cudaStreamSynchronize(kv->stream));
+    kv->seqs.resize(g.max_seqs);
+    kv->refs.assign(g.n_pages, 0);
+    for (int p = 0; p < g.n_pages; p++) kv->free_pages.push(p);
+    *out = kv.release();
+    return DTTS_OK;
+} catch (const std::bad_alloc &) {
+    set_error("out of host memory");
+    return DTTS_ERR_OOM;
+}
+
+int dtts_kv_destroy(dtts_kv *kv) {
+    if (!kv) return DTTS_OK;
+    DeviceGuard dg(kv->device);
+    cudaStreamSynchronize(kv->stream);
+    delete kv;
+    return DTTS_OK;
+}
+
+int dtts_kv_set_stream(dtts_kv *kv, void *stream) {
+    DTTS_CHECK(kv, DTTS_ERR_ARG, "null cache");
+    cudaStream_t s = stream ? static_cast<cudaStream_t>(stream) : kv->own_stream;
+    if (s == kv->stream) return DTTS_OK;
+    DeviceGuard dg(kv->device);
+    // work already enqueued on the old stream stays before what follows on the new one
+    cudaStreamCaptureStatus a = cudaStreamCaptureStatusNone, b = cudaStreamCaptureStatusNone;
+    DTTS_CUDA(cudaStreamIsCapturing(kv->stream, &a));
+    DTTS_CUDA(cudaStreamIsCapturing(s, &b));
+    if (a == cudaStreamCaptureStatusNone && b == cudaStreamCaptureStatusNone) {
+        DTTS_CUDA(cudaEventRecord(kv->handoff, kv->stream));
+        DTTS_CUDA(cudaStreamWaitEvent(s, kv->handoff, 0));
+    }
+    kv->stream = s;
+    return DTTS_OK;
+}
+
+int dtts_kv_sync(dtts_kv *kv) {
+    DTTS_CHECK(kv, DTTS_ERR_ARG, "null cache");
+    DeviceGuard dg(kv->device);
+    int st = stream_wait(kv->stream, 300.0);
+    if (st) return st;
+    int err = 0;
+    DTTS_CUDA(cudaMemcpy(&err, kv->d_err, 4, cudaMemcpyDeviceToHost));
+    if (err) {
+        cudaMemset(kv->d_err, 0, 4);
+        set_error("device wait limit reached (code %d)", err);
+        return DTTS_ERR_TIMEOUT;
+    }
+    return DTTS_OK;
+}
+
+int dtts_kv_open(dtts_kv *kv, int *seq) {
+    DTTS_CHECK(kv && seq, DTTS_ERR_ARG, "null argument");
+    for (int s = 0; s < kv->g.max_seqs; s++)
+        if (!kv->seqs[s].open) {
+            kv->seqs[s] = dtts_kv::Seq();
+            kv->seqs[s].open = true;
+            *seq = s;
+            return DTTS_OK;
+        }
+    set_error("all %d sequences are open", kv->g.max_seqs);
+    return DTTS_ERR_OOM;
+}
+
+int dtts_kv_close(dtts_kv *kv, int n, const int *seqs) try {
+    DTTS_CHECK(kv && (n == 0 || seqs) && n >= 0, DTTS_ERR_ARG, "null argument");
+    for (int i = 0; i < n; i++) DTTS_CHECK(seq_ok(kv, seqs[i]), DTTS_ERR_ARG, "sequence %d is not open", seqs[i]);
+    std::vector<int> listed(seqs, seqs + n);
+    std::sort(listed.begin(), listed.end());
+    DTTS_CHECK(std::adjacent_find(listed.begin(), listed.end()) == listed.end(), DTTS_ERR_ARG,
+               "a sequence is listed twice");
+    for (int s : listed) {
+        for (int p : kv->seqs[s].pages) kv->drop_page(p);
+        kv->seqs[s] = dtts_kv::Seq();
+    }
+    for (int s : kv->b_seq)
+        if (std::binary_search(listed.begin(), listed.end(), s)) { kv->drop_batch(); break; }
+    return DTTS_OK;
+} catch (const std::bad_alloc &) {
+    set_error("out of host memory");
+    return DTTS_ERR_OOM;
+}
+
+int dtts_kv_fork(dtts_kv *kv, int src, int n, int *dst) try {
+    DTTS_CHECK(kv && (n == 0 || dst) && n >= 0, DTTS_ERR_ARG, "null argument");
+    DTTS_CHECK(seq_ok(kv, src), DTTS_ERR_ARG, "sequence %d is not open", src);
+    DeviceGuard dg(kv->device);
+    int st = kv->not_capturing("fork");
+    if (st) return st;
+    std::vector<int> to;
+    for (int s = 0; s < kv->g.max_seqs && (int)to.size() < n; s++)
+        if (!kv->seqs[s].open) to.push_back(s);
+    DTTS_CHECK((int)to.size() == n, DTTS_ERR_OOM, "%d sequences wanted, %zu free", n, to.size());
+    if ((st = kv->flush())) return st;   // the source's row on the device is current
+    const int pages = (int)kv->seqs[src].pages.size();
+    for (int i = 0; i < n && pages; i += kForks) {
+        Forks f;
+        f.n = std::min(kForks, n - i);
+        f.src = src;
+        f.pages = pages;
+        for (int j = 0; j < f.n; j++) f.dst[j] = to[i + j];
+        DTTS_CUDA(launch_k(kLaunchPdl, kv_fork_tables_kernel, dim3(f.n), dim3(128), 0, kv->stream,
+                           kv->meta + 5 * kv->g.max_seqs, kv->g.max_pages, f));
+    }
+    for (int s : to) {
+        kv->seqs[s] = kv->seqs[src];
+        for (int p = 0; p < pages; p++) {
+            kv->meta_h[kv->table_at(s, p)] = kv->meta_h[kv->table_at(src, p)];
+            if (kv->seqs[s].pages[p] >= 0) kv->refs[kv->seqs[s].pages[p]]++;
+        }
+    }
+    std::copy(to.begin(), to.end(), dst);
+    return DTTS_OK;
+} catch (const std::bad_alloc &) {
+    set_error("out of host memory");
+    return DTTS_ERR_OOM;
+}
+
+int dtts_kv_truncate(dtts_kv *kv, int seq, int n_tokens) {
+    DTTS_CHECK(kv, DTTS_ERR_ARG, "null cache");
+    DTTS_CHECK(seq_ok(kv, seq), DTTS_ERR_ARG, "sequence %d is not open", seq);
+    dtts_kv::Seq &s = kv->seqs[seq];
+    DTTS_CHECK(n_tokens >= 0 && n_tokens <= s.len, DTTS_ERR_ARG, "sequence %d holds %d tokens, not %d", seq, s.len,
+               n_tokens);
+    const int keep = (n_tokens + kv->g.P - 1) / kv->g.P;
+    DTTS_CHECK(keep == 0 || n_tokens == s.len || s.pages[keep - 1] >= 0, DTTS_ERR_ARG,
+               "row %d of sequence %d was freed by a trim", n_tokens - 1, seq);
+    if (n_tokens == s.len) return DTTS_OK;
+    for (size_t p = keep; p < s.pages.size(); p++) kv->drop_page(s.pages[p]);
+    s.pages.resize(keep);
+    s.hole_hi = std::min(s.hole_hi, keep);
+    if (s.hole_lo >= s.hole_hi) s.hole_lo = s.hole_hi = 0;
+    s.pos -= s.len - n_tokens;
+    s.len = n_tokens;
+    for (int b : kv->b_seq)
+        if (b == seq) { kv->drop_batch(); break; }
+    return DTTS_OK;
+}
+
+int dtts_kv_trim(dtts_kv *kv, int seq, int window, int sinks) {
+    DTTS_CHECK(kv, DTTS_ERR_ARG, "null cache");
+    DTTS_CHECK(seq_ok(kv, seq), DTTS_ERR_ARG, "sequence %d is not open", seq);
+    DTTS_CHECK(window >= 1 && sinks >= 0, DTTS_ERR_ARG, "window %d, sinks %d", window, sinks);
+    dtts_kv::Seq &s = kv->seqs[seq];
+    const int P = kv->g.P;
+    // the next token, at row len, sees rows > len - window and rows < sinks
+    const long long lo = std::max(0ll, (long long)s.len - window + 1);
+    const long long a = ((long long)sinks + P - 1) / P, b = std::min<long long>(lo / P, (long long)s.pages.size());
+    if (a >= b) return DTTS_OK;
+    bool any = false;
+    for (long long p = a; p < b; p++)
+        if (s.pages[p] >= 0) {
+            kv->drop_page(s.pages[p]);
+            s.pages[p] = -1;
+            kv->poke(kv->table_at(seq, (int)p), -1);
+            any = true;
+        }
+    if (!any) return DTTS_OK;
+    if (s.hole_lo >= s.hole_hi) {
+        s.hole_lo = (int)a;
+        s.hole_hi = (int)b;
+    } else {
+        s.hole_lo = std::min(s.hole_lo, (int)a);
+        s.hole_hi = std::max(s.hole_hi, (int)b);
+    }
+    for (int e : kv->b_seq)
+        if (e == seq) { kv->drop_batch(); break; }
+    return DTTS_OK;
+}
+
+int dtts_kv_compact(dtts_kv *kv, int seq, int n_keep, const int *keep) try {
+    DTTS_CHECK(kv && (n_keep == 0 || keep) && n_keep >= 0, DTTS_ERR_ARG, "null argument");
+    DTTS_CHECK(seq_ok(kv, seq), DTTS_ERR_ARG, "sequence %d is not open", seq);
+    DeviceGuard dg(kv->device);
+    int st = kv->not_capturing("compact");
+    if (st) return st;
+    dtts_kv::Seq &s = kv->seqs[seq];
+    const KvGeom &g = kv->g;
+    DTTS_CHECK(n_keep <= s.len, DTTS_ERR_ARG, "sequence %d holds %d rows, not %d", seq, s.len, n_keep);
+    for (int j = 0; j < n_keep; j++) {
+        DTTS_CHECK(keep[j] >= 0 && keep[j] < s.len && (j == 0 || keep[j] > keep[j - 1]), DTTS_ERR_ARG,
+                   "kept rows must ascend within 0..%d (entry %d is %d)", s.len - 1, j, keep[j]);
+        DTTS_CHECK(s.pages[keep[j] >> g.lgP] >= 0, DTTS_ERR_ARG, "row %d of sequence %d was freed by a trim", keep[j], seq);
+    }
+    // pages of the unchanged start stay; the rest goes to fresh pages
+    int same = 0;
+    while (same < n_keep && keep[same] == same) same++;
+    const int stay = same == n_keep && n_keep == s.len ? (int)s.pages.size() : same >> g.lgP;
+    const int total = (n_keep + g.P - 1) / g.P, fresh = std::max(0, total - stay);
+    if (stay == (int)s.pages.size() && n_keep == s.len) return DTTS_OK;
+    DTTS_CHECK(fresh <= (int)kv->free_pages.size(), DTTS_ERR_OOM, "%d pages needed, %zu free", fresh,
+               kv->free_pages.size());
+    const int j0 = stay << g.lgP, n = n_keep - j0, scratch = g.max_seqs;
+    std::vector<int> pages(s.pages.begin(), s.pages.begin() + stay);
+    for (int p = stay; p < total; p++) {
+        pages.push_back(kv->take_page());
+        kv->poke(kv->table_at(scratch, p), pages.back());
+    }
+    if ((st = kv->flush())) return st;
+    if (n > 0) {
+        for (int i = 0; i < n; i += kPuts) {
+            Puts p;
+            p.n = std::min(kPuts, n - i);
+            std::memcpy(p.value, keep + j0 + i, (size_t)p.n * 4);
+            DTTS_CUDA(launch_k(kLaunchPdl, kv_put_kernel, dim3(1), dim3(256), 0, kv->stream, kv->keep + i, p));
+        }
+        const long long units = (long long)n * (2 * g.RB / 16 + (g.i4 ? 2 : 0));
+        const int gx = (int)std::min<long long>((units + 255) / 256, 1024);
+        DTTS_CUDA(launch_k(kLaunchPdl, kv_gather_kernel, dim3(gx, g.L * g.H), dim3(256), 0, kv->stream, g,
+                           (const int *)(kv->meta + 5 * g.max_seqs), kv->pool, (const int *)kv->keep, n, j0, seq, scratch));
+    }
+    for (int p = 0; p < total; p++) kv->poke(kv->table_at(seq, p), pages[p]);
+    if ((st = kv->flush())) return st;
+    for (size_t p = stay; p < s.pages.size(); p++) kv->drop_page(s.pages[p]);
+    s.pages.swap(pages);
+    s.len = n_keep;
+    s.hole_lo = s.hole_hi = 0;
+    for (int b : kv->b_seq)
+        if (b == seq) { kv->drop_batch(); break; }
+    return DTTS_OK;
+} catch (const std::bad_alloc &) {
+    set_error("out of host memory");
+    return DTTS_ERR_OOM;
+}
+
+int dtts_kv_length(dtts_kv *kv, int seq, int *tokens, int *position) {
+    DTTS_CHECK(kv, DTTS_ERR_ARG, "null cache");
+    DTTS_CHECK(seq_ok(kv, seq), DTTS_ERR_ARG, "sequence %d is not open", seq);
+    if (tokens) *tokens = kv->seqs[seq].len;
+    if (position) *position = kv->seqs[seq].pos;
+    return DTTS_OK;
+}
+
+int dtts_kv_free_pages(dtts_kv *kv, int *n) {
+    DTTS_CHECK(kv && n, DTTS_ERR_ARG, "null argument");
+    *n = (int)kv->free_pages.size();
+    return DTTS_OK;
+}
+
+int dtts_kv_extend(dtts_kv *kv, int n_seq, const int *seqs, const int *n_new) try {
+    DTTS_CHECK(kv && seqs && n_new, DTTS_ERR_ARG, "null argument");
+    DTTS_CHECK(n_seq >= 1 && n_seq <= kv->g.max_seqs, DTTS_ERR_ARG, "%d sequences (1..%d)", n_seq, kv->g.max_seqs);
+    for (int b = 0; b < n_seq; b++) {
+        DTTS_CHECK(seq_ok(kv, seqs[b]), DTTS_ERR_ARG, "sequence %d is not open", seqs[b]);
+        DTTS_CHECK(n_new[b] >= 0, DTTS_ERR_ARG, "%d new tokens", n_new[b]);
+    }
+    DeviceGuard dg(kv->device);
+    return kv->extend(n_seq, seqs, n_new);
+} catch (const std::bad_alloc &) {
+    set_error("out of host memory");
+    return DTTS_ERR_OOM;
+}
+
+int dtts_kv_write(dtts_kv *kv, int layer, const void *k, const void *v, long long k_row, long long k_head,
+                  long long v_row, long long v_head) {
+    DTTS_CHECK(kv, DTTS_ERR_ARG, "null cache");
+    const KvGeom &g = kv->g;
+    DTTS_CHECK(layer >= 0 && layer < g.L, DTTS_ERR_ARG, "layer %d of %d", layer, g.L);
+    DTTS_CHECK(!kv->b_seq.empty(), DTTS_ERR_ARG, "no current batch: call dtts_kv_extend first");
+    if (kv->b_rows == 0) return DTTS_OK;
+    DTTS_CHECK(k && v, DTTS_ERR_ARG, "null argument");
+    DTTS_CHECK(aligned16(k) && aligned16(v) && !((k_row | k_head | v_row | v_head) & 7), DTTS_ERR_ARG,
+               "rows must start on 16-byte boundaries");
+    DeviceGuard dg(kv->device);
+    int st = kv->flush();
+    if (st) return st;
+    const int per_block = 256 / (g.D / 4);
+    const long long items = (long long)kv->b_rows * g.H;
+    DTTS_CHECK((items + per_block - 1) / per_block <= INT32_MAX, DTTS_ERR_ARG, "%d rows in one batch", kv->b_rows);
+    DTTS_CUDA(launch_k(kLaunchPdl, kv_write_kernel, dim3((unsigned)((items + per_block - 1) / per_block)), dim3(256), 0,
+                       kv->stream, g, kv->kv_meta(), kv->pool + (long long)layer * g.H * g.seg, (int)kv->b_seq.size(),
+                       kv->b_rows, (const bf16 *)k, (const bf16 *)v, k_row, k_head, v_row, v_head));
+    return DTTS_OK;
+}
+
+int dtts_kv_read(dtts_kv *kv, int layer, int n_layers, int n, const int *seqs, const int *first, const int *count,
+                 void *k, void *v, int dtype) try {
+    DTTS_CHECK(kv && (n == 0 || (seqs && first && count)) && n >= 0, DTTS_ERR_ARG, "null argument");
+    const KvGeom &g = kv->g;
+    DTTS_CHECK(dtype == DTTS_DTYPE_F32 || dtype == DTTS_DTYPE_BF16, DTTS_ERR_UNSUPPORTED, "dtype %d", dtype);
+    DTTS_CHECK(layer >= 0 && n_layers >= 1 && layer < g.L && n_layers <= g.L - layer, DTTS_ERR_ARG,
+               "layers %d..%d of %d", layer, layer + n_layers - 1, g.L);
+    long long rows = 0;
+    for (int i = 0; i < n; i++) {
+        DTTS_CHECK(seq_ok(kv, seqs[i]), DTTS_ERR_ARG, "sequence %d is not open", seqs[i]);
+        const dtts_kv::Seq &s = kv->seqs[seqs[i]];
+        DTTS_CHECK(first[i] >= 0 && count[i] >= 0 && (long long)first[i] + count[i] <= s.len, DTTS_ERR_ARG,
+                   "rows %d..%lld of sequence %d, which holds %d", first[i], (long long)first[i] + count[i] - 1, seqs[i],
+                   s.len);
+        if (count[i] && s.hole_lo < s.hole_hi)
+            for (int p = first[i] >> g.lgP; p <= (first[i] + count[i] - 1) >> g.lgP; p++)
+                DTTS_CHECK(s.pages[p] >= 0, DTTS_ERR_ARG, "rows %d.. of sequence %d were freed by a trim", p * g.P, seqs[i]);
+        rows += count[i];
+    }
+    if (rows == 0) return DTTS_OK;
+    DTTS_CHECK(k && v && aligned16(k) && aligned16(v), DTTS_ERR_ARG, "outputs must be on 16-byte boundaries");
+    DTTS_CHECK(rows <= INT32_MAX / 2, DTTS_ERR_ARG, "%lld rows in one call", rows);
+    DeviceGuard dg(kv->device);
+    int st = kv->flush();
+    if (st) return st;
+    const int per_block = 256 / (g.D / 4);
+    int start = 0;
+    for (int i = 0; i < n; i += kReads) {
+        Reads r;
+        r.n = std::min(kReads, n - i);
+        r.rows = (int)rows;
+        r.n_layers = n_layers;
+        for (int j = 0; j < r.n; j++) {
+            r.seq[j] = seqs[i + j];
+            r.first[j] = first[i + j];
+            r.start[j] = start;
+            start += count[i + j];
+        }
+        r.start[r.n] = start;
+        const long long items = (long long)(start - r.start[0]) * g.H;
+        if (!items) continue;
+        const dim3 grid((unsigned)((items + per_block - 1) / per_block), n_layers);
+        const uint8_t *pool = kv->pool + (long long)layer * g.H * g.seg;
+        const int *table = kv->meta + 5 * g.max_seqs;
+        if (dtype == DTTS_DTYPE_F32)
+            DTTS_CUDA(launch_k(kLaunchPdl, kv_read_kernel<true>, grid, dim3(256), 0, kv->stream, g, table, pool, r, k, v));
+        else
+            DTTS_CUDA(launch_k(kLaunchPdl, kv_read_kernel<false>, grid, dim3(256), 0, kv->stream, g, table, pool, r, k, v));
+    }
+    return DTTS_OK;
+} catch (const std::bad_alloc &) {
+    set_error("out of host memory");
+    return DTTS_ERR_OOM;
+}
+
+int dtts_kv_attend(dtts_kv *kv, int layer, const dtts_kv_attend_args *a) {
+    DTTS_CHECK(kv && a, DTTS_ERR_ARG, "null argument");
+    const KvGeom &g = kv->g;
+    DTTS_CHECK(layer >= 0 && layer < g.L, DTTS_ERR_ARG, "layer %d of %d", layer, g.L);
+    DTTS_CHECK(!kv->b_seq.empty(), DTTS_ERR_ARG, "no current batch: call dtts_kv_extend first");
+    DTTS_CHECK(a->n_heads >= 1 && a->n_heads % g.H == 0 && a->n_heads / g.H <= 128, DTTS_ERR_ARG,
+               "%d query heads over %d key heads (a multiple, 128 to one at most)", a->n_heads, g.H);
+    DTTS_CHECK(a->window >= 0 && a->sinks >= 0, DTTS_ERR_ARG, "window %d, sinks %d", a->window, a->sinks);
+    DTTS_CHECK(a->scale > 0.f && a->scale < INFINITY, DTTS_ERR_ARG, "scale %g", (double)a->scale);
+    const int n_seq = (int)kv->b_seq.size(), G = a->n_heads / g.H;
+    for (int b = 0; b < n_seq; b++) {
+        const dtts_kv::Seq &s = kv->seqs[kv->b_seq[b]];
+        if (s.hole_lo >= s.hole_hi || kv->b_cnt[b] == 0) continue;
+        const long long lo = a->window ? std::max(0ll, (long long)kv->b_len[b] - kv->b_cnt[b] - a->window + 1) : 0;
+        DTTS_CHECK(lo >= (long long)s.hole_hi * g.P && std::min<long long>(a->sinks, lo) <= (long long)s.hole_lo * g.P,
+                   DTTS_ERR_ARG, "the window reaches rows of sequence %d that a trim freed", kv->b_seq[b]);
+    }
+    if (kv->b_rows == 0) return DTTS_OK;
+    DTTS_CHECK(a->q && a->out, DTTS_ERR_ARG, "null argument");
+    DTTS_CHECK(aligned16(a->q) && aligned16(a->out) && !((a->q_row | a->q_head | a->out_row | a->out_head) & 7),
+               DTTS_ERR_ARG, "rows must start on 16-byte boundaries");
+    DeviceGuard dg(kv->device);
+    int st = kv->flush();
+    if (st) return st;
+    KvAttendArgs p;
+    p.g = g;
+    p.m = kv->kv_meta();
+    p.pool = kv->pool + (long long)layer * g.H * g.seg;
+    p.q = (const bf16 *)a->q;
+    p.out = (bf16 *)a->out;
+    p.q_row = a->q_row; p.q_head = a->q_head; p.o_row = a->out_row; p.o_head = a->out_head;
+    p.n_seq = n_seq; p.G = G; p.total_rows = kv->b_rows;
+    p.scale_log2 = a->scale * 1.4426950408889634f;
+    p.window = a->window; p.sinks = a->sinks;
+    p.ws = kv->ws; p.cnt = kv->cnt; p.err = kv->d_err;
+    // both kernels run where a batch mixes steps and prompts; each takes its own sequences
+    for (int many = 0; many < 2; many++) {
+        const int kt = kv_key_tile(g, many);
+        long long tiles = 0, max_tiles = 0;
+        int max_rows = 0;
+        for (int b = 0; b < n_seq; b++) {
+            const long long rows = (long long)kv->b_cnt[b] * G;
+            if (rows == 0 || (rows > kKvFewRows) != (many == 1)) continue;
+            const long long i0 = kv->b_len[b] - kv->b_cnt[b];
+            const long long lo = a->window ? std::max(0ll, i0 - a->window + 1) : 0;
+            const long long nt = (kv->b_len[b] + kt - 1) / kt - lo / kt + (std::min<long long>(a->sinks, lo) + kt - 1) / kt;
+            const long long rt = many ? (rows + 127) / 128 : 1;
+            tiles += nt * rt * g.H;
+            max_tiles = std::max(max_tiles, nt);
+            max_rows = (int)std::min<long long>(INT32_MAX, std::max<long long>(max_rows, rows));
+        }
+        if (!max_rows) continue;
+        const int rt = many ? (max_rows + 127) / 128 : 1;
+        const long long units = (long long)n_seq * g.H * rt;
+        DTTS_CHECK(units <= INT32_MAX / 256, DTTS_ERR_ARG, "%lld row tiles in one batch", units);
+        // parts of a key range: enough for every SM, each a few tiles long
+        const int slot_rows = many ? 128 : kKvFewRows;
+        const long long slots = kWsFloats / ((long long)slot_rows * (g.D + 2));
+        const long long want = many ? kv->num_sms : 4ll * kv->num_sms;
+        const long long min_tiles = many ? 2 : 4;
+        const long long per = std::max(min_tiles, (tiles + want - 1) / want);
+        long long splits = (max_tiles + per - 1) / per;
+        if (units > kMaxUnits / 2) splits = 1;
+        splits = std::max(1ll, std::min(splits, slots / units));
+        p.splits = (int)splits;
+        p.tiles_per_split = (int)per;
+        DTTS_CUDA(launch_kv_attend(p, many == 1, many ? rt : max_rows, kv->stream));
+    }
+    return DTTS_OK;
+}
+
+}  // extern "C"

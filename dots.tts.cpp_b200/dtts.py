@@ -15,7 +15,7 @@ LIB_PATH = os.path.join(HERE, "libdtts.so")
 
 OK, ERR_ARG, ERR_CUDA, ERR_OOM, ERR_TIMEOUT, ERR_NONFINITE, ERR_UNSUPPORTED, ERR_IO, ERR_NO_DEVICE = \
     0, -1, -2, -3, -4, -5, -6, -7, -8
-DTYPE_BF16, DTYPE_FP8, DTYPE_F32 = 0, 1, 2
+DTYPE_BF16, DTYPE_FP8, DTYPE_F32, DTYPE_INT4 = 0, 1, 2, 3
 MEM_HOST, MEM_DEVICE = 0, 1
 CFG_V4, CFG_V3 = 0, 1
 LAYOUT_FM_MASK, LAYOUT_FULL = 0, 1
@@ -25,6 +25,7 @@ ROPE_HALF, ROPE_ADJACENT = 0, 1
 _fp = C.POINTER(C.c_float)
 _u8p = C.POINTER(C.c_uint8)
 _vp = C.c_void_p
+_ip = C.POINTER(C.c_int)
 
 
 class DitBlockW(C.Structure):
@@ -112,6 +113,9 @@ EXPORTS = [
     "dtts_dit_last_launch_count", "dtts_dit_tune", "dtts_dit_set_fused_ln", "dtts_fm_create", "dtts_fm_destroy", "dtts_fm_start",
     "dtts_fm_append_latents", "dtts_fm_append_hidden", "dtts_fm_length", "dtts_fm_read", "dtts_fm_solve", "dtts_fm_layout",
     "dtts_llm_create", "dtts_llm_destroy", "dtts_llm_set_stream", "dtts_llm_prefill", "dtts_llm_step", "dtts_llm_length",
+    "dtts_kv_create", "dtts_kv_destroy", "dtts_kv_set_stream", "dtts_kv_sync", "dtts_kv_open", "dtts_kv_close",
+    "dtts_kv_fork", "dtts_kv_truncate", "dtts_kv_trim", "dtts_kv_compact", "dtts_kv_length", "dtts_kv_free_pages",
+    "dtts_kv_extend", "dtts_kv_write", "dtts_kv_attend", "dtts_kv_read",
     "dtts_voc_create", "dtts_voc_destroy", "dtts_voc_set_stream", "dtts_voc_decode", "dtts_voc_aa_filter",
     "dtts_selftest_voc_activation", "dtts_selftest_wait_limit", "dtts_selftest_conv", "dtts_attn_create", "dtts_attn_destroy", "dtts_attn_forward",
     "dtts_attn_profile_core", "dtts_attn_forward_f32_noalloc", "dtts_pe_create", "dtts_pe_create_from_safetensors", "dtts_pe_destroy",
@@ -226,6 +230,22 @@ def lib(path: str = LIB_PATH):
     L.dtts_llm_prefill.argtypes = [_vp, _vp, C.c_int, C.c_int, _vp, C.c_int]
     L.dtts_llm_step.argtypes = [_vp, _vp, C.c_int, _vp, C.c_int]
     L.dtts_llm_length.argtypes = [_vp, C.POINTER(C.c_int)]
+    L.dtts_kv_create.argtypes = [C.POINTER(KVConfig), C.c_int, C.POINTER(_vp)]
+    for f in ("destroy", "sync"):
+        getattr(L, "dtts_kv_" + f).argtypes = [_vp]
+    L.dtts_kv_set_stream.argtypes = [_vp, _vp]
+    L.dtts_kv_open.argtypes = [_vp, _ip]
+    L.dtts_kv_close.argtypes = [_vp, C.c_int, _vp]
+    L.dtts_kv_fork.argtypes = [_vp, C.c_int, C.c_int, _vp]
+    L.dtts_kv_truncate.argtypes = [_vp, C.c_int, C.c_int]
+    L.dtts_kv_trim.argtypes = [_vp, C.c_int, C.c_int, C.c_int]
+    L.dtts_kv_compact.argtypes = [_vp, C.c_int, C.c_int, _vp]
+    L.dtts_kv_length.argtypes = [_vp, C.c_int, _ip, _ip]
+    L.dtts_kv_free_pages.argtypes = [_vp, _ip]
+    L.dtts_kv_extend.argtypes = [_vp, C.c_int, _vp, _vp]
+    L.dtts_kv_write.argtypes = [_vp, C.c_int, _vp, _vp] + [C.c_longlong] * 4
+    L.dtts_kv_attend.argtypes = [_vp, C.c_int, C.POINTER(KVAttendArgs)]
+    L.dtts_kv_read.argtypes = [_vp, C.c_int, C.c_int, C.c_int, _vp, _vp, _vp, _vp, _vp, C.c_int]
     L.dtts_voc_create.argtypes = [C.POINTER(VocW), C.c_int, C.c_int, C.POINTER(_vp)]
     L.dtts_voc_destroy.argtypes = [_vp]
     L.dtts_voc_set_stream.argtypes = [_vp, _vp]
@@ -487,6 +507,143 @@ class FMHistory:
         a.layout, a.z_out, a.mem, a.use_graph = layout, _addr(z_out), MEM_HOST, int(use_graph)
         check(lib().dtts_fm_solve(self.h, C.byref(a)))
         return z_out
+
+
+class KVConfig(C.Structure):
+    """dtts_kv_config (include/dtts.h)."""
+    _fields_ = [(n, C.c_int) for n in ("n_layers", "n_kv_heads", "head_dim", "page_tokens", "n_pages", "max_seqs",
+                                       "max_tokens", "dtype")]
+
+
+class KVAttendArgs(C.Structure):
+    """dtts_kv_attend_args (include/dtts.h)."""
+    _fields_ = [("q", _vp), ("q_row", C.c_longlong), ("q_head", C.c_longlong), ("out", _vp),
+                ("out_row", C.c_longlong), ("out_head", C.c_longlong), ("n_heads", C.c_int), ("scale", C.c_float),
+                ("window", C.c_int), ("sinks", C.c_int)]
+
+
+def _ints(a):
+    """Sequence or int32 array -> (keep-alive, address, length)."""
+    a = np.ascontiguousarray(a, np.int32).ravel()
+    return a, a.ctypes.data, a.size
+
+
+class KVCache:
+    """The paged K/V cache (dtts_kv_*).  k, v, q and out are bf16 device tensors
+    [rows][heads][head_dim] (anything with data_ptr(), stride(), element_size()
+    and is_contiguous()) whose last dimension is dense; calls only enqueue."""
+
+    def __init__(self, n_layers, n_kv_heads, head_dim, n_pages, max_seqs, max_tokens, page_tokens=64,
+                 dtype=DTYPE_BF16, device=0):
+        c = KVConfig(n_layers, n_kv_heads, head_dim, page_tokens, n_pages, max_seqs, max_tokens, dtype)
+        h = _vp()
+        check(lib().dtts_kv_create(C.byref(c), device, C.byref(h)))
+        self._init(h, n_layers, n_kv_heads, head_dim)
+
+    def _init(self, h, n_layers, n_kv_heads, head_dim):
+        self.h, self._lib = h, lib()
+        self.n_layers, self.n_kv_heads, self.head_dim = n_layers, n_kv_heads, head_dim
+        self._args = KVAttendArgs()
+
+    def close(self):
+        if getattr(self, "h", None):
+            lib().dtts_kv_destroy(self.h)
+            self.h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+    def set_stream(self, stream_ptr):
+        check(self._lib.dtts_kv_set_stream(self.h, stream_ptr))
+
+    def sync(self):
+        check(self._lib.dtts_kv_sync(self.h))
+
+    def open(self):
+        s = C.c_int()
+        check(self._lib.dtts_kv_open(self.h, C.byref(s)))
+        return s.value
+
+    def close_seqs(self, seqs):
+        a, p, n = _ints(seqs)
+        check(self._lib.dtts_kv_close(self.h, n, p))
+
+    def fork(self, seq, n=1):
+        out = np.zeros(max(n, 0), np.int32)
+        check(self._lib.dtts_kv_fork(self.h, seq, n, out.ctypes.data))
+        return out.tolist()
+
+    def truncate(self, seq, n_tokens):
+        check(self._lib.dtts_kv_truncate(self.h, seq, n_tokens))
+
+    def trim(self, seq, window, sinks=0):
+        check(self._lib.dtts_kv_trim(self.h, seq, window, sinks))
+
+    def compact(self, seq, keep):
+        a, p, n = _ints(keep)
+        check(self._lib.dtts_kv_compact(self.h, seq, n, p))
+
+    def length(self, seq):
+        n = C.c_int()
+        check(self._lib.dtts_kv_length(self.h, seq, C.byref(n), None))
+        return n.value
+
+    def position(self, seq):
+        n = C.c_int()
+        check(self._lib.dtts_kv_length(self.h, seq, None, C.byref(n)))
+        return n.value
+
+    def free_pages(self):
+        n = C.c_int()
+        check(self._lib.dtts_kv_free_pages(self.h, C.byref(n)))
+        return n.value
+
+    def extend(self, seqs, n_new):
+        a, p, n = _ints(seqs)
+        c, q, m = _ints(n_new)
+        if n != m:
+            raise ValueError(f"{n} sequences, {m} counts")
+        check(self._lib.dtts_kv_extend(self.h, n, p, q))
+
+    def _strides(self, x, heads, what):
+        shape = tuple(x.shape)
+        if len(shape) != 3 or shape[1] != heads or shape[2] != self.head_dim or x.element_size() != 2 or \
+                (shape[2] > 1 and x.stride(2) != 1):
+            raise ValueError(f"{what}: bf16 [rows][{heads}][{self.head_dim}] with a dense last dimension expected")
+        return x.stride(0), x.stride(1)
+
+    def write(self, layer, k, v):
+        kr, kh = self._strides(k, self.n_kv_heads, "k")
+        vr, vh = self._strides(v, self.n_kv_heads, "v")
+        check(self._lib.dtts_kv_write(self.h, layer, k.data_ptr(), v.data_ptr(), kr, kh, vr, vh))
+
+    def attend(self, layer, q, out, scale=None, window=0, sinks=0):
+        a = self._args
+        a.n_heads = q.shape[1]
+        a.q, a.out = q.data_ptr(), out.data_ptr()
+        a.q_row, a.q_head = self._strides(q, a.n_heads, "q")
+        a.out_row, a.out_head = self._strides(out, a.n_heads, "out")
+        a.scale = self.head_dim ** -0.5 if scale is None else scale
+        a.window, a.sinks = window, sinks
+        check(self._lib.dtts_kv_attend(self.h, layer, C.byref(a)))
+        return out
+
+    def read(self, layer, seqs, first, count, k, v, n_layers=1):
+        """k, v: dense fp32 or bf16 [n_layers][sum of counts][heads][head_dim]."""
+        s, ps, n = _ints(seqs)
+        f, pf, nf = _ints(first)
+        c, pc, nc = _ints(count)
+        size = n_layers * int(c.sum()) * self.n_kv_heads * self.head_dim
+        if not n == nf == nc:
+            raise ValueError("seqs, first and count differ in length")
+        if k.element_size() != v.element_size() or not (k.is_contiguous() and v.is_contiguous()) or \
+                k.numel() != size or v.numel() != size:
+            raise ValueError(f"k and v: dense, {size} elements of one type expected")
+        dtype = DTYPE_F32 if k.element_size() == 4 else DTYPE_BF16
+        check(self._lib.dtts_kv_read(self.h, layer, n_layers, n, ps, pf, pc, k.data_ptr(), v.data_ptr(), dtype))
 
 
 class LLMLayerW(C.Structure):

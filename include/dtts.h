@@ -61,7 +61,8 @@ extern "C" {
                                  (LayerNorm outputs: row absmax; attention and GELU outputs:
                                  a per-row bound, see dtts_fp8_quantize_rows); adaLN,
                                  input/output layers, attention core and residual as bf16 */
-#define DTTS_DTYPE_F32   2   /* fp32 everywhere (attention sublayer only)              */
+#define DTTS_DTYPE_F32   2   /* fp32 everywhere (attention sublayer; dtts_kv_read outputs) */
+#define DTTS_DTYPE_INT4  3   /* K/V cache pages only: 4-bit rows, see dtts_kv_config    */
 
 #define DTTS_MEM_HOST    0
 #define DTTS_MEM_DEVICE  1
@@ -325,6 +326,87 @@ int dtts_pe_stream_reset(dtts_pe *p, int B);
  * whole prefix (adjacent pairing). */
 int dtts_pe_decode(dtts_pe *p, const float *frames, int B, int n_frames, float *out, int mem);
 int dtts_pe_stream_length(dtts_pe *p, int *tokens);
+
+/* ------------------------------------------------------------------ paged K/V cache
+ * Keys and values of many sequences in a pool of pages, and the attention that reads them (no
+ * counterpart in the reference, whose LLM keeps one dense fp32 cache per run,
+ * src/llm_manual.cpp:237).  Sequences have their own lengths, can share pages (fork), give pages
+ * back (close, truncate, trim) and drop rows (compact).  The tables live on the host, so every
+ * request that does not fit is refused before anything changes.
+ *
+ * A step: dtts_kv_extend grows the sequences of a batch and makes it the current batch; then, for
+ * every layer, dtts_kv_write stores the new tokens' rows and dtts_kv_attend attends with their
+ * queries.  "Rows" of the batch are the new tokens of its sequences, in the order given.
+ * dtts_llm_extend runs the whole decoder this way.
+ *
+ * k, v, q and out are device pointers to bf16 on the cache's device: element [row][head][dim] at
+ * row * row_stride + head * head_stride + dim (strides in elements).  Base addresses are multiples
+ * of 16 bytes and strides multiples of 8 elements; strides may exceed the dense ones (a fused q|k|v
+ * projection) or come in any order.  Calls only enqueue work on the cache's stream (dtts_kv_sync
+ * waits and reports device errors) and must be serialised by the caller, like an engine's.
+ * dtts_kv_write, dtts_kv_attend and dtts_kv_read may be captured into a CUDA graph; a replay acts on
+ * the batch that is current on the stream then (same number of sequences and new tokens as at the
+ * capture, any lengths).  All work of a cache shares its workspace: replays of graphs captured from one
+ * cache must not overlap with each other or with its calls.  The calls that change tables
+ * (extend, fork, compact) return DTTS_ERR_UNSUPPORTED while the stream is capturing.
+ *
+ * 4-bit rows (DTTS_DTYPE_INT4): for every 32 consecutive values x of a row (a token's head) one
+ * scale s = clamp(bf16(max|x| / 7), 2^-14, 9344), held in half, and integers
+ * c = clamp(round_half_even(x / s), -7, 7); the value held is c s.  4.5 bits a value.  Magnitudes
+ * above 65408 saturate; a group with a NaN or infinity reads back as NaN. */
+typedef struct dtts_kv dtts_kv;
+typedef struct dtts_kv_config {
+    int n_layers, n_kv_heads;
+    int head_dim;                     /* 64 or 128                                          */
+    int page_tokens;                  /* tokens of a page: 16, 32, 64 or 128                */
+    int n_pages;                      /* pages of the pool (each holds every layer)         */
+    int max_seqs;                     /* sequences open at the same time                    */
+    int max_tokens;                   /* rows of the longest sequence                       */
+    int dtype;                        /* DTTS_DTYPE_BF16 or DTTS_DTYPE_INT4                 */
+} dtts_kv_config;
+int dtts_kv_create(const dtts_kv_config *c, int device, dtts_kv **out);
+int dtts_kv_destroy(dtts_kv *kv);
+/* NULL: the cache's own stream; the legacy default stream is the handle 1 (cudaStreamLegacy).  Work
+ * enqueued so far stays before what follows, unless either stream is capturing. */
+int dtts_kv_set_stream(dtts_kv *kv, void *cuda_stream);
+int dtts_kv_sync(dtts_kv *kv);
+int dtts_kv_open(dtts_kv *kv, int *seq);                       /* a new, empty sequence           */
+int dtts_kv_close(dtts_kv *kv, int n, const int *seqs);        /* frees sequences and their pages */
+/* n new sequences with the rows of src.  Pages are shared; a shared, partly filled last page is
+ * copied when a sequence that shares it grows. */
+int dtts_kv_fork(dtts_kv *kv, int src, int n, int *dst);
+int dtts_kv_truncate(dtts_kv *kv, int seq, int n_tokens);      /* drops the rows behind n_tokens  */
+/* Frees the pages that no later token sees through a window of `window` tokens with `sinks` first
+ * rows visible.  Row numbers stay; calls that would reach a freed row are refused. */
+int dtts_kv_trim(dtts_kv *kv, int seq, int window, int sinks);
+/* Keeps the n_keep listed rows (ascending) and repacks them densely; the position of the next token
+ * stays.  Needs free pages for the repacked part while it runs. */
+int dtts_kv_compact(dtts_kv *kv, int seq, int n_keep, const int *keep);
+/* rows held, and position of the next token (they differ after a compaction); either may be NULL */
+int dtts_kv_length(dtts_kv *kv, int seq, int *tokens, int *position);
+int dtts_kv_free_pages(dtts_kv *kv, int *n);
+/* Adds n_new[b] >= 0 tokens to each of the n_seq sequences and makes them the current batch.  Closing,
+ * truncating, trimming or compacting one of its sequences ends the batch. */
+int dtts_kv_extend(dtts_kv *kv, int n_seq, const int *seqs, const int *n_new);
+int dtts_kv_write(dtts_kv *kv, int layer, const void *k, const void *v, long long k_row, long long k_head,
+                  long long v_row, long long v_head);
+typedef struct dtts_kv_attend_args {
+    const void *q;                    /* [rows][n_heads][head_dim]                          */
+    long long q_row, q_head;          /* strides in elements                                */
+    void *out;                        /* like q                                             */
+    long long out_row, out_head;
+    int n_heads;                      /* a multiple of n_kv_heads; query head h reads key head
+                                         h / (n_heads / n_kv_heads)                         */
+    float scale;                      /* of the scores, > 0                                 */
+    int window;                       /* row i sees rows j <= i with j > i - window ...     */
+    int sinks;                        /* ... or j < sinks; window 0: every row j <= i       */
+} dtts_kv_attend_args;
+int dtts_kv_attend(dtts_kv *kv, int layer, const dtts_kv_attend_args *a);
+/* Rows first[i] .. first[i] + count[i] - 1 of sequence seqs[i], i < n, one after another, for
+ * n_layers layers: k, v [n_layers][sum of counts][n_kv_heads][head_dim], dense, DTTS_DTYPE_F32 (exact)
+ * or DTTS_DTYPE_BF16 (rounded to nearest even). */
+int dtts_kv_read(dtts_kv *kv, int layer, int n_layers, int n, const int *seqs, const int *first, const int *count,
+                 void *k, void *v, int dtype);
 
 /* ------------------------------------------------------------------ LLM decoder step
  * The autoregressive loop's Qwen2.5-1.5B step (src/llm_manual.cpp): a batch of B sequences

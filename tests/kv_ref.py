@@ -1,0 +1,76 @@
+"""The paged K/V cache's definitions in 64 bits (numpy / torch double, CPU).
+
+Tolerance of attention against them, per output element, from the kernels' roundings (a rounding is off by at
+most half a step: bf16 2^-8, half 2^-11, fp32 2^-24, relative):
+  * the bf16 output: 2^-8 |out|;
+  * P in half (int4 rows): 2^-11 sum_j p_j |v_j|, and 2^-25 sum_j |v_j| for subnormal P (p <= 1 before the
+    division by l >= 1); in two bf16 terms (bf16 rows): 2^-16 sum_j p_j |v_j|, below the former;
+  * a score s = scale sum_d q_d k_d in fp32: at most D / 16 additions of 16-term products, each step off by at
+    most 2^-22 of B = scale sum_d |q_d k_d|: 2^-19 B for D <= 128, on p through exp twice (numerator and l);
+    exp2 itself 2^-22, corrections of the running maximum and l: n / 16 steps of 2^-23 each, P V the same."""
+import math
+
+import numpy as np
+import torch
+
+
+def bf16_round(x):
+    return torch.as_tensor(x, dtype=torch.float32).to(torch.bfloat16)
+
+
+def codes(x):
+    """int4 rows of x (bf16 [..., D]): (integers, scales), in 64 bits."""
+    y = x.double()
+    y = y.reshape(*y.shape[:-1], -1, 32)
+    top = y.abs().amax(-1, keepdim=True)
+    s = (top / 7).to(torch.bfloat16).double().clamp(2.0 ** -14, 9344.0)
+    c = torch.round(y / s).clamp(-7, 7)
+    bad = ~torch.isfinite(y).all(-1, keepdim=True)
+    c = torch.where(bad, torch.zeros_like(c), c)
+    s = torch.where(bad, torch.full_like(s, math.nan), s)
+    return c, s
+
+
+def held(x, int4):
+    """The values the cache holds for rows x (bf16), as double."""
+    if not int4:
+        return x.double()
+    c, s = codes(x)
+    return (c * s).reshape(x.shape)
+
+
+def visible(n, i, window, sinks):
+    j = torch.arange(n)
+    ok = j <= i
+    if window:
+        ok &= (j > i - window) | (j < sinks)
+    return ok
+
+
+def attend(q, k, v, i0, window=0, sinks=0, scale=None):
+    """q [t][Hq][D], held k, v [n][H][D] (double): rows i0 .. i0 + t - 1.  Returns (out, tolerance)."""
+    t, hq, D = q.shape
+    n, H = k.shape[:2]
+    G = hq // H
+    scale = D ** -0.5 if scale is None else scale
+    q = q.double()
+    out, tol = torch.zeros_like(q), torch.zeros_like(q)
+    for x in range(t):
+        j = visible(n, i0 + x, window, sinks).nonzero()[:, 0]
+        for h in range(hq):
+            kk, vv = k[j, h // G], v[j, h // G]
+            s = kk @ q[x, h] * scale
+            p = torch.softmax(s, 0)
+            o = p @ vv
+            a = p @ vv.abs()
+            B = float((kk.abs() @ q[x, h].abs()).max() * scale)
+            out[x, h] = o
+            tol[x, h] = 2.0 ** -8 * o.abs() + a * (2.0 ** -11 + 2.0 ** -19 * B + (len(j) / 16 + 64) * 2.0 ** -22) + \
+                2.0 ** -25 * vv.abs().sum(0)
+    return out, tol
+
+
+def assert_close(got, want, tol, what=""):
+    err = (got.double().cpu() - want).abs()
+    bad = ~(err <= tol)
+    assert not bad.any(), f"{what}: {int(bad.sum())} of {bad.numel()} off, worst {float((err / tol).max()):.2f} of the tolerance"
