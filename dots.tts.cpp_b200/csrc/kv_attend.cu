@@ -5,6 +5,7 @@
 #include "kv.cuh"
 
 #include <cmath>
+#include <type_traits>
 
 namespace dtts {
 namespace {
@@ -275,8 +276,8 @@ __global__ void __launch_bounds__(128) kv_attend_few_kernel(const __grid_constan
             top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
             top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
             const int ex = (int)(top >> 7);   // biased exponent; 0: zeros and subnormals, 255: inf or NaN
-            const int sh = ex == 255 ? 0 : min(14 + 127 - ex, 127);
-            const float up = __uint_as_float((uint32_t)(max(sh, -126) + 127) << 23);
+            const int sh = ex == 255 ? 0 : min(14 + 127 - ex, 100);
+            const float up = __uint_as_float((uint32_t)(sh + 127) << 23);
 #pragma unroll
             for (int j = 0; j < NG; j++) {
                 const uint32_t e[4] = {w[j].x, w[j].y, w[j].z, w[j].w};
@@ -292,9 +293,7 @@ __global__ void __launch_bounds__(128) kv_attend_few_kernel(const __grid_constan
                 qf[nt][2 * j + 1][1] = h2_bits(__floats2half2_rn(x[3], x[7]));
             }
             // column g's factor is 2^-sh scale; lanes need those of columns 2 t, 2 t + 1
-            const float down = __uint_as_float((uint32_t)(127 - min(max(sh, -126), 126)) << 23) *
-                               (sh == 127 ? 0.5f : 1.0f);
-            f *= down;
+            f *= __uint_as_float((uint32_t)(127 - sh) << 23);
         } else {
 #pragma unroll
             for (int j = 0; j < NG; j++) {
@@ -610,26 +609,472 @@ __global__ void __launch_bounds__(128) kv_attend_few_kernel(const __grid_constan
 }
 
 // ---------------------------------------------------------------- many rows
-// One warp a row, plain arithmetic.
-template <int D>
-__global__ void __launch_bounds__(128) kv_attend_rows_kernel(const __grid_constant__ KvAttendArgs a, int row_tiles) {
-    pdl_wait();
-    pdl_trigger();
-    const int tile = blockIdx.x % row_tiles, unit = blockIdx.x / row_tiles;
-    const int b = unit / a.g.H, head = unit % a.g.H;
-    const int cnt = a.m.cnt[b], len = a.m.len[b], row0 = a.m.start[b], G = a.G;
-    const long long rows = (long long)cnt * G;
-    if (rows <= kKvFewRows || (long long)row0 + cnt > a.total_rows) return;
-    const int *trow = a.m.table + (long long)a.m.seq[b] * a.g.max_pages;
-    const KeyTiles kt(64, len - cnt, len, a.window, a.sinks);
-    for (long long r = tile * 128ll + (threadIdx.x >> 5); r < min(rows, tile * 128ll + 128); r += 4) {
-        const int tok = (int)(r / G), hg = (int)(r % G), lane = threadIdx.x & 31;
-        float m, l, o[D / 32];
-        kv_row_plain<D>(a, trow, head, a.q + (row0 + tok) * a.q_row + (head * G + hg) * a.q_head, len - cnt + tok, 64, kt, 0,
-                        kt.n, m, l, o);
-        for (int c = 0; c < D / 32; c++)
-            a.out[(row0 + tok) * a.o_row + (head * G + hg) * a.o_head + lane + 32 * c] = __float2bfloat16_rn(o[c] / l);
+// tcgen05 pieces that only this kernel uses: A operand from TMEM, 32-column
+// stores, and the MN-major descriptor of a [keys][dims] tile of 64-dim chunks
+// (rows of 128 bytes, 128-byte swizzle): 8-key groups 1024 bytes apart, chunks
+// kChunk bytes apart.
+constexpr int kChunk = 128 * 128;   // 128 rows x 64 elements of 2 bytes
+DTTS_DEV void tc_mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d_tmem),
+        "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+DTTS_DEV void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], "
+        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};\n"
+        ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+          "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]),
+          "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]),
+          "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(taddr)
+        : "memory");
+}
+DTTS_DEV void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+DTTS_DEV uint64_t sdesc_mn128(uint32_t saddr) {
+    return (sdesc_k128(saddr) & ~(0x3fffull << 16)) | ((uint64_t)(kChunk >> 4) << 16);
+}
+// byte offset of 16-byte unit u (8 elements) of row r in a tile of 64-element chunks
+DTTS_DEV int tile_unit(int r, int u) { return (u >> 3) * kChunk + r * 128 + (((u & 7) ^ (r & 7)) << 4); }
+
+template <int D, bool I4>
+struct ManyCfg {
+    static constexpr int KT = 128, kTile = D / 64 * kChunk;   // one operand tile of 128 rows
+    static constexpr int kSoftmax = 256, kProducers = 96, kThreads = kSoftmax + kProducers + 32;
+    static constexpr int kSmem = 6 * kTile + 256 + 1024;      // Q x 2, K x 2, V x 2, barriers
+    static constexpr int RB = I4 ? D / 2 : 2 * D, SB = I4 ? D / 16 : 0;
+    static constexpr uint32_t kF16 = I4 ? 0u : (1u << 7) | (1u << 10);   // operand type: half or bf16
+    __host__ __device__ static constexpr uint32_t idesc(int n) {
+        return (1u << 4) | kF16 | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
     }
+};
+
+// pairs (0, 4), (1, 5), (2, 6), (3, 7) of a word's values, as one 16-byte unit
+DTTS_DEV uint4 dequant_unit(uint32_t w, __half2 s) {
+    __half2 h[4];
+    unpack_nibbles(w, h);
+    return make_uint4(h2_bits(__hmul2(h[0], s)), h2_bits(__hmul2(h[1], s)), h2_bits(__hmul2(h[2], s)),
+                      h2_bits(__hmul2(h[3], s)));
+}
+// where dim i of 8 stands inside such a unit
+__host__ __device__ constexpr int unit_dim(bool i4, int pos) { return i4 ? (pos >> 1) + (pos & 1) * 4 : pos; }
+
+// Attention of up to 256 rows (new token x query head of one kv head, two tiles of
+// 128) of one sequence over a part of its keys, in blocks of 128 keys.
+//   warps 0-3, 4-7: softmax of tile 0, 1, one row a thread (S from TMEM, P back into
+//                   the same columns, O rescaled when the row maximum has grown by
+//                   more than 2^8, so P <= 2^8 stays in half's range);
+//   warps 8-10:     K and V blocks from the pages into swizzled tiles (4-bit rows
+//                   become exact halves on the way), two stages;
+//   warp 11:        S = Q K^T and O += P V on tcgen05 (P from TMEM, V MN-major).
+// The two tiles alternate: while one's softmax runs, the other's products do.
+// Bound by the softmax's exponentials (128 x 128 a block and tile at 16 a clock and
+// SM, as long as its two products take) and by shared memory reads of the operands.
+// 4-bit rows: all operands half, Q after an exact power-of-two scaling of the row, P
+// rounded by 2^-11.  bf16 rows: P is rounded to bf16 (2^-8 of the P-weighted mean
+// of |v|, the size of the output's own rounding): a second term would cost half as
+// much tensor time again.
+template <int D, bool I4>
+__global__ void __launch_bounds__(384, 1) kv_attend_many_kernel(const __grid_constant__ KvAttendArgs a, int pairs) {
+    using C = ManyCfg<D, I4>;
+    constexpr int KT = C::KT, NU = D / 8;   // 16-byte units a row
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t *sm = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint8_t *sQ = sm, *sK = sm + 2 * C::kTile, *sV = sm + 4 * C::kTile;
+    uint64_t *bars = reinterpret_cast<uint64_t *>(sm + 6 * C::kTile);
+    uint64_t *q_full = bars, *s_full = bars + 2, *p_full = bars + 4, *o_full = bars + 6;
+    uint64_t *k_full = bars + 8, *k_empty = bars + 10, *v_full = bars + 12, *v_empty = bars + 14, *drain = bars + 16;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 17);
+    int *flag = reinterpret_cast<int *>(tmem_slot + 1);
+    volatile int *abort_flag = flag + 1;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    pdl_wait();
+
+    const int split = blockIdx.x % a.splits, u = blockIdx.x / a.splits;
+    const int bh = u % (a.n_seq * a.g.H), pair = pairs - 1 - u / (a.n_seq * a.g.H);   // longest key ranges first
+    const int b = bh / a.g.H, head = bh % a.g.H, unit = bh * pairs + pair;
+    const int cnt = a.m.cnt[b], len = a.m.len[b], row0 = a.m.start[b], G = a.G;
+    const long long all = (long long)cnt * G;
+    if (all <= kKvFewRows || (long long)pair * 256 >= all || (long long)row0 + cnt > a.total_rows) return;
+    const int base = pair * 256, rows = (int)min(256ll, all - base), tiles = rows > 128 ? 2 : 1;
+    const int *trow = a.m.table + (long long)a.m.seq[b] * a.g.max_pages;
+    const int i0 = len - cnt, i_first = i0 + base / G, i_last = i0 + (base + rows - 1) / G;
+    const KeyTiles kt(KT, i_first, i_last + 1, a.window, a.sinks);
+    const int parts = min(a.splits, max(1, (kt.n + a.tiles_per_split - 1) / a.tiles_per_split));
+    if (split >= parts) return;
+    const int c0 = (int)((long long)kt.n * split / parts), c1 = (int)((long long)kt.n * (split + 1) / parts), n = c1 - c0;
+
+    if (tid == 0) {
+        for (int w = 0; w < 2; w++) {
+            mbar_init(q_full + w, 128);
+            mbar_init(s_full + w, 1);
+            mbar_init(p_full + w, 128);
+            mbar_init(o_full + w, 1);
+            mbar_init(k_full + w, C::kProducers);
+            mbar_init(k_empty + w, 1);
+            mbar_init(v_full + w, C::kProducers);
+            mbar_init(v_empty + w, 1);
+        }
+        mbar_init(drain, 1);
+        *flag = 0;
+        *abort_flag = 0;
+        fence_mbar_init();
+    }
+    if (warp == 11) {
+        tmem_alloc(tmem_slot, 512);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tbase = *tmem_slot;   // S0 | S1 | O0 | O1
+    // only now: the next kernel's CTAs may take TMEM before they wait for this grid
+    pdl_trigger();
+
+    if (warp == 11) {
+        if (lane == 0) {
+            bool ok = true;
+            auto scores = [&](int w, int k) {   // S_w = Q_w K^T of block k
+                const uint32_t qa = smem_u32(sQ + w * C::kTile), ka = smem_u32(sK + (k & 1) * C::kTile);
+#pragma unroll
+                for (int x = 0; x < D / 16; x++) {
+                    const uint32_t off = (x >> 2) * kChunk + (x & 3) * 32;
+                    tc_mma_bf16(tbase + w * 128, sdesc_k128(qa + off), sdesc_k128(ka + off), C::idesc(128), x ? 1u : 0u);
+                }
+                tc_commit(s_full + w);
+            };
+            ok = ok && mbar_wait(k_full, 0, abort_flag, a.err, DEVERR_TIMEOUT_MMA);
+            for (int w = 0; w < tiles && ok; w++) {
+                ok = mbar_wait(q_full + w, 0, abort_flag, a.err, DEVERR_TIMEOUT_MMA);
+                if (!ok) break;
+                tc_fence_after();
+                scores(w, 0);
+            }
+            if (ok) tc_commit(k_empty);
+            for (int k = 0; k < n && ok; k++) {
+                ok = mbar_wait(v_full + (k & 1), (k >> 1) & 1, abort_flag, a.err, DEVERR_TIMEOUT_MMA);
+                for (int w = 0; w < tiles && ok; w++) {
+                    ok = mbar_wait(p_full + w, k & 1, abort_flag, a.err, DEVERR_TIMEOUT_MMA);
+                    if (!ok) break;
+                    tc_fence_after();
+                    const uint32_t va = smem_u32(sV + (k & 1) * C::kTile);
+#pragma unroll
+                    for (int x = 0; x < KT / 16; x++)
+                        tc_mma_ts(tbase + 256 + w * 128, tbase + w * 128 + 8 * x, sdesc_mn128(va + x * 2048),
+                                  C::idesc(D) | (1u << 16), k || x ? 1u : 0u);
+                    tc_commit(o_full + w);
+                    if (k + 1 == n) continue;
+                    // S_w takes the columns P_w is read from: only after that product is done
+                    ok = mbar_wait(k_full + ((k + 1) & 1), ((k + 1) >> 1) & 1, abort_flag, a.err, DEVERR_TIMEOUT_MMA) &&
+                         mbar_wait(o_full + w, k & 1, abort_flag, a.err, DEVERR_TIMEOUT_MMA);
+                    if (!ok) break;
+                    tc_fence_after();
+                    scores(w, k + 1);
+                }
+                if (!ok) break;
+                tc_commit(v_empty + (k & 1));
+                if (k + 1 < n) tc_commit(k_empty + ((k + 1) & 1));
+            }
+            // every product done before TMEM is given back (also after an abort)
+            tc_commit(drain);
+            const unsigned long long t0 = globaltimer_ns();
+            while (!mbar_try_wait(drain, 0) && globaltimer_ns() - t0 < kWaitLimitNs) {}
+        }
+        __syncwarp();
+    } else if (warp >= 8) {
+        // ---- pages -> tiles
+        const int pt = tid - C::kSoftmax, P = a.g.P, lg = a.g.lgP;
+        auto seg_of = [&](int j) -> const uint8_t * {
+            if (j >= len) return nullptr;
+            const int page = trow[j >> lg];
+            return page >= 0 && page < a.g.n_pages ? a.pool + kv_seg_off(a.g, page, 0, head) : nullptr;
+        };
+        if constexpr (I4) {
+            // K: the words of unit t are dims 32 j + 8 t of all groups j; V: unit t is group t.
+            // A block's raw rows are loaded while the one before is unpacked.
+            constexpr int kN = (KT * 4 + C::kProducers - 1) / C::kProducers;
+            struct Raw {
+                uint4 w[kN];
+                uint2 sc[kN];
+            } rk, rv;
+            auto load = [&](auto is_v, int k, Raw &raw) {
+                constexpr bool V = decltype(is_v)::value;
+                constexpr int per = V ? D / 32 : 4;   // items a row
+                const int j0 = kt.tile(c0 + k) * KT;
+#pragma unroll
+                for (int x = 0; x < kN; x++) {
+                    const int it = pt + x * C::kProducers, r = it / per, t = it % per;
+                    raw.w[x] = make_uint4(0u, 0u, 0u, 0u);
+                    raw.sc[x] = make_uint2(0u, 0u);
+                    if (r >= KT) continue;
+                    const uint8_t *seg = seg_of(j0 + r);
+                    if (!seg) continue;
+                    const int pr = (j0 + r) & (P - 1);
+                    const uint8_t *row = seg + (V ? P * C::RB : 0) + pr * C::RB;
+                    const uint8_t *srow = seg + 2 * P * C::RB + (V ? P * C::SB : 0) + pr * C::SB;
+                    if (V || D == 128) {
+                        raw.w[x] = *reinterpret_cast<const uint4 *>(row + (V ? t ^ kv_swz_v(true, D, pr) : t) * 16);
+                    } else {
+                        const uint2 y = *reinterpret_cast<const uint2 *>(row + t * 8);
+                        raw.w[x].x = y.x;
+                        raw.w[x].y = y.y;
+                    }
+                    if (V) raw.sc[x].x = *reinterpret_cast<const uint16_t *>(srow + t * 2) * 0x10001u;
+                    else if (D == 128) raw.sc[x] = *reinterpret_cast<const uint2 *>(srow);
+                    else raw.sc[x].x = *reinterpret_cast<const uint32_t *>(srow);
+                }
+            };
+            auto store = [&](auto is_v, int k, const Raw &raw) {
+                constexpr bool V = decltype(is_v)::value;
+                constexpr int per = V ? D / 32 : 4;
+                uint8_t *dst = (V ? sV : sK) + (k & 1) * C::kTile;
+                if (k >= 2 && !mbar_wait((V ? v_empty : k_empty) + (k & 1), ((k >> 1) - 1) & 1, abort_flag, a.err,
+                                         DEVERR_TIMEOUT_PRODUCER))
+                    return false;
+#pragma unroll
+                for (int x = 0; x < kN; x++) {
+                    const int it = pt + x * C::kProducers, r = it / per, t = it % per;
+                    if (r >= KT) continue;
+                    const uint32_t e[4] = {raw.w[x].x, raw.w[x].y, raw.w[x].z, raw.w[x].w};
+#pragma unroll
+                    for (int q = 0; q < (V ? 4 : D / 32); q++) {
+                        if (V) {
+                            *reinterpret_cast<uint4 *>(dst + tile_unit(r, 4 * t + q)) = dequant_unit(e[q], bits_h2(raw.sc[x].x));
+                        } else {
+                            // odd rows take their words in pair-swapped order, so that the two rows of a
+                            // quarter warp fill all eight units of the swizzle
+                            const int j = q ^ (r & 1);
+                            const uint32_t s2 = (q >> 1) ? raw.sc[x].y : raw.sc[x].x;
+                            const uint32_t sj = (r & 1) ^ (q & 1) ? s2 >> 16 : s2 & 0xffffu;
+                            *reinterpret_cast<uint4 *>(dst + tile_unit(r, 4 * j + t)) =
+                                dequant_unit(r & 1 ? e[q ^ 1] : e[q], bits_h2(sj * 0x10001u));
+                        }
+                    }
+                }
+                fence_proxy_async_smem();
+                mbar_arrive((V ? v_full : k_full) + (k & 1));
+                return true;
+            };
+            using K_ = std::integral_constant<bool, false>;
+            using V_ = std::integral_constant<bool, true>;
+            load(K_{}, 0, rk);
+            for (int k = 0; k < n; k++) {
+                load(V_{}, k, rv);
+                if (!store(K_{}, k, rk)) break;
+                if (k + 1 < n) load(K_{}, k + 1, rk);
+                if (!store(V_{}, k, rv)) break;
+            }
+        } else {
+            // blocks K0 V0 K1 V1 ...: a block is announced when the second one behind it has been requested
+            auto full_of = [&](int i) { return (i & 1 ? v_full : k_full) + ((i >> 1) & 1); };
+            int issued = 0;
+            for (; issued < 2 * n; issued++) {
+                const int k = issued >> 1, is_v = issued & 1, j0 = kt.tile(c0 + k) * KT;
+                uint8_t *dst = (is_v ? sV : sK) + (k & 1) * C::kTile;
+                if (k >= 2 && !mbar_wait((is_v ? v_empty : k_empty) + (k & 1), ((k >> 1) - 1) & 1, abort_flag, a.err,
+                                         DEVERR_TIMEOUT_PRODUCER))
+                    break;
+                for (int it = pt; it < KT * NU; it += C::kProducers) {
+                    const int r = it / NU, un = it % NU, pr = (j0 + r) & (P - 1);
+                    const uint8_t *seg = seg_of(j0 + r);
+                    const uint32_t d = smem_u32(dst + tile_unit(r, un));
+                    const int su = un ^ (is_v ? kv_swz_v(false, D, pr) : kv_swz_k(false, pr));
+                    const uint8_t *src = seg ? seg + (is_v ? P * C::RB : 0) + pr * C::RB + su * 16 : a.pool;
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(d), "l"(src), "r"(seg ? 16 : 0) : "memory");
+                }
+                asm volatile("cp.async.commit_group;" ::: "memory");
+                if (issued >= 2) {
+                    asm volatile("cp.async.wait_group 2;" ::: "memory");
+                    fence_proxy_async_smem();
+                    mbar_arrive(full_of(issued - 2));
+                }
+            }
+            asm volatile("cp.async.wait_all;" ::: "memory");
+            fence_proxy_async_smem();
+            for (int i = max(0, issued - 2); i < issued; i++) mbar_arrive(full_of(i));
+        }
+    } else {
+        // ---- softmax, a row a thread
+        const int w = warp >> 2, r = tid & 127, rr = w * 128 + r;
+        if (w < tiles) {
+            const bool live = rr < rows;
+            const int tok = (base + (live ? rr : 0)) / G, hg = (base + (live ? rr : 0)) % G, qi = live ? i0 + tok : -1;
+            const bf16 *qp = a.q + (long long)(row0 + tok) * a.q_row + (long long)(head * G + hg) * a.q_head;
+            float c = a.scale_log2;
+            {
+                uint4 x[NU];
+                uint32_t top = 0;
+#pragma unroll
+                for (int i = 0; i < NU; i++) {
+                    x[i] = live ? reinterpret_cast<const uint4 *>(qp)[i] : make_uint4(0u, 0u, 0u, 0u);
+                    const uint32_t e[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+#pragma unroll
+                    for (int y = 0; y < 4; y++) top = max(top, max(e[y] & 0x7fffu, (e[y] >> 16) & 0x7fffu));
+                }
+                float up = 1.f;
+                if constexpr (I4) {
+                    // as in the few-row kernel: the largest |q| of the row to [2^14, 2^15)
+                    const int ex = (int)(top >> 7), sh = ex == 255 ? 0 : min(14 + 127 - ex, 100);
+                    up = __uint_as_float((uint32_t)(sh + 127) << 23);
+                    c = fmaxf(c * __uint_as_float((uint32_t)(127 - sh) << 23), 1.17549435e-38f);   // -inf * c stays -inf
+                }
+#pragma unroll
+                for (int i = 0; i < NU; i++) {
+                    if constexpr (I4) {
+                        const uint32_t e[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+                        float f[8];
+#pragma unroll
+                        for (int y = 0; y < 4; y++) {
+                            f[2 * y] = __uint_as_float(e[y] << 16) * up;
+                            f[2 * y + 1] = __uint_as_float(e[y] & 0xffff0000u) * up;
+                        }
+                        x[i] = make_uint4(h2_bits(__floats2half2_rn(f[0], f[4])), h2_bits(__floats2half2_rn(f[1], f[5])),
+                                          h2_bits(__floats2half2_rn(f[2], f[6])), h2_bits(__floats2half2_rn(f[3], f[7])));
+                    }
+                    *reinterpret_cast<uint4 *>(sQ + w * C::kTile + tile_unit(r, i)) = x[i];
+                }
+            }
+            fence_proxy_async_smem();
+            mbar_arrive(q_full + w);
+            const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+            const uint32_t ts = tbase + w * 128 + lanes, to = tbase + 256 + w * 128 + lanes;
+            const int q_min = i0 + (base + w * 128) / G, q_max = i0 + (base + min(rows, w * 128 + 128) - 1) / G;
+            float m = -INFINITY, l = 0.f;
+            bool ok = true;
+            for (int k = 0; k < n; k++) {
+                const int j0 = kt.tile(c0 + k) * KT;
+                ok = mbar_wait(s_full + w, k & 1, abort_flag, a.err, DEVERR_TIMEOUT_EPILOGUE);
+                if (__any_sync(0xffffffffu, !ok)) { ok = false; break; }
+                tc_fence_after();
+                float s[4][32];
+                tmem_ld32x2(ts, ts + 32, s[0], s[1]);
+                tmem_ld32x2(ts + 64, ts + 96, s[2], s[3]);
+                if (!(j0 + KT - 1 <= q_min && (a.window == 0 || j0 > q_max - a.window || j0 + KT - 1 < a.sinks))) {
+#pragma unroll
+                    for (int x = 0; x < 4; x++)
+#pragma unroll
+                        for (int y = 0; y < 32; y++)
+                            if (!kv_visible(j0 + 32 * x + y, qi, a.window, a.sinks)) s[x][y] = -INFINITY;
+                }
+                float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                for (int y = 0; y < 32; y++)
+#pragma unroll
+                    for (int x = 0; x < 4; x++) mx[x] = fmaxf(mx[x], s[x][y]);
+                const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * c;
+                if (__any_sync(0xffffffffu, top > m + 8.f || (m == -INFINITY && top > m))) {
+                    const float mn = fmaxf(m, top), corr = mn == -INFINITY ? 1.f : exp2f(m - mn);
+                    if (k > 0) {
+#pragma unroll 1
+                        for (int x = 0; x < D; x += 32) {
+                            float o[32];
+                            uint32_t p[32];
+                            tmem_ld32(to + x, o);
+#pragma unroll
+                            for (int y = 0; y < 32; y++) p[y] = __float_as_uint(o[y] * corr);
+                            tmem_st32(to + x, p);
+                        }
+                        tmem_wait_st();
+                    }
+                    l *= corr;
+                    m = mn;
+                }
+                const float mu = m == -INFINITY ? 0.f : m;
+                float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int x = 0; x < 2; x++) {
+                    uint32_t p[32];
+#pragma unroll
+                    for (int y = 0; y < 32; y++) {
+                        const float p0 = ex2_hw(fmaf(s[2 * x + (y >> 4)][(2 * y) & 31], c, -mu));
+                        const float p1 = ex2_hw(fmaf(s[2 * x + (y >> 4)][(2 * y + 1) & 31], c, -mu));
+                        sum[y & 3] += p0 + p1;
+                        p[y] = I4 ? h2_bits(__floats2half2_rn(p0, p1)) : pack_bf16x2(p0, p1);
+                    }
+                    tmem_st32(ts + 32 * x, p);
+                }
+                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                tmem_wait_st();
+                tc_fence_before();
+                mbar_arrive(p_full + w);
+            }
+            if (ok) ok = mbar_wait(o_full + w, (n - 1) & 1, abort_flag, a.err, DEVERR_TIMEOUT_EPILOGUE);
+            if (!__any_sync(0xffffffffu, !ok)) {
+                tc_fence_after();
+                bf16 *op = a.out + (long long)(row0 + tok) * a.o_row + (long long)(head * G + hg) * a.o_head;
+                float *wp = a.ws + (((long long)unit * a.splits + split) * 256 + rr) * (D + 2);
+                const float inv = 1.0f / l;   // l = 0: every score was -inf, and 0 * inf is the formula's NaN
+                bool bad = false;
+#pragma unroll 1
+                for (int x = 0; x < D; x += 32) {
+                    float o[32];
+                    tmem_ld32(to + x, o);
+#pragma unroll
+                    for (int y = 0; y < 4; y++) {
+                        float v[8];
+#pragma unroll
+                        for (int i = 0; i < 8; i++) {
+                            v[unit_dim(I4, i)] = o[8 * y + i];
+                            bad |= o[8 * y + i] != o[8 * y + i];
+                        }
+                        if (!live) continue;
+                        if (parts == 1)
+                            *reinterpret_cast<uint4 *>(op + x + 8 * y) =
+                                make_uint4(pack_bf16x2(v[0] * inv, v[1] * inv), pack_bf16x2(v[2] * inv, v[3] * inv),
+                                           pack_bf16x2(v[4] * inv, v[5] * inv), pack_bf16x2(v[6] * inv, v[7] * inv));
+                        else
+#pragma unroll
+                            for (int i = 0; i < 4; i++)
+                                reinterpret_cast<float2 *>(wp + x + 8 * y)[i] = make_float2(v[2 * i], v[2 * i + 1]);
+                    }
+                }
+                if (live && parts > 1) {
+                    wp[D] = m;
+                    wp[D + 1] = l;
+                }
+                // a NaN: recompute the row so that key rows it cannot see do not reach it
+                for (unsigned todo = __ballot_sync(0xffffffffu, bad && live); todo; todo &= todo - 1) {
+                    const int x = __ffs(todo) - 1, xr = base + w * 128 + (warp & 3) * 32 + x, xt = xr / G, xh = xr % G;
+                    float mm, ll, oo[D / 32];
+                    kv_row_plain<D>(a, trow, head, a.q + (long long)(row0 + xt) * a.q_row + (long long)(head * G + xh) * a.q_head,
+                                    i0 + xt, KT, kt, c0, c1, mm, ll, oo);
+                    float *xw = a.ws + (((long long)unit * a.splits + split) * 256 + xr - base) * (D + 2);
+                    bf16 *xo = a.out + (long long)(row0 + xt) * a.o_row + (long long)(head * G + xh) * a.o_head;
+                    for (int i = 0; i < D / 32; i++) {
+                        if (parts == 1) xo[lane + 32 * i] = __float2bfloat16_rn(oo[i] / ll);
+                        else xw[lane + 32 * i] = oo[i];
+                    }
+                    if (parts > 1 && lane == 0) { xw[D] = mm; xw[D + 1] = ll; }
+                    __syncwarp();
+                }
+            }
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 11) {
+        tc_fence_after();
+        tmem_dealloc(tbase, 512);
+    }
+    if (parts > 1 && kv_last_part(a.cnt + unit, parts, flag))
+        kv_join_parts<D>(a.ws + (long long)unit * a.splits * 256 * (D + 2), 256ll * (D + 2), parts, rows, [&](int r) {
+            const int x = base + r;
+            return a.out + (long long)(row0 + x / G) * a.o_row + (long long)(head * G + x % G) * a.o_head;
+        });
+}
+
+template <int D, bool I4>
+cudaError_t prepare_many() {
+    return cudaFuncSetAttribute(kv_attend_many_kernel<D, I4>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                ManyCfg<D, I4>::kSmem);
+}
+template <int D, bool I4>
+cudaError_t launch_many(const KvAttendArgs &a, int pairs, cudaStream_t s) {
+    return launch_k(kLaunchPdl, kv_attend_many_kernel<D, I4>, dim3((unsigned)a.n_seq * a.g.H * pairs * a.splits),
+                    dim3(ManyCfg<D, I4>::kThreads), ManyCfg<D, I4>::kSmem, s, a, pairs);
 }
 
 template <int D, bool I4, int NT>
@@ -649,7 +1094,7 @@ cudaError_t launch_few(const KvAttendArgs &a, int rows, cudaStream_t s) {
 
 // rows of a key tile of the few-row or the many-row kernel
 int kv_key_tile(const KvGeom &g, bool many) {
-    if (many) return 64;
+    if (many) return 128;
     if (g.i4) return g.D == 128 ? FewCfg<128, true>::KT : FewCfg<64, true>::KT;
     return g.D == 128 ? FewCfg<128, false>::KT : FewCfg<64, false>::KT;
 }
@@ -658,21 +1103,21 @@ cudaError_t kv_attend_prepare() {
     cudaError_t e = cudaSuccess;
     if ((e = prepare_few<128, true, 1>()) || (e = prepare_few<128, true, 2>()) || (e = prepare_few<128, false, 1>()) ||
         (e = prepare_few<128, false, 2>()) || (e = prepare_few<64, true, 1>()) || (e = prepare_few<64, true, 2>()) ||
-        (e = prepare_few<64, false, 1>()) || (e = prepare_few<64, false, 2>()))
+        (e = prepare_few<64, false, 1>()) || (e = prepare_few<64, false, 2>()) || (e = prepare_many<128, true>()) ||
+        (e = prepare_many<128, false>()) || (e = prepare_many<64, true>()) || (e = prepare_many<64, false>()))
         return e;
     return cudaSuccess;
 }
 
-// many: sequences of more than kKvFewRows rows, in rows_or_tiles row tiles of 128
-// at most; otherwise sequences of up to that many, rows_or_tiles at most
-cudaError_t launch_kv_attend(const KvAttendArgs &a, bool many, int rows_or_tiles, cudaStream_t s) {
+// many: sequences of more than kKvFewRows rows, in rows_or_pairs pairs of row tiles
+// (256 rows) at most; otherwise sequences of up to that many, rows_or_pairs at most
+cudaError_t launch_kv_attend(const KvAttendArgs &a, bool many, int rows_or_pairs, cudaStream_t s) {
     if (many) {
-        const dim3 grid((unsigned)a.n_seq * a.g.H * rows_or_tiles);
-        return a.g.D == 128 ? launch_k(kLaunchPdl, kv_attend_rows_kernel<128>, grid, dim3(128), 0, s, a, rows_or_tiles)
-                            : launch_k(kLaunchPdl, kv_attend_rows_kernel<64>, grid, dim3(128), 0, s, a, rows_or_tiles);
+        if (a.g.i4) return a.g.D == 128 ? launch_many<128, true>(a, rows_or_pairs, s) : launch_many<64, true>(a, rows_or_pairs, s);
+        return a.g.D == 128 ? launch_many<128, false>(a, rows_or_pairs, s) : launch_many<64, false>(a, rows_or_pairs, s);
     }
-    if (a.g.i4) return a.g.D == 128 ? launch_few<128, true>(a, rows_or_tiles, s) : launch_few<64, true>(a, rows_or_tiles, s);
-    return a.g.D == 128 ? launch_few<128, false>(a, rows_or_tiles, s) : launch_few<64, false>(a, rows_or_tiles, s);
+    if (a.g.i4) return a.g.D == 128 ? launch_few<128, true>(a, rows_or_pairs, s) : launch_few<64, true>(a, rows_or_pairs, s);
+    return a.g.D == 128 ? launch_few<128, false>(a, rows_or_pairs, s) : launch_few<64, false>(a, rows_or_pairs, s);
 }
 
 }  // namespace dtts

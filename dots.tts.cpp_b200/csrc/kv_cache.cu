@@ -16,7 +16,7 @@ using namespace dtts;
 
 namespace dtts {
 cudaError_t kv_attend_prepare();
-cudaError_t launch_kv_attend(const KvAttendArgs &a, bool many, int rows_or_tiles, cudaStream_t s);
+cudaError_t launch_kv_attend(const KvAttendArgs &a, bool many, int rows_or_pairs, cudaStream_t s);
 int kv_key_tile(const KvGeom &g, bool many);
 }  // namespace dtts
 
@@ -719,7 +719,7 @@ int dtts_kv_attend(dtts_kv *kv, int layer, const dtts_kv_attend_args *a) {
     DTTS_CHECK(a->n_heads >= 1 && a->n_heads % g.H == 0 && a->n_heads / g.H <= 128, DTTS_ERR_ARG,
                "%d query heads over %d key heads (a multiple, 128 to one at most)", a->n_heads, g.H);
     DTTS_CHECK(a->window >= 0 && a->sinks >= 0, DTTS_ERR_ARG, "window %d, sinks %d", a->window, a->sinks);
-    DTTS_CHECK(a->scale > 0.f && a->scale < INFINITY, DTTS_ERR_ARG, "scale %g", (double)a->scale);
+    DTTS_CHECK(a->scale > 0.f && a->scale <= 1e30f, DTTS_ERR_ARG, "scale %g", (double)a->scale);
     const int n_seq = (int)kv->b_seq.size(), G = a->n_heads / g.H;
     for (int b = 0; b < n_seq; b++) {
         const dtts_kv::Seq &s = kv->seqs[kv->b_seq[b]];
@@ -757,17 +757,17 @@ int dtts_kv_attend(dtts_kv *kv, int layer, const dtts_kv_attend_args *a) {
             const long long i0 = kv->b_len[b] - kv->b_cnt[b];
             const long long lo = a->window ? std::max(0ll, i0 - a->window + 1) : 0;
             const long long nt = (kv->b_len[b] + kt - 1) / kt - lo / kt + (std::min<long long>(a->sinks, lo) + kt - 1) / kt;
-            const long long rt = many ? (rows + 127) / 128 : 1;
+            const long long rt = many ? (rows + 255) / 256 : 1;
             tiles += nt * rt * g.H;
             max_tiles = std::max(max_tiles, nt);
             max_rows = (int)std::min<long long>(INT32_MAX, std::max<long long>(max_rows, rows));
         }
         if (!max_rows) continue;
-        const int rt = many ? (max_rows + 127) / 128 : 1;
+        const int rt = many ? (max_rows + 255) / 256 : 1;
         const long long units = (long long)n_seq * g.H * rt;
         DTTS_CHECK(units <= INT32_MAX / 256, DTTS_ERR_ARG, "%lld row tiles in one batch", units);
         // parts of a key range: enough for every SM, each a few tiles long
-        const int slot_rows = many ? 128 : kKvFewRows;
+        const int slot_rows = many ? 256 : kKvFewRows;
         const long long slots = kWsFloats / ((long long)slot_rows * (g.D + 2));
         const long long want = many ? kv->num_sms : 4ll * kv->num_sms;
         const long long min_tiles = many ? 2 : 4;

@@ -397,7 +397,7 @@ typedef struct dtts_kv_attend_args {
     long long out_row, out_head;
     int n_heads;                      /* a multiple of n_kv_heads; query head h reads key head
                                          h / (n_heads / n_kv_heads)                         */
-    float scale;                      /* of the scores, > 0                                 */
+    float scale;                      /* of the scores, > 0 and <= 1e30                      */
     int window;                       /* row i sees rows j <= i with j > i - window ...     */
     int sinks;                        /* ... or j < sinks; window 0: every row j <= i       */
 } dtts_kv_attend_args;

@@ -4,7 +4,8 @@ Tolerance of attention against them, per output element, from the kernels' round
 most half a step: bf16 2^-8, half 2^-11, fp32 2^-24, relative):
   * the bf16 output: 2^-8 |out|;
   * P in half (int4 rows): 2^-11 sum_j p_j |v_j|, and 2^-25 sum_j |v_j| for subnormal P (p <= 1 before the
-    division by l >= 1); in two bf16 terms (bf16 rows): 2^-16 sum_j p_j |v_j|, below the former;
+    division by l >= 1); in two bf16 terms (bf16 rows, at most 16 query rows): 2^-16 sum_j p_j |v_j|, below the
+    former; in bf16 (bf16 rows, more query rows): 2^-8 sum_j p_j |v_j|;
   * a score s = scale sum_d q_d k_d in fp32: at most D / 16 additions of 16-term products, each step off by at
     most 2^-22 of B = scale sum_d |q_d k_d|: 2^-19 B for D <= 128, on p through exp twice (numerator and l);
     exp2 itself 2^-22, corrections of the running maximum and l: n / 16 steps of 2^-23 each, P V the same."""
@@ -47,12 +48,13 @@ def visible(n, i, window, sinks):
     return ok
 
 
-def attend(q, k, v, i0, window=0, sinks=0, scale=None):
+def attend(q, k, v, i0, window=0, sinks=0, scale=None, int4=True):
     """q [t][Hq][D], held k, v [n][H][D] (double): rows i0 .. i0 + t - 1.  Returns (out, tolerance)."""
     t, hq, D = q.shape
     n, H = k.shape[:2]
     G = hq // H
     scale = D ** -0.5 if scale is None else scale
+    p_step = 2.0 ** -8 if not int4 and t * G > 16 else 2.0 ** -11
     q = q.double()
     out, tol = torch.zeros_like(q), torch.zeros_like(q)
     for x in range(t):
@@ -65,7 +67,7 @@ def attend(q, k, v, i0, window=0, sinks=0, scale=None):
             a = p @ vv.abs()
             B = float((kk.abs() @ q[x, h].abs()).max() * scale)
             out[x, h] = o
-            tol[x, h] = 2.0 ** -8 * o.abs() + a * (2.0 ** -11 + 2.0 ** -19 * B + (len(j) / 16 + 64) * 2.0 ** -22) + \
+            tol[x, h] = 2.0 ** -8 * o.abs() + a * (p_step + 2.0 ** -19 * B + (len(j) / 16 + 64) * 2.0 ** -22) + \
                 2.0 ** -25 * vv.abs().sum(0)
     return out, tol
 

@@ -141,7 +141,7 @@ def attend_case(dtype, D, Hq, H, page, lens, news, window=0, sinks=0, seed=3, sc
     row = 1
     for b, (n, t) in enumerate(zip(lens, news)):
         want, tol = R.attend(q[row - 1:row - 1 + t], R.held(rows[b][0], dtype == I4), R.held(rows[b][1], dtype == I4),
-                             n - t, window, sinks, scale)
+                             n - t, window, sinks, scale, dtype == I4)
         R.assert_close(out[row:row + t], want, tol, f"sequence {b} of {n} rows, {t} new")
         row += t
     kv.close()
