@@ -8,6 +8,7 @@
 #include <type_traits>
 
 namespace dtts {
+bool pdl_enabled();
 namespace {
 
 DTTS_DEV bool kv_visible(int j, int i, int window, int sinks) {
@@ -1073,7 +1074,7 @@ cudaError_t prepare_many() {
 }
 template <int D, bool I4>
 cudaError_t launch_many(const KvAttendArgs &a, int pairs, cudaStream_t s) {
-    return launch_k(kLaunchPdl, kv_attend_many_kernel<D, I4>, dim3((unsigned)a.n_seq * a.g.H * pairs * a.splits),
+    return launch_k(pdl_enabled() ? kLaunchPdl : 0u, kv_attend_many_kernel<D, I4>, dim3((unsigned)a.n_seq * a.g.H * pairs * a.splits),
                     dim3(ManyCfg<D, I4>::kThreads), ManyCfg<D, I4>::kSmem, s, a, pairs);
 }
 
@@ -1086,8 +1087,8 @@ template <int D, bool I4>
 cudaError_t launch_few(const KvAttendArgs &a, int rows, cudaStream_t s) {
     const dim3 grid((unsigned)a.n_seq * a.g.H * a.splits);
     if (rows <= 8)
-        return launch_k(kLaunchPdl, kv_attend_few_kernel<D, I4, 1>, grid, dim3(128), FewCfg<D, I4>::kSmem, s, a);
-    return launch_k(kLaunchPdl, kv_attend_few_kernel<D, I4, 2>, grid, dim3(128), FewCfg<D, I4>::kSmem, s, a);
+        return launch_k(pdl_enabled() ? kLaunchPdl : 0u, kv_attend_few_kernel<D, I4, 1>, grid, dim3(128), FewCfg<D, I4>::kSmem, s, a);
+    return launch_k(pdl_enabled() ? kLaunchPdl : 0u, kv_attend_few_kernel<D, I4, 2>, grid, dim3(128), FewCfg<D, I4>::kSmem, s, a);
 }
 
 }  // namespace

@@ -7,6 +7,7 @@
 #include "kv_host.h"
 
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 #include <cstring>
 #include <memory>
@@ -15,12 +16,15 @@
 using namespace dtts;
 
 namespace dtts {
+bool pdl_enabled();
 cudaError_t kv_attend_prepare();
 cudaError_t launch_kv_attend(const KvAttendArgs &a, bool many, int rows_or_pairs, cudaStream_t s);
 int kv_key_tile(const KvGeom &g, bool many);
 }  // namespace dtts
 
 namespace {
+
+unsigned kv_pdl() { return pdl_enabled() ? kLaunchPdl : 0u; }
 
 constexpr int kWsFloats = 9 * 1024 * 1024;     // 36 MB of partial results
 constexpr int kMaxUnits = 1 << 16;             // split units with an arrival counter
@@ -224,7 +228,7 @@ int dtts_kv::flush() {
             p.index[j] = pokes[i + j];
             p.value[j] = meta_h[pokes[i + j]];   // an index listed twice gets its last value both times
         }
-        DTTS_CUDA(launch_k(kLaunchPdl, kv_poke_kernel, dim3(1), dim3(256), 0, stream, meta, p));
+        DTTS_CUDA(launch_k(kv_pdl(), kv_poke_kernel, dim3(1), dim3(256), 0, stream, meta, p));
     }
     pokes.clear();
     return DTTS_OK;
@@ -235,7 +239,6 @@ void dtts_kv::drop_batch() {
     b_cnt.clear();
     b_len.clear();
     b_rows = 0;
-    b_id++;
 }
 
 int dtts_kv::not_capturing(const char *what) const {
@@ -284,7 +287,6 @@ int dtts_kv::extend(int n_seq, const int *sq, const int *n_new) {
     b_cnt.assign(n_new, n_new + n_seq);
     b_len.resize(n_seq);
     b_rows = (int)rows;
-    b_id++;
     int start = 0;
     for (int b = 0; b < n_seq; b++) {
         Seq &s = seqs[sq[b]];
@@ -320,8 +322,114 @@ int dtts_kv::extend(int n_seq, const int *sq, const int *n_new) {
     }
     if (c.n) copies.push_back(c);
     for (const Copies &cc : copies)
-        DTTS_CUDA(launch_k(kLaunchPdl, kv_copy_pages_kernel, dim3(g.L * g.H, cc.n), dim3(256), 0, stream, g, pool, cc));
+        DTTS_CUDA(launch_k(kv_pdl(), kv_copy_pages_kernel, dim3(g.L * g.H, cc.n), dim3(256), 0, stream, g, pool, cc));
     return flush();
+}
+
+namespace {
+// whether `cnt` queries from row i0 on see only rows that no trim has freed
+bool reachable(const dtts_kv &kv, const dtts_kv::Seq &s, int i0, int cnt, int window, int sinks) {
+    if (s.hole_lo >= s.hole_hi || cnt == 0) return true;
+    const long long lo = window ? std::max(0ll, (long long)i0 - window + 1) : 0;
+    return lo >= (long long)s.hole_hi * kv.g.P && std::min<long long>(sinks, lo) <= (long long)s.hole_lo * kv.g.P;
+}
+}  // namespace
+
+int dtts_kv::check_window(int n_seq, const int *sq, const int *n_new, int window, int sinks) const {
+    DTTS_CHECK(window >= 0 && sinks >= 0, DTTS_ERR_ARG, "window %d, sinks %d", window, sinks);
+    for (int b = 0; b < n_seq; b++)
+        if (!reachable(*this, seqs[sq[b]], seqs[sq[b]].len, n_new[b], window, sinks)) {
+            set_error("the window reaches rows of sequence %d that a trim freed", sq[b]);
+            return DTTS_ERR_ARG;
+        }
+    return DTTS_OK;
+}
+
+int dtts_kv::max_splits(int n_seq) const {
+    const long long units = (long long)n_seq * g.H, slots = kWsFloats / ((long long)kKvFewRows * (g.D + 2));
+    return units > kMaxUnits / 2 ? 1 : (int)std::max(1ll, slots / units);
+}
+
+int dtts_kv::plan_attend(const dtts_kv_attend_args &a, KvAttendPlan *plan) const {
+    DTTS_CHECK(!b_seq.empty(), DTTS_ERR_ARG, "no current batch: call dtts_kv_extend first");
+    DTTS_CHECK(a.n_heads >= 1 && a.n_heads % g.H == 0 && a.n_heads / g.H <= 128, DTTS_ERR_ARG,
+               "%d query heads over %d key heads (a multiple, 128 to one at most)", a.n_heads, g.H);
+    DTTS_CHECK(a.window >= 0 && a.sinks >= 0, DTTS_ERR_ARG, "window %d, sinks %d", a.window, a.sinks);
+    DTTS_CHECK(a.scale > 0.f && a.scale <= 1e30f, DTTS_ERR_ARG, "scale %g", (double)a.scale);
+    const int n_seq = (int)b_seq.size(), G = a.n_heads / g.H;
+    for (int b = 0; b < n_seq; b++)
+        if (!reachable(*this, seqs[b_seq[b]], b_len[b] - b_cnt[b], b_cnt[b], a.window, a.sinks)) {
+            set_error("the window reaches rows of sequence %d that a trim freed", b_seq[b]);
+            return DTTS_ERR_ARG;
+        }
+    plan->rows_or_pairs[0] = plan->rows_or_pairs[1] = 0;
+    if (b_rows == 0) return DTTS_OK;
+    DTTS_CHECK(a.q && a.out, DTTS_ERR_ARG, "null argument");
+    DTTS_CHECK(aligned16(a.q) && aligned16(a.out) && !((a.q_row | a.q_head | a.out_row | a.out_head) & 7), DTTS_ERR_ARG,
+               "rows must start on 16-byte boundaries");
+    KvAttendArgs p;
+    p.g = g;
+    p.m = kv_meta();
+    p.pool = pool;
+    p.q = (const bf16 *)a.q;
+    p.out = (bf16 *)a.out;
+    p.q_row = a.q_row; p.q_head = a.q_head; p.o_row = a.out_row; p.o_head = a.out_head;
+    p.n_seq = n_seq; p.G = G; p.total_rows = b_rows;
+    p.scale_log2 = a.scale * 1.4426950408889634f;
+    p.window = a.window; p.sinks = a.sinks;
+    p.ws = ws; p.cnt = cnt; p.err = d_err;
+    // both kernels run where a batch mixes steps and prompts; each takes its own sequences
+    for (int many = 0; many < 2; many++) {
+        const int kt = kv_key_tile(g, many);
+        long long tiles = 0, max_tiles = 0;
+        int max_rows = 0;
+        for (int b = 0; b < n_seq; b++) {
+            const long long rows = (long long)b_cnt[b] * G;
+            if (rows == 0 || (rows > kKvFewRows) != (many == 1)) continue;
+            const long long lo = a.window ? std::max(0ll, (long long)b_len[b] - b_cnt[b] - a.window + 1) : 0;
+            const long long nt = (b_len[b] + kt - 1) / kt - lo / kt + (std::min<long long>(a.sinks, lo) + kt - 1) / kt;
+            tiles += nt * (many ? (rows + 255) / 256 : 1) * g.H;
+            max_tiles = std::max(max_tiles, nt);
+            max_rows = (int)std::min<long long>(INT32_MAX / 2, std::max<long long>(max_rows, rows));
+        }
+        if (!max_rows) continue;
+        const int rt = many ? (max_rows + 255) / 256 : 1;
+        const long long units = (long long)n_seq * g.H * rt;
+        DTTS_CHECK(units <= INT32_MAX / 256, DTTS_ERR_ARG, "%lld row tiles in one batch", units);
+        // parts of a key range: enough for every SM, each a few tiles long
+        const int slot_rows = many ? 256 : kKvFewRows;
+        const long long slots = kWsFloats / ((long long)slot_rows * (g.D + 2));
+        const long long want = many ? num_sms : 4ll * num_sms;
+        const long long min_tiles = many ? 2 : 4;
+        const long long per = std::max(min_tiles, (tiles + want - 1) / want);
+        long long splits = (max_tiles + per - 1) / per;
+        if (units > kMaxUnits / 2) splits = 1;
+        splits = std::max(1ll, std::min(splits, slots / units));
+        p.splits = (int)splits;
+        p.tiles_per_split = (int)per;
+        plan->args[many] = p;
+        plan->rows_or_pairs[many] = many ? rt : max_rows;
+    }
+    return DTTS_OK;
+}
+
+int dtts_kv::attend(const KvAttendPlan &plan, int layer) {
+    for (int many = 0; many < 2; many++) {
+        if (!plan.rows_or_pairs[many]) continue;
+        KvAttendArgs p = plan.args[many];
+        p.pool += (long long)layer * g.H * g.seg;
+        DTTS_CUDA(launch_kv_attend(p, many == 1, plan.rows_or_pairs[many], stream));
+    }
+    return DTTS_OK;
+}
+
+int dtts_kv::check_batch(int n_seq, const int *sq, const int *n_new) const {
+    DTTS_CHECK(n_seq >= 1 && n_seq <= g.max_seqs, DTTS_ERR_ARG, "%d sequences (1..%d)", n_seq, g.max_seqs);
+    for (int b = 0; b < n_seq; b++) {
+        DTTS_CHECK(seq_ok(this, sq[b]), DTTS_ERR_ARG, "sequence %d is not open", sq[b]);
+        DTTS_CHECK(n_new[b] >= 0, DTTS_ERR_ARG, "%d new tokens", n_new[b]);
+    }
+    return DTTS_OK;
 }
 
 extern "C" {
@@ -350,6 +458,8 @@ int dtts_kv_create(const dtts_kv_config *c, int device, dtts_kv **out) try {
     std::unique_ptr<dtts_kv> kv(new dtts_kv());
     kv->device = device;
     kv->num_sms = nsm;
+    static std::atomic<long long> uids{0};
+    kv->uid = ++uids;
     kv->max_tokens = c->max_tokens;
     KvGeom &g = kv->g;
     g.L = c->n_layers; g.H = c->n_kv_heads; g.D = c->head_dim; g.P = P;
@@ -395,7 +505,7 @@ int dtts_kv_create(const dtts_kv_config *c, int device, dtts_kv **out) try {
 int dtts_kv_destroy(dtts_kv *kv) {
     if (!kv) return DTTS_OK;
     DeviceGuard dg(kv->device);
-    cudaStreamSynchronize(kv->stream);
+    cudaDeviceSynchronize();   // its work may be on streams that no longer exist
     delete kv;
     return DTTS_OK;
 }
@@ -482,7 +592,7 @@ int dtts_kv_fork(dtts_kv *kv, int src, int n, int *dst) try {
         f.src = src;
         f.pages = pages;
         for (int j = 0; j < f.n; j++) f.dst[j] = to[i + j];
-        DTTS_CUDA(launch_k(kLaunchPdl, kv_fork_tables_kernel, dim3(f.n), dim3(128), 0, kv->stream,
+        DTTS_CUDA(launch_k(kv_pdl(), kv_fork_tables_kernel, dim3(f.n), dim3(128), 0, kv->stream,
                            kv->meta + 5 * kv->g.max_seqs, kv->g.max_pages, f));
     }
     for (int s : to) {
@@ -585,11 +695,11 @@ int dtts_kv_compact(dtts_kv *kv, int seq, int n_keep, const int *keep) try {
             Puts p;
             p.n = std::min(kPuts, n - i);
             std::memcpy(p.value, keep + j0 + i, (size_t)p.n * 4);
-            DTTS_CUDA(launch_k(kLaunchPdl, kv_put_kernel, dim3(1), dim3(256), 0, kv->stream, kv->keep + i, p));
+            DTTS_CUDA(launch_k(kv_pdl(), kv_put_kernel, dim3(1), dim3(256), 0, kv->stream, kv->keep + i, p));
         }
         const long long units = (long long)n * (2 * g.RB / 16 + (g.i4 ? 2 : 0));
         const int gx = (int)std::min<long long>((units + 255) / 256, 1024);
-        DTTS_CUDA(launch_k(kLaunchPdl, kv_gather_kernel, dim3(gx, g.L * g.H), dim3(256), 0, kv->stream, g,
+        DTTS_CUDA(launch_k(kv_pdl(), kv_gather_kernel, dim3(gx, g.L * g.H), dim3(256), 0, kv->stream, g,
                            (const int *)(kv->meta + 5 * g.max_seqs), kv->pool, (const int *)kv->keep, n, j0, seq, scratch));
     }
     for (int p = 0; p < total; p++) kv->poke(kv->table_at(seq, p), pages[p]);
@@ -622,11 +732,8 @@ int dtts_kv_free_pages(dtts_kv *kv, int *n) {
 
 int dtts_kv_extend(dtts_kv *kv, int n_seq, const int *seqs, const int *n_new) try {
     DTTS_CHECK(kv && seqs && n_new, DTTS_ERR_ARG, "null argument");
-    DTTS_CHECK(n_seq >= 1 && n_seq <= kv->g.max_seqs, DTTS_ERR_ARG, "%d sequences (1..%d)", n_seq, kv->g.max_seqs);
-    for (int b = 0; b < n_seq; b++) {
-        DTTS_CHECK(seq_ok(kv, seqs[b]), DTTS_ERR_ARG, "sequence %d is not open", seqs[b]);
-        DTTS_CHECK(n_new[b] >= 0, DTTS_ERR_ARG, "%d new tokens", n_new[b]);
-    }
+    int st = kv->check_batch(n_seq, seqs, n_new);
+    if (st) return st;
     DeviceGuard dg(kv->device);
     return kv->extend(n_seq, seqs, n_new);
 } catch (const std::bad_alloc &) {
@@ -650,7 +757,7 @@ int dtts_kv_write(dtts_kv *kv, int layer, const void *k, const void *v, long lon
     const int per_block = 256 / (g.D / 4);
     const long long items = (long long)kv->b_rows * g.H;
     DTTS_CHECK((items + per_block - 1) / per_block <= INT32_MAX, DTTS_ERR_ARG, "%d rows in one batch", kv->b_rows);
-    DTTS_CUDA(launch_k(kLaunchPdl, kv_write_kernel, dim3((unsigned)((items + per_block - 1) / per_block)), dim3(256), 0,
+    DTTS_CUDA(launch_k(kv_pdl(), kv_write_kernel, dim3((unsigned)((items + per_block - 1) / per_block)), dim3(256), 0,
                        kv->stream, g, kv->kv_meta(), kv->pool + (long long)layer * g.H * g.seg, (int)kv->b_seq.size(),
                        kv->b_rows, (const bf16 *)k, (const bf16 *)v, k_row, k_head, v_row, v_head));
     return DTTS_OK;
@@ -701,9 +808,9 @@ int dtts_kv_read(dtts_kv *kv, int layer, int n_layers, int n, const int *seqs, c
         const uint8_t *pool = kv->pool + (long long)layer * g.H * g.seg;
         const int *table = kv->meta + 5 * g.max_seqs;
         if (dtype == DTTS_DTYPE_F32)
-            DTTS_CUDA(launch_k(kLaunchPdl, kv_read_kernel<true>, grid, dim3(256), 0, kv->stream, g, table, pool, r, k, v));
+            DTTS_CUDA(launch_k(kv_pdl(), kv_read_kernel<true>, grid, dim3(256), 0, kv->stream, g, table, pool, r, k, v));
         else
-            DTTS_CUDA(launch_k(kLaunchPdl, kv_read_kernel<false>, grid, dim3(256), 0, kv->stream, g, table, pool, r, k, v));
+            DTTS_CUDA(launch_k(kv_pdl(), kv_read_kernel<false>, grid, dim3(256), 0, kv->stream, g, table, pool, r, k, v));
     }
     return DTTS_OK;
 } catch (const std::bad_alloc &) {
@@ -713,73 +820,13 @@ int dtts_kv_read(dtts_kv *kv, int layer, int n_layers, int n, const int *seqs, c
 
 int dtts_kv_attend(dtts_kv *kv, int layer, const dtts_kv_attend_args *a) {
     DTTS_CHECK(kv && a, DTTS_ERR_ARG, "null argument");
-    const KvGeom &g = kv->g;
-    DTTS_CHECK(layer >= 0 && layer < g.L, DTTS_ERR_ARG, "layer %d of %d", layer, g.L);
-    DTTS_CHECK(!kv->b_seq.empty(), DTTS_ERR_ARG, "no current batch: call dtts_kv_extend first");
-    DTTS_CHECK(a->n_heads >= 1 && a->n_heads % g.H == 0 && a->n_heads / g.H <= 128, DTTS_ERR_ARG,
-               "%d query heads over %d key heads (a multiple, 128 to one at most)", a->n_heads, g.H);
-    DTTS_CHECK(a->window >= 0 && a->sinks >= 0, DTTS_ERR_ARG, "window %d, sinks %d", a->window, a->sinks);
-    DTTS_CHECK(a->scale > 0.f && a->scale <= 1e30f, DTTS_ERR_ARG, "scale %g", (double)a->scale);
-    const int n_seq = (int)kv->b_seq.size(), G = a->n_heads / g.H;
-    for (int b = 0; b < n_seq; b++) {
-        const dtts_kv::Seq &s = kv->seqs[kv->b_seq[b]];
-        if (s.hole_lo >= s.hole_hi || kv->b_cnt[b] == 0) continue;
-        const long long lo = a->window ? std::max(0ll, (long long)kv->b_len[b] - kv->b_cnt[b] - a->window + 1) : 0;
-        DTTS_CHECK(lo >= (long long)s.hole_hi * g.P && std::min<long long>(a->sinks, lo) <= (long long)s.hole_lo * g.P,
-                   DTTS_ERR_ARG, "the window reaches rows of sequence %d that a trim freed", kv->b_seq[b]);
-    }
-    if (kv->b_rows == 0) return DTTS_OK;
-    DTTS_CHECK(a->q && a->out, DTTS_ERR_ARG, "null argument");
-    DTTS_CHECK(aligned16(a->q) && aligned16(a->out) && !((a->q_row | a->q_head | a->out_row | a->out_head) & 7),
-               DTTS_ERR_ARG, "rows must start on 16-byte boundaries");
-    DeviceGuard dg(kv->device);
-    int st = kv->flush();
+    DTTS_CHECK(layer >= 0 && layer < kv->g.L, DTTS_ERR_ARG, "layer %d of %d", layer, kv->g.L);
+    KvAttendPlan p;
+    int st = kv->plan_attend(*a, &p);
     if (st) return st;
-    KvAttendArgs p;
-    p.g = g;
-    p.m = kv->kv_meta();
-    p.pool = kv->pool + (long long)layer * g.H * g.seg;
-    p.q = (const bf16 *)a->q;
-    p.out = (bf16 *)a->out;
-    p.q_row = a->q_row; p.q_head = a->q_head; p.o_row = a->out_row; p.o_head = a->out_head;
-    p.n_seq = n_seq; p.G = G; p.total_rows = kv->b_rows;
-    p.scale_log2 = a->scale * 1.4426950408889634f;
-    p.window = a->window; p.sinks = a->sinks;
-    p.ws = kv->ws; p.cnt = kv->cnt; p.err = kv->d_err;
-    // both kernels run where a batch mixes steps and prompts; each takes its own sequences
-    for (int many = 0; many < 2; many++) {
-        const int kt = kv_key_tile(g, many);
-        long long tiles = 0, max_tiles = 0;
-        int max_rows = 0;
-        for (int b = 0; b < n_seq; b++) {
-            const long long rows = (long long)kv->b_cnt[b] * G;
-            if (rows == 0 || (rows > kKvFewRows) != (many == 1)) continue;
-            const long long i0 = kv->b_len[b] - kv->b_cnt[b];
-            const long long lo = a->window ? std::max(0ll, i0 - a->window + 1) : 0;
-            const long long nt = (kv->b_len[b] + kt - 1) / kt - lo / kt + (std::min<long long>(a->sinks, lo) + kt - 1) / kt;
-            const long long rt = many ? (rows + 255) / 256 : 1;
-            tiles += nt * rt * g.H;
-            max_tiles = std::max(max_tiles, nt);
-            max_rows = (int)std::min<long long>(INT32_MAX, std::max<long long>(max_rows, rows));
-        }
-        if (!max_rows) continue;
-        const int rt = many ? (max_rows + 255) / 256 : 1;
-        const long long units = (long long)n_seq * g.H * rt;
-        DTTS_CHECK(units <= INT32_MAX / 256, DTTS_ERR_ARG, "%lld row tiles in one batch", units);
-        // parts of a key range: enough for every SM, each a few tiles long
-        const int slot_rows = many ? 256 : kKvFewRows;
-        const long long slots = kWsFloats / ((long long)slot_rows * (g.D + 2));
-        const long long want = many ? kv->num_sms : 4ll * kv->num_sms;
-        const long long min_tiles = many ? 2 : 4;
-        const long long per = std::max(min_tiles, (tiles + want - 1) / want);
-        long long splits = (max_tiles + per - 1) / per;
-        if (units > kMaxUnits / 2) splits = 1;
-        splits = std::max(1ll, std::min(splits, slots / units));
-        p.splits = (int)splits;
-        p.tiles_per_split = (int)per;
-        DTTS_CUDA(launch_kv_attend(p, many == 1, many ? rt : max_rows, kv->stream));
-    }
-    return DTTS_OK;
+    DeviceGuard dg(kv->device);
+    if ((st = kv->flush())) return st;
+    return kv->attend(p, layer);
 }
 
 }  // extern "C"

@@ -9,6 +9,14 @@
 #include "kv.cuh"
 #include "runtime.h"
 
+namespace dtts {
+// Launches of one attention call on the current batch; the same for every layer.
+struct KvAttendPlan {
+    KvAttendArgs args[2];       // sequences of few rows, of many rows
+    int rows_or_pairs[2];       // 0: no such sequence
+};
+}  // namespace dtts
+
 struct dtts_kv {
     struct Seq {
         bool open = false;
@@ -33,7 +41,7 @@ struct dtts_kv {
     // current batch
     std::vector<int> b_seq, b_cnt, b_len;
     int b_rows = 0;
-    long long b_id = 0;                   // changes with the batch and with anything that moves its rows
+    long long uid = 0;                    // no two caches of a process share it
 
     ~dtts_kv();
     dtts::KvMeta kv_meta() const;
@@ -55,5 +63,12 @@ struct dtts_kv {
     }
     void drop_batch();
     int not_capturing(const char *what) const;
+    int check_batch(int n_seq, const int *sq, const int *n_new) const;
     int extend(int n_seq, const int *sq, const int *n_new);
+    // Whether attention of n_new[b] further tokens would reach rows that a trim freed.
+    int check_window(int n_seq, const int *sq, const int *n_new, int window, int sinks) const;
+    int max_splits(int n_seq) const;      // of the few-row kernel, for the workspace
+    // Checks the arguments against the current batch and sizes the launches.
+    int plan_attend(const dtts_kv_attend_args &a, dtts::KvAttendPlan *p) const;
+    int attend(const dtts::KvAttendPlan &p, int layer);
 };

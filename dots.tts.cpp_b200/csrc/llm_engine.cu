@@ -9,14 +9,17 @@
 // k and v appended to a bf16 cache -> grouped-query attention (12 query heads
 // over 2 key/value heads of 128, causal) -> o_proj (+bias) into the fp32
 // residual -> RMSNorm -> gate|up projection -> SiLU(gate) * up -> down_proj
-// into the residual; then the final RMSNorm.
+// into the residual; then the final RMSNorm.  dtts_llm_extend runs the same
+// layers over a paged cache (kv_host.h): sequences of different lengths, bf16 or
+// 4-bit rows, an optional sliding window.
 #include "kernels.cuh"
-#include "runtime.h"
+#include "kv_host.h"
 
 #include <algorithm>
 #include <cmath>
 #include <cstring>
 #include <memory>
+#include <new>
 #include <vector>
 
 using namespace dtts;
@@ -98,6 +101,66 @@ __global__ void __launch_bounds__(256) llm_rope_cache_kernel(float *__restrict__
             if (zero) row[kLH + kLKV + j] = 0.f;
             vc[(((long long)b * kLNKV + hv) * cap + p) * kLHD + d] = __float2bfloat16_rn(x);
         }
+    }
+}
+
+// RoPE and cache rows for a batch over a paged cache: q to bf16 [M][1536], k and v
+// (rounded to bf16, as the dense cache holds them) to the rows' pages.  One block
+// of 160 threads per token: warp 0 rotates and stores the two k heads, warp 1
+// stores v, warps 2-4 rotate q; a thread of a rotation has dims 8 u .. 8 u + 7 and
+// 64 + 8 u .. of a head.  zero as above.
+DTTS_DEV void llm_rope8(float *row, const float4 *cs4, int c, uint4 *lo, uint4 *hi, int zero) {
+    float4 *a = reinterpret_cast<float4 *>(row + c), *b = reinterpret_cast<float4 *>(row + c + 64);
+    const float4 x0 = a[0], x1 = a[1], y0 = b[0], y1 = b[1];
+    if (zero) a[0] = a[1] = b[0] = b[1] = make_float4(0.f, 0.f, 0.f, 0.f);
+    const float x[8] = {x0.x, x0.y, x0.z, x0.w, x1.x, x1.y, x1.z, x1.w};
+    const float y[8] = {y0.x, y0.y, y0.z, y0.w, y1.x, y1.y, y1.z, y1.w};
+    float p[8], q[8];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const float4 cs = cs4[i];   // (cos, sin) of two dims
+        p[2 * i] = x[2 * i] * cs.x - y[2 * i] * cs.y;
+        q[2 * i] = y[2 * i] * cs.x + x[2 * i] * cs.y;
+        p[2 * i + 1] = x[2 * i + 1] * cs.z - y[2 * i + 1] * cs.w;
+        q[2 * i + 1] = y[2 * i + 1] * cs.z + x[2 * i + 1] * cs.w;
+    }
+    *lo = make_uint4(pack_bf16x2(p[0], p[1]), pack_bf16x2(p[2], p[3]), pack_bf16x2(p[4], p[5]), pack_bf16x2(p[6], p[7]));
+    *hi = make_uint4(pack_bf16x2(q[0], q[1]), pack_bf16x2(q[2], q[3]), pack_bf16x2(q[4], q[5]), pack_bf16x2(q[6], q[7]));
+}
+__global__ void __launch_bounds__(160) llm_rope_pages_kernel(float *__restrict__ qkv, const __grid_constant__ KvGeom g,
+                                                             const __grid_constant__ KvMeta m, uint8_t *__restrict__ pool,
+                                                             int n_seq, const float2 *__restrict__ rope, int max_seq,
+                                                             bf16 *__restrict__ qout, int zero) {
+    pdl_wait();
+    pdl_trigger();
+    const int row = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int b = kv_find_entry(m.start, n_seq, row), off = row - m.start[b];
+    const bool on = off < m.cnt[b];
+    const int tok = m.len[b] - m.cnt[b] + off, pos = min(m.pos[b] + off, max_seq - 1);
+    const int page = on ? m.table[(long long)m.seq[b] * g.max_pages + (tok >> g.lgP)] : -1;
+    const bool held = page >= 0 && page < g.n_pages;
+    float *x = qkv + (long long)row * kLQKV;
+    const float4 *cs = reinterpret_cast<const float4 *>(rope + (long long)pos * 64 + 8 * (lane & 7));
+    uint4 lo = make_uint4(0u, 0u, 0u, 0u), hi = lo;
+    if (warp == 0) {
+        const int head = (lane >> 3) & 1, u = lane & 7;
+        if (lane < 16) llm_rope8(x, cs, kLH + head * kLHD + 8 * u, &lo, &hi, zero);
+        uint8_t *seg = pool + kv_seg_off(g, held ? page : 0, 0, head);
+        kv_store8(g, seg, false, tok & (g.P - 1), u, lo, held && lane < 16);
+        kv_store8(g, seg, false, tok & (g.P - 1), 8 + u, hi, held && lane < 16);
+    } else if (warp == 1) {
+        const int head = lane >> 4, w = lane & 15;
+        float4 *v = reinterpret_cast<float4 *>(x + kLH + kLKV + head * kLHD + 8 * w);
+        const float4 a = v[0], c = v[1];
+        if (zero) v[0] = v[1] = make_float4(0.f, 0.f, 0.f, 0.f);
+        lo = make_uint4(pack_bf16x2(a.x, a.y), pack_bf16x2(a.z, a.w), pack_bf16x2(c.x, c.y), pack_bf16x2(c.z, c.w));
+        kv_store8(g, pool + kv_seg_off(g, held ? page : 0, 0, head), true, tok & (g.P - 1), w, lo, held);
+    } else {
+        const int head = (warp - 2) * 4 + (lane >> 3), c = head * kLHD + 8 * (lane & 7);
+        llm_rope8(x, cs, c, &lo, &hi, zero);
+        bf16 *q = qout + (long long)row * kLH + c;
+        *reinterpret_cast<uint4 *>(q) = lo;
+        *reinterpret_cast<uint4 *>(q + 64) = hi;
     }
 }
 
@@ -260,7 +323,13 @@ struct dtts_llm {
     int *d_len = nullptr;                // cache length on the device (graph-captured steps)
     int *d_err = nullptr;
     // step graphs, one per batch size; dropped when the workspace moves
-    struct Graph { int B; cudaGraphExec_t exec; };
+    // (paged: also the cache, the window and the split of its attention; uid 0: the dense cache)
+    struct Graph {
+        int B;
+        long long uid;
+        int window, sinks, splits;
+        cudaGraphExec_t exec;
+    };
     std::vector<Graph> graphs;
     void drop_graphs() {
         for (Graph &g : graphs) cudaGraphExecDestroy(g.exec);
@@ -313,9 +382,11 @@ struct dtts_llm {
 
     // emb already in h ([B * T][1536]); runs every layer and the final norm into
     // `out`, then advances d_len; dev_pos: positions from d_len, not pos0
-    int enqueue(int B, int T, int pos0, bool dev_pos, float *out) {
+    // kv, plan: instead of the dense cache, the M rows of the paged cache's batch
+    int enqueue(int B, int T, int pos0, bool dev_pos, float *out, dtts_kv *kv = nullptr,
+                const KvAttendPlan *plan = nullptr) {
         const int *pd = dev_pos ? d_len : nullptr;
-        const int M = B * T;
+        const int M = kv ? kv->b_rows : B * T;
         const bool small = M <= 256;
         const int bn = small ? 128 : 256;
         const size_t layer_stride = (size_t)max_batch * kLNKV * max_seq * kLHD;
@@ -341,11 +412,19 @@ struct dtts_llm {
                 o.ep.bias = L.bqkv; o.ep.out = qkv; o.ep.ldo = kLQKV;
                 DTTS_CUDA(launch_gemm(o, num_sms, stream));
             }
-            launch_k(pdl, llm_rope_cache_kernel, dim3(M), dim3(256), 0, stream, qkv, T, pos0, pd, (const float2 *)rope,
-                     q, kc + l * layer_stride, vc + l * layer_stride, max_seq, small ? 1 : 0);
-            launch_k(pdl, llm_attn_kernel, dim3((M * kLNH + 7) / 8), dim3(256), 0, stream, (const float *)q,
-                     (const bf16 *)(kc + l * layer_stride), (const bf16 *)(vc + l * layer_stride), T, pos0, pd,
-                     max_seq, M, ao);
+            if (kv) {
+                launch_k(pdl, llm_rope_pages_kernel, dim3(M), dim3(160), 0, stream, qkv, kv->g, kv->kv_meta(),
+                         kv->pool + (long long)l * kv->g.H * kv->g.seg, (int)kv->b_seq.size(), (const float2 *)rope, max_seq,
+                         (bf16 *)q, small ? 1 : 0);
+                int st = kv->attend(*plan, l);
+                if (st) return st;
+            } else {
+                launch_k(pdl, llm_rope_cache_kernel, dim3(M), dim3(256), 0, stream, qkv, T, pos0, pd, (const float2 *)rope,
+                         q, kc + l * layer_stride, vc + l * layer_stride, max_seq, small ? 1 : 0);
+                launch_k(pdl, llm_attn_kernel, dim3((M * kLNH + 7) / 8), dim3(256), 0, stream, (const float *)q,
+                         (const bf16 *)(kc + l * layer_stride), (const bf16 *)(vc + l * layer_stride), T, pos0, pd,
+                         max_seq, M, ao);
+            }
             {
                 GemmOp o = op(t_ao, small ? L.to_s : L.to, M, kLH, kLH, EPI_RESID, bn);
                 o.tr = t_h; o.ep.bias = L.bo; o.ep.resid = h; o.ep.ldr = kLH;
@@ -378,7 +457,7 @@ struct dtts_llm {
         }
         launch_k(pdl, llm_rms_norm_kernel<false>, dim3((M + 7) / 8), dim3(256), 0, stream, (const float *)h,
                  (const float *)final_norm, (void *)out, M);
-        launch_advance_len(d_len, T, stream, true);
+        if (!kv) launch_advance_len(d_len, T, stream, true);
         DTTS_CUDA(cudaGetLastError());
         return DTTS_OK;
     }
@@ -399,18 +478,10 @@ struct dtts_llm {
             // decode step: one graph per batch size, positions from d_len
             cudaGraphExec_t exec = nullptr;
             for (Graph &g : graphs)
-                if (g.B == B) exec = g.exec;
+                if (g.B == B && g.uid == 0) exec = g.exec;
             if (!exec) {
-                cudaGraph_t graph = nullptr;
-                DTTS_CUDA(cudaStreamBeginCapture(stream, cudaStreamCaptureModeThreadLocal));
-                st = enqueue(B, 1, 0, true, outd);
-                cudaError_t ce = cudaStreamEndCapture(stream, &graph);
-                if (st) { if (graph) cudaGraphDestroy(graph); return st; }
-                DTTS_CUDA(ce);
-                ce = cudaGraphInstantiate(&exec, graph, 0);
-                cudaGraphDestroy(graph);
-                DTTS_CUDA(ce);
-                graphs.push_back({B, exec});
+                if ((st = capture(&exec, [&] { return enqueue(B, 1, 0, true, outd); }))) return st;
+                graphs.push_back({B, 0, 0, 0, 0, exec});
             }
             DTTS_CUDA(cudaGraphLaunch(exec, stream));
         } else if ((st = enqueue(B, T, cur_len, false, outd))) {
@@ -419,12 +490,101 @@ struct dtts_llm {
         DTTS_CUDA(cudaMemcpyAsync(hidden, outd, (size_t)M * kLH * 4,
                                   mem == DTTS_MEM_HOST ? cudaMemcpyDeviceToHost : cudaMemcpyDeviceToDevice, stream));
         cur_len += T;
-        if (mem != DTTS_MEM_HOST) return DTTS_OK;
-        if ((st = stream_wait(stream, 300.0))) return st;
+        return mem == DTTS_MEM_HOST ? finish() : DTTS_OK;
+    }
+
+    template <typename F>
+    int capture(cudaGraphExec_t *exec, F body) {
+        cudaGraph_t graph = nullptr;
+        DTTS_CUDA(cudaStreamBeginCapture(stream, cudaStreamCaptureModeThreadLocal));
+        int st = body();
+        cudaError_t ce = cudaStreamEndCapture(stream, &graph);
+        if (st) { if (graph) cudaGraphDestroy(graph); return st; }
+        DTTS_CUDA(ce);
+        ce = cudaGraphInstantiate(exec, graph, 0);
+        cudaGraphDestroy(graph);
+        DTTS_CUDA(ce);
+        return DTTS_OK;
+    }
+
+    int finish() {
+        int st = stream_wait(stream, 300.0);
+        if (st) return st;
         int err = 0;
         DTTS_CUDA(cudaMemcpy(&err, d_err, 4, cudaMemcpyDeviceToHost));
         if (err) { cudaMemset(d_err, 0, 4); set_error("device wait limit reached (code %d)", err); return DTTS_ERR_TIMEOUT; }
         return DTTS_OK;
+    }
+
+    // The new tokens of a ragged batch over a paged cache.  A step (one token for
+    // every sequence) is a graph: its kernels read lengths and tables on the device,
+    // so one graph serves every step with the same batch size and split of the
+    // attention (rounded up to a power of two; a part then holds at least 4 tiles).
+    int extend(dtts_kv *kv, int n_seq, const int *seqs, const int *n_new, const float *emb, int window, int sinks,
+               float *hidden, int mem) {
+        long long M = 0;
+        bool step = true;
+        for (int b = 0; b < n_seq; b++) {
+            DTTS_CHECK(kv->seqs[seqs[b]].pos + (long long)n_new[b] <= max_seq, DTTS_ERR_ARG,
+                       "sequence %d would reach position %lld (limit %d)", seqs[b],
+                       kv->seqs[seqs[b]].pos + (long long)n_new[b], max_seq);
+            M += n_new[b];
+            step = step && n_new[b] == 1;
+        }
+        DTTS_CHECK(M <= (1 << 24), DTTS_ERR_ARG, "%lld tokens in one call", M);
+        DeviceGuard g(device);
+        // the cache works on the engine's stream during the call; its own stream waits for what is enqueued here
+        struct Streams {
+            dtts_kv *kv;
+            cudaStream_t back;
+            ~Streams() { dtts_kv_set_stream(kv, back); }
+        } streams{kv, kv->stream};
+        int st = dtts_kv_set_stream(kv, stream);
+        if (st || (st = kv->not_capturing("extend"))) return st;
+        if ((st = ensure(M + 1))) return st;
+        dtts_kv_attend_args aa;
+        std::memset(&aa, 0, sizeof(aa));
+        aa.q = q; aa.q_row = kLH; aa.q_head = kLHD;
+        aa.out = ao; aa.out_row = kLH; aa.out_head = kLHD;
+        aa.n_heads = kLNH;
+        aa.scale = 1.0f / sqrtf((float)kLHD);
+        aa.window = window; aa.sinks = sinks;
+        if ((st = kv->check_window(n_seq, seqs, n_new, window, sinks))) return st;
+        if ((st = kv->extend(n_seq, seqs, n_new))) return st;
+        if (M == 0) return DTTS_OK;
+        KvAttendPlan plan;
+        if ((st = kv->plan_attend(aa, &plan))) return st;
+        float *outd = qkv;
+        DTTS_CUDA(cudaMemcpyAsync(h, emb, (size_t)M * kLH * 4,
+                                  mem == DTTS_MEM_HOST ? cudaMemcpyHostToDevice : cudaMemcpyDeviceToDevice, stream));
+        if (step) {
+            KvAttendArgs &p = plan.args[0];
+            int pow2 = 1;
+            while (pow2 < p.splits) pow2 *= 2;
+            const int splits = std::min(pow2, kv->max_splits(n_seq));
+            cudaGraphExec_t exec = nullptr;
+            for (Graph &g : graphs)
+                if (g.B == n_seq && g.uid == kv->uid && g.window == window && g.sinks == sinks && g.splits == splits)
+                    exec = g.exec;
+            if (!exec) {
+                p.splits = splits;
+                p.tiles_per_split = 4;
+                if (graphs.size() >= 64) {
+                    DTTS_CUDA(cudaStreamSynchronize(stream));
+                    drop_graphs();
+                }
+                if ((st = capture(&exec, [&] { return enqueue(n_seq, 1, 0, false, outd, kv, &plan); }))) return st;
+                graphs.push_back({n_seq, kv->uid, window, sinks, splits, exec});
+            }
+            DTTS_CUDA(cudaGraphLaunch(exec, stream));
+        } else if ((st = enqueue(n_seq, 0, 0, false, outd, kv, &plan))) {
+            return st;
+        }
+        DTTS_CUDA(cudaMemcpyAsync(hidden, outd, (size_t)M * kLH * 4,
+                                  mem == DTTS_MEM_HOST ? cudaMemcpyDeviceToHost : cudaMemcpyDeviceToDevice, stream));
+        if (mem != DTTS_MEM_HOST) return DTTS_OK;
+        if ((st = finish())) return st;
+        return dtts_kv_sync(kv);
     }
 };
 
@@ -526,6 +686,36 @@ int dtts_llm_step(dtts_llm *e, const float *emb, int B, float *hidden, int mem) 
     DTTS_CHECK(e, DTTS_ERR_ARG, "null engine");
     DTTS_CHECK(B == e->cur_B && e->cur_len > 0, DTTS_ERR_ARG, "step needs a prefill of the same %d sequences", B);
     return e->run(emb, B, 1, hidden, mem);
+}
+
+int dtts_llm_kv_create(dtts_llm *e, int n_pages, int max_seqs, int page_tokens, int dtype, dtts_kv **out) {
+    DTTS_CHECK(e && out, DTTS_ERR_ARG, "null argument");
+    *out = nullptr;
+    dtts_kv_config c;
+    c.n_layers = e->n_layers;
+    c.n_kv_heads = kLNKV;
+    c.head_dim = kLHD;
+    c.page_tokens = page_tokens;
+    c.n_pages = n_pages;
+    c.max_seqs = max_seqs;
+    c.max_tokens = e->max_seq;
+    c.dtype = dtype;
+    return dtts_kv_create(&c, e->device, out);
+}
+
+int dtts_llm_extend(dtts_llm *e, dtts_kv *kv, int n_seq, const int *seqs, const int *n_new, const float *emb, int window,
+                    int sinks, float *hidden, int mem) try {
+    DTTS_CHECK(e && kv && seqs && n_new && emb && hidden, DTTS_ERR_ARG, "null argument");
+    DTTS_CHECK(mem == DTTS_MEM_HOST || mem == DTTS_MEM_DEVICE, DTTS_ERR_ARG, "bad mem kind");
+    DTTS_CHECK(kv->device == e->device && kv->g.L == e->n_layers && kv->g.H == kLNKV && kv->g.D == kLHD, DTTS_ERR_ARG,
+               "the cache has %d layers of %d x %d on device %d, the engine needs %d of %d x %d on device %d", kv->g.L,
+               kv->g.H, kv->g.D, kv->device, e->n_layers, kLNKV, kLHD, e->device);
+    int st = kv->check_batch(n_seq, seqs, n_new);
+    if (st) return st;
+    return e->extend(kv, n_seq, seqs, n_new, emb, window, sinks, hidden, mem);
+} catch (const std::bad_alloc &) {
+    set_error("out of host memory");
+    return DTTS_ERR_OOM;
 }
 
 int dtts_llm_length(dtts_llm *e, int *tokens) {

@@ -113,6 +113,7 @@ EXPORTS = [
     "dtts_dit_last_launch_count", "dtts_dit_tune", "dtts_dit_set_fused_ln", "dtts_fm_create", "dtts_fm_destroy", "dtts_fm_start",
     "dtts_fm_append_latents", "dtts_fm_append_hidden", "dtts_fm_length", "dtts_fm_read", "dtts_fm_solve", "dtts_fm_layout",
     "dtts_llm_create", "dtts_llm_destroy", "dtts_llm_set_stream", "dtts_llm_prefill", "dtts_llm_step", "dtts_llm_length",
+    "dtts_llm_kv_create", "dtts_llm_extend",
     "dtts_kv_create", "dtts_kv_destroy", "dtts_kv_set_stream", "dtts_kv_sync", "dtts_kv_open", "dtts_kv_close",
     "dtts_kv_fork", "dtts_kv_truncate", "dtts_kv_trim", "dtts_kv_compact", "dtts_kv_length", "dtts_kv_free_pages",
     "dtts_kv_extend", "dtts_kv_write", "dtts_kv_attend", "dtts_kv_read",
@@ -230,6 +231,8 @@ def lib(path: str = LIB_PATH):
     L.dtts_llm_prefill.argtypes = [_vp, _vp, C.c_int, C.c_int, _vp, C.c_int]
     L.dtts_llm_step.argtypes = [_vp, _vp, C.c_int, _vp, C.c_int]
     L.dtts_llm_length.argtypes = [_vp, C.POINTER(C.c_int)]
+    L.dtts_llm_kv_create.argtypes = [_vp, C.c_int, C.c_int, C.c_int, C.c_int, C.POINTER(_vp)]
+    L.dtts_llm_extend.argtypes = [_vp, _vp, C.c_int, _vp, _vp, _vp, C.c_int, C.c_int, _vp, C.c_int]
     L.dtts_kv_create.argtypes = [C.POINTER(KVConfig), C.c_int, C.POINTER(_vp)]
     for f in ("destroy", "sync"):
         getattr(L, "dtts_kv_" + f).argtypes = [_vp]
@@ -681,6 +684,7 @@ class LLM:
         h = _vp()
         check(lib().dtts_llm_create(C.byref(s), device, max_batch, max_seq, C.byref(h)))
         self.h = h
+        self.n_layers = n_layers
 
     def close(self):
         if getattr(self, "h", None):
@@ -715,6 +719,28 @@ class LLM:
         n = C.c_int()
         check(lib().dtts_llm_length(self.h, C.byref(n)))
         return n.value
+
+    def kv_cache(self, n_pages, max_seqs, page_tokens=64, dtype=DTYPE_BF16):
+        """A paged cache of this engine's geometry (KVCache), for extend()."""
+        h = _vp()
+        check(lib().dtts_llm_kv_create(self.h, n_pages, max_seqs, page_tokens, dtype, C.byref(h)))
+        kv = KVCache.__new__(KVCache)
+        kv._init(h, self.n_layers, 2, 128)
+        return kv
+
+    def extend(self, kv, seqs, n_new, emb, out=None, window=0, sinks=0, mem=MEM_HOST):
+        """Appends n_new[b] tokens to sequence seqs[b] of kv: emb [sum of n_new][1536] -> hidden."""
+        s, ps, n = _ints(seqs)
+        c, pc, m = _ints(n_new)
+        if n != m:
+            raise ValueError(f"{n} sequences, {m} counts")
+        if mem == MEM_HOST:
+            emb = _f32(emb)
+            out = np.zeros_like(emb) if out is None else out
+        if tuple(emb.shape) != (int(c.sum()), 1536) or tuple(out.shape) != tuple(emb.shape):
+            raise ValueError(f"emb and out: [{int(c.sum())}][1536] expected")
+        check(lib().dtts_llm_extend(self.h, kv.h, n, ps, pc, _addr(emb), window, sinks, _addr(out), mem))
+        return out
 
 
 def voc_struct(w: dict):

@@ -438,6 +438,16 @@ int dtts_llm_prefill(dtts_llm *e, const float *emb, int B, int n_tok, float *hid
  * hidden [B][1536]; B must match the prefill. */
 int dtts_llm_step(dtts_llm *e, const float *emb, int B, float *hidden, int mem);
 int dtts_llm_length(dtts_llm *e, int *tokens);
+/* The same decoder over a paged cache (dtts_kv_*), for streams that start, fork and end on their own:
+ * appends n_new[b] >= 0 tokens to each of the n_seq sequences, prompts and steps mixed freely; emb and
+ * hidden are [sum of n_new][1536] in the order of seqs.  Row i of a sequence attends with the window and
+ * sinks of dtts_kv_attend_args; token positions continue from the sequence's position.  K and V are rounded
+ * to bf16 (and then, in a 4-bit cache, to 4 bits), q to bf16.  dtts_llm_kv_create makes a cache of the
+ * engine's geometry for sequences of up to max_seq tokens; the call works on the engine's stream, before which
+ * the work already enqueued on the cache's stream comes, and the cache's stream waits for it. */
+int dtts_llm_kv_create(dtts_llm *e, int n_pages, int max_seqs, int page_tokens, int dtype, dtts_kv **out);
+int dtts_llm_extend(dtts_llm *e, dtts_kv *kv, int n_seq, const int *seqs, const int *n_new, const float *emb,
+                    int window, int sinks, float *hidden, int mem);
 
 /* ------------------------------------------------------------------ vocoder
  * BigVGAN v2 decoder (src/modules/vocoder/bigvgan_cpp.cpp, include/bigvgan_cpp.h): the

@@ -200,3 +200,360 @@ def test_scores_of_any_size(dtype):
     attend_case(dtype, 128, 12, 2, 64, [300, 40], [1, 40], scale=1.0)
     attend_case(dtype, 128, 12, 2, 64, [300, 40], [1, 40], scale=1e-4)
     attend_case(dtype, 64, 4, 4, 32, [200], [1], k_gain=50.0)
+
+
+# ---------------------------------------------------------------- non-finite values
+@pytest.mark.parametrize("dtype", [BF, I4])
+@pytest.mark.parametrize("value", [float("nan"), float("inf")])
+def test_rows_that_a_query_cannot_see_do_not_reach_it(dtype, value):
+    """Non-finite K and V behind the window, between sinks and window, and in later rows of the same prompt."""
+    g = rng(11)
+    for n, t, window, sinks, bad in ((300, 1, 100, 4, [4, 150, 199]), (300, 2, 100, 70, [70, 197]),
+                                     (200, 200, 50, 2, [120]), (150, 150, 0, 0, [149, 77]), (2000, 1, 64, 1, [1, 1900])):
+        kv = make(dtype=dtype, n_pages=40)
+        s = kv.open()
+        k, v, q = rand(g, n, 2, 128), rand(g, n, 2, 128), rand(g, t, 12, 128)
+        for j in bad:
+            k[j, 0, 5], v[j, 1, 40] = value, value
+        fill(kv, [s], [(k[:n - t], v[:n - t])])
+        fill(kv, [s], [(k[n - t:], v[n - t:])])
+        out = torch.empty(t, 12, 128, dtype=torch.bfloat16, device="cuda")
+        kv.attend(0, q.cuda(), out, window=window, sinks=sinks)
+        want, tol = R.attend(q, R.held(k, dtype == I4), R.held(v, dtype == I4), n - t, window, sinks, None, dtype == I4)
+        got = out.cpu()
+        assert torch.equal(torch.isnan(got), torch.isnan(want)), f"{n} rows, {t} new"
+        ok = torch.isfinite(want)
+        R.assert_close(torch.where(ok, got.double(), 0), torch.where(ok, want, 0), torch.where(ok, tol, 1e-30), "finite rows")
+        kv.close()
+
+
+def test_stale_rows_of_a_reused_page_are_not_read():
+    """Pages that held NaN are given to another sequence whose last page they fill only partly."""
+    g = rng(12)
+    for dtype in (BF, I4):
+        kv = make(dtype=dtype, n_pages=3)
+        s = kv.open()
+        fill(kv, [s], [(torch.full((192, 2, 128), float("nan")).bfloat16(),) * 2])
+        kv.close_seqs([s])
+        for n in (1, 65, 130):
+            s = kv.open()
+            k, v, q = rand(g, n, 2, 128), rand(g, n, 2, 128), rand(g, n, 12, 128)
+            fill(kv, [s], [(k, v)])
+            out = torch.empty(n, 12, 128, dtype=torch.bfloat16, device="cuda")
+            kv.attend(0, q.cuda(), out)
+            want, tol = R.attend(q, R.held(k, dtype == I4), R.held(v, dtype == I4), 0, int4=dtype == I4)
+            R.assert_close(out, want, tol, f"{n} rows")
+            kv.close_seqs([s])
+        kv.close()
+
+
+# ---------------------------------------------------------------- pages
+@pytest.mark.parametrize("dtype", [BF, I4])
+def test_forks_share_pages_until_they_grow(dtype):
+    g = rng(13)
+    L, n = 3, 150
+    kv = make(dtype=dtype, layers=L, n_pages=20)
+    s = kv.open()
+    base = [(rand(g, n, 2, 128), rand(g, n, 2, 128)) for _ in range(L)]
+    kv.extend([s], [n])
+    for l in range(L):
+        kv.write(l, base[l][0].cuda(), base[l][1].cuda())
+    forks = kv.fork(s, 3)
+    assert kv.free_pages() == 17 and [kv.length(f) for f in forks] == [n] * 3
+    more = [[(rand(g, 2, 2, 128), rand(g, 2, 2, 128)) for _ in range(L)] for _ in range(4)]
+    kv.extend([s] + forks, [2] * 4)
+    assert kv.free_pages() == 14                       # three copies of the shared last page
+    for l in range(L):
+        kv.write(l, torch.cat([more[b][l][0] for b in range(4)]).cuda(), torch.cat([more[b][l][1] for b in range(4)]).cuda())
+    for b, f in enumerate([s] + forks):
+        k, v = read(kv, f, 0, n + 2, n_layers=L)
+        for l in range(L):
+            assert torch.equal(k[l].double(), R.held(torch.cat([base[l][0], more[b][l][0]]), dtype == I4))
+            assert torch.equal(v[l].double(), R.held(torch.cat([base[l][1], more[b][l][1]]), dtype == I4))
+    kv.close_seqs([s, forks[1]])
+    k, _ = read(kv, forks[0], 0, n, n_layers=L)        # the shared pages outlive the sequence they came from
+    assert torch.equal(k[2].double(), R.held(base[2][0], dtype == I4))
+    (again,) = kv.fork(forks[2])
+    kv.truncate(again, 128)                            # at a page border: growing needs no copy
+    free = kv.free_pages()
+    kv.extend([again], [1])
+    assert kv.free_pages() == free - 1
+    kv.close_seqs([forks[0], forks[2], again])
+    assert kv.free_pages() == 20
+    kv.close()
+
+
+def test_fork_of_an_empty_sequence_and_many_forks():
+    kv = make(n_pages=600, max_seqs=1200, max_tokens=64, page=16)
+    s = kv.open()
+    assert kv.fork(s, 0) == []
+    f = kv.fork(s, 1000)
+    kv.extend(f[:500], [3] * 500)
+    g = rng(14)
+    k, v = rand(g, 1500, 2, 128), rand(g, 1500, 2, 128)
+    kv.write(0, k.cuda(), v.cuda())
+    ko = torch.empty(1, 1500, 2, 128, device="cuda")
+    vo = torch.empty_like(ko)
+    kv.read(0, f[:500], [0] * 500, [3] * 500, ko, vo)
+    assert torch.equal(ko[0].cpu().double(), R.held(k, True)) and torch.equal(vo[0].cpu().double(), R.held(v, True))
+    kv.close_seqs(f)
+    assert kv.free_pages() == 600
+    kv.close()
+
+
+@pytest.mark.parametrize("dtype", [BF, I4])
+@pytest.mark.parametrize("D,page", [(128, 64), (64, 16), (128, 16), (64, 128)])
+def test_compact_keeps_the_listed_rows(dtype, D, page):
+    g = rng(15)
+    L, n = 2, 333
+    kv = make(H=3, D=D, page=page, dtype=dtype, layers=L, n_pages=80)
+    s = kv.open()
+    k, v = rand(g, L, n, 3, D), rand(g, L, n, 3, D)
+    kv.extend([s], [n])
+    for l in range(L):
+        kv.write(l, k[l].cuda(), v[l].cuda())
+    for keep in (list(range(n)), list(range(200)) + list(range(230, n)), [0, 1, 2] + list(range(50, 333, 2)),
+                 list(range(7, 19)), [332], []):
+        (f,) = kv.fork(s)
+        kv.compact(f, keep)
+        assert kv.length(f) == len(keep) and kv.position(f) == n
+        if keep:
+            gk, gv = read(kv, f, 0, len(keep), n_layers=L)
+            assert torch.equal(gk.double(), R.held(k[:, keep], dtype == I4))
+            assert torch.equal(gv.double(), R.held(v[:, keep], dtype == I4))
+        kv.extend([f], [1])                            # grows without touching the rows of the source
+        kv.write(0, torch.zeros(1, 3, D, dtype=torch.bfloat16, device="cuda"), torch.zeros(1, 3, D, dtype=torch.bfloat16, device="cuda"))
+        gk, _ = read(kv, s, 0, n, n_layers=L)
+        assert torch.equal(gk.double(), R.held(k, dtype == I4))
+        kv.close_seqs([f])
+    kv.close()
+
+
+@pytest.mark.parametrize("dtype", [BF, I4])
+def test_trim_frees_what_no_query_sees(dtype):
+    g = rng(16)
+    window, sinks, n = 100, 20, 400
+    kv = make(dtype=dtype, page=32, n_pages=20)
+    s = kv.open()
+    k, v = rand(g, n + 30, 2, 128), rand(g, n + 30, 2, 128)
+    fill(kv, [s], [(k[:n], v[:n])])
+    before = kv.free_pages()
+    kv.trim(s, window, sinks)
+    # the next token, row 400, sees rows 0..19 and 301..; whole pages in between: rows 32..287, 8 pages
+    assert kv.free_pages() == before + 8
+    fill(kv, [s], [(k[n:n + 1], v[n:n + 1])])
+    q = rand(g, 30, 12, 128)
+    out = torch.empty(1, 12, 128, dtype=torch.bfloat16, device="cuda")
+    kv.attend(0, q[:1].cuda(), out, window=window, sinks=sinks)
+    held = [R.held(x, dtype == I4) for x in (k, v)]
+    want, tol = R.attend(q[:1], held[0][:n + 1], held[1][:n + 1], n, window, sinks, int4=dtype == I4)
+    R.assert_close(out, want, tol, "step")
+    for bad in (dict(window=0), dict(window=200, sinks=20), dict(window=100, sinks=33)):
+        with pytest.raises(dtts.DttsError) as e:
+            kv.attend(0, q[:1].cuda(), out, **bad)
+        assert e.value.status == dtts.ERR_ARG
+    kv.attend(0, q[:1].cuda(), out, window=113, sinks=32)     # rows 288 .. 400 and 0 .. 31 are there
+    with pytest.raises(dtts.DttsError):
+        kv.attend(0, q[:1].cuda(), out, window=114)
+    with pytest.raises(dtts.DttsError):
+        read(kv, s, 31, 2)
+    with pytest.raises(dtts.DttsError):
+        kv.compact(s, [0, 32])
+    with pytest.raises(dtts.DttsError):
+        kv.truncate(s, 100)
+    kv.truncate(s, 390)
+    kv.truncate(s, 300)
+    kv.truncate(s, 32)
+    fill(kv, [s], [(k[32:40], v[32:40])])
+    kv.attend(0, q[:8].cuda(), torch.empty(8, 12, 128, dtype=torch.bfloat16, device="cuda"))   # nothing freed is left
+    gk, _ = read(kv, s, 0, 40)
+    assert torch.equal(gk[0].double(), held[0][:40])
+    kv.close()
+
+
+def test_refusals():
+    kv = make(n_pages=4, max_seqs=3, max_tokens=300)
+    s = kv.open()
+    x = torch.zeros(8, 2, 128, dtype=torch.bfloat16, device="cuda")
+    q = torch.zeros(8, 12, 128, dtype=torch.bfloat16, device="cuda")
+
+    def refused(status, f, *a, **k):
+        with pytest.raises(dtts.DttsError) as e:
+            f(*a, **k)
+        assert e.value.status == status, e.value
+
+    refused(dtts.ERR_ARG, kv.write, 0, x, x)                       # no batch
+    refused(dtts.ERR_ARG, kv.attend, 0, q, q)
+    refused(dtts.ERR_OOM, kv.extend, [s], [257])
+    refused(dtts.ERR_ARG, kv.extend, [s], [301])
+    refused(dtts.ERR_ARG, kv.extend, [s], [-1])
+    refused(dtts.ERR_ARG, kv.extend, [s, s], [1, 1])
+    refused(dtts.ERR_ARG, kv.extend, [s, 2], [1, 1])
+    refused(dtts.ERR_ARG, kv.extend, [], [])
+    for bad in (-1, 3, 1 << 30):
+        refused(dtts.ERR_ARG, kv.extend, [bad], [1])
+        refused(dtts.ERR_ARG, kv.close_seqs, [bad])
+        refused(dtts.ERR_ARG, kv.fork, bad)
+        refused(dtts.ERR_ARG, kv.truncate, bad, 0)
+        refused(dtts.ERR_ARG, kv.trim, bad, 1)
+        refused(dtts.ERR_ARG, kv.compact, bad, [])
+        refused(dtts.ERR_ARG, kv.length, bad)
+    assert kv.length(s) == 0 and kv.free_pages() == 4
+    kv.extend([s], [8])
+    for layer in (-1, 1):
+        refused(dtts.ERR_ARG, kv.write, layer, x, x)
+        refused(dtts.ERR_ARG, kv.attend, layer, q, q)
+    refused(dtts.ERR_ARG, kv.write, 0, x.flatten()[1:1 + 7 * 256].view(7, 2, 128), x)      # off a 16-byte boundary
+    refused(dtts.ERR_ARG, kv.write, 0, torch.zeros(8, 2, 130, dtype=torch.bfloat16, device="cuda")[..., :128], x)
+    refused(dtts.ERR_ARG, kv.attend, 0, q[:, :11], q[:, :11])
+    refused(dtts.ERR_ARG, kv.attend, 0, q, q, window=-1)
+    refused(dtts.ERR_ARG, kv.attend, 0, q, q, sinks=-1)
+    for scale in (0.0, -1.0, float("nan"), float("inf"), 1e31):
+        refused(dtts.ERR_ARG, kv.attend, 0, q, q, scale=scale)
+    f32 = torch.zeros(1, 9, 2, 128, device="cuda")
+    refused(dtts.ERR_ARG, kv.read, 0, [s], [0], [9], f32, f32.clone())
+    refused(dtts.ERR_ARG, kv.read, 0, [s], [-1], [9], f32, f32.clone())
+    refused(dtts.ERR_ARG, kv.read, 1, [s], [0], [9], f32, f32.clone())
+    refused(dtts.ERR_ARG, kv.compact, s, [1, 1])
+    refused(dtts.ERR_ARG, kv.compact, s, [2, 1])
+    refused(dtts.ERR_ARG, kv.compact, s, [7, 8])
+    refused(dtts.ERR_ARG, kv.truncate, s, 9)
+    refused(dtts.ERR_ARG, kv.trim, s, 0)
+    refused(dtts.ERR_ARG, kv.close_seqs, [s, s])
+    refused(dtts.ERR_OOM, kv.fork, s, 3)
+    (f,) = kv.fork(s)
+    kv.extend([s], [1])                                            # copies the shared page
+    kv.extend([f], [184])                                          # the pool is full now
+    refused(dtts.ERR_OOM, kv.extend, [s], [64])
+    refused(dtts.ERR_OOM, kv.compact, f, list(range(1, 192)))
+    assert kv.length(s) == 9 and kv.length(f) == 192
+    kv.close_seqs([f])
+    refused(dtts.ERR_ARG, kv.write, 0, x, x)                       # its batch ended with it
+    kv.close()
+    big = dtts.KVConfig(1 << 10, 32, 128, 128, 1 << 20, 4, 128, I4)   # petabytes
+    import ctypes as C
+    h = C.c_void_p()
+    assert dtts.lib().dtts_kv_create(C.byref(big), 0, C.byref(h)) == dtts.ERR_OOM and not h.value
+    make().close()                                                 # and the next one works
+
+
+# ---------------------------------------------------------------- streams and graphs
+def test_captured_step_follows_the_sequences():
+    """write + attend captured once; replays act on the batch that is current, across page borders and after a
+    sequence was replaced."""
+    g = rng(17)
+    for dtype in (BF, I4):
+        kv = make(dtype=dtype, n_pages=40)
+        a, b = kv.open(), kv.open()
+        ka, va = rand(g, 230, 2, 128), rand(g, 230, 2, 128)
+        kb, vb = rand(g, 230, 2, 128), rand(g, 230, 2, 128)
+        fill(kv, [a, b], [(ka[:60], va[:60]), (kb[:190], vb[:190])])
+        kn = torch.zeros(2, 2, 128, dtype=torch.bfloat16, device="cuda")
+        vn, q, out = torch.zeros_like(kn), torch.zeros(2, 12, 128, dtype=torch.bfloat16, device="cuda"), torch.zeros(2, 12, 128, dtype=torch.bfloat16, device="cuda")
+        kv.extend([a, b], [1, 1])
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=torch.cuda.current_stream()):
+            kv.write(0, kn, vn)
+            kv.attend(0, q, out, window=150, sinks=2)
+            with pytest.raises(dtts.DttsError) as e:
+                kv.extend([a, b], [1, 1])
+            assert e.value.status == dtts.ERR_UNSUPPORTED
+            with pytest.raises(dtts.DttsError):
+                kv.fork(a)
+            with pytest.raises(dtts.DttsError):
+                kv.compact(a, [0])
+        la, lb, cb = 60, 190, b
+        for i in range(12):
+            if i:
+                if i == 6:
+                    kv.close_seqs([cb])
+                    cb, lb = kv.open(), 3
+                    fill(kv, [cb], [(kb[:3], vb[:3])])
+                kv.extend([a, cb], [1, 1])
+            kn.copy_(torch.stack([ka[la], kb[lb]]))
+            vn.copy_(torch.stack([va[la], vb[lb]]))
+            qq = rand(g, 2, 12, 128)
+            q.copy_(qq)
+            graph.replay()
+            la, lb = la + 1, lb + 1
+            for row, k, v, n in ((0, ka, va, la), (1, kb, vb, lb)):
+                want, tol = R.attend(qq[row:row + 1], R.held(k[:n], dtype == I4), R.held(v[:n], dtype == I4), n - 1, 150, 2)
+                R.assert_close(out[row:row + 1], want, tol, f"replay {i}, row {row}")
+        del graph
+        kv.close()
+
+
+def test_work_moves_to_another_stream_in_order():
+    g = rng(18)
+    kv = make(dtype=I4, n_pages=300, max_tokens=16384)
+    s = kv.open()
+    n = 12000
+    k, v, q = rand(g, n, 2, 128).cuda(), rand(g, n, 2, 128).cuda(), rand(g, 4, 12, 128).cuda()
+    out = torch.empty_like(q)
+    torch.cuda.synchronize()
+    other = torch.cuda.Stream()
+    for i in range(3):
+        kv.extend([s], [n if i == 0 else 0])
+        if i == 0:
+            kv.write(0, k, v)
+        kv.set_stream(other.cuda_stream if i % 2 == 0 else torch.cuda.current_stream().cuda_stream)
+        (f,) = kv.fork(s)
+        kv.compact(f, list(range(0, n, 2)))
+        kv.extend([f], [1])
+        kv.write(0, k[:1], v[:1])
+        kv.set_stream(None)
+        gk = torch.empty(1, 6001, 2, 128, device="cuda")
+        gv = torch.empty_like(gk)
+        torch.cuda.synchronize()
+        kv.read(0, [f], [0], [6001], gk, gv)
+        kv.sync()
+        assert torch.equal(gk[0].cpu().double(), R.held(torch.cat([k[::2], k[:1]]).cpu(), True))
+        kv.close_seqs([f])
+    kv.set_stream(1)                       # the legacy default stream
+    kv.extend([s], [0])
+    kv.attend(0, q, out)                   # no rows: nothing to do
+    kv.close()
+
+
+def test_strided_queries_and_outputs():
+    g = rng(19)
+    for t in (1, 30):
+        kv = make(dtype=I4)
+        s = kv.open()
+        k, v = rand(g, 100, 2, 128), rand(g, 100, 2, 128)
+        fill(kv, [s], [(k[:100 - t], v[:100 - t])])
+        fill(kv, [s], [(k[100 - t:], v[100 - t:])])
+        qkv = rand(g, t, 16, 128).cuda()
+        out = torch.full((12, t, 136), 5.0, dtype=torch.bfloat16, device="cuda")
+        kv.attend(0, qkv[:, :12], out[:, :, :128].transpose(0, 1))
+        want, tol = R.attend(qkv[:, :12].cpu(), R.held(k, True), R.held(v, True), 100 - t)
+        R.assert_close(out[:, :, :128].transpose(0, 1), want, tol)
+        assert (out[:, :, 128:] == 5).all()
+        kv.close()
+
+
+def test_pool_beyond_32_bits():
+    """Pages past 4 GiB of the pool: the first 2000 of 2100 pages of 2.6 MB are taken."""
+    g = rng(20)
+    L, n = 40, 130
+    kv = make(dtype=BF, layers=L, n_pages=2100, max_tokens=64 * 2000)
+    kv.extend([kv.open()], [64 * 2000])
+    s = kv.open()
+    k, v, q = rand(g, n, 2, 128), rand(g, n, 2, 128), rand(g, n, 12, 128)
+    for l in (0, L - 1):
+        for t in (n, 1):
+            kv.truncate(s, 0)
+            kv.extend([s], [n - t])
+            kv.write(l, k[:n - t].cuda(), v[:n - t].cuda())
+            kv.extend([s], [t])
+            kv.write(l, k[n - t:].cuda(), v[n - t:].cuda())
+            out = torch.empty(t, 12, 128, dtype=torch.bfloat16, device="cuda")
+            kv.attend(l, q[:t].cuda(), out)
+            want, tol = R.attend(q[:t], k.double(), v.double(), n - t, int4=False)
+            R.assert_close(out, want, tol, f"layer {l}, {t} new")
+    (f,) = kv.fork(s)
+    kv.extend([f], [1])
+    kv.compact(f, list(range(5, n)))
+    got, _ = read(kv, f, 0, n - 5, layer=L - 1)
+    assert torch.equal(got[0].double(), k[5:].double())
+    kv.close()

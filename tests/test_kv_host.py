@@ -1,0 +1,68 @@
+"""Host-side checks of the paged K/V cache that need no GPU: refusals before any device is touched, and the
+definition of 4-bit rows the GPU tests rely on."""
+import ctypes as C
+
+import pytest
+import torch
+
+import dtts
+import kv_ref as R
+
+
+def _config(**change):
+    c = dict(n_layers=2, n_kv_heads=2, head_dim=128, page_tokens=64, n_pages=8, max_seqs=2, max_tokens=256,
+             dtype=dtts.DTYPE_INT4)
+    c.update(change)
+    return dtts.KVConfig(*[c[n] for n, _ in dtts.KVConfig._fields_])
+
+
+@pytest.mark.parametrize("change,status", [
+    (dict(dtype=dtts.DTYPE_FP8), dtts.ERR_UNSUPPORTED), (dict(dtype=dtts.DTYPE_F32), dtts.ERR_UNSUPPORTED),
+    (dict(dtype=9), dtts.ERR_UNSUPPORTED), (dict(head_dim=96), dtts.ERR_UNSUPPORTED), (dict(head_dim=0), dtts.ERR_UNSUPPORTED),
+    (dict(page_tokens=8), dtts.ERR_UNSUPPORTED), (dict(page_tokens=48), dtts.ERR_UNSUPPORTED),
+    (dict(page_tokens=256), dtts.ERR_UNSUPPORTED), (dict(n_layers=0), dtts.ERR_ARG), (dict(n_layers=-1), dtts.ERR_ARG),
+    (dict(n_kv_heads=0), dtts.ERR_ARG), (dict(n_layers=1000, n_kv_heads=100), dtts.ERR_ARG), (dict(n_pages=0), dtts.ERR_ARG),
+    (dict(max_seqs=0), dtts.ERR_ARG), (dict(max_seqs=65536), dtts.ERR_ARG), (dict(max_tokens=0), dtts.ERR_ARG),
+    (dict(max_tokens=(1 << 24) + 1), dtts.ERR_ARG), (dict(max_seqs=60000, max_tokens=1 << 24, page_tokens=16), dtts.ERR_ARG)])
+def test_bad_configurations_are_refused(dtts_mod, change, status):
+    h = C.c_void_p(5)
+    assert dtts.lib().dtts_kv_create(C.byref(_config(**change)), 0, C.byref(h)) == status
+    assert not h.value and dtts.lib().dtts_last_error()
+
+
+def test_null_arguments_are_refused(dtts_mod):
+    L = dtts.lib()
+    n = C.c_int()
+    h = C.c_void_p()
+    assert L.dtts_kv_create(None, 0, C.byref(h)) == dtts.ERR_ARG
+    assert L.dtts_kv_create(C.byref(_config()), 0, None) == dtts.ERR_ARG
+    assert L.dtts_kv_destroy(None) == dtts.OK
+    calls = [L.dtts_kv_set_stream(None, None), L.dtts_kv_sync(None), L.dtts_kv_open(None, C.byref(n)),
+             L.dtts_kv_close(None, 0, None), L.dtts_kv_fork(None, 0, 0, None), L.dtts_kv_truncate(None, 0, 0),
+             L.dtts_kv_trim(None, 0, 1, 0), L.dtts_kv_compact(None, 0, 0, None), L.dtts_kv_length(None, 0, None, None),
+             L.dtts_kv_free_pages(None, C.byref(n)), L.dtts_kv_extend(None, 1, None, None),
+             L.dtts_kv_write(None, 0, None, None, 0, 0, 0, 0), L.dtts_kv_attend(None, 0, None),
+             L.dtts_kv_read(None, 0, 1, 0, None, None, None, None, None, dtts.DTYPE_F32),
+             L.dtts_llm_kv_create(None, 1, 1, 64, dtts.DTYPE_BF16, C.byref(h)),
+             L.dtts_llm_extend(None, None, 1, None, None, None, 0, 0, None, dtts.MEM_HOST)]
+    assert calls == [dtts.ERR_ARG] * len(calls)
+
+
+def test_no_device_is_an_error(dtts_mod):
+    if dtts_mod.device_count() > 0:
+        pytest.skip("a device is visible here")
+    h = C.c_void_p()
+    assert dtts.lib().dtts_kv_create(C.byref(_config()), 0, C.byref(h)) == dtts.ERR_NO_DEVICE and not h.value
+
+
+def test_four_bit_rows_are_within_half_a_step():
+    g = torch.Generator()
+    g.manual_seed(1)
+    x = (torch.randn(64, 3, 128, generator=g) * torch.logspace(-3, 3, 64)[:, None, None]).bfloat16()
+    c, s = R.codes(x)
+    assert c.abs().max() == 7 and torch.equal(s.to(torch.float16).double(), s)
+    err = (R.held(x, True) - x.double()).reshape(64, 3, 4, 32).abs()
+    # half a step, and where bf16(max / 7) was rounded down the largest value is clamped: 7 * 2^-8 of a step more
+    assert (err <= s * (0.5 + 7 * 2.0 ** -8)).all()
+    # every value is exact in half
+    assert torch.equal(R.held(x, True).to(torch.float16).double(), R.held(x, True))
