@@ -1,10 +1,11 @@
 // The paged K/V cache: page layout, device metadata and the row codec shared by
 // its kernels (kv_cache.cu: rows and pages; kv_attend.cu: attention).
 //
-// Pool: [page][layer][kv head] segments; a segment holds P token rows as
-//   K rows [P][RB] | V rows [P][RB] | K scales [P][SB] | V scales [P][SB]
+// Pool: [page][layer][kv head] segments; a segment holds P token rows (16, 32, 64
+// or 128) in blocks of 16 rows, each
+//   K rows [16][RB] | V rows [16][RB] | K scales [16][SB] | V scales [16][SB]
 // with RB = 2 D bytes (bf16) or D / 2 (int4), SB = 0 or D / 16 (one half per 32
-// values).  All parts are multiples of 16 bytes (P is 16, 32, 64 or 128).
+// values).  So any run of whole blocks of a page is one contiguous copy.
 //
 // Row codec, int4: for every 32 consecutive values x (bf16) of a row
 //   s = clamp(bf16(max|x| / 7), 2^-14, 9344),  c = clamp(rint(x / s), -7, 7),
@@ -47,6 +48,14 @@ struct KvMeta {
 
 __host__ __device__ inline long long kv_seg_off(const KvGeom &g, int page, int layer, int head) {
     return (long long)page * g.page_stride + ((long long)layer * g.H + head) * g.seg;
+}
+
+// byte offset of row r and of its scales within a segment
+__host__ __device__ inline int kv_row_off(const KvGeom &g, bool is_v, int r) {
+    return (r >> 4) * 32 * (g.RB + g.SB) + (is_v ? 16 * g.RB : 0) + (r & 15) * g.RB;
+}
+__host__ __device__ inline int kv_scale_off(const KvGeom &g, bool is_v, int r) {
+    return (r >> 4) * 32 * (g.RB + g.SB) + 32 * g.RB + (is_v ? 16 * g.SB : 0) + (r & 15) * g.SB;
 }
 
 // XOR of the 16-byte unit index inside row r (r: row within the page or tile)
@@ -106,15 +115,15 @@ DTTS_DEV float kv_nibble(uint32_t w, int i) { return (float)((int)((w >> (4 * i)
 // dims 8 w .. 8 w + 7 of row r of a segment (r within the page), as floats
 DTTS_DEV void kv_load8(const KvGeom &g, const uint8_t *seg, bool is_v, int r, int w, float (&x)[8]) {
     if (g.i4) {
-        const uint8_t *row = seg + (is_v ? g.P * g.RB : 0) + r * g.RB;
+        const uint8_t *row = seg + kv_row_off(g, is_v, r);
         const uint32_t q = *reinterpret_cast<const uint32_t *>(row + (is_v ? kv_word_v(g.D, w, r) : kv_word_k(g.D, w)));
         const float s = __half2float(*reinterpret_cast<const __half *>(
-            seg + 2 * g.P * g.RB + (is_v ? g.P * g.SB : 0) + r * g.SB + (w >> 2) * 2));
+            seg + kv_scale_off(g, is_v, r) + (w >> 2) * 2));
 #pragma unroll
         for (int i = 0; i < 8; i++) x[i] = kv_nibble(q, i) * s;
     } else {
         const int u = w ^ (is_v ? kv_swz_v(false, g.D, r) : kv_swz_k(false, r));
-        const uint4 q = *reinterpret_cast<const uint4 *>(seg + (is_v ? g.P * g.RB : 0) + r * g.RB + u * 16);
+        const uint4 q = *reinterpret_cast<const uint4 *>(seg + kv_row_off(g, is_v, r) + u * 16);
         const uint32_t e[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
         for (int i = 0; i < 4; i++) {
@@ -138,13 +147,13 @@ DTTS_DEV void kv_store8(const KvGeom &g, uint8_t *seg, bool is_v, int r, int w, 
         __half s;
         const uint32_t c = kv_encode8(x, &s);
         if (!on) return;
-        uint8_t *row = seg + (is_v ? g.P * g.RB : 0) + r * g.RB;
+        uint8_t *row = seg + kv_row_off(g, is_v, r);
         *reinterpret_cast<uint32_t *>(row + (is_v ? kv_word_v(g.D, w, r) : kv_word_k(g.D, w))) = c;
         if ((w & 3) == 0)
-            *reinterpret_cast<__half *>(seg + 2 * g.P * g.RB + (is_v ? g.P * g.SB : 0) + r * g.SB + (w >> 2) * 2) = s;
+            *reinterpret_cast<__half *>(seg + kv_scale_off(g, is_v, r) + (w >> 2) * 2) = s;
     } else if (on) {
         const int u = w ^ (is_v ? kv_swz_v(false, g.D, r) : kv_swz_k(false, r));
-        *reinterpret_cast<uint4 *>(seg + (is_v ? g.P * g.RB : 0) + r * g.RB + u * 16) = q;
+        *reinterpret_cast<uint4 *>(seg + kv_row_off(g, is_v, r) + u * 16) = q;
     }
 }
 

@@ -31,14 +31,14 @@ struct KeyTiles {
 DTTS_DEV float kv_elem(const KvGeom &g, const uint8_t *seg, bool is_v, int r, int d) {
     if (g.i4) {
         const int w = d >> 3;
-        const uint8_t *row = seg + (is_v ? g.P * g.RB : 0) + r * g.RB;
+        const uint8_t *row = seg + kv_row_off(g, is_v, r);
         const uint32_t q = *reinterpret_cast<const uint32_t *>(row + (is_v ? kv_word_v(g.D, w, r) : kv_word_k(g.D, w)));
         const float s = __half2float(*reinterpret_cast<const __half *>(
-            seg + 2 * g.P * g.RB + (is_v ? g.P * g.SB : 0) + r * g.SB + (d >> 5) * 2));
+            seg + kv_scale_off(g, is_v, r) + (d >> 5) * 2));
         return kv_nibble(q, d & 7) * s;
     }
     const int u = (d >> 3) ^ (is_v ? kv_swz_v(false, g.D, r) : kv_swz_k(false, r));
-    return __bfloat162float(*reinterpret_cast<const bf16 *>(seg + (is_v ? g.P * g.RB : 0) + r * g.RB + u * 16 + (d & 7) * 2));
+    return __bfloat162float(*reinterpret_cast<const bf16 *>(seg + kv_row_off(g, is_v, r) + u * 16 + (d & 7) * 2));
 }
 
 // One query row against key tiles [v0, v1) by one warp in plain arithmetic: only
@@ -125,6 +125,9 @@ DTTS_DEV bool kv_last_part(int *cnt, int parts, int *flag) {
 }
 
 // ---------------------------------------------------------------- few rows
+DTTS_DEV void mbar_expect_tx(uint64_t *bar, uint32_t bytes) {
+    asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes) : "memory");
+}
 DTTS_DEV uint32_t movmatrix_t(uint32_t x) {
     uint32_t y;
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
@@ -141,18 +144,48 @@ DTTS_DEV void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uin
                      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+// as mma16816<true>, the accumulators starting at c0, c1 (both rows)
+DTTS_DEV void mma16816_from(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1,
+                            float c0, float c1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%10,%11};"
+                 : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c0), "f"(c1));
+}
 DTTS_DEV uint32_t h2_bits(__half2 h) { return *reinterpret_cast<uint32_t *>(&h); }
 DTTS_DEV __half2 bits_h2(uint32_t u) { return *reinterpret_cast<__half2 *>(&u); }
 
-// Nibbles (0, 4), (1, 5), (2, 6), (3, 7) of w as half pairs c - 8: OR with the
-// bits of 1024 gives 1024 + c exactly (c in bits 0-3) or 1024 + 16 c (bits 4-7).
-DTTS_DEV void unpack_nibbles(uint32_t w, __half2 (&h)[4]) {
-    const __half2 k1032 = __float2half2_rn(1032.f), k72 = __float2half2_rn(-72.f), sixteenth = __float2half2_rn(0.0625f);
+// (w & mask) | magic in one instruction; both constants stay in registers
+DTTS_DEV uint32_t and_or(uint32_t w, uint32_t mask, uint32_t magic) {
+    uint32_t y;
+    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(y) : "r"(w), "r"(mask), "r"(magic));
+    return y;
+}
+struct NibbleMasks {
+    uint32_t lo, hi, magic;
+    DTTS_DEV NibbleMasks() {
+        // volatile: as constants they would be folded into two instructions a use
+        asm volatile("mov.b32 %0, 0x000f000f;" : "=r"(lo));
+        asm volatile("mov.b32 %0, 0x00f000f0;" : "=r"(hi));
+        asm volatile("mov.b32 %0, 0x64006400;" : "=r"(magic));
+    }
+};
+// Nibbles (0, 4), (1, 5), (2, 6), (3, 7) of w as half pairs: OR with the bits of
+// 1024 gives 1024 + n exactly (n in bits 0-3) or 1024 + 16 n (bits 4-7).
+// unpack_raw: n - 8 in pairs 0 and 2, 1024 + 16 n in pairs 1 and 3;
+// unpack_nibbles: n - 8 in all.
+DTTS_DEV void unpack_raw(uint32_t w, const NibbleMasks &k, __half2 (&h)[4]) {
+    const __half2 k1032 = __float2half2_rn(1032.f);
     const uint32_t x = w >> 8;
-    h[0] = __hsub2(bits_h2((w & 0x000f000fu) | 0x64006400u), k1032);
-    h[1] = __hfma2(bits_h2((w & 0x00f000f0u) | 0x64006400u), sixteenth, k72);
-    h[2] = __hsub2(bits_h2((x & 0x000f000fu) | 0x64006400u), k1032);
-    h[3] = __hfma2(bits_h2((x & 0x00f000f0u) | 0x64006400u), sixteenth, k72);
+    h[0] = __hsub2(bits_h2(and_or(w, k.lo, k.magic)), k1032);
+    h[1] = bits_h2(and_or(w, k.hi, k.magic));
+    h[2] = __hsub2(bits_h2(and_or(x, k.lo, k.magic)), k1032);
+    h[3] = bits_h2(and_or(x, k.hi, k.magic));
+}
+DTTS_DEV void unpack_nibbles(uint32_t w, const NibbleMasks &k, __half2 (&h)[4]) {
+    const __half2 k72 = __float2half2_rn(-72.f), sixteenth = __float2half2_rn(0.0625f);
+    unpack_raw(w, k, h);
+    h[1] = __hfma2(h[1], sixteenth, k72);
+    h[3] = __hfma2(h[3], sixteenth, k72);
 }
 
 // Row of a 16-row block that row k of a fragment stands for: adjacent k have rows
@@ -161,29 +194,36 @@ __host__ __device__ constexpr int frag_row(int k) { return (k & 8) | ((k & 7) < 
 
 template <int D, bool I4>
 struct FewCfg {
-    static constexpr int kWarps = 4, kThreads = kWarps * 32;
-    static constexpr int KT = I4 ? 64 : (D == 64 ? 32 : 16);   // keys a tile
+    static constexpr int kWarps = I4 ? 8 : 4, kThreads = kWarps * 32;
+    static constexpr int KT = I4 || D == 64 ? 32 : 16;         // keys a tile
     static constexpr int RB = I4 ? D / 2 : 2 * D, SB = I4 ? D / 16 : 0;
-    static constexpr int kStage = KT * 2 * (RB + SB);
-    static constexpr int kStages = I4 ? (D == 128 ? 2 : 4) : 3;
+    static constexpr int kBlock = 32 * (RB + SB);              // 16 rows of K and V with their scales
+    static constexpr int kStage = KT / 16 * kBlock;
+    static constexpr int kStages = 3;
     static constexpr int kRing = kWarps * kStages * kStage;
     static constexpr int kMerge = kWarps * kKvFewRows * (D + 2) * 4;   // the warps' results, over the rings
     static constexpr int kSmem = (kRing > kMerge ? kRing : kMerge) + kWarps * kStages * 8 + 16;
 };
 
 // Attention of at most 8 NT rows (new tokens x query heads of one kv head) of one
-// sequence.  Each warp takes every fourth key tile of the CTA's part: bulk copies
-// bring a tile's pages into the warp's own ring while earlier tiles are computed,
-// so DRAM latency is covered without registers.  Products are m16n8k16 with the
-// keys (S^T = K Q^T) and then the dims (O^T = V^T P^T) as the 16-row side: a
-// group of up to 8 query rows costs one column block, and K and V bytes become
-// fragments in registers.  P^T comes from S^T by an in-register 8 x 8 transpose.
-// int4: K enters as the integers c with the group's scale applied to the fp32
-// partial sums, V as the exact half values c s; Q as half after an exact scaling
-// by a power of two.  P is half (2^-12 relative, against 2^-9 of the bf16
-// output); with bf16 rows P is split into two bf16 terms (2^-17).
+// sequence.  Each warp takes every kWarps-th key tile of the CTA's part: bulk
+// copies bring a tile's pages into the warp's own ring while earlier tiles are
+// computed, so DRAM latency is covered without registers.  Products are m16n8k16
+// with the keys (S^T = K Q^T) and then the dims (O^T = V^T P^T) as the 16-row
+// side: a group of up to 8 query rows costs one column block, and K and V bytes
+// become fragments in registers.  P^T comes from S^T by an in-register 8 x 8
+// transpose.
+// int4: K enters as its integers with the group's scale applied to the fp32
+// partial sums.  Pairs 1 and 3 of a word enter as 64 + n (1024 + 16 n against q /
+// 16), and the products' accumulators start at -72 sum of those q: the products
+// are exact and a group's sums stay within 80 s sum |q|.  V enters as the exact half
+// values c s; Q as half after an exact scaling by a power of two.  P is half (2^-12
+// relative, against 2^-9 of the bf16 output); with bf16 rows P is split into two
+// bf16 terms (2^-17).
+// The running maximum m of a column is raised only when a score passes it by 2^8
+// (P <= 2^8 is as exact as P <= 1), so most tiles need no exchange between lanes.
 template <int D, bool I4, int NT>
-__global__ void __launch_bounds__(128) kv_attend_few_kernel(const __grid_constant__ KvAttendArgs a) {
+__global__ void __launch_bounds__(FewCfg<D, I4>::kThreads, NT == 1 ? 2 : 1) kv_attend_few_kernel(const __grid_constant__ KvAttendArgs a) {
     using C = FewCfg<D, I4>;
     constexpr int KT = C::KT, NK = KT / 16, MI = D / 16, NG = D / 32;
     extern __shared__ __align__(128) uint8_t smem[];
@@ -204,11 +244,11 @@ __global__ void __launch_bounds__(128) kv_attend_few_kernel(const __grid_constan
     const int split = blockIdx.x % a.splits, unit = blockIdx.x / a.splits;
     const int b = unit / a.g.H, head = unit % a.g.H;
     const int cnt = a.m.cnt[b], len = a.m.len[b], row0 = a.m.start[b], G = a.G;
+    const int *trow = a.m.table + (long long)a.m.seq[b] * a.g.max_pages;
     const long long rows_ll = (long long)cnt * G;
     if (rows_ll < 1 || rows_ll > kKvFewRows) return;   // none, or the other kernel's
     const int rows = min((int)rows_ll, 8 * NT);
     if ((long long)row0 + cnt > a.total_rows) return;
-    const int *trow = a.m.table + (long long)a.m.seq[b] * a.g.max_pages;
     const int i0 = len - cnt;
     const KeyTiles kt(KT, i0, len, a.window, a.sinks);
     const int parts = min(a.splits, max(1, (kt.n + a.tiles_per_split - 1) / a.tiles_per_split));
@@ -217,42 +257,48 @@ __global__ void __launch_bounds__(128) kv_attend_few_kernel(const __grid_constan
 
     uint8_t *ring = smem + warp * C::kStages * C::kStage;
     uint64_t *bar = bars + warp * C::kStages;
-    const int P = a.g.P, chunk = min(P, KT);
-    // lane = 4 chunk + part copies one part (K, V, their scales) of one page's rows
-    auto issue = [&](int v, int stage) {
-        const int j0 = kt.tile(v) * KT;
-        uint32_t bytes = 0, dst = 0;
-        const uint8_t *src = nullptr;
-        const int c = lane >> 2, part = lane & 3, j = j0 + c * chunk;
-        if (c * chunk < KT && j < len && (I4 || part < 2)) {
-            const int last = min(len, j + chunk) - 1;
-            // a chunk that lies wholly between the sinks and the first query's window stays out
-            const bool seen = a.window == 0 || last > i0 - a.window || j < a.sinks;
-            const int page = trow[j >> a.g.lgP];
-            if (seen && page >= 0 && page < a.g.n_pages) {
-                const int n = (last - j + 16) & ~15;   // rows, whole 16-row blocks
-                const int r = j & (P - 1), rb = part < 2 ? C::RB : C::SB;
-                const long long off = (part < 2 ? (long long)part * P * C::RB
-                                                : 2ll * P * C::RB + (long long)(part - 2) * P * C::SB) + (long long)r * rb;
-                bytes = n * rb;
-                src = a.pool + kv_seg_off(a.g, page, 0, head) + off;
-                dst = (part < 2 ? part * KT * C::RB : 2 * KT * C::RB + (part - 2) * KT * C::SB) + c * chunk * rb;
-            }
-        }
-        const uint32_t total = __reduce_add_sync(0xffffffffu, bytes);
-        if (lane == 0) mbar_arrive_expect_tx(bar + stage, total);
-        __syncwarp();
-        if (bytes) bulk_load_1d(ring + stage * C::kStage + dst, src, bytes, bar + stage);
-    };
+    const int P = a.g.P, chunk = min(P, KT);   // rows of a tile that are one copy
     const int n_mine = (c1 - c0 - warp + C::kWarps - 1) / C::kWarps;
+    const uint8_t *head_pool = a.pool + kv_seg_off(a.g, 0, 0, head);
+    auto tile_row = [&](int it) { return kt.tile(c0 + warp + it * C::kWarps) * KT; };
+    // the page of the tile's first rows, loaded one issue ahead; -1: no tile, or freed
+    auto page_of = [&](int it) { return it < n_mine ? trow[tile_row(it) >> a.g.lgP] : -1; };
+    // one lane requests the tile: a copy per page it touches (two where a page has 16 rows)
+    auto issue = [&](int it, int stage, int page) {
+        if (lane != 0) return;
+        const int j0 = tile_row(it), rows_in = min(len - j0, KT);
+        uint8_t *dst = ring + stage * C::kStage;
+        if (chunk == KT) {
+            const uint32_t bytes = (unsigned)page < (unsigned)a.g.n_pages ? ((rows_in + 15) >> 4) * C::kBlock : 0;
+            mbar_arrive_expect_tx(bar + stage, bytes);
+            if (bytes)
+                bulk_load_1d(dst, head_pool + page * a.g.page_stride + ((j0 & (P - 1)) >> 4) * C::kBlock, bytes, bar + stage);
+            return;
+        }
+        for (int r = 0; r < rows_in; r += 16) {
+            if (r) page = trow[(j0 + r) >> a.g.lgP];
+            const bool on = (unsigned)page < (unsigned)a.g.n_pages;
+            // the phase completes with the last piece's arrival; pieces before it only add bytes
+            if (on) mbar_expect_tx(bar + stage, C::kBlock);
+            if (on) bulk_load_1d(dst + (r >> 4) * C::kBlock, head_pool + page * a.g.page_stride, C::kBlock, bar + stage);
+        }
+        mbar_arrive(bar + stage);
+    };
+    {
+        int pg[C::kStages];
 #pragma unroll
-    for (int s = 0; s < C::kStages; s++)
-        if (s < n_mine) issue(c0 + warp + s * C::kWarps, s);
+        for (int s = 0; s < C::kStages; s++) pg[s] = page_of(s);
+#pragma unroll
+        for (int s = 0; s < C::kStages; s++)
+            if (s < n_mine) issue(s, s, pg[s]);
+    }
+    int next_page = page_of(C::kStages);
 
     // Q^T fragments: lane (g, t) holds dims 32 j + 8 t .. + 7 of column g
     uint32_t qf[NT][2 * NG][2];
-    float fac[NT][2];   // score factor of columns 2 t, 2 t + 1
-    int qi[NT][2];      // their query rows
+    float fac[NT][2];            // score factor of columns 2 t, 2 t + 1
+    float off[NT][I4 ? NG : 1][2];   // where their partial sums start
+    int qi[NT][2], qlo[NT][2];   // their query rows and the last row before their windows
 #pragma unroll
     for (int nt = 0; nt < NT; nt++) {
         const int col = nt * 8 + g;
@@ -288,12 +334,21 @@ __global__ void __launch_bounds__(128) kv_attend_few_kernel(const __grid_constan
                     x[2 * i] = __uint_as_float(e[i] << 16) * up;
                     x[2 * i + 1] = __uint_as_float(e[i] & 0xffff0000u) * up;
                 }
+                // pairs 1 and 3 stand against 16 (64 + n): a sixteenth of q, rounded at 2^-24 for the smallest
+                const __half2 q1 = __floats2half2_rn(x[1] * 0.0625f, x[5] * 0.0625f);
+                const __half2 q3 = __floats2half2_rn(x[3] * 0.0625f, x[7] * 0.0625f);
                 qf[nt][2 * j][0] = h2_bits(__floats2half2_rn(x[0], x[4]));
-                qf[nt][2 * j][1] = h2_bits(__floats2half2_rn(x[1], x[5]));
+                qf[nt][2 * j][1] = h2_bits(q1);
                 qf[nt][2 * j + 1][0] = h2_bits(__floats2half2_rn(x[2], x[6]));
-                qf[nt][2 * j + 1][1] = h2_bits(__floats2half2_rn(x[3], x[7]));
+                qf[nt][2 * j + 1][1] = h2_bits(q3);
+                const float2 f1 = __half22float2(q1), f3 = __half22float2(q3);
+                float sum = (f1.x + f1.y) + (f3.x + f3.y);
+                sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+                sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+                sum *= -16.f * 72.f;
+                off[nt][j][0] = __shfl_sync(0xffffffffu, sum, 8 * t);
+                off[nt][j][1] = __shfl_sync(0xffffffffu, sum, 8 * t + 4);
             }
-            // column g's factor is 2^-sh scale; lanes need those of columns 2 t, 2 t + 1
             f *= __uint_as_float((uint32_t)(127 - sh) << 23);
         } else {
 #pragma unroll
@@ -304,12 +359,18 @@ __global__ void __launch_bounds__(128) kv_attend_few_kernel(const __grid_constan
                 qf[nt][2 * j + 1][1] = w[j].w;
             }
         }
+        f = fmaxf(f, 1.17549435e-38f);   // -inf * f stays -inf
+        // column g's factor; lanes need those of columns 2 t, 2 t + 1
         fac[nt][0] = __shfl_sync(0xffffffffu, f, 8 * t);
         fac[nt][1] = __shfl_sync(0xffffffffu, f, 8 * t + 4);
-        // a column without a row sees nothing
-        qi[nt][0] = nt * 8 + 2 * t < rows ? i0 + (nt * 8 + 2 * t) / G : -1;
-        qi[nt][1] = nt * 8 + 2 * t + 1 < rows ? i0 + (nt * 8 + 2 * t + 1) / G : -1;
+#pragma unroll
+        for (int c = 0; c < 2; c++) {
+            const int col2 = nt * 8 + 2 * t + c;
+            qi[nt][c] = col2 < rows ? i0 + col2 / G : -1;   // a column without a row sees nothing
+            qlo[nt][c] = a.window ? qi[nt][c] - a.window : -1;
+        }
     }
+    const NibbleMasks nib;
 
     float o[MI][NT][4], m[NT][2], l[NT][2];
 #pragma unroll
@@ -322,18 +383,15 @@ __global__ void __launch_bounds__(128) kv_attend_few_kernel(const __grid_constan
             for (int c = 0; c < 4; c++) o[i][nt][c] = 0.f;
     }
 
-    for (int it = 0; it < n_mine; it++) {
-        const int stage = it % C::kStages, v = c0 + warp + it * C::kWarps, j0 = kt.tile(v) * KT;
-        if (!mbar_wait(bar + stage, (it / C::kStages) & 1, abort_flag, a.err, DEVERR_TIMEOUT_PRODUCER)) break;
-        const uint8_t *sK = ring + stage * C::kStage, *sV = sK + KT * C::RB;
-        const __half *sKs = reinterpret_cast<const __half *>(sK + 2 * KT * C::RB);
-        const __half *sVs = sKs + KT * NG;
-        // every row of the tile visible to every query row
-        const bool full = j0 + KT - 1 <= i0 && (a.window == 0 || j0 > len - 1 - a.window || j0 + KT - 1 < a.sinks);
+    // one tile in shared memory; FULL: every row of it visible to every query row
+    auto tile = [&](auto full_c, const uint8_t *sT, int j0) {
+        constexpr bool FULL = decltype(full_c)::value;
         float s[NK][NT][4];
 #pragma unroll
         for (int kb = 0; kb < NK; kb++) {
-            const int ra = kb * 16 + frag_row(g), rb = ra + 8;
+            const uint8_t *sK = sT + kb * C::kBlock;
+            const __half *sKs = reinterpret_cast<const __half *>(sK + 32 * C::RB);
+            const int ra = frag_row(g), rb = ra + 8;
 #pragma unroll
             for (int nt = 0; nt < NT; nt++)
 #pragma unroll
@@ -355,15 +413,15 @@ __global__ void __launch_bounds__(128) kv_attend_few_kernel(const __grid_constan
 #pragma unroll
                 for (int j = 0; j < NG; j++) {
                     __half2 ha[4], hb[4];
-                    unpack_nibbles(wa[j], ha);
-                    unpack_nibbles(wb[j], hb);
+                    unpack_raw(wa[j], nib, ha);
+                    unpack_raw(wb[j], nib, hb);
                     const float fa = j & 1 ? __high2float(sa[j / 2]) : __low2float(sa[j / 2]);
                     const float fb = j & 1 ? __high2float(sb[j / 2]) : __low2float(sb[j / 2]);
 #pragma unroll
                     for (int nt = 0; nt < NT; nt++) {
-                        float d[4] = {0.f, 0.f, 0.f, 0.f};
-                        mma16816<true>(d, h2_bits(ha[0]), h2_bits(hb[0]), h2_bits(ha[1]), h2_bits(hb[1]),
-                                       qf[nt][2 * j][0], qf[nt][2 * j][1]);
+                        float d[4];
+                        mma16816_from(d, h2_bits(ha[0]), h2_bits(hb[0]), h2_bits(ha[1]), h2_bits(hb[1]), qf[nt][2 * j][0],
+                                      qf[nt][2 * j][1], off[nt][j][0], off[nt][j][1]);
                         mma16816<true>(d, h2_bits(ha[2]), h2_bits(hb[2]), h2_bits(ha[3]), h2_bits(hb[3]),
                                        qf[nt][2 * j + 1][0], qf[nt][2 * j + 1][1]);
                         s[kb][nt][0] = fmaf(d[0], fa, s[kb][nt][0]);
@@ -384,47 +442,60 @@ __global__ void __launch_bounds__(128) kv_attend_few_kernel(const __grid_constan
                     }
                 }
             }
+            if constexpr (!FULL) {
 #pragma unroll
-            for (int nt = 0; nt < NT; nt++)
+                for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-                for (int c = 0; c < 4; c++) {
-                    s[kb][nt][c] *= fac[nt][c & 1];
-                    if (!full && !kv_visible(j0 + (c < 2 ? ra : rb), qi[nt][c & 1], a.window, a.sinks))
-                        s[kb][nt][c] = -INFINITY;
-                }
+                    for (int c = 0; c < 4; c++) {
+                        const int j = j0 + kb * 16 + (c < 2 ? ra : rb);
+                        const bool seen = (j <= qi[nt][c & 1]) & ((j > qlo[nt][c & 1]) | (j < a.sinks));
+                        s[kb][nt][c] = seen ? s[kb][nt][c] : -INFINITY;
+                    }
+            }
         }
         // online softmax of the tile; l stays per lane until the end
-        bool moved = false;
-        float corr[NT][2];
+        bool grow = false;
+        float top[NT][2];
 #pragma unroll
         for (int nt = 0; nt < NT; nt++)
 #pragma unroll
             for (int c = 0; c < 2; c++) {
-                float mx = m[nt][c];
+                float mx = -INFINITY;
 #pragma unroll
                 for (int kb = 0; kb < NK; kb++) mx = fmaxf(mx, fmaxf(s[kb][nt][c], s[kb][nt][c + 2]));
+                top[nt][c] = mx * fac[nt][c];
+                grow |= top[nt][c] > m[nt][c] + 8.f;   // m = -inf: any score
+            }
+        if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
-                for (int x = 4; x < 32; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
-                const float mu = mx == -INFINITY ? 0.f : mx;
-                corr[nt][c] = ex2_hw(m[nt][c] - mu);
-                moved |= m[nt][c] != mx;
-                m[nt][c] = mx;
-                float sum = 0.f;
+            for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                for (int c = 0; c < 2; c++) {
+                    float mx = fmaxf(m[nt][c], top[nt][c]);
+#pragma unroll
+                    for (int x = 4; x < 32; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
+                    const float corr = mx == -INFINITY ? 1.f : ex2_hw(m[nt][c] - mx);
+                    m[nt][c] = mx;
+                    l[nt][c] *= corr;
+#pragma unroll
+                    for (int i = 0; i < MI; i++) {
+                        o[i][nt][c] *= corr;
+                        o[i][nt][c + 2] *= corr;
+                    }
+                }
+        }
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+            for (int c = 0; c < 2; c++) {
+                const float mu = m[nt][c] == -INFINITY ? 0.f : m[nt][c];
 #pragma unroll
                 for (int kb = 0; kb < NK; kb++) {
-                    s[kb][nt][c] = ex2_hw(s[kb][nt][c] - mu);
-                    s[kb][nt][c + 2] = ex2_hw(s[kb][nt][c + 2] - mu);
-                    sum += s[kb][nt][c] + s[kb][nt][c + 2];
+                    s[kb][nt][c] = ex2_hw(fmaf(s[kb][nt][c], fac[nt][c], -mu));
+                    s[kb][nt][c + 2] = ex2_hw(fmaf(s[kb][nt][c + 2], fac[nt][c], -mu));
+                    l[nt][c] += s[kb][nt][c] + s[kb][nt][c + 2];
                 }
-                l[nt][c] = l[nt][c] * corr[nt][c] + sum;
             }
-        if (__any_sync(0xffffffffu, moved))
-#pragma unroll
-            for (int i = 0; i < MI; i++)
-#pragma unroll
-                for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-                    for (int c = 0; c < 4; c++) o[i][nt][c] *= corr[nt][c & 1];
 #pragma unroll
         for (int kb = 0; kb < NK; kb++) {
             // P^T fragments
@@ -445,12 +516,17 @@ __global__ void __launch_bounds__(128) kv_attend_few_kernel(const __grid_constan
             // the four keys of this lane's V^T columns 2 t, 2 t + 1, 2 t + 8, 2 t + 9
             int r[4];
 #pragma unroll
-            for (int c = 0; c < 4; c++) r[c] = kb * 16 + frag_row(2 * t + (c & 1)) + (c >> 1) * 8;
-            bool dead[4];   // a row no query sees may hold anything: its V counts as zero
+            for (int c = 0; c < 4; c++) r[c] = frag_row(2 * t + (c & 1)) + (c >> 1) * 8;
+            const uint8_t *sV = sT + kb * C::kBlock + 16 * C::RB;
+            const __half *sVs = reinterpret_cast<const __half *>(sV + 16 * (C::RB + C::SB));
+            // a row no query sees may hold anything: its V counts as zero
+            bool dead[4] = {false, false, false, false};
+            if constexpr (!FULL) {
 #pragma unroll
-            for (int c = 0; c < 4; c++) {
-                const int j = j0 + r[c];
-                dead[c] = !full && (j >= len || (a.window && j <= i0 - a.window && j >= a.sinks));
+                for (int c = 0; c < 4; c++) {
+                    const int j = j0 + kb * 16 + r[c];
+                    dead[c] = (j >= len) | ((a.window != 0) & (j <= i0 - a.window) & (j >= a.sinks));
+                }
             }
             if constexpr (I4) {
                 __half2 sc[2];
@@ -459,7 +535,7 @@ __global__ void __launch_bounds__(128) kv_attend_few_kernel(const __grid_constan
 #pragma unroll
                     for (int c = 0; c < 4; c++) {
                         x[c] = sVs[r[c] * NG + (D == 128 ? g >> 1 : g >> 2)];
-                        if (dead[c]) x[c] = __ushort_as_half(0);
+                        if (!FULL) x[c] = dead[c] ? __ushort_as_half(0) : x[c];
                     }
                     sc[0] = __halves2half2(x[0], x[1]);
                     sc[1] = __halves2half2(x[2], x[3]);
@@ -480,8 +556,8 @@ __global__ void __launch_bounds__(128) kv_attend_few_kernel(const __grid_constan
                     for (int hf = 0; hf < 2; hf++) {   // dims 4 hf .. 4 hf + 3 of the word
                         __half2 va[4], vb[4];
                         const uint32_t sel = hf ? 0x7632 : 0x5410;
-                        unpack_nibbles(__byte_perm(w[0][x], w[1][x], sel), va);
-                        unpack_nibbles(__byte_perm(w[2][x], w[3][x], sel), vb);
+                        unpack_nibbles(__byte_perm(w[0][x], w[1][x], sel), nib, va);
+                        unpack_nibbles(__byte_perm(w[2][x], w[3][x], sel), nib, vb);
 #pragma unroll
                         for (int n = 0; n < 4; n++) { va[n] = __hmul2(va[n], sc[0]); vb[n] = __hmul2(vb[n], sc[1]); }
 #pragma unroll
@@ -500,7 +576,9 @@ __global__ void __launch_bounds__(128) kv_attend_few_kernel(const __grid_constan
                     for (int c = 0; c < 4; c++) {
                         *reinterpret_cast<uint4 *>(w[c]) =
                             *reinterpret_cast<const uint4 *>(sV + r[c] * C::RB + 16 * ((U * g + x) ^ kv_swz_v(false, D, r[c])));
-                        if (dead[c]) w[c][0] = w[c][1] = w[c][2] = w[c][3] = 0u;
+#pragma unroll
+                        for (int n = 0; n < 4; n++)
+                            if (!FULL) w[c][n] = dead[c] ? 0u : w[c][n];
                     }
 #pragma unroll
                     for (int n = 0; n < 4; n++) {
@@ -515,8 +593,21 @@ __global__ void __launch_bounds__(128) kv_attend_few_kernel(const __grid_constan
                 }
             }
         }
+    };
+    for (int it = 0, stage = 0, ph = 0; it < n_mine; it++) {
+        const int j0 = tile_row(it);
+        if (!mbar_wait(bar + stage, ph, abort_flag, a.err, DEVERR_TIMEOUT_PRODUCER)) break;
+        const uint8_t *sT = ring + stage * C::kStage;
+        if (j0 + KT - 1 <= i0 && (a.window == 0 || j0 > len - 1 - a.window || j0 + KT - 1 < a.sinks))
+            tile(std::true_type{}, sT, j0);
+        else
+            tile(std::false_type{}, sT, j0);
         __syncwarp();   // every lane has read the stage
-        if (it + C::kStages < n_mine) issue(c0 + warp + (it + C::kStages) * C::kWarps, stage);
+        if (it + C::kStages < n_mine) {
+            issue(it + C::kStages, stage, next_page);
+            next_page = page_of(it + C::kStages + 1);
+        }
+        if (++stage == C::kStages) { stage = 0; ph ^= 1; }
     }
     // a wait that ran out: let this warp's copies land before the rings are reused
     if (*abort_flag) {
@@ -654,9 +745,9 @@ struct ManyCfg {
 };
 
 // pairs (0, 4), (1, 5), (2, 6), (3, 7) of a word's values, as one 16-byte unit
-DTTS_DEV uint4 dequant_unit(uint32_t w, __half2 s) {
+DTTS_DEV uint4 dequant_unit(uint32_t w, const NibbleMasks &k, __half2 s) {
     __half2 h[4];
-    unpack_nibbles(w, h);
+    unpack_nibbles(w, k, h);
     return make_uint4(h2_bits(__hmul2(h[0], s)), h2_bits(__hmul2(h[1], s)), h2_bits(__hmul2(h[2], s)),
                       h2_bits(__hmul2(h[3], s)));
 }
@@ -797,6 +888,7 @@ __global__ void __launch_bounds__(384, 1) kv_attend_many_kernel(const __grid_con
             // K: the words of unit t are dims 32 j + 8 t of all groups j; V: unit t is group t.
             // A block's raw rows are loaded while the one before is unpacked.
             constexpr int kN = (KT * 4 + C::kProducers - 1) / C::kProducers;
+            const NibbleMasks nib;
             struct Raw {
                 uint4 w[kN];
                 uint2 sc[kN];
@@ -814,8 +906,8 @@ __global__ void __launch_bounds__(384, 1) kv_attend_many_kernel(const __grid_con
                     const uint8_t *seg = seg_of(j0 + r);
                     if (!seg) continue;
                     const int pr = (j0 + r) & (P - 1);
-                    const uint8_t *row = seg + (V ? P * C::RB : 0) + pr * C::RB;
-                    const uint8_t *srow = seg + 2 * P * C::RB + (V ? P * C::SB : 0) + pr * C::SB;
+                    const uint8_t *row = seg + kv_row_off(a.g, V, pr);
+                    const uint8_t *srow = seg + kv_scale_off(a.g, V, pr);
                     if (V || D == 128) {
                         raw.w[x] = *reinterpret_cast<const uint4 *>(row + (V ? t ^ kv_swz_v(true, D, pr) : t) * 16);
                     } else {
@@ -843,7 +935,7 @@ __global__ void __launch_bounds__(384, 1) kv_attend_many_kernel(const __grid_con
 #pragma unroll
                     for (int q = 0; q < (V ? 4 : D / 32); q++) {
                         if (V) {
-                            *reinterpret_cast<uint4 *>(dst + tile_unit(r, 4 * t + q)) = dequant_unit(e[q], bits_h2(raw.sc[x].x));
+                            *reinterpret_cast<uint4 *>(dst + tile_unit(r, 4 * t + q)) = dequant_unit(e[q], nib, bits_h2(raw.sc[x].x));
                         } else {
                             // odd rows take their words in pair-swapped order, so that the two rows of a
                             // quarter warp fill all eight units of the swizzle
@@ -851,7 +943,7 @@ __global__ void __launch_bounds__(384, 1) kv_attend_many_kernel(const __grid_con
                             const uint32_t s2 = (q >> 1) ? raw.sc[x].y : raw.sc[x].x;
                             const uint32_t sj = (r & 1) ^ (q & 1) ? s2 >> 16 : s2 & 0xffffu;
                             *reinterpret_cast<uint4 *>(dst + tile_unit(r, 4 * j + t)) =
-                                dequant_unit(r & 1 ? e[q ^ 1] : e[q], bits_h2(sj * 0x10001u));
+                                dequant_unit(r & 1 ? e[q ^ 1] : e[q], nib, bits_h2(sj * 0x10001u));
                         }
                     }
                 }
@@ -883,7 +975,7 @@ __global__ void __launch_bounds__(384, 1) kv_attend_many_kernel(const __grid_con
                     const uint8_t *seg = seg_of(j0 + r);
                     const uint32_t d = smem_u32(dst + tile_unit(r, un));
                     const int su = un ^ (is_v ? kv_swz_v(false, D, pr) : kv_swz_k(false, pr));
-                    const uint8_t *src = seg ? seg + (is_v ? P * C::RB : 0) + pr * C::RB + su * 16 : a.pool;
+                    const uint8_t *src = seg ? seg + kv_row_off(a.g, is_v, pr) + su * 16 : a.pool;
                     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(d), "l"(src), "r"(seg ? 16 : 0) : "memory");
                 }
                 asm volatile("cp.async.commit_group;" ::: "memory");
@@ -1087,8 +1179,8 @@ template <int D, bool I4>
 cudaError_t launch_few(const KvAttendArgs &a, int rows, cudaStream_t s) {
     const dim3 grid((unsigned)a.n_seq * a.g.H * a.splits);
     if (rows <= 8)
-        return launch_k(pdl_enabled() ? kLaunchPdl : 0u, kv_attend_few_kernel<D, I4, 1>, grid, dim3(128), FewCfg<D, I4>::kSmem, s, a);
-    return launch_k(pdl_enabled() ? kLaunchPdl : 0u, kv_attend_few_kernel<D, I4, 2>, grid, dim3(128), FewCfg<D, I4>::kSmem, s, a);
+        return launch_k(pdl_enabled() ? kLaunchPdl : 0u, kv_attend_few_kernel<D, I4, 1>, grid, dim3(FewCfg<D, I4>::kThreads), FewCfg<D, I4>::kSmem, s, a);
+    return launch_k(pdl_enabled() ? kLaunchPdl : 0u, kv_attend_few_kernel<D, I4, 2>, grid, dim3(FewCfg<D, I4>::kThreads), FewCfg<D, I4>::kSmem, s, a);
 }
 
 }  // namespace
@@ -1098,6 +1190,11 @@ int kv_key_tile(const KvGeom &g, bool many) {
     if (many) return 128;
     if (g.i4) return g.D == 128 ? FewCfg<128, true>::KT : FewCfg<64, true>::KT;
     return g.D == 128 ? FewCfg<128, false>::KT : FewCfg<64, false>::KT;
+}
+
+// fewest key tiles a part of the few-row kernel is given: two rounds of its warps
+int kv_min_tiles(const KvGeom &g) {
+    return 2 * (g.i4 ? FewCfg<128, true>::kWarps : FewCfg<128, false>::kWarps);
 }
 
 cudaError_t kv_attend_prepare() {

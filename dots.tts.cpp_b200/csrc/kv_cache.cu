@@ -20,6 +20,7 @@ bool pdl_enabled();
 cudaError_t kv_attend_prepare();
 cudaError_t launch_kv_attend(const KvAttendArgs &a, bool many, int rows_or_pairs, cudaStream_t s);
 int kv_key_tile(const KvGeom &g, bool many);
+int kv_min_tiles(const KvGeom &g);
 }  // namespace dtts
 
 namespace {
@@ -132,9 +133,8 @@ __global__ void __launch_bounds__(256) kv_read_kernel(const __grid_constant__ Kv
     }
 }
 
-// The first `rows` rows of pages src to pages dst, all layers and heads: four
-// contiguous runs a segment (K, V and their scales), copied in 16-byte units
-// (a scale run is rounded up, inside its part).
+// The first `rows` rows of pages src to pages dst, all layers and heads: whole
+// 16-row blocks, one contiguous run a segment.
 constexpr int kCopies = 320;
 struct Copies {
     int n;
@@ -147,17 +147,9 @@ __global__ void __launch_bounds__(256) kv_copy_pages_kernel(const __grid_constan
     const int e = blockIdx.y, n = c.rows[e];
     const uint8_t *src = pool + (long long)c.src[e] * g.page_stride + (long long)blockIdx.x * g.seg;
     uint8_t *dst = pool + (long long)c.dst[e] * g.page_stride + (long long)blockIdx.x * g.seg;
-    const int ur = n * g.RB / 16, us = (n * g.SB + 15) / 16;
-    for (int i = threadIdx.x; i < 2 * (ur + us); i += blockDim.x) {
-        int off;
-        if (i < 2 * ur)
-            off = (i < ur ? 0 : g.P * g.RB - ur * 16) + i * 16;
-        else {
-            const int j = i - 2 * ur;
-            off = 2 * g.P * g.RB + (j < us ? 0 : g.P * g.SB - us * 16) + j * 16;
-        }
-        *reinterpret_cast<uint4 *>(dst + off) = *reinterpret_cast<const uint4 *>(src + off);
-    }
+    const int units = (n + 15) / 16 * 2 * (g.RB + g.SB);
+    for (int i = threadIdx.x; i < units; i += blockDim.x)
+        reinterpret_cast<uint4 *>(dst)[i] = reinterpret_cast<const uint4 *>(src)[i];
 }
 
 // Rows keep[j] of table row src to rows j0 + j of table row dst (j < n), all
@@ -182,17 +174,17 @@ __global__ void __launch_bounds__(256) kv_gather_kernel(const __grid_constant__ 
         const int ra = a & (g.P - 1), rb = b & (g.P - 1);
         if (u < 2 * u_row) {
             const bool is_v = u >= u_row;
-            const int w = is_v ? u - u_row : u, part = is_v ? g.P * g.RB : 0;
+            const int w = is_v ? u - u_row : u;
             const int ua = w ^ (is_v ? kv_swz_v(g.i4, g.D, ra) : kv_swz_k(g.i4, ra));
             const int ub = w ^ (is_v ? kv_swz_v(g.i4, g.D, rb) : kv_swz_k(g.i4, rb));
-            *reinterpret_cast<uint4 *>(sb + part + rb * g.RB + ub * 16) =
-                *reinterpret_cast<const uint4 *>(sa + part + ra * g.RB + ua * 16);
+            *reinterpret_cast<uint4 *>(sb + kv_row_off(g, is_v, rb) + ub * 16) =
+                *reinterpret_cast<const uint4 *>(sa + kv_row_off(g, is_v, ra) + ua * 16);
         } else {
-            const int part = 2 * g.P * g.RB + (u - 2 * u_row) * g.P * g.SB;
-            if (g.SB == 8)
-                *reinterpret_cast<uint2 *>(sb + part + rb * 8) = *reinterpret_cast<const uint2 *>(sa + part + ra * 8);
-            else
-                *reinterpret_cast<uint32_t *>(sb + part + rb * 4) = *reinterpret_cast<const uint32_t *>(sa + part + ra * 4);
+            const bool is_v = u > 2 * u_row;
+            sa += kv_scale_off(g, is_v, ra);
+            sb += kv_scale_off(g, is_v, rb);
+            if (g.SB == 8) *reinterpret_cast<uint2 *>(sb) = *reinterpret_cast<const uint2 *>(sa);
+            else *reinterpret_cast<uint32_t *>(sb) = *reinterpret_cast<const uint32_t *>(sa);
         }
     }
 }
@@ -378,31 +370,44 @@ int dtts_kv::plan_attend(const dtts_kv_attend_args &a, KvAttendPlan *plan) const
     p.scale_log2 = a.scale * 1.4426950408889634f;
     p.window = a.window; p.sinks = a.sinks;
     p.ws = ws; p.cnt = cnt; p.err = d_err;
+    std::vector<std::pair<long long, long long>> parts;
     // both kernels run where a batch mixes steps and prompts; each takes its own sequences
     for (int many = 0; many < 2; many++) {
         const int kt = kv_key_tile(g, many);
         long long tiles = 0, max_tiles = 0;
         int max_rows = 0;
+        parts.clear();   // (key tiles, row tiles) of this kernel's sequences
         for (int b = 0; b < n_seq; b++) {
             const long long rows = (long long)b_cnt[b] * G;
             if (rows == 0 || (rows > kKvFewRows) != (many == 1)) continue;
             const long long lo = a.window ? std::max(0ll, (long long)b_len[b] - b_cnt[b] - a.window + 1) : 0;
             const long long nt = (b_len[b] + kt - 1) / kt - lo / kt + (std::min<long long>(a.sinks, lo) + kt - 1) / kt;
-            tiles += nt * (many ? (rows + 255) / 256 : 1) * g.H;
+            const long long rt = many ? (rows + 255) / 256 : 1;
+            tiles += nt * rt * g.H;
             max_tiles = std::max(max_tiles, nt);
             max_rows = (int)std::min<long long>(INT32_MAX / 2, std::max<long long>(max_rows, rows));
+            parts.emplace_back(nt, rt);
         }
         if (!max_rows) continue;
         const int rt = many ? (max_rows + 255) / 256 : 1;
         const long long units = (long long)n_seq * g.H * rt;
         DTTS_CHECK(units <= INT32_MAX / 256, DTTS_ERR_ARG, "%lld row tiles in one batch", units);
-        // parts of a key range: enough for every SM, each a few tiles long
+        // Parts of the key ranges: as short as they may be with all CTAs resident at once, but not
+        // shorter than what hides a CTA's start and the join.
+        const long long resident = (many ? 1ll : 2ll) * num_sms, min_tiles = many ? 2 : kv_min_tiles(g);
+        auto ctas = [&](long long per) {
+            long long n = 0;
+            for (auto &x : parts) n += (x.first + per - 1) / per * x.second * g.H;
+            return n;
+        };
+        long long per = std::max(min_tiles, (tiles + resident - 1) / resident), hi = std::max(per, max_tiles);
+        while (per < hi) {   // the smallest part length with at most `resident` CTAs, or no split at all
+            const long long mid = (per + hi) / 2;
+            if (ctas(mid) <= resident) hi = mid; else per = mid + 1;
+        }
+        long long splits = (max_tiles + per - 1) / per;
         const int slot_rows = many ? 256 : kKvFewRows;
         const long long slots = kWsFloats / ((long long)slot_rows * (g.D + 2));
-        const long long want = many ? num_sms : 4ll * num_sms;
-        const long long min_tiles = many ? 2 : 4;
-        const long long per = std::max(min_tiles, (tiles + want - 1) / want);
-        long long splits = (max_tiles + per - 1) / per;
         if (units > kMaxUnits / 2) splits = 1;
         splits = std::max(1ll, std::min(splits, slots / units));
         p.splits = (int)splits;
@@ -818,7 +823,7 @@ int dtts_kv_read(dtts_kv *kv, int layer, int n_layers, int n, const int *seqs, c
     return DTTS_ERR_OOM;
 }
 
-int dtts_kv_attend(dtts_kv *kv, int layer, const dtts_kv_attend_args *a) {
+int dtts_kv_attend(dtts_kv *kv, int layer, const dtts_kv_attend_args *a) try {
     DTTS_CHECK(kv && a, DTTS_ERR_ARG, "null argument");
     DTTS_CHECK(layer >= 0 && layer < kv->g.L, DTTS_ERR_ARG, "layer %d of %d", layer, kv->g.L);
     KvAttendPlan p;
@@ -827,6 +832,9 @@ int dtts_kv_attend(dtts_kv *kv, int layer, const dtts_kv_attend_args *a) {
     DeviceGuard dg(kv->device);
     if ((st = kv->flush())) return st;
     return kv->attend(p, layer);
+} catch (const std::bad_alloc &) {
+    set_error("out of host memory");
+    return DTTS_ERR_OOM;
 }
 
 }  // extern "C"

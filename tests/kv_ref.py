@@ -7,7 +7,10 @@ most half a step: bf16 2^-8, half 2^-11, fp32 2^-24, relative):
     division by l >= 1); in two bf16 terms (bf16 rows, at most 16 query rows): 2^-16 sum_j p_j |v_j|, below the
     former; in bf16 (bf16 rows, more query rows): 2^-8 sum_j p_j |v_j|;
   * a score s = scale sum_d q_d k_d in fp32: at most D / 16 additions of 16-term products, each step off by at
-    most 2^-22 of B = scale sum_d |q_d k_d|: 2^-19 B for D <= 128, on p through exp twice (numerator and l);
+    most 2^-22 of B = scale sum_d |q_d k_d|: 2^-19 B for D <= 128, on p through exp twice (numerator and l).
+    int4 rows, few query rows: a code c enters as 64 + n, n = c + 8 < 16, and 72 q is taken off again, so the
+    sums of a group reach scale sum_d |q_d| 80 s, s = max|k| / 7 of the group; two products and one fused
+    multiply-add a group, each off by 2^-23 of that: with B' = scale sum_d |q_d| 80 s_d, 2^-21 B' in all;
     exp2 itself 2^-22, corrections of the running maximum and l: n / 16 steps of 2^-23 each, P V the same."""
 import math
 
@@ -65,9 +68,12 @@ def attend(q, k, v, i0, window=0, sinks=0, scale=None, int4=True):
             p = torch.softmax(s, 0)
             o = p @ vv
             a = p @ vv.abs()
-            B = float((kk.abs() @ q[x, h].abs()).max() * scale)
+            B = float((kk.abs() @ q[x, h].abs()).max() * scale) * 2.0 ** -19
+            if int4:
+                top = kk.abs().reshape(len(j), -1, 32).amax(-1, keepdim=True).expand(-1, -1, 32).reshape(len(j), D)
+                B += float((top @ q[x, h].abs()).max() * scale) * 80 / 7 * 2.0 ** -21
             out[x, h] = o
-            tol[x, h] = 2.0 ** -8 * o.abs() + a * (p_step + 2.0 ** -19 * B + (len(j) / 16 + 64) * 2.0 ** -22) + \
+            tol[x, h] = 2.0 ** -8 * o.abs() + a * (p_step + B + (len(j) / 16 + 64) * 2.0 ** -22) + \
                 2.0 ** -25 * vv.abs().sum(0)
     return out, tol
 
