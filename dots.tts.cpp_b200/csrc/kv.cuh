@@ -173,6 +173,17 @@ struct KvAttendArgs {
     int *cnt;                                 // arrivals per split unit, zero between calls
     int *err;
 };
+// What sizes the launches of a cache's attention kernels.
+struct KvShapes {
+    int few_key_tile, few_min_tiles;   // rows of a key tile; fewest tiles a part is given
+    int few_ctas[2];                   // resident CTAs per SM: up to 8, up to 16 query rows
+};
+constexpr int kKvManyKeyTile = 128;
+// Sets the kernels' attributes on the current device.
+cudaError_t kv_attend_prepare(const KvGeom &g, KvShapes *k);
+// many: sequences of more than kKvFewRows rows, in rows_or_pairs pairs of row tiles
+// (256 rows) at most; otherwise sequences of up to that many, rows_or_pairs at most
+cudaError_t launch_kv_attend(const KvAttendArgs &a, bool many, int rows_or_pairs, cudaStream_t s);
 // rows (new tokens x query heads per kv head) that the few-row kernel takes
 constexpr int kKvFewRows = 16;
 

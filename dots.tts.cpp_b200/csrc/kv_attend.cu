@@ -194,12 +194,12 @@ __host__ __device__ constexpr int frag_row(int k) { return (k & 8) | ((k & 7) < 
 
 template <int D, bool I4>
 struct FewCfg {
-    static constexpr int kWarps = I4 ? 8 : 4, kThreads = kWarps * 32;
-    static constexpr int KT = I4 || D == 64 ? 32 : 16;         // keys a tile
+    static constexpr int kWarps = 4, kThreads = kWarps * 32;
+    static constexpr int KT = I4 ? 64 : D == 64 ? 32 : 16;     // keys a tile
     static constexpr int RB = I4 ? D / 2 : 2 * D, SB = I4 ? D / 16 : 0;
     static constexpr int kBlock = 32 * (RB + SB);              // 16 rows of K and V with their scales
     static constexpr int kStage = KT / 16 * kBlock;
-    static constexpr int kStages = 3;
+    static constexpr int kStages = 2;
     static constexpr int kRing = kWarps * kStages * kStage;
     static constexpr int kMerge = kWarps * kKvFewRows * (D + 2) * 4;   // the warps' results, over the rings
     static constexpr int kSmem = (kRing > kMerge ? kRing : kMerge) + kWarps * kStages * 8 + 16;
@@ -223,7 +223,7 @@ struct FewCfg {
 // The running maximum m of a column is raised only when a score passes it by 2^8
 // (P <= 2^8 is as exact as P <= 1), so most tiles need no exchange between lanes.
 template <int D, bool I4, int NT>
-__global__ void __launch_bounds__(FewCfg<D, I4>::kThreads, NT == 1 ? 2 : 1) kv_attend_few_kernel(const __grid_constant__ KvAttendArgs a) {
+__global__ void __launch_bounds__(FewCfg<D, I4>::kThreads, NT == 1 ? 3 : 1) kv_attend_few_kernel(const __grid_constant__ KvAttendArgs a) {
     using C = FewCfg<D, I4>;
     constexpr int KT = C::KT, NK = KT / 16, MI = D / 16, NG = D / 32;
     extern __shared__ __align__(128) uint8_t smem[];
@@ -734,7 +734,7 @@ DTTS_DEV int tile_unit(int r, int u) { return (u >> 3) * kChunk + r * 128 + (((u
 
 template <int D, bool I4>
 struct ManyCfg {
-    static constexpr int KT = 128, kTile = D / 64 * kChunk;   // one operand tile of 128 rows
+    static constexpr int KT = kKvManyKeyTile, kTile = D / 64 * kChunk;   // one operand tile of 128 rows
     static constexpr int kSoftmax = 256, kProducers = 96, kThreads = kSoftmax + kProducers + 32;
     static constexpr int kSmem = 6 * kTile + 256 + 1024;      // Q x 2, K x 2, V x 2, barriers
     static constexpr int RB = I4 ? D / 2 : 2 * D, SB = I4 ? D / 16 : 0;
@@ -1160,20 +1160,28 @@ __global__ void __launch_bounds__(384, 1) kv_attend_many_kernel(const __grid_con
 }
 
 template <int D, bool I4>
-cudaError_t prepare_many() {
-    return cudaFuncSetAttribute(kv_attend_many_kernel<D, I4>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                ManyCfg<D, I4>::kSmem);
-}
-template <int D, bool I4>
 cudaError_t launch_many(const KvAttendArgs &a, int pairs, cudaStream_t s) {
     return launch_k(pdl_enabled() ? kLaunchPdl : 0u, kv_attend_many_kernel<D, I4>, dim3((unsigned)a.n_seq * a.g.H * pairs * a.splits),
                     dim3(ManyCfg<D, I4>::kThreads), ManyCfg<D, I4>::kSmem, s, a, pairs);
 }
 
 template <int D, bool I4, int NT>
-cudaError_t prepare_few() {
-    return cudaFuncSetAttribute(kv_attend_few_kernel<D, I4, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                FewCfg<D, I4>::kSmem);
+cudaError_t prepare_few(int *ctas) {
+    cudaError_t e = cudaFuncSetAttribute(kv_attend_few_kernel<D, I4, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         FewCfg<D, I4>::kSmem);
+    if (e != cudaSuccess) return e;
+    return cudaOccupancyMaxActiveBlocksPerMultiprocessor(ctas, kv_attend_few_kernel<D, I4, NT>, FewCfg<D, I4>::kThreads,
+                                                         FewCfg<D, I4>::kSmem);
+}
+template <int D, bool I4>
+cudaError_t prepare(KvShapes *k) {
+    k->few_key_tile = FewCfg<D, I4>::KT;
+    k->few_min_tiles = 2 * FewCfg<D, I4>::kWarps;
+    cudaError_t e = prepare_few<D, I4, 1>(&k->few_ctas[0]);
+    if (e == cudaSuccess) e = prepare_few<D, I4, 2>(&k->few_ctas[1]);
+    if (e != cudaSuccess) return e;
+    return cudaFuncSetAttribute(kv_attend_many_kernel<D, I4>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                ManyCfg<D, I4>::kSmem);
 }
 template <int D, bool I4>
 cudaError_t launch_few(const KvAttendArgs &a, int rows, cudaStream_t s) {
@@ -1185,30 +1193,11 @@ cudaError_t launch_few(const KvAttendArgs &a, int rows, cudaStream_t s) {
 
 }  // namespace
 
-// rows of a key tile of the few-row or the many-row kernel
-int kv_key_tile(const KvGeom &g, bool many) {
-    if (many) return 128;
-    if (g.i4) return g.D == 128 ? FewCfg<128, true>::KT : FewCfg<64, true>::KT;
-    return g.D == 128 ? FewCfg<128, false>::KT : FewCfg<64, false>::KT;
+cudaError_t kv_attend_prepare(const KvGeom &g, KvShapes *k) {
+    if (g.i4) return g.D == 128 ? prepare<128, true>(k) : prepare<64, true>(k);
+    return g.D == 128 ? prepare<128, false>(k) : prepare<64, false>(k);
 }
 
-// fewest key tiles a part of the few-row kernel is given: two rounds of its warps
-int kv_min_tiles(const KvGeom &g) {
-    return 2 * (g.i4 ? FewCfg<128, true>::kWarps : FewCfg<128, false>::kWarps);
-}
-
-cudaError_t kv_attend_prepare() {
-    cudaError_t e = cudaSuccess;
-    if ((e = prepare_few<128, true, 1>()) || (e = prepare_few<128, true, 2>()) || (e = prepare_few<128, false, 1>()) ||
-        (e = prepare_few<128, false, 2>()) || (e = prepare_few<64, true, 1>()) || (e = prepare_few<64, true, 2>()) ||
-        (e = prepare_few<64, false, 1>()) || (e = prepare_few<64, false, 2>()) || (e = prepare_many<128, true>()) ||
-        (e = prepare_many<128, false>()) || (e = prepare_many<64, true>()) || (e = prepare_many<64, false>()))
-        return e;
-    return cudaSuccess;
-}
-
-// many: sequences of more than kKvFewRows rows, in rows_or_pairs pairs of row tiles
-// (256 rows) at most; otherwise sequences of up to that many, rows_or_pairs at most
 cudaError_t launch_kv_attend(const KvAttendArgs &a, bool many, int rows_or_pairs, cudaStream_t s) {
     if (many) {
         if (a.g.i4) return a.g.D == 128 ? launch_many<128, true>(a, rows_or_pairs, s) : launch_many<64, true>(a, rows_or_pairs, s);

@@ -17,10 +17,6 @@ using namespace dtts;
 
 namespace dtts {
 bool pdl_enabled();
-cudaError_t kv_attend_prepare();
-cudaError_t launch_kv_attend(const KvAttendArgs &a, bool many, int rows_or_pairs, cudaStream_t s);
-int kv_key_tile(const KvGeom &g, bool many);
-int kv_min_tiles(const KvGeom &g);
 }  // namespace dtts
 
 namespace {
@@ -373,7 +369,7 @@ int dtts_kv::plan_attend(const dtts_kv_attend_args &a, KvAttendPlan *plan) const
     std::vector<std::pair<long long, long long>> parts;
     // both kernels run where a batch mixes steps and prompts; each takes its own sequences
     for (int many = 0; many < 2; many++) {
-        const int kt = kv_key_tile(g, many);
+        const int kt = many ? kKvManyKeyTile : shapes.few_key_tile;
         long long tiles = 0, max_tiles = 0;
         int max_rows = 0;
         parts.clear();   // (key tiles, row tiles) of this kernel's sequences
@@ -394,7 +390,8 @@ int dtts_kv::plan_attend(const dtts_kv_attend_args &a, KvAttendPlan *plan) const
         DTTS_CHECK(units <= INT32_MAX / 256, DTTS_ERR_ARG, "%lld row tiles in one batch", units);
         // Parts of the key ranges: as short as they may be with all CTAs resident at once, but not
         // shorter than what hides a CTA's start and the join.
-        const long long resident = (many ? 1ll : 2ll) * num_sms, min_tiles = many ? 2 : kv_min_tiles(g);
+        const long long resident = (long long)(many ? 1 : std::max(1, shapes.few_ctas[max_rows > 8])) * num_sms;
+        const long long min_tiles = many ? 2 : shapes.few_min_tiles;
         auto ctas = [&](long long per) {
             long long n = 0;
             for (auto &x : parts) n += (x.first + per - 1) / per * x.second * g.H;
@@ -478,7 +475,7 @@ int dtts_kv_create(const dtts_kv_config *c, int device, dtts_kv **out) try {
     DTTS_CUDA(cudaStreamCreateWithFlags(&kv->own_stream, cudaStreamNonBlocking));
     kv->stream = kv->own_stream;
     DTTS_CUDA(cudaEventCreateWithFlags(&kv->handoff, cudaEventDisableTiming));
-    DTTS_CUDA(kv_attend_prepare());
+    DTTS_CUDA(kv_attend_prepare(g, &kv->shapes));
     const size_t pool_bytes = (size_t)g.page_stride * g.n_pages;
     kv->pool = (uint8_t *)kv->mem.alloc(pool_bytes);
     kv->meta = (int *)kv->mem.alloc((size_t)ints * 4);

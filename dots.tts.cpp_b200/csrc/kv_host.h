@@ -26,6 +26,7 @@ struct dtts_kv {
     };
     int device = 0, num_sms = 148;
     dtts::KvGeom g{};
+    dtts::KvShapes shapes{};
     long long max_tokens = 0;
     cudaStream_t own_stream = nullptr, stream = nullptr;
     cudaEvent_t handoff = nullptr;
