@@ -263,7 +263,7 @@ __global__ void __launch_bounds__(FewCfg<D, I4>::kThreads, NT == 1 ? 3 : 1) kv_a
     auto tile_row = [&](int it) { return kt.tile(c0 + warp + it * C::kWarps) * KT; };
     // the page of the tile's first rows, loaded one issue ahead; -1: no tile, or freed
     auto page_of = [&](int it) { return it < n_mine ? trow[tile_row(it) >> a.g.lgP] : -1; };
-    // one lane requests the tile: a copy per page it touches (two where a page has 16 rows)
+    // one lane requests the tile: a copy per page it touches
     auto issue = [&](int it, int stage, int page) {
         if (lane != 0) return;
         const int j0 = tile_row(it), rows_in = min(len - j0, KT);
@@ -275,12 +275,13 @@ __global__ void __launch_bounds__(FewCfg<D, I4>::kThreads, NT == 1 ? 3 : 1) kv_a
                 bulk_load_1d(dst, head_pool + page * a.g.page_stride + ((j0 & (P - 1)) >> 4) * C::kBlock, bytes, bar + stage);
             return;
         }
-        for (int r = 0; r < rows_in; r += 16) {
+        for (int r = 0; r < rows_in; r += chunk) {   // whole pages
             if (r) page = trow[(j0 + r) >> a.g.lgP];
-            const bool on = (unsigned)page < (unsigned)a.g.n_pages;
-            // the phase completes with the last piece's arrival; pieces before it only add bytes
-            if (on) mbar_expect_tx(bar + stage, C::kBlock);
-            if (on) bulk_load_1d(dst + (r >> 4) * C::kBlock, head_pool + page * a.g.page_stride, C::kBlock, bar + stage);
+            if ((unsigned)page >= (unsigned)a.g.n_pages) continue;
+            // the phase completes with the arrival behind the last piece; the pieces only add bytes
+            const uint32_t bytes = ((min(rows_in - r, chunk) + 15) >> 4) * C::kBlock;
+            mbar_expect_tx(bar + stage, bytes);
+            bulk_load_1d(dst + (r >> 4) * C::kBlock, head_pool + page * a.g.page_stride, bytes, bar + stage);
         }
         mbar_arrive(bar + stage);
     };
