@@ -79,9 +79,9 @@ DTTS_DEV float merge_weight(float m, float top) { return m == -INFINITY ? 0.f : 
 // Joins the parts of `rows` rows (row stride D + 2 floats: O, m, l; part stride
 // `part` floats) and stores rows r -> out_of(r).  Parts are taken in order, so
 // the result does not depend on which CTA arrived last.
-template <int D, typename OutOf>
+template <int D, int N, typename OutOf>
 DTTS_DEV void kv_join_parts(const float *ws, long long part, int parts, int rows, OutOf out_of) {
-    for (int e = threadIdx.x; e < rows * (D / 8); e += blockDim.x) {
+    for (int e = threadIdx.x; e < rows * (D / 8); e += N) {
         const int r = e / (D / 8), c = e % (D / 8);
         const float *w = ws + (long long)r * (D + 2);
         float top = -INFINITY;
@@ -108,17 +108,25 @@ DTTS_DEV void kv_join_parts(const float *ws, long long part, int parts, int rows
     }
 }
 
+// Barrier over threads 0 .. N - 1 of the CTA, N = 0: all of them.
+template <int N>
+DTTS_DEV void sync_first() {
+    if (N == 0) __syncthreads();
+    else asm volatile("bar.sync 1, %0;" ::"n"(N) : "memory");
+}
+
 // Counts the parts of a unit that have been written; true in the CTA that sees
 // the last one, which resets the counter for the next call.
+template <int N>
 DTTS_DEV bool kv_last_part(int *cnt, int parts, int *flag) {
     __threadfence();
-    __syncthreads();
+    sync_first<N>();
     if (threadIdx.x == 0) {
         const int old = atomicAdd(cnt, 1);
         *flag = old == parts - 1;
         if (old == parts - 1) *cnt = 0;
     }
-    __syncthreads();
+    sync_first<N>();
     const bool last = *flag;
     if (last) __threadfence();
     return last;
@@ -391,7 +399,7 @@ __global__ void __launch_bounds__(FewCfg<D, I4>::kThreads, NT == 1 ? 3 : 1) kv_a
 #pragma unroll
         for (int kb = 0; kb < NK; kb++) {
             const uint8_t *sK = sT + kb * C::kBlock;
-            const __half *sKs = reinterpret_cast<const __half *>(sK + 32 * C::RB);
+            [[maybe_unused]] const __half *sKs = reinterpret_cast<const __half *>(sK + 32 * C::RB);
             const int ra = frag_row(g), rb = ra + 8;
 #pragma unroll
             for (int nt = 0; nt < NT; nt++)
@@ -500,7 +508,8 @@ __global__ void __launch_bounds__(FewCfg<D, I4>::kThreads, NT == 1 ? 3 : 1) kv_a
 #pragma unroll
         for (int kb = 0; kb < NK; kb++) {
             // P^T fragments
-            uint32_t ph[NT][2], pl[NT][2];
+            uint32_t ph[NT][2];
+            [[maybe_unused]] uint32_t pl[NT][2];
 #pragma unroll
             for (int nt = 0; nt < NT; nt++)
 #pragma unroll
@@ -519,7 +528,7 @@ __global__ void __launch_bounds__(FewCfg<D, I4>::kThreads, NT == 1 ? 3 : 1) kv_a
 #pragma unroll
             for (int c = 0; c < 4; c++) r[c] = frag_row(2 * t + (c & 1)) + (c >> 1) * 8;
             const uint8_t *sV = sT + kb * C::kBlock + 16 * C::RB;
-            const __half *sVs = reinterpret_cast<const __half *>(sV + 16 * (C::RB + C::SB));
+            [[maybe_unused]] const __half *sVs = reinterpret_cast<const __half *>(sV + 16 * (C::RB + C::SB));
             // a row no query sees may hold anything: its V counts as zero
             bool dead[4] = {false, false, false, false};
             if constexpr (!FULL) {
@@ -695,8 +704,8 @@ __global__ void __launch_bounds__(FewCfg<D, I4>::kThreads, NT == 1 ? 3 : 1) kv_a
         }
     }
     if (parts == 1) return;
-    if (kv_last_part(a.cnt + unit, parts, flag))
-        kv_join_parts<D>(a.ws + (long long)unit * a.splits * WS, WS, parts, rows, [&](int r) {
+    if (kv_last_part<0>(a.cnt + unit, parts, flag))
+        kv_join_parts<D, C::kThreads>(a.ws + (long long)unit * a.splits * WS, WS, parts, rows, [&](int r) {
             return a.out + (long long)(row0 + r / G) * a.o_row + (long long)(head * G + r % G) * a.o_head;
         });
 }
@@ -736,7 +745,9 @@ DTTS_DEV int tile_unit(int r, int u) { return (u >> 3) * kChunk + r * 128 + (((u
 template <int D, bool I4>
 struct ManyCfg {
     static constexpr int KT = kKvManyKeyTile, kTile = D / 64 * kChunk;   // one operand tile of 128 rows
-    static constexpr int kSoftmax = 256, kProducers = 96, kThreads = kSoftmax + kProducers + 32;
+    static constexpr int kSoftmax = 256, kProducerWarps = 7, kThreads = 512;
+    // registers a thread: 128 at launch (512 x 128 = 65536), then 256 x (176 + 80) = 65536
+    static constexpr int kSoftmaxRegs = 176, kOtherRegs = 80;
     static constexpr int kSmem = 6 * kTile + 256 + 1024;      // Q x 2, K x 2, V x 2, barriers
     static constexpr int RB = I4 ? D / 2 : 2 * D, SB = I4 ? D / 16 : 0;
     static constexpr uint32_t kF16 = I4 ? 0u : (1u << 7) | (1u << 10);   // operand type: half or bf16
@@ -755,14 +766,40 @@ DTTS_DEV uint4 dequant_unit(uint32_t w, const NibbleMasks &k, __half2 s) {
 // where dim i of 8 stands inside such a unit
 __host__ __device__ constexpr int unit_dim(bool i4, int pos) { return i4 ? (pos >> 1) + (pos & 1) * 4 : pos; }
 
+// Waits like mbar_wait, asleep in the barrier for up to a microsecond a try, so that
+// a waiting role leaves the issue slots to the working ones.
+DTTS_DEV bool kv_wait(uint64_t *bar, uint32_t parity, volatile int *abort_flag, int *err, int code) {
+    const uint32_t addr = smem_u32(bar);
+    unsigned long long t0 = 0;
+    while (true) {
+        uint32_t ok;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, 1000;\n\t"
+            "selp.u32 %0, 1, 0, p;\n\t}\n"
+            : "=r"(ok)
+            : "r"(addr), "r"(parity)
+            : "memory");
+        if (ok) return true;
+        if (*abort_flag) return false;
+        const unsigned long long t = globaltimer_ns();
+        if (t0 == 0) t0 = t;
+        if (t - t0 > kWaitLimitNs) {
+            if (err) atomicCAS(err, 0, code);
+            *abort_flag = 1;
+            return false;
+        }
+    }
+}
+
 // Attention of up to 256 rows (new token x query head of one kv head, two tiles of
 // 128) of one sequence over a part of its keys, in blocks of 128 keys.
 //   warps 0-3, 4-7: softmax of tile 0, 1, one row a thread (S from TMEM, P back into
 //                   the same columns, O rescaled when the row maximum has grown by
 //                   more than 2^8, so P <= 2^8 stays in half's range);
-//   warps 8-10:     K and V blocks from the pages into swizzled tiles (4-bit rows
-//                   become exact halves on the way), two stages;
-//   warp 11:        S = Q K^T and O += P V on tcgen05 (P from TMEM, V MN-major).
+//   warps 8-14:     K and V rows from the pages into swizzled tiles (4-bit rows become
+//                   exact halves on the way), 16 rows of K or V a job, two stages;
+//   warp 15:        S = Q K^T and O += P V on tcgen05 (P from TMEM, V MN-major).
 // The two tiles alternate: while one's softmax runs, the other's products do.
 // Bound by the softmax's exponentials (128 x 128 a block and tile at 16 a clock and
 // SM, as long as its two products take) and by shared memory reads of the operands.
@@ -771,7 +808,7 @@ __host__ __device__ constexpr int unit_dim(bool i4, int pos) { return i4 ? (pos 
 // of |v|, the size of the output's own rounding): a second term would cost half as
 // much tensor time again.
 template <int D, bool I4>
-__global__ void __launch_bounds__(384, 1) kv_attend_many_kernel(const __grid_constant__ KvAttendArgs a, int pairs) {
+__global__ void __launch_bounds__(512, 1) kv_attend_many_kernel(const __grid_constant__ KvAttendArgs a, int pairs) {
     using C = ManyCfg<D, I4>;
     constexpr int KT = C::KT, NU = D / 8;   // 16-byte units a row
     extern __shared__ uint8_t smem_raw[];
@@ -806,9 +843,9 @@ __global__ void __launch_bounds__(384, 1) kv_attend_many_kernel(const __grid_con
             mbar_init(s_full + w, 1);
             mbar_init(p_full + w, 128);
             mbar_init(o_full + w, 1);
-            mbar_init(k_full + w, C::kProducers);
+            mbar_init(k_full + w, 8);
             mbar_init(k_empty + w, 1);
-            mbar_init(v_full + w, C::kProducers);
+            mbar_init(v_full + w, 8);
             mbar_init(v_empty + w, 1);
         }
         mbar_init(drain, 1);
@@ -816,7 +853,7 @@ __global__ void __launch_bounds__(384, 1) kv_attend_many_kernel(const __grid_con
         *abort_flag = 0;
         fence_mbar_init();
     }
-    if (warp == 11) {
+    if (warp == 15) {
         tmem_alloc(tmem_slot, 512);
         tmem_relinquish();
     }
@@ -827,7 +864,9 @@ __global__ void __launch_bounds__(384, 1) kv_attend_many_kernel(const __grid_con
     // only now: the next kernel's CTAs may take TMEM before they wait for this grid
     pdl_trigger();
 
-    if (warp == 11) {
+    if (warp >= 8) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kOtherRegs));
+    else asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::kSoftmaxRegs));
+    if (warp == 15) {
         if (lane == 0) {
             bool ok = true;
             auto scores = [&](int w, int k) {   // S_w = Q_w K^T of block k
@@ -839,18 +878,18 @@ __global__ void __launch_bounds__(384, 1) kv_attend_many_kernel(const __grid_con
                 }
                 tc_commit(s_full + w);
             };
-            ok = ok && mbar_wait(k_full, 0, abort_flag, a.err, DEVERR_TIMEOUT_MMA);
+            ok = ok && kv_wait(k_full, 0, abort_flag, a.err, DEVERR_TIMEOUT_MMA);
             for (int w = 0; w < tiles && ok; w++) {
-                ok = mbar_wait(q_full + w, 0, abort_flag, a.err, DEVERR_TIMEOUT_MMA);
+                ok = kv_wait(q_full + w, 0, abort_flag, a.err, DEVERR_TIMEOUT_MMA);
                 if (!ok) break;
                 tc_fence_after();
                 scores(w, 0);
             }
             if (ok) tc_commit(k_empty);
             for (int k = 0; k < n && ok; k++) {
-                ok = mbar_wait(v_full + (k & 1), (k >> 1) & 1, abort_flag, a.err, DEVERR_TIMEOUT_MMA);
+                ok = kv_wait(v_full + (k & 1), (k >> 1) & 1, abort_flag, a.err, DEVERR_TIMEOUT_MMA);
                 for (int w = 0; w < tiles && ok; w++) {
-                    ok = mbar_wait(p_full + w, k & 1, abort_flag, a.err, DEVERR_TIMEOUT_MMA);
+                    ok = kv_wait(p_full + w, k & 1, abort_flag, a.err, DEVERR_TIMEOUT_MMA);
                     if (!ok) break;
                     tc_fence_after();
                     const uint32_t va = smem_u32(sV + (k & 1) * C::kTile);
@@ -861,8 +900,8 @@ __global__ void __launch_bounds__(384, 1) kv_attend_many_kernel(const __grid_con
                     tc_commit(o_full + w);
                     if (k + 1 == n) continue;
                     // S_w takes the columns P_w is read from: only after that product is done
-                    ok = mbar_wait(k_full + ((k + 1) & 1), ((k + 1) >> 1) & 1, abort_flag, a.err, DEVERR_TIMEOUT_MMA) &&
-                         mbar_wait(o_full + w, k & 1, abort_flag, a.err, DEVERR_TIMEOUT_MMA);
+                    ok = kv_wait(k_full + ((k + 1) & 1), ((k + 1) >> 1) & 1, abort_flag, a.err, DEVERR_TIMEOUT_MMA) &&
+                         kv_wait(o_full + w, k & 1, abort_flag, a.err, DEVERR_TIMEOUT_MMA);
                     if (!ok) break;
                     tc_fence_after();
                     scores(w, k + 1);
@@ -878,117 +917,144 @@ __global__ void __launch_bounds__(384, 1) kv_attend_many_kernel(const __grid_con
         }
         __syncwarp();
     } else if (warp >= 8) {
-        // ---- pages -> tiles
-        const int pt = tid - C::kSoftmax, P = a.g.P, lg = a.g.lgP;
-        auto seg_of = [&](int j) -> const uint8_t * {
-            if (j >= len) return nullptr;
-            const int page = trow[j >> lg];
-            return page >= 0 && page < a.g.n_pages ? a.pool + kv_seg_off(a.g, page, 0, head) : nullptr;
+        // ---- pages -> tiles.  A job is 16 rows of K or V, one block of a page: jobs K0 .. K7, V0 .. V7
+        // of key block 0, then of block 1, ...; producer warp pw takes jobs pw, pw + 7, ...  A job's page
+        // number is loaded two jobs ahead, its rows one job ahead.
+        const int P = a.g.P, lg = a.g.lgP, jobs = 16 * n;
+        const uint8_t *head_pool = a.pool + kv_seg_off(a.g, 0, 0, head);
+        auto row_of = [&](int job) { return kt.tile(c0 + (job >> 4)) * KT + (job & 7) * 16; };
+        auto page_of = [&](int job) {   // -1: nothing to load
+            if (job >= jobs) return -1;
+            const int j = row_of(job);
+            return j < len ? trow[j >> lg] : -1;
         };
+        // the job's block of 16 rows and how many of them exist
+        auto block_of = [&](int job, int page, int &live) -> const uint8_t * {
+            const int j = row_of(job);
+            live = (unsigned)page < (unsigned)a.g.n_pages ? len - j : 0;
+            return head_pool + (live > 0 ? page : 0) * a.g.page_stride + ((j & (P - 1)) >> 4) * (32 * (C::RB + C::SB));
+        };
+        auto wait_empty = [&](int job) {
+            const int k = job >> 4;
+            return k < 2 || kv_wait((job & 8 ? v_empty : k_empty) + (k & 1), ((k >> 1) - 1) & 1, abort_flag, a.err,
+                                    DEVERR_TIMEOUT_PRODUCER);
+        };
+        auto announce = [&](int job) {
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive((job & 8 ? v_full : k_full) + ((job >> 4) & 1));
+        };
+        constexpr int kStep = C::kProducerWarps;
+        int job = warp - 8;
         if constexpr (I4) {
-            // K: the words of unit t are dims 32 j + 8 t of all groups j; V: unit t is group t.
-            // A block's raw rows are loaded while the one before is unpacked.
-            constexpr int kN = (KT * 4 + C::kProducers - 1) / C::kProducers;
+            // K: lane = 4 r + t takes the words of dims 32 j + 8 t (all groups j) of rows r and r + 8;
+            // V: a lane takes 16-byte units (a group of dims each), two of them where D = 128
             const NibbleMasks nib;
+            constexpr int kV = D / 64, kPerRow = D / 32;   // V: units a lane, units a row
             struct Raw {
-                uint4 w[kN];
-                uint2 sc[kN];
-            } rk, rv;
-            auto load = [&](auto is_v, int k, Raw &raw) {
-                constexpr bool V = decltype(is_v)::value;
-                constexpr int per = V ? D / 32 : 4;   // items a row
-                const int j0 = kt.tile(c0 + k) * KT;
+                uint4 w[2];
+                uint2 s[2];
+            };
+            auto load = [&](int jb, int page, Raw &raw) {
+                int live;
+                const uint8_t *blk = block_of(jb, page, live);
+                if (jb & 8) {
 #pragma unroll
-                for (int x = 0; x < kN; x++) {
-                    const int it = pt + x * C::kProducers, r = it / per, t = it % per;
-                    raw.w[x] = make_uint4(0u, 0u, 0u, 0u);
-                    raw.sc[x] = make_uint2(0u, 0u);
-                    if (r >= KT) continue;
-                    const uint8_t *seg = seg_of(j0 + r);
-                    if (!seg) continue;
-                    const int pr = (j0 + r) & (P - 1);
-                    const uint8_t *row = seg + kv_row_off(a.g, V, pr);
-                    const uint8_t *srow = seg + kv_scale_off(a.g, V, pr);
-                    if (V || D == 128) {
-                        raw.w[x] = *reinterpret_cast<const uint4 *>(row + (V ? t ^ kv_swz_v(true, D, pr) : t) * 16);
-                    } else {
-                        const uint2 y = *reinterpret_cast<const uint2 *>(row + t * 8);
-                        raw.w[x].x = y.x;
-                        raw.w[x].y = y.y;
+                    for (int x = 0; x < kV; x++) {
+                        const int it = lane + 32 * x, r = it / kPerRow, u = it % kPerRow;
+                        raw.w[x] = make_uint4(0u, 0u, 0u, 0u);
+                        raw.s[x].x = 0u;
+                        if (r >= live) continue;
+                        raw.w[x] = *reinterpret_cast<const uint4 *>(blk + (16 + r) * C::RB + 16 * (u ^ kv_swz_v(true, D, r)));
+                        raw.s[x].x = *reinterpret_cast<const uint16_t *>(blk + 32 * C::RB + (16 + r) * C::SB + 2 * u);
                     }
-                    if (V) raw.sc[x].x = *reinterpret_cast<const uint16_t *>(srow + t * 2) * 0x10001u;
-                    else if (D == 128) raw.sc[x] = *reinterpret_cast<const uint2 *>(srow);
-                    else raw.sc[x].x = *reinterpret_cast<const uint32_t *>(srow);
+                } else {
+#pragma unroll
+                    for (int x = 0; x < 2; x++) {
+                        const int r = (lane >> 2) + 8 * x, q = lane & 3;
+                        raw.w[x] = make_uint4(0u, 0u, 0u, 0u);
+                        raw.s[x] = make_uint2(0u, 0u);
+                        if (r >= live) continue;
+                        if constexpr (D == 128) {
+                            raw.w[x] = *reinterpret_cast<const uint4 *>(blk + r * C::RB + 16 * q);
+                            raw.s[x] = *reinterpret_cast<const uint2 *>(blk + 32 * C::RB + r * C::SB);
+                        } else {
+                            const uint2 y = *reinterpret_cast<const uint2 *>(blk + r * C::RB + 8 * q);
+                            raw.w[x].x = y.x;
+                            raw.w[x].y = y.y;
+                            raw.s[x].x = *reinterpret_cast<const uint32_t *>(blk + 32 * C::RB + r * C::SB);
+                        }
+                    }
                 }
             };
-            auto store = [&](auto is_v, int k, const Raw &raw) {
-                constexpr bool V = decltype(is_v)::value;
-                constexpr int per = V ? D / 32 : 4;
-                uint8_t *dst = (V ? sV : sK) + (k & 1) * C::kTile;
-                if (k >= 2 && !mbar_wait((V ? v_empty : k_empty) + (k & 1), ((k >> 1) - 1) & 1, abort_flag, a.err,
-                                         DEVERR_TIMEOUT_PRODUCER))
-                    return false;
+            auto store = [&](int jb, const Raw &raw) {
+                uint8_t *dst = (jb & 8 ? sV : sK) + ((jb >> 4) & 1) * C::kTile;
+                const int r0 = (jb & 7) * 16;
+                if (jb & 8) {
 #pragma unroll
-                for (int x = 0; x < kN; x++) {
-                    const int it = pt + x * C::kProducers, r = it / per, t = it % per;
-                    if (r >= KT) continue;
-                    const uint32_t e[4] = {raw.w[x].x, raw.w[x].y, raw.w[x].z, raw.w[x].w};
+                    for (int x = 0; x < kV; x++) {
+                        const int it = lane + 32 * x, r = r0 + it / kPerRow, u = it % kPerRow;
+                        const uint32_t e[4] = {raw.w[x].x, raw.w[x].y, raw.w[x].z, raw.w[x].w};
 #pragma unroll
-                    for (int q = 0; q < (V ? 4 : D / 32); q++) {
-                        if (V) {
-                            *reinterpret_cast<uint4 *>(dst + tile_unit(r, 4 * t + q)) = dequant_unit(e[q], nib, bits_h2(raw.sc[x].x));
-                        } else {
+                        for (int q = 0; q < 4; q++)
+                            *reinterpret_cast<uint4 *>(dst + tile_unit(r, 4 * u + q)) =
+                                dequant_unit(e[q], nib, bits_h2(raw.s[x].x * 0x10001u));
+                    }
+                } else {
+#pragma unroll
+                    for (int x = 0; x < 2; x++) {
+                        const int r = r0 + (lane >> 2) + 8 * x, kq = lane & 3;
+                        const uint32_t e[4] = {raw.w[x].x, raw.w[x].y, raw.w[x].z, raw.w[x].w};
+#pragma unroll
+                        for (int q = 0; q < D / 32; q++) {
                             // odd rows take their words in pair-swapped order, so that the two rows of a
                             // quarter warp fill all eight units of the swizzle
                             const int j = q ^ (r & 1);
-                            const uint32_t s2 = (q >> 1) ? raw.sc[x].y : raw.sc[x].x;
+                            const uint32_t s2 = (q >> 1) ? raw.s[x].y : raw.s[x].x;
                             const uint32_t sj = (r & 1) ^ (q & 1) ? s2 >> 16 : s2 & 0xffffu;
-                            *reinterpret_cast<uint4 *>(dst + tile_unit(r, 4 * j + t)) =
+                            *reinterpret_cast<uint4 *>(dst + tile_unit(r, 4 * j + kq)) =
                                 dequant_unit(r & 1 ? e[q ^ 1] : e[q], nib, bits_h2(sj * 0x10001u));
                         }
                     }
                 }
-                fence_proxy_async_smem();
-                mbar_arrive((V ? v_full : k_full) + (k & 1));
-                return true;
             };
-            using K_ = std::integral_constant<bool, false>;
-            using V_ = std::integral_constant<bool, true>;
-            load(K_{}, 0, rk);
-            for (int k = 0; k < n; k++) {
-                load(V_{}, k, rv);
-                if (!store(K_{}, k, rk)) break;
-                if (k + 1 < n) load(K_{}, k + 1, rk);
-                if (!store(V_{}, k, rv)) break;
+            Raw cur, next;
+            load(job, page_of(job), cur);
+            int page = page_of(job + kStep);
+            for (; job < jobs; job += kStep) {
+                if (job + kStep < jobs) load(job + kStep, page, next);
+                page = page_of(job + 2 * kStep);
+                if (!wait_empty(job)) break;
+                store(job, cur);
+                announce(job);
+                cur = next;
             }
         } else {
-            // blocks K0 V0 K1 V1 ...: a block is announced when the second one behind it has been requested
-            auto full_of = [&](int i) { return (i & 1 ? v_full : k_full) + ((i >> 1) & 1); };
-            int issued = 0;
-            for (; issued < 2 * n; issued++) {
-                const int k = issued >> 1, is_v = issued & 1, j0 = kt.tile(c0 + k) * KT;
-                uint8_t *dst = (is_v ? sV : sK) + (k & 1) * C::kTile;
-                if (k >= 2 && !mbar_wait((is_v ? v_empty : k_empty) + (k & 1), ((k >> 1) - 1) & 1, abort_flag, a.err,
-                                         DEVERR_TIMEOUT_PRODUCER))
-                    break;
-                for (int it = pt; it < KT * NU; it += C::kProducers) {
-                    const int r = it / NU, un = it % NU, pr = (j0 + r) & (P - 1);
-                    const uint8_t *seg = seg_of(j0 + r);
-                    const uint32_t d = smem_u32(dst + tile_unit(r, un));
-                    const int su = un ^ (is_v ? kv_swz_v(false, D, pr) : kv_swz_k(false, pr));
-                    const uint8_t *src = seg ? seg + kv_row_off(a.g, is_v, pr) + su * 16 : a.pool;
-                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(d), "l"(src), "r"(seg ? 16 : 0) : "memory");
+            // a job is announced when the second one behind it has been requested
+            int issued = 0, page = page_of(job);
+            for (; job < jobs; job += kStep, issued++) {
+                int live;
+                const uint8_t *blk = block_of(job, page, live);
+                page = page_of(job + kStep);
+                if (!wait_empty(job)) break;
+                const int is_v = (job >> 3) & 1, r0 = (job & 7) * 16;
+                const uint32_t dst = smem_u32((is_v ? sV : sK) + ((job >> 4) & 1) * C::kTile);
+#pragma unroll
+                for (int x = 0; x < 16 * NU / 32; x++) {
+                    const int it = lane + 32 * x, r = it / NU, u = it % NU;
+                    const int su = u ^ (is_v ? kv_swz_v(false, D, r) : kv_swz_k(false, r));
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + tile_unit(r0 + r, u)),
+                                 "l"(blk + (is_v * 16 + r) * C::RB + su * 16), "r"(r < live ? 16 : 0)
+                                 : "memory");
                 }
                 asm volatile("cp.async.commit_group;" ::: "memory");
                 if (issued >= 2) {
                     asm volatile("cp.async.wait_group 2;" ::: "memory");
-                    fence_proxy_async_smem();
-                    mbar_arrive(full_of(issued - 2));
+                    announce(job - 2 * kStep);
                 }
             }
             asm volatile("cp.async.wait_all;" ::: "memory");
-            fence_proxy_async_smem();
-            for (int i = max(0, issued - 2); i < issued; i++) mbar_arrive(full_of(i));
+            for (int i = min(issued, 2); i > 0; i--) announce(job - i * kStep);
         }
     } else {
         // ---- softmax, a row a thread
@@ -1040,7 +1106,7 @@ __global__ void __launch_bounds__(384, 1) kv_attend_many_kernel(const __grid_con
             bool ok = true;
             for (int k = 0; k < n; k++) {
                 const int j0 = kt.tile(c0 + k) * KT;
-                ok = mbar_wait(s_full + w, k & 1, abort_flag, a.err, DEVERR_TIMEOUT_EPILOGUE);
+                ok = kv_wait(s_full + w, k & 1, abort_flag, a.err, DEVERR_TIMEOUT_EPILOGUE);
                 if (__any_sync(0xffffffffu, !ok)) { ok = false; break; }
                 tc_fence_after();
                 float s[4][32];
@@ -1095,7 +1161,7 @@ __global__ void __launch_bounds__(384, 1) kv_attend_many_kernel(const __grid_con
                 tc_fence_before();
                 mbar_arrive(p_full + w);
             }
-            if (ok) ok = mbar_wait(o_full + w, (n - 1) & 1, abort_flag, a.err, DEVERR_TIMEOUT_EPILOGUE);
+            if (ok) ok = kv_wait(o_full + w, (n - 1) & 1, abort_flag, a.err, DEVERR_TIMEOUT_EPILOGUE);
             if (!__any_sync(0xffffffffu, !ok)) {
                 tc_fence_after();
                 bf16 *op = a.out + (long long)(row0 + tok) * a.o_row + (long long)(head * G + hg) * a.o_head;
@@ -1149,12 +1215,12 @@ __global__ void __launch_bounds__(384, 1) kv_attend_many_kernel(const __grid_con
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == 11) {
+    if (warp == 15) {
         tc_fence_after();
         tmem_dealloc(tbase, 512);
     }
-    if (parts > 1 && kv_last_part(a.cnt + unit, parts, flag))
-        kv_join_parts<D>(a.ws + (long long)unit * a.splits * 256 * (D + 2), 256ll * (D + 2), parts, rows, [&](int r) {
+    if (parts > 1 && warp < 8 && kv_last_part<C::kSoftmax>(a.cnt + unit, parts, flag))
+        kv_join_parts<D, C::kSoftmax>(a.ws + (long long)unit * a.splits * 256 * (D + 2), 256ll * (D + 2), parts, rows, [&](int r) {
             const int x = base + r;
             return a.out + (long long)(row0 + x / G) * a.o_row + (long long)(head * G + x % G) * a.o_head;
         });
