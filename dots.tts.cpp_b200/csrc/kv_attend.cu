@@ -766,6 +766,13 @@ DTTS_DEV uint4 dequant_unit(uint32_t w, const NibbleMasks &k, __half2 s) {
 // where dim i of 8 stands inside such a unit
 __host__ __device__ constexpr int unit_dim(bool i4, int pos) { return i4 ? (pos >> 1) + (pos & 1) * 4 : pos; }
 
+// true in one lane of a converged warp
+DTTS_DEV bool elect_one() {
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}\n" : "=r"(p));
+    return p != 0;
+}
+
 // Waits like mbar_wait, asleep in the barrier for up to a microsecond a try, so that
 // a waiting role leaves the issue slots to the working ones.
 DTTS_DEV bool kv_wait(uint64_t *bar, uint32_t parity, volatile int *abort_flag, int *err, int code) {
@@ -866,55 +873,73 @@ __global__ void __launch_bounds__(512, 1) kv_attend_many_kernel(const __grid_con
 
     if (warp >= 8) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kOtherRegs));
     else asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::kSoftmaxRegs));
+    // the same answer in all lanes of the warp
+    auto wait_all = [&](uint64_t *bar, uint32_t parity, int code) {
+        return __all_sync(0xffffffffu, kv_wait(bar, parity, abort_flag, a.err, code)) != 0;
+    };
     if (warp == 15) {
-        if (lane == 0) {
-            bool ok = true;
-            auto scores = [&](int w, int k) {   // S_w = Q_w K^T of block k
-                const uint32_t qa = smem_u32(sQ + w * C::kTile), ka = smem_u32(sK + (k & 1) * C::kTile);
+        // The whole warp runs the loop, so that addresses and descriptors stay uniform; one elected lane issues.
+        const bool lead = elect_one();
+        bool ok = true;
+        const uint64_t qd = sdesc_k128(smem_u32(sQ)), kd = sdesc_k128(smem_u32(sK)), vd = sdesc_mn128(smem_u32(sV));
+        constexpr uint64_t kTileD = C::kTile >> 4;   // descriptor units of 16 bytes
+        auto scores = [&](int w, int k) {   // S_w = Q_w K^T of block k
+            const uint64_t qw = qd + w * kTileD, kw = kd + (k & 1) * kTileD;
+            const uint32_t d = tbase + w * 128;
+            if (lead) {
 #pragma unroll
                 for (int x = 0; x < D / 16; x++) {
-                    const uint32_t off = (x >> 2) * kChunk + (x & 3) * 32;
-                    tc_mma_bf16(tbase + w * 128, sdesc_k128(qa + off), sdesc_k128(ka + off), C::idesc(128), x ? 1u : 0u);
+                    const uint64_t off = ((x >> 2) * kChunk + (x & 3) * 32) >> 4;
+                    tc_mma_bf16(d, qw + off, kw + off, C::idesc(128), x ? 1u : 0u);
                 }
                 tc_commit(s_full + w);
-            };
-            ok = ok && kv_wait(k_full, 0, abort_flag, a.err, DEVERR_TIMEOUT_MMA);
+            }
+            __syncwarp();
+        };
+        ok = wait_all(k_full, 0, DEVERR_TIMEOUT_MMA);
+        for (int w = 0; w < tiles && ok; w++) {
+            ok = wait_all(q_full + w, 0, DEVERR_TIMEOUT_MMA);
+            if (!ok) break;
+            tc_fence_after();
+            scores(w, 0);
+        }
+        if (ok && lead) tc_commit(k_empty);
+        __syncwarp();
+        for (int k = 0; k < n && ok; k++) {
+            ok = wait_all(v_full + (k & 1), (k >> 1) & 1, DEVERR_TIMEOUT_MMA);
             for (int w = 0; w < tiles && ok; w++) {
-                ok = kv_wait(q_full + w, 0, abort_flag, a.err, DEVERR_TIMEOUT_MMA);
+                ok = wait_all(p_full + w, k & 1, DEVERR_TIMEOUT_MMA);
                 if (!ok) break;
                 tc_fence_after();
-                scores(w, 0);
-            }
-            if (ok) tc_commit(k_empty);
-            for (int k = 0; k < n && ok; k++) {
-                ok = kv_wait(v_full + (k & 1), (k >> 1) & 1, abort_flag, a.err, DEVERR_TIMEOUT_MMA);
-                for (int w = 0; w < tiles && ok; w++) {
-                    ok = kv_wait(p_full + w, k & 1, abort_flag, a.err, DEVERR_TIMEOUT_MMA);
-                    if (!ok) break;
-                    tc_fence_after();
-                    const uint32_t va = smem_u32(sV + (k & 1) * C::kTile);
+                const uint64_t vw = vd + (k & 1) * kTileD;
+                const uint32_t d = tbase + 256 + w * 128, p = tbase + w * 128;
+                if (lead) {
 #pragma unroll
                     for (int x = 0; x < KT / 16; x++)
-                        tc_mma_ts(tbase + 256 + w * 128, tbase + w * 128 + 8 * x, sdesc_mn128(va + x * 2048),
-                                  C::idesc(D) | (1u << 16), k || x ? 1u : 0u);
+                        tc_mma_ts(d, p + 8 * x, vw + x * (2048 >> 4), C::idesc(D) | (1u << 16), k || x ? 1u : 0u);
                     tc_commit(o_full + w);
-                    if (k + 1 == n) continue;
-                    // S_w takes the columns P_w is read from: only after that product is done
-                    ok = kv_wait(k_full + ((k + 1) & 1), ((k + 1) >> 1) & 1, abort_flag, a.err, DEVERR_TIMEOUT_MMA) &&
-                         kv_wait(o_full + w, k & 1, abort_flag, a.err, DEVERR_TIMEOUT_MMA);
-                    if (!ok) break;
-                    tc_fence_after();
-                    scores(w, k + 1);
                 }
+                __syncwarp();
+                if (k + 1 == n) continue;
+                // S_w takes the columns P_w is read from: only after that product is done
+                ok = wait_all(k_full + ((k + 1) & 1), ((k + 1) >> 1) & 1, DEVERR_TIMEOUT_MMA) &&
+                     wait_all(o_full + w, k & 1, DEVERR_TIMEOUT_MMA);
                 if (!ok) break;
+                tc_fence_after();
+                scores(w, k + 1);
+            }
+            if (!ok) break;
+            if (lead) {
                 tc_commit(v_empty + (k & 1));
                 if (k + 1 < n) tc_commit(k_empty + ((k + 1) & 1));
             }
-            // every product done before TMEM is given back (also after an abort)
-            tc_commit(drain);
-            const unsigned long long t0 = globaltimer_ns();
-            while (!mbar_try_wait(drain, 0) && globaltimer_ns() - t0 < kWaitLimitNs) {}
+            __syncwarp();
         }
+        // every product done before TMEM is given back (also after an abort)
+        if (lead) tc_commit(drain);
+        __syncwarp();
+        const unsigned long long t0 = globaltimer_ns();
+        while (!mbar_try_wait(drain, 0) && globaltimer_ns() - t0 < kWaitLimitNs) {}
         __syncwarp();
     } else if (warp >= 8) {
         // ---- pages -> tiles.  A job is 16 rows of K or V, one block of a page: jobs K0 .. K7, V0 .. V7
@@ -936,8 +961,7 @@ __global__ void __launch_bounds__(512, 1) kv_attend_many_kernel(const __grid_con
         };
         auto wait_empty = [&](int job) {
             const int k = job >> 4;
-            return k < 2 || kv_wait((job & 8 ? v_empty : k_empty) + (k & 1), ((k >> 1) - 1) & 1, abort_flag, a.err,
-                                    DEVERR_TIMEOUT_PRODUCER);
+            return k < 2 || wait_all((job & 8 ? v_empty : k_empty) + (k & 1), ((k >> 1) - 1) & 1, DEVERR_TIMEOUT_PRODUCER);
         };
         auto announce = [&](int job) {
             fence_proxy_async_smem();
@@ -1106,8 +1130,8 @@ __global__ void __launch_bounds__(512, 1) kv_attend_many_kernel(const __grid_con
             bool ok = true;
             for (int k = 0; k < n; k++) {
                 const int j0 = kt.tile(c0 + k) * KT;
-                ok = kv_wait(s_full + w, k & 1, abort_flag, a.err, DEVERR_TIMEOUT_EPILOGUE);
-                if (__any_sync(0xffffffffu, !ok)) { ok = false; break; }
+                ok = wait_all(s_full + w, k & 1, DEVERR_TIMEOUT_EPILOGUE);
+                if (!ok) break;
                 tc_fence_after();
                 float s[4][32];
                 tmem_ld32x2(ts, ts + 32, s[0], s[1]);
@@ -1161,8 +1185,7 @@ __global__ void __launch_bounds__(512, 1) kv_attend_many_kernel(const __grid_con
                 tc_fence_before();
                 mbar_arrive(p_full + w);
             }
-            if (ok) ok = kv_wait(o_full + w, (n - 1) & 1, abort_flag, a.err, DEVERR_TIMEOUT_EPILOGUE);
-            if (!__any_sync(0xffffffffu, !ok)) {
+            if (ok && wait_all(o_full + w, (n - 1) & 1, DEVERR_TIMEOUT_EPILOGUE)) {
                 tc_fence_after();
                 bf16 *op = a.out + (long long)(row0 + tok) * a.o_row + (long long)(head * G + hg) * a.o_head;
                 float *wp = a.ws + (((long long)unit * a.splits + split) * 256 + rr) * (D + 2);
