@@ -735,6 +735,37 @@ DTTS_DEV void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
           "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(taddr)
         : "memory");
 }
+// 32 columns on their way to r; r may be used after tmem_ld_wait(r), which waits
+// for all loads of the warp
+DTTS_DEV void tmem_ld32_issue(uint32_t taddr, uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+          "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+          "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(taddr)
+        : "memory");
+}
+DTTS_DEV void tmem_ld_wait(uint32_t (&r)[32]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                   "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]),
+                   "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]),
+                   "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29])
+                 :
+                 : "memory");
+    asm volatile("" : "+r"(r[30]), "+r"(r[31])::"memory");   // an asm has 30 operands at most
+}
+DTTS_DEV void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};\n" ::"r"(r[0]),
+        "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+        "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(taddr)
+        : "memory");
+}
 DTTS_DEV void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 DTTS_DEV uint64_t sdesc_mn128(uint32_t saddr) {
     return (sdesc_k128(saddr) & ~(0x3fffull << 16)) | ((uint64_t)(kChunk >> 4) << 16);
@@ -765,6 +796,9 @@ DTTS_DEV uint4 dequant_unit(uint32_t w, const NibbleMasks &k, __half2 s) {
 }
 // where dim i of 8 stands inside such a unit
 __host__ __device__ constexpr int unit_dim(bool i4, int pos) { return i4 ? (pos >> 1) + (pos & 1) * 4 : pos; }
+
+// the lowest n bits, n clamped to 0 .. 32
+DTTS_DEV uint32_t low_bits(int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; }
 
 // true in one lane of a converged warp
 DTTS_DEV bool elect_one() {
@@ -1126,6 +1160,7 @@ __global__ void __launch_bounds__(512, 1) kv_attend_many_kernel(const __grid_con
             const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
             const uint32_t ts = tbase + w * 128 + lanes, to = tbase + 256 + w * 128 + lanes;
             const int q_min = i0 + (base + w * 128) / G, q_max = i0 + (base + min(rows, w * 128 + 128) - 1) / G;
+            const int qlo = a.window ? qi - a.window : -1;   // the last row before the window
             float m = -INFINITY, l = 0.f;
             bool ok = true;
             for (int k = 0; k < n; k++) {
@@ -1133,52 +1168,64 @@ __global__ void __launch_bounds__(512, 1) kv_attend_many_kernel(const __grid_con
                 ok = wait_all(s_full + w, k & 1, DEVERR_TIMEOUT_EPILOGUE);
                 if (!ok) break;
                 tc_fence_after();
-                float s[4][32];
-                tmem_ld32x2(ts, ts + 32, s[0], s[1]);
-                tmem_ld32x2(ts + 64, ts + 96, s[2], s[3]);
-                if (!(j0 + KT - 1 <= q_min && (a.window == 0 || j0 > q_max - a.window || j0 + KT - 1 < a.sinks))) {
+                const bool all = j0 + KT - 1 <= q_min && (a.window == 0 || j0 > q_max - a.window || j0 + KT - 1 < a.sinks);
+                // scores of columns 32 x .. 32 x + 31, -inf where this row does not see the key
+                auto mask = [&](uint32_t (&s)[32], int x) {
+                    if (all) return;
+                    const uint32_t seen = low_bits(qi - j0 - 32 * x + 1) &
+                                          (~low_bits(qlo - j0 - 32 * x + 1) | low_bits(a.sinks - j0 - 32 * x));
 #pragma unroll
-                    for (int x = 0; x < 4; x++)
-#pragma unroll
-                        for (int y = 0; y < 32; y++)
-                            if (!kv_visible(j0 + 32 * x + y, qi, a.window, a.sinks)) s[x][y] = -INFINITY;
-                }
-                float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-                for (int y = 0; y < 32; y++)
-#pragma unroll
-                    for (int x = 0; x < 4; x++) mx[x] = fmaxf(mx[x], s[x][y]);
-                const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * c;
-                if (__any_sync(0xffffffffu, top > m + 8.f || (m == -INFINITY && top > m))) {
+                    for (int y = 0; y < 32; y++) s[y] = (seen >> y) & 1u ? s[y] : 0xff800000u;
+                };
+                auto raise = [&](float top) {   // the running maximum to top, O and l with it
                     const float mn = fmaxf(m, top), corr = mn == -INFINITY ? 1.f : exp2f(m - mn);
                     if (k > 0) {
 #pragma unroll 1
                         for (int x = 0; x < D; x += 32) {
                             float o[32];
-                            uint32_t p[32];
+                            uint32_t q[32];
                             tmem_ld32(to + x, o);
 #pragma unroll
-                            for (int y = 0; y < 32; y++) p[y] = __float_as_uint(o[y] * corr);
-                            tmem_st32(to + x, p);
+                            for (int y = 0; y < 32; y++) q[y] = __float_as_uint(o[y] * corr);
+                            tmem_st32(to + x, q);
                         }
                         tmem_wait_st();
                     }
                     l *= corr;
                     m = mn;
+                };
+                // Two passes over the block's scores, each with one chunk of columns on its way while the one
+                // before is computed: the maximum, then P, which replaces the scores.
+                uint32_t s[2][32];
+                float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                tmem_ld32_issue(ts, s[0]);
+                tmem_ld_wait(s[0]);
+#pragma unroll
+                for (int x = 0; x < 4; x++) {
+                    tmem_ld32_issue(ts + 32 * ((x + 1) & 3), s[(x + 1) & 1]);
+                    mask(s[x & 1], x);
+#pragma unroll
+                    for (int y = 0; y < 32; y++) mx[y & 3] = fmaxf(mx[y & 3], __uint_as_float(s[x & 1][y]));
+                    tmem_ld_wait(s[(x + 1) & 1]);
                 }
+                const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * c;
+                if (__any_sync(0xffffffffu, top > m + 8.f)) raise(top);   // m = -inf: any score
                 const float mu = m == -INFINITY ? 0.f : m;
                 float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int x = 0; x < 2; x++) {
-                    uint32_t p[32];
+                for (int x = 0; x < 4; x++) {
+                    if (x < 3) tmem_ld32_issue(ts + 32 * (x + 1), s[(x + 1) & 1]);
+                    mask(s[x & 1], x);
+                    uint32_t p[16];
 #pragma unroll
-                    for (int y = 0; y < 32; y++) {
-                        const float p0 = ex2_hw(fmaf(s[2 * x + (y >> 4)][(2 * y) & 31], c, -mu));
-                        const float p1 = ex2_hw(fmaf(s[2 * x + (y >> 4)][(2 * y + 1) & 31], c, -mu));
+                    for (int y = 0; y < 16; y++) {
+                        const float p0 = ex2_hw(fmaf(__uint_as_float(s[x & 1][2 * y]), c, -mu));
+                        const float p1 = ex2_hw(fmaf(__uint_as_float(s[x & 1][2 * y + 1]), c, -mu));
                         sum[y & 3] += p0 + p1;
                         p[y] = I4 ? h2_bits(__floats2half2_rn(p0, p1)) : pack_bf16x2(p0, p1);
                     }
-                    tmem_st32(ts + 32 * x, p);
+                    if (x < 3) tmem_ld_wait(s[(x + 1) & 1]);
+                    tmem_st16(ts + 16 * x, p);   // columns that both passes have read
                 }
                 l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
                 tmem_wait_st();
