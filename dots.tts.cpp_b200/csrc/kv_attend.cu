@@ -724,17 +724,6 @@ DTTS_DEV void tc_mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32
         "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate)
         : "memory");
 }
-DTTS_DEV void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], "
-        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};\n"
-        ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
-          "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]),
-          "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]),
-          "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(taddr)
-        : "memory");
-}
 // 32 columns on their way to r; r may be used after tmem_ld_wait(r), which waits
 // for all loads of the warp
 DTTS_DEV void tmem_ld32_issue(uint32_t taddr, uint32_t (&r)[32]) {
@@ -766,6 +755,18 @@ DTTS_DEV void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
         "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(taddr)
         : "memory");
 }
+DTTS_DEV void tmem_ld16(uint32_t taddr, float (&v)[16]) {
+    uint32_t r[16];
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n\t"
+        "tcgen05.wait::ld.sync.aligned;\n"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr)
+        : "memory");
+#pragma unroll
+    for (int i = 0; i < 16; i++) v[i] = __uint_as_float(r[i]);
+}
 DTTS_DEV void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 DTTS_DEV uint64_t sdesc_mn128(uint32_t saddr) {
     return (sdesc_k128(saddr) & ~(0x3fffull << 16)) | ((uint64_t)(kChunk >> 4) << 16);
@@ -776,7 +777,7 @@ DTTS_DEV int tile_unit(int r, int u) { return (u >> 3) * kChunk + r * 128 + (((u
 template <int D, bool I4>
 struct ManyCfg {
     static constexpr int KT = kKvManyKeyTile, kTile = D / 64 * kChunk;   // one operand tile of 128 rows
-    static constexpr int kSoftmax = 256, kProducerWarps = 7, kThreads = 512;
+    static constexpr int kSoftmax = 256, kProducerWarps = 6, kThreads = 512;
     // registers a thread: 128 at launch (512 x 128 = 65536), then 256 x (176 + 80) = 65536
     static constexpr int kSoftmaxRegs = 176, kOtherRegs = 80;
     static constexpr int kSmem = 6 * kTile + 256 + 1024;      // Q x 2, K x 2, V x 2, barriers
@@ -811,6 +812,15 @@ DTTS_DEV bool elect_one() {
 // a waiting role leaves the issue slots to the working ones.
 DTTS_DEV bool kv_wait(uint64_t *bar, uint32_t parity, volatile int *abort_flag, int *err, int code) {
     const uint32_t addr = smem_u32(bar);
+    uint32_t done;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}\n"
+        : "=r"(done)
+        : "r"(addr), "r"(parity)
+        : "memory");
+    if (done) return true;
     unsigned long long t0 = 0;
     while (true) {
         uint32_t ok;
@@ -835,15 +845,19 @@ DTTS_DEV bool kv_wait(uint64_t *bar, uint32_t parity, volatile int *abort_flag, 
 
 // Attention of up to 256 rows (new token x query head of one kv head, two tiles of
 // 128) of one sequence over a part of its keys, in blocks of 128 keys.
-//   warps 0-3, 4-7: softmax of tile 0, 1, one row a thread (S from TMEM, P back into
-//                   the same columns, O rescaled when the row maximum has grown by
-//                   more than 2^8, so P <= 2^8 stays in half's range);
-//   warps 8-14:     K and V rows from the pages into swizzled tiles (4-bit rows become
+//   warps 0-3, 4-7: softmax of tile 0, 1, one row a thread, half a block (64 keys) at
+//                   a time: S from TMEM, P back into the same columns, O rescaled
+//                   when the row maximum has grown by more than 2^8 (so P <= 2^8 stays
+//                   in half's range);
+//   warps 8-13:     K and V rows from the pages into swizzled tiles (4-bit rows become
 //                   exact halves on the way), 16 rows of K or V a job, two stages;
-//   warp 15:        S = Q K^T and O += P V on tcgen05 (P from TMEM, V MN-major).
-// The two tiles alternate: while one's softmax runs, the other's products do.
-// Bound by the softmax's exponentials (128 x 128 a block and tile at 16 a clock and
-// SM, as long as its two products take) and by shared memory reads of the operands.
+//   warps 14, 15:   S = Q K^T and O += P V of tile 0, 1 on tcgen05 (P from TMEM, V
+//                   MN-major); while one warp waits, the other's products run.
+// A tile has two score buffers of 64 columns: the scores of the next half are
+// computed while the softmax of this one runs and P V of the one before, so no role
+// waits for a round trip.  Bound by the softmax's exponentials (128 x 128 a block
+// and tile at 16 a clock and SM) and by the operands' shared memory reads, which take
+// longer than the products themselves (S: 128 x 64 x 16 a step reads 6 KB in 32 clocks).
 // 4-bit rows: all operands half, Q after an exact power-of-two scaling of the row, P
 // rounded by 2^-11.  bf16 rows: P is rounded to bf16 (2^-8 of the P-weighted mean
 // of |v|, the size of the output's own rounding): a second term would cost half as
@@ -856,9 +870,10 @@ __global__ void __launch_bounds__(512, 1) kv_attend_many_kernel(const __grid_con
     uint8_t *sm = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint8_t *sQ = sm, *sK = sm + 2 * C::kTile, *sV = sm + 4 * C::kTile;
     uint64_t *bars = reinterpret_cast<uint64_t *>(sm + 6 * C::kTile);
-    uint64_t *q_full = bars, *s_full = bars + 2, *p_full = bars + 4, *o_full = bars + 6;
-    uint64_t *k_full = bars + 8, *k_empty = bars + 10, *v_full = bars + 12, *v_empty = bars + 14, *drain = bars + 16;
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 17);
+    // s_full, p_full, pv_done: [tile][half]
+    uint64_t *q_full = bars, *s_full = bars + 2, *p_full = bars + 6, *pv_done = bars + 10;
+    uint64_t *k_full = bars + 14, *k_empty = bars + 16, *v_full = bars + 18, *v_empty = bars + 20, *drain = bars + 22;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 24);
     int *flag = reinterpret_cast<int *>(tmem_slot + 1);
     volatile int *abort_flag = flag + 1;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -877,19 +892,23 @@ __global__ void __launch_bounds__(512, 1) kv_attend_many_kernel(const __grid_con
     const int parts = min(a.splits, max(1, (kt.n + a.tiles_per_split - 1) / a.tiles_per_split));
     if (split >= parts) return;
     const int c0 = (int)((long long)kt.n * split / parts), c1 = (int)((long long)kt.n * (split + 1) / parts), n = c1 - c0;
+    // half blocks of 64 keys; the last one stays out where no row sees it
+    const int halves = 2 * n - (kt.tile(c1 - 1) * KT + 64 > i_last ? 1 : 0);
 
     if (tid == 0) {
         for (int w = 0; w < 2; w++) {
             mbar_init(q_full + w, 128);
-            mbar_init(s_full + w, 1);
-            mbar_init(p_full + w, 128);
-            mbar_init(o_full + w, 1);
+            for (int h = 0; h < 2; h++) {
+                mbar_init(s_full + 2 * w + h, 1);
+                mbar_init(p_full + 2 * w + h, 128);
+                mbar_init(pv_done + 2 * w + h, 1);
+            }
             mbar_init(k_full + w, 8);
-            mbar_init(k_empty + w, 1);
+            mbar_init(k_empty + w, tiles);
             mbar_init(v_full + w, 8);
-            mbar_init(v_empty + w, 1);
+            mbar_init(v_empty + w, tiles);
+            mbar_init(drain + w, 1);
         }
-        mbar_init(drain, 1);
         *flag = 0;
         *abort_flag = 0;
         fence_mbar_init();
@@ -911,69 +930,68 @@ __global__ void __launch_bounds__(512, 1) kv_attend_many_kernel(const __grid_con
     auto wait_all = [&](uint64_t *bar, uint32_t parity, int code) {
         return __all_sync(0xffffffffu, kv_wait(bar, parity, abort_flag, a.err, code)) != 0;
     };
-    if (warp == 15) {
+    if (warp >= 14) {
+        const int w = warp - 14;
         // The whole warp runs the loop, so that addresses and descriptors stay uniform; one elected lane issues.
         const bool lead = elect_one();
-        bool ok = true;
-        const uint64_t qd = sdesc_k128(smem_u32(sQ)), kd = sdesc_k128(smem_u32(sK)), vd = sdesc_mn128(smem_u32(sV));
         constexpr uint64_t kTileD = C::kTile >> 4;   // descriptor units of 16 bytes
-        auto scores = [&](int w, int k) {   // S_w = Q_w K^T of block k
-            const uint64_t qw = qd + w * kTileD, kw = kd + (k & 1) * kTileD;
-            const uint32_t d = tbase + w * 128;
+        constexpr uint64_t kHalfD = (64 * 128) >> 4;
+        const uint64_t qd = sdesc_k128(smem_u32(sQ)) + w * kTileD, kd = sdesc_k128(smem_u32(sK)), vd = sdesc_mn128(smem_u32(sV));
+        uint64_t *sf = s_full + 2 * w, *pf = p_full + 2 * w, *pd = pv_done + 2 * w;
+        auto scores = [&](int i) {   // of half block i: Q K^T, 64 keys
+            const uint64_t kw = kd + ((i >> 1) & 1) * kTileD + (i & 1) * kHalfD;
+            const uint32_t d = tbase + w * 128 + (i & 1) * 64;
             if (lead) {
 #pragma unroll
                 for (int x = 0; x < D / 16; x++) {
                     const uint64_t off = ((x >> 2) * kChunk + (x & 3) * 32) >> 4;
-                    tc_mma_bf16(d, qw + off, kw + off, C::idesc(128), x ? 1u : 0u);
+                    tc_mma_bf16(d, qd + off, kw + off, C::idesc(64), x ? 1u : 0u);
                 }
-                tc_commit(s_full + w);
+                tc_commit(sf + (i & 1));
             }
             __syncwarp();
         };
-        ok = wait_all(k_full, 0, DEVERR_TIMEOUT_MMA);
-        for (int w = 0; w < tiles && ok; w++) {
-            ok = wait_all(q_full + w, 0, DEVERR_TIMEOUT_MMA);
-            if (!ok) break;
-            tc_fence_after();
-            scores(w, 0);
-        }
-        if (ok && lead) tc_commit(k_empty);
-        __syncwarp();
-        for (int k = 0; k < n && ok; k++) {
-            ok = wait_all(v_full + (k & 1), (k >> 1) & 1, DEVERR_TIMEOUT_MMA);
-            for (int w = 0; w < tiles && ok; w++) {
-                ok = wait_all(p_full + w, k & 1, DEVERR_TIMEOUT_MMA);
+        if (w < tiles) {
+            bool ok = wait_all(k_full, 0, DEVERR_TIMEOUT_MMA) && wait_all(q_full + w, 0, DEVERR_TIMEOUT_MMA);
+            if (ok) {
+                tc_fence_after();
+                scores(0);
+            }
+            for (int i = 0; i < halves && ok; i++) {
+                const int k = i >> 1, h = i & 1;
+                if (i + 1 < halves) {
+                    // the next half's scores take the columns that P of the half before this one is read from
+                    if (h == 1) ok = wait_all(k_full + ((k + 1) & 1), ((k + 1) >> 1) & 1, DEVERR_TIMEOUT_MMA);
+                    if (ok && i >= 1) ok = wait_all(pd + (h ^ 1), ((i - 1) >> 1) & 1, DEVERR_TIMEOUT_MMA);
+                    if (!ok) break;
+                    tc_fence_after();
+                    scores(i + 1);
+                }
+                if (h == 0) {
+                    if (lead) tc_commit(k_empty + (k & 1));   // both halves' scores are issued
+                    __syncwarp();
+                    ok = wait_all(v_full + (k & 1), (k >> 1) & 1, DEVERR_TIMEOUT_MMA);
+                }
+                ok = ok && wait_all(pf + h, k & 1, DEVERR_TIMEOUT_MMA);
                 if (!ok) break;
                 tc_fence_after();
-                const uint64_t vw = vd + (k & 1) * kTileD;
-                const uint32_t d = tbase + 256 + w * 128, p = tbase + w * 128;
+                const uint64_t vw = vd + (k & 1) * kTileD + h * kHalfD;
+                const uint32_t d = tbase + 256 + w * 128, p = tbase + w * 128 + h * 64;
                 if (lead) {
 #pragma unroll
-                    for (int x = 0; x < KT / 16; x++)
-                        tc_mma_ts(d, p + 8 * x, vw + x * (2048 >> 4), C::idesc(D) | (1u << 16), k || x ? 1u : 0u);
-                    tc_commit(o_full + w);
+                    for (int x = 0; x < 4; x++)
+                        tc_mma_ts(d, p + 8 * x, vw + x * (2048 >> 4), C::idesc(D) | (1u << 16), i || x ? 1u : 0u);
+                    tc_commit(pd + h);
+                    if (h == 1) tc_commit(v_empty + (k & 1));
                 }
                 __syncwarp();
-                if (k + 1 == n) continue;
-                // S_w takes the columns P_w is read from: only after that product is done
-                ok = wait_all(k_full + ((k + 1) & 1), ((k + 1) >> 1) & 1, DEVERR_TIMEOUT_MMA) &&
-                     wait_all(o_full + w, k & 1, DEVERR_TIMEOUT_MMA);
-                if (!ok) break;
-                tc_fence_after();
-                scores(w, k + 1);
             }
-            if (!ok) break;
-            if (lead) {
-                tc_commit(v_empty + (k & 1));
-                if (k + 1 < n) tc_commit(k_empty + ((k + 1) & 1));
-            }
-            __syncwarp();
         }
         // every product done before TMEM is given back (also after an abort)
-        if (lead) tc_commit(drain);
+        if (lead) tc_commit(drain + w);
         __syncwarp();
         const unsigned long long t0 = globaltimer_ns();
-        while (!mbar_try_wait(drain, 0) && globaltimer_ns() - t0 < kWaitLimitNs) {}
+        while (!mbar_try_wait(drain + w, 0) && globaltimer_ns() - t0 < kWaitLimitNs) {}
         __syncwarp();
     } else if (warp >= 8) {
         // ---- pages -> tiles.  A job is 16 rows of K or V, one block of a page: jobs K0 .. K7, V0 .. V7
@@ -1163,12 +1181,13 @@ __global__ void __launch_bounds__(512, 1) kv_attend_many_kernel(const __grid_con
             const int qlo = a.window ? qi - a.window : -1;   // the last row before the window
             float m = -INFINITY, l = 0.f;
             bool ok = true;
-            for (int k = 0; k < n; k++) {
-                const int j0 = kt.tile(c0 + k) * KT;
-                ok = wait_all(s_full + w, k & 1, DEVERR_TIMEOUT_EPILOGUE);
+            for (int i = 0; i < halves; i++) {
+                const int h = i & 1, j0 = kt.tile(c0 + (i >> 1)) * KT + 64 * h;
+                const uint32_t ti = ts + 64 * h;
+                ok = wait_all(s_full + 2 * w + h, (i >> 1) & 1, DEVERR_TIMEOUT_EPILOGUE);
                 if (!ok) break;
                 tc_fence_after();
-                const bool all = j0 + KT - 1 <= q_min && (a.window == 0 || j0 > q_max - a.window || j0 + KT - 1 < a.sinks);
+                const bool all = j0 + 63 <= q_min && (a.window == 0 || j0 > q_max - a.window || j0 + 63 < a.sinks);
                 // scores of columns 32 x .. 32 x + 31, -inf where this row does not see the key
                 auto mask = [&](uint32_t (&s)[32], int x) {
                     if (all) return;
@@ -1177,62 +1196,60 @@ __global__ void __launch_bounds__(512, 1) kv_attend_many_kernel(const __grid_con
 #pragma unroll
                     for (int y = 0; y < 32; y++) s[y] = (seen >> y) & 1u ? s[y] : 0xff800000u;
                 };
-                auto raise = [&](float top) {   // the running maximum to top, O and l with it
-                    const float mn = fmaxf(m, top), corr = mn == -INFINITY ? 1.f : exp2f(m - mn);
-                    if (k > 0) {
-#pragma unroll 1
-                        for (int x = 0; x < D; x += 32) {
-                            float o[32];
-                            uint32_t q[32];
-                            tmem_ld32(to + x, o);
+                uint32_t s[2][32];
+                float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                tmem_ld32_issue(ti, s[0]);
+                tmem_ld_wait(s[0]);
+                tmem_ld32_issue(ti + 32, s[1]);
+                mask(s[0], 0);
 #pragma unroll
-                            for (int y = 0; y < 32; y++) q[y] = __float_as_uint(o[y] * corr);
-                            tmem_st32(to + x, q);
+                for (int y = 0; y < 32; y++) mx[y & 3] = fmaxf(mx[y & 3], __uint_as_float(s[0][y]));
+                tmem_ld_wait(s[1]);
+                mask(s[1], 1);
+#pragma unroll
+                for (int y = 0; y < 32; y++) mx[y & 3] = fmaxf(mx[y & 3], __uint_as_float(s[1][y]));
+                const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * c;
+                if (__any_sync(0xffffffffu, top > m + 8.f)) {   // m = -inf: any score
+                    // the running maximum rises to top, O and l with it
+                    const float mn = fmaxf(m, top), corr = mn == -INFINITY ? 1.f : exp2f(m - mn);
+                    if (i > 0) {
+                        ok = wait_all(pv_done + 2 * w + (h ^ 1), ((i - 1) >> 1) & 1, DEVERR_TIMEOUT_EPILOGUE);
+                        if (!ok) break;
+                        tc_fence_after();
+#pragma unroll 1
+                        for (int x = 0; x < D; x += 16) {
+                            float o[16];
+                            uint32_t q[16];
+                            tmem_ld16(to + x, o);
+#pragma unroll
+                            for (int y = 0; y < 16; y++) q[y] = __float_as_uint(o[y] * corr);
+                            tmem_st16(to + x, q);
                         }
-                        tmem_wait_st();
                     }
                     l *= corr;
                     m = mn;
-                };
-                // Two passes over the block's scores, each with one chunk of columns on its way while the one
-                // before is computed: the maximum, then P, which replaces the scores.
-                uint32_t s[2][32];
-                float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-                tmem_ld32_issue(ts, s[0]);
-                tmem_ld_wait(s[0]);
-#pragma unroll
-                for (int x = 0; x < 4; x++) {
-                    tmem_ld32_issue(ts + 32 * ((x + 1) & 3), s[(x + 1) & 1]);
-                    mask(s[x & 1], x);
-#pragma unroll
-                    for (int y = 0; y < 32; y++) mx[y & 3] = fmaxf(mx[y & 3], __uint_as_float(s[x & 1][y]));
-                    tmem_ld_wait(s[(x + 1) & 1]);
                 }
-                const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * c;
-                if (__any_sync(0xffffffffu, top > m + 8.f)) raise(top);   // m = -inf: any score
                 const float mu = m == -INFINITY ? 0.f : m;
                 float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int x = 0; x < 4; x++) {
-                    if (x < 3) tmem_ld32_issue(ts + 32 * (x + 1), s[(x + 1) & 1]);
-                    mask(s[x & 1], x);
+                for (int x = 0; x < 2; x++) {
                     uint32_t p[16];
 #pragma unroll
                     for (int y = 0; y < 16; y++) {
-                        const float p0 = ex2_hw(fmaf(__uint_as_float(s[x & 1][2 * y]), c, -mu));
-                        const float p1 = ex2_hw(fmaf(__uint_as_float(s[x & 1][2 * y + 1]), c, -mu));
+                        const float p0 = ex2_hw(fmaf(__uint_as_float(s[x][2 * y]), c, -mu));
+                        const float p1 = ex2_hw(fmaf(__uint_as_float(s[x][2 * y + 1]), c, -mu));
                         sum[y & 3] += p0 + p1;
                         p[y] = I4 ? h2_bits(__floats2half2_rn(p0, p1)) : pack_bf16x2(p0, p1);
                     }
-                    if (x < 3) tmem_ld_wait(s[(x + 1) & 1]);
-                    tmem_st16(ts + 16 * x, p);   // columns that both passes have read
+                    tmem_st16(ti + 16 * x, p);
                 }
                 l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
                 tmem_wait_st();
                 tc_fence_before();
-                mbar_arrive(p_full + w);
+                mbar_arrive(p_full + 2 * w + h);
             }
-            if (ok && wait_all(o_full + w, (n - 1) & 1, DEVERR_TIMEOUT_EPILOGUE)) {
+            const int last = halves - 1;   // its product follows all others into O
+            if (ok && wait_all(pv_done + 2 * w + (last & 1), (last >> 1) & 1, DEVERR_TIMEOUT_EPILOGUE)) {
                 tc_fence_after();
                 bf16 *op = a.out + (long long)(row0 + tok) * a.o_row + (long long)(head * G + hg) * a.o_head;
                 float *wp = a.ws + (((long long)unit * a.splits + split) * 256 + rr) * (D + 2);
