@@ -798,6 +798,24 @@ DTTS_DEV uint4 dequant_unit(uint32_t w, const NibbleMasks &k, __half2 s) {
 // where dim i of 8 stands inside such a unit
 __host__ __device__ constexpr int unit_dim(bool i4, int pos) { return i4 ? (pos >> 1) + (pos & 1) * 4 : pos; }
 
+// two fp32 operations in one instruction
+DTTS_DEV float2 fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("{\n\t.reg .b64 a, b, c, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
+        "fma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}\n"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return d;
+}
+DTTS_DEV float2 add2(float2 a, float2 b) {
+    float2 d;
+    asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tadd.rn.f32x2 d, a, b;\n\t"
+        "mov.b64 {%0, %1}, d;\n\t}\n"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+
 // the lowest n bits, n clamped to 0 .. 32
 DTTS_DEV uint32_t low_bits(int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; }
 
@@ -1023,10 +1041,17 @@ __global__ void __launch_bounds__(512, 1) kv_attend_many_kernel(const __grid_con
         constexpr int kStep = C::kProducerWarps;
         int job = warp - 8;
         if constexpr (I4) {
-            // K: lane = 4 r + t takes the words of dims 32 j + 8 t (all groups j) of rows r and r + 8;
-            // V: a lane takes 16-byte units (a group of dims each), two of them where D = 128
+            // A lane takes unit un = lane / 8 of rows lane % 8 and lane % 8 + 8: a quarter warp then stores eight
+            // rows of one unit, which the tile's swizzle spreads over all banks.  K: the words of dims 32 j +
+            // 8 un of all groups j; V: the dims of group un (D = 64: two groups a row, row by un / 2).
             const NibbleMasks nib;
-            constexpr int kV = D / 64, kPerRow = D / 32;   // V: units a lane, units a row
+            constexpr int kV = D / 64;   // V units a lane
+            const int lr = lane & 7, un = lane >> 3, vr = D == 128 ? lr : lr + 8 * (un >> 1), vu = D == 128 ? un : un & 1;
+            const uint32_t k_at = lr * C::RB + un * (D / 8), ks_at = 32 * C::RB + lr * C::SB;
+            const uint32_t v_at = (16 + vr) * C::RB + 16 * (vu ^ kv_swz_v(true, D, vr));
+            const uint32_t vs_at = 32 * C::RB + (16 + vr) * C::SB + 2 * vu;
+            const uint32_t k_to = lr * 128 + ((un ^ lr) << 4);                                        // + j: see below
+            const uint32_t v_to = (vu >> 1) * kChunk + vr * 128 + (((4 * (vu & 1)) ^ lr) << 4);       // vr % 8 = lr
             struct Raw {
                 uint4 w[2];
                 uint2 s[2];
@@ -1037,74 +1062,67 @@ __global__ void __launch_bounds__(512, 1) kv_attend_many_kernel(const __grid_con
                 if (jb & 8) {
 #pragma unroll
                     for (int x = 0; x < kV; x++) {
-                        const int it = lane + 32 * x, r = it / kPerRow, u = it % kPerRow;
                         raw.w[x] = make_uint4(0u, 0u, 0u, 0u);
                         raw.s[x].x = 0u;
-                        if (r >= live) continue;
-                        raw.w[x] = *reinterpret_cast<const uint4 *>(blk + (16 + r) * C::RB + 16 * (u ^ kv_swz_v(true, D, r)));
-                        raw.s[x].x = *reinterpret_cast<const uint16_t *>(blk + 32 * C::RB + (16 + r) * C::SB + 2 * u);
+                        if (vr + 8 * x >= live) continue;
+                        raw.w[x] = *reinterpret_cast<const uint4 *>(blk + v_at + 8 * x * C::RB);   // 8 rows on: the same swap
+                        raw.s[x].x = *reinterpret_cast<const uint16_t *>(blk + vs_at + 8 * x * C::SB);
                     }
                 } else {
 #pragma unroll
                     for (int x = 0; x < 2; x++) {
-                        const int r = (lane >> 2) + 8 * x, q = lane & 3;
                         raw.w[x] = make_uint4(0u, 0u, 0u, 0u);
                         raw.s[x] = make_uint2(0u, 0u);
-                        if (r >= live) continue;
+                        if (lr + 8 * x >= live) continue;
                         if constexpr (D == 128) {
-                            raw.w[x] = *reinterpret_cast<const uint4 *>(blk + r * C::RB + 16 * q);
-                            raw.s[x] = *reinterpret_cast<const uint2 *>(blk + 32 * C::RB + r * C::SB);
+                            raw.w[x] = *reinterpret_cast<const uint4 *>(blk + k_at + 8 * x * C::RB);
+                            raw.s[x] = *reinterpret_cast<const uint2 *>(blk + ks_at + 8 * x * C::SB);
                         } else {
-                            const uint2 y = *reinterpret_cast<const uint2 *>(blk + r * C::RB + 8 * q);
+                            const uint2 y = *reinterpret_cast<const uint2 *>(blk + k_at + 8 * x * C::RB);
                             raw.w[x].x = y.x;
                             raw.w[x].y = y.y;
-                            raw.s[x].x = *reinterpret_cast<const uint32_t *>(blk + 32 * C::RB + r * C::SB);
+                            raw.s[x].x = *reinterpret_cast<const uint32_t *>(blk + ks_at + 8 * x * C::SB);
                         }
                     }
                 }
             };
             auto store = [&](int jb, const Raw &raw) {
-                uint8_t *dst = (jb & 8 ? sV : sK) + ((jb >> 4) & 1) * C::kTile;
-                const int r0 = (jb & 7) * 16;
+                uint8_t *dst = (jb & 8 ? sV : sK) + ((jb >> 4) & 1) * C::kTile + (jb & 7) * (16 * 128);
                 if (jb & 8) {
 #pragma unroll
                     for (int x = 0; x < kV; x++) {
-                        const int it = lane + 32 * x, r = r0 + it / kPerRow, u = it % kPerRow;
                         const uint32_t e[4] = {raw.w[x].x, raw.w[x].y, raw.w[x].z, raw.w[x].w};
+                        const __half2 sc = bits_h2(__byte_perm(raw.s[x].x, 0u, 0x1010));
 #pragma unroll
                         for (int q = 0; q < 4; q++)
-                            *reinterpret_cast<uint4 *>(dst + tile_unit(r, 4 * u + q)) =
-                                dequant_unit(e[q], nib, bits_h2(raw.s[x].x * 0x10001u));
+                            *reinterpret_cast<uint4 *>(dst + x * 1024 + (v_to ^ (q << 4))) = dequant_unit(e[q], nib, sc);
                     }
                 } else {
 #pragma unroll
                     for (int x = 0; x < 2; x++) {
-                        const int r = r0 + (lane >> 2) + 8 * x, kq = lane & 3;
                         const uint32_t e[4] = {raw.w[x].x, raw.w[x].y, raw.w[x].z, raw.w[x].w};
 #pragma unroll
-                        for (int q = 0; q < D / 32; q++) {
-                            // odd rows take their words in pair-swapped order, so that the two rows of a
-                            // quarter warp fill all eight units of the swizzle
-                            const int j = q ^ (r & 1);
-                            const uint32_t s2 = (q >> 1) ? raw.s[x].y : raw.s[x].x;
-                            const uint32_t sj = (r & 1) ^ (q & 1) ? s2 >> 16 : s2 & 0xffffu;
-                            *reinterpret_cast<uint4 *>(dst + tile_unit(r, 4 * j + kq)) =
-                                dequant_unit(r & 1 ? e[q ^ 1] : e[q], nib, bits_h2(sj * 0x10001u));
+                        for (int j = 0; j < D / 32; j++) {   // unit 4 j + un: chunk j / 2, place (4 (j % 2) + un) ^ row
+                            const __half2 sc = bits_h2(__byte_perm((j >> 1) ? raw.s[x].y : raw.s[x].x, 0u, j & 1 ? 0x3232 : 0x1010));
+                            *reinterpret_cast<uint4 *>(dst + (j >> 1) * kChunk + x * 1024 + (k_to ^ ((j & 1) << 6))) =
+                                dequant_unit(e[j], nib, sc);
                         }
                     }
                 }
             };
-            Raw cur, next;
-            load(job, page_of(job), cur);
+            Raw ra, rb;   // this job's rows and the next one's, in turn
+            load(job, page_of(job), ra);
             int page = page_of(job + kStep);
-            for (; job < jobs; job += kStep) {
+            auto one = [&](Raw &cur, Raw &next) {
                 if (job + kStep < jobs) load(job + kStep, page, next);
                 page = page_of(job + 2 * kStep);
-                if (!wait_empty(job)) break;
+                if (!wait_empty(job)) return false;
                 store(job, cur);
                 announce(job);
-                cur = next;
-            }
+                job += kStep;
+                return job < jobs;
+            };
+            while (one(ra, rb) && one(rb, ra)) {}
         } else {
             // a job is announced when the second one behind it has been requested
             int issued = 0, page = page_of(job);
@@ -1196,21 +1214,35 @@ __global__ void __launch_bounds__(512, 1) kv_attend_many_kernel(const __grid_con
 #pragma unroll
                     for (int y = 0; y < 32; y++) s[y] = (seen >> y) & 1u ? s[y] : 0xff800000u;
                 };
-                uint32_t s[2][32];
-                float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                uint32_t s[2][32], p[2][16];
                 tmem_ld32_issue(ti, s[0]);
-                tmem_ld_wait(s[0]);
                 tmem_ld32_issue(ti + 32, s[1]);
-                mask(s[0], 0);
-#pragma unroll
-                for (int y = 0; y < 32; y++) mx[y & 3] = fmaxf(mx[y & 3], __uint_as_float(s[0][y]));
+                tmem_ld_wait(s[0]);
                 tmem_ld_wait(s[1]);
+                mask(s[0], 0);
                 mask(s[1], 1);
+                // Exponentials against the running maximum as it stands, the half's own maximum beside them;
+                // where that passes it by 2^8 (m = -inf: any score) it is raised, and O and l with it, and the
+                // exponentials are done again.
+                float2 sum[2];
+                while (true) {
+                    float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                    const float mu = m == -INFINITY ? 0.f : m;
+                    const float2 c2 = make_float2(c, c), mu2 = make_float2(-mu, -mu);
+                    sum[0] = sum[1] = make_float2(0.f, 0.f);
 #pragma unroll
-                for (int y = 0; y < 32; y++) mx[y & 3] = fmaxf(mx[y & 3], __uint_as_float(s[1][y]));
-                const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * c;
-                if (__any_sync(0xffffffffu, top > m + 8.f)) {   // m = -inf: any score
-                    // the running maximum rises to top, O and l with it
+                    for (int x = 0; x < 2; x++)
+#pragma unroll
+                        for (int y = 0; y < 16; y++) {
+                            const float2 s2 = make_float2(__uint_as_float(s[x][2 * y]), __uint_as_float(s[x][2 * y + 1]));
+                            const float2 e = fma2(s2, c2, mu2);
+                            const float2 p2 = make_float2(ex2_hw(e.x), ex2_hw(e.y));
+                            mx[y & 3] = fmaxf(mx[y & 3], fmaxf(s2.x, s2.y));
+                            sum[y & 1] = add2(sum[y & 1], p2);
+                            p[x][y] = I4 ? h2_bits(__float22half2_rn(p2)) : pack_bf16x2(p2.x, p2.y);
+                        }
+                    const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * c;
+                    if (!__any_sync(0xffffffffu, top > m + 8.f)) break;
                     const float mn = fmaxf(m, top), corr = mn == -INFINITY ? 1.f : exp2f(m - mn);
                     if (i > 0) {
                         ok = wait_all(pv_done + 2 * w + (h ^ 1), ((i - 1) >> 1) & 1, DEVERR_TIMEOUT_EPILOGUE);
@@ -1229,21 +1261,10 @@ __global__ void __launch_bounds__(512, 1) kv_attend_many_kernel(const __grid_con
                     l *= corr;
                     m = mn;
                 }
-                const float mu = m == -INFINITY ? 0.f : m;
-                float sum[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int x = 0; x < 2; x++) {
-                    uint32_t p[16];
-#pragma unroll
-                    for (int y = 0; y < 16; y++) {
-                        const float p0 = ex2_hw(fmaf(__uint_as_float(s[x][2 * y]), c, -mu));
-                        const float p1 = ex2_hw(fmaf(__uint_as_float(s[x][2 * y + 1]), c, -mu));
-                        sum[y & 3] += p0 + p1;
-                        p[y] = I4 ? h2_bits(__floats2half2_rn(p0, p1)) : pack_bf16x2(p0, p1);
-                    }
-                    tmem_st16(ti + 16 * x, p);
-                }
-                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                if (!ok) break;
+                tmem_st16(ti, p[0]);
+                tmem_st16(ti + 16, p[1]);
+                l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
                 tmem_wait_st();
                 tc_fence_before();
                 mbar_arrive(p_full + 2 * w + h);
