@@ -108,25 +108,17 @@ DTTS_DEV void kv_join_parts(const float *ws, long long part, int parts, int rows
     }
 }
 
-// Barrier over threads 0 .. N - 1 of the CTA, N = 0: all of them.
-template <int N>
-DTTS_DEV void sync_first() {
-    if (N == 0) __syncthreads();
-    else asm volatile("bar.sync 1, %0;" ::"n"(N) : "memory");
-}
-
 // Counts the parts of a unit that have been written; true in the CTA that sees
 // the last one, which resets the counter for the next call.
-template <int N>
 DTTS_DEV bool kv_last_part(int *cnt, int parts, int *flag) {
     __threadfence();
-    sync_first<N>();
+    __syncthreads();
     if (threadIdx.x == 0) {
         const int old = atomicAdd(cnt, 1);
         *flag = old == parts - 1;
         if (old == parts - 1) *cnt = 0;
     }
-    sync_first<N>();
+    __syncthreads();
     const bool last = *flag;
     if (last) __threadfence();
     return last;
@@ -704,7 +696,7 @@ __global__ void __launch_bounds__(FewCfg<D, I4>::kThreads, NT == 1 ? 3 : 1) kv_a
         }
     }
     if (parts == 1) return;
-    if (kv_last_part<0>(a.cnt + unit, parts, flag))
+    if (kv_last_part(a.cnt + unit, parts, flag))
         kv_join_parts<D, C::kThreads>(a.ws + (long long)unit * a.splits * WS, WS, parts, rows, [&](int r) {
             return a.out + (long long)(row0 + r / G) * a.o_row + (long long)(head * G + r % G) * a.o_head;
         });
@@ -773,6 +765,64 @@ DTTS_DEV uint64_t sdesc_mn128(uint32_t saddr) {
 }
 // byte offset of 16-byte unit u (8 elements) of row r in a tile of 64-element chunks
 DTTS_DEV int tile_unit(int r, int u) { return (u >> 3) * kChunk + r * 128 + (((u & 7) ^ (r & 7)) << 4); }
+
+// 256 query rows of one (sequence, key head) pair
+struct ManyUnit {
+    bool on;
+    int b, head, cnt, len, row0, base, rows, i0, i_last, parts;
+    KeyTiles kt;
+    DTTS_DEV ManyUnit(const KvAttendArgs &a, int bh, int pair)
+        : b(bh / a.g.H), head(bh % a.g.H), cnt(a.m.cnt[b]), len(a.m.len[b]), row0(a.m.start[b]), base(pair * 256),
+          rows((int)min(256ll, max(0ll, (long long)cnt * a.G - (long long)pair * 256))), i0(len - cnt),
+          i_last(i0 + (base + rows - 1) / a.G),
+          kt(kKvManyKeyTile, i0 + base / a.G, i_last + 1, a.window, a.sinks) {
+        on = (long long)cnt * a.G > kKvFewRows && rows > 0 && (long long)row0 + cnt <= a.total_rows;
+        parts = min(a.splits, max(1, (kt.n + a.tiles_per_split - 1) / a.tiles_per_split));
+    }
+};
+// A part's result: O as [D / 4][256 rows][4], then m [256], l [256], so that a warp's rows are contiguous.
+template <int D>
+DTTS_DEV float *many_part(const KvAttendArgs &a, int unit, int split) {
+    return a.ws + ((long long)unit * a.splits + split) * 256 * (D + 2);
+}
+
+// Joins the parts of a unit, a row a thread, 16 dims a block (blockIdx.y).
+template <int D>
+__global__ void __launch_bounds__(256) kv_join_many_kernel(const __grid_constant__ KvAttendArgs a, int pairs) {
+    pdl_wait();
+    pdl_trigger();
+    const int unit = blockIdx.x, x0 = blockIdx.y * 16, r = threadIdx.x;
+    const ManyUnit n(a, unit / pairs, unit % pairs);
+    if (!n.on || n.parts == 1 || r >= n.rows) return;
+    float top = -INFINITY;
+#pragma unroll 4
+    for (int s = 0; s < n.parts; s++) top = fmaxf(top, many_part<D>(a, unit, s)[256 * D + r]);
+    float l = 0.f, o[16];
+#pragma unroll
+    for (int i = 0; i < 16; i++) o[i] = 0.f;
+#pragma unroll 2
+    for (int s = 0; s < n.parts; s++) {
+        const float *p = many_part<D>(a, unit, s);
+        const float f = merge_weight(p[256 * D + r], top);
+        l += f * p[256 * (D + 1) + r];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const float4 v = reinterpret_cast<const float4 *>(p)[(x0 / 4 + i) * 256 + r];
+            o[4 * i] += f * v.x;
+            o[4 * i + 1] += f * v.y;
+            o[4 * i + 2] += f * v.z;
+            o[4 * i + 3] += f * v.w;
+        }
+    }
+    const float inv = 1.0f / l;   // l = 0: every score was -inf, and 0 * inf is the formula's NaN
+    const int row = n.base + r;
+    uint4 *dst = reinterpret_cast<uint4 *>(a.out + (long long)(n.row0 + row / a.G) * a.o_row +
+                                           (long long)(n.head * a.G + row % a.G) * a.o_head + x0);
+#pragma unroll
+    for (int i = 0; i < 2; i++)
+        dst[i] = make_uint4(pack_bf16x2(o[8 * i] * inv, o[8 * i + 1] * inv), pack_bf16x2(o[8 * i + 2] * inv, o[8 * i + 3] * inv),
+                            pack_bf16x2(o[8 * i + 4] * inv, o[8 * i + 5] * inv), pack_bf16x2(o[8 * i + 6] * inv, o[8 * i + 7] * inv));
+}
 
 template <int D, bool I4>
 struct ManyCfg {
@@ -892,23 +942,19 @@ __global__ void __launch_bounds__(512, 1) kv_attend_many_kernel(const __grid_con
     uint64_t *q_full = bars, *s_full = bars + 2, *p_full = bars + 6, *pv_done = bars + 10;
     uint64_t *k_full = bars + 14, *k_empty = bars + 16, *v_full = bars + 18, *v_empty = bars + 20, *drain = bars + 22;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 24);
-    int *flag = reinterpret_cast<int *>(tmem_slot + 1);
-    volatile int *abort_flag = flag + 1;
+    volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     pdl_wait();
 
     const int split = blockIdx.x % a.splits, u = blockIdx.x / a.splits;
     const int bh = u % (a.n_seq * a.g.H), pair = pairs - 1 - u / (a.n_seq * a.g.H);   // longest key ranges first
-    const int b = bh / a.g.H, head = bh % a.g.H, unit = bh * pairs + pair;
-    const int cnt = a.m.cnt[b], len = a.m.len[b], row0 = a.m.start[b], G = a.G;
-    const long long all = (long long)cnt * G;
-    if (all <= kKvFewRows || (long long)pair * 256 >= all || (long long)row0 + cnt > a.total_rows) return;
-    const int base = pair * 256, rows = (int)min(256ll, all - base), tiles = rows > 128 ? 2 : 1;
-    const int *trow = a.m.table + (long long)a.m.seq[b] * a.g.max_pages;
-    const int i0 = len - cnt, i_first = i0 + base / G, i_last = i0 + (base + rows - 1) / G;
-    const KeyTiles kt(KT, i_first, i_last + 1, a.window, a.sinks);
-    const int parts = min(a.splits, max(1, (kt.n + a.tiles_per_split - 1) / a.tiles_per_split));
-    if (split >= parts) return;
+    const int unit = bh * pairs + pair;
+    const ManyUnit mu(a, bh, pair);
+    if (!mu.on || split >= mu.parts) return;
+    const int head = mu.head, len = mu.len, row0 = mu.row0, G = a.G, base = mu.base, rows = mu.rows, parts = mu.parts;
+    const int tiles = rows > 128 ? 2 : 1, i0 = mu.i0, i_last = mu.i_last;
+    const KeyTiles &kt = mu.kt;
+    const int *trow = a.m.table + (long long)a.m.seq[mu.b] * a.g.max_pages;
     const int c0 = (int)((long long)kt.n * split / parts), c1 = (int)((long long)kt.n * (split + 1) / parts), n = c1 - c0;
     // half blocks of 64 keys; the last one stays out where no row sees it
     const int halves = 2 * n - (kt.tile(c1 - 1) * KT + 64 > i_last ? 1 : 0);
@@ -927,7 +973,6 @@ __global__ void __launch_bounds__(512, 1) kv_attend_many_kernel(const __grid_con
             mbar_init(v_empty + w, tiles);
             mbar_init(drain + w, 1);
         }
-        *flag = 0;
         *abort_flag = 0;
         fence_mbar_init();
     }
@@ -1156,41 +1201,48 @@ __global__ void __launch_bounds__(512, 1) kv_attend_many_kernel(const __grid_con
         if (w < tiles) {
             const bool live = rr < rows;
             const int tok = (base + (live ? rr : 0)) / G, hg = (base + (live ? rr : 0)) % G, qi = live ? i0 + tok : -1;
-            const bf16 *qp = a.q + (long long)(row0 + tok) * a.q_row + (long long)(head * G + hg) * a.q_head;
+            // Q: the warp loads its 32 rows two (D = 64: four) at a time, 16 bytes a lane; row offsets and scale
+            // factors pass between the row's owner and the lanes that hold it
+            constexpr int kRows = 32 / NU, kSteps = 32 / kRows, kBatch = 8;
+            const long long q_off = (long long)(row0 + tok) * a.q_row + (long long)(head * G + hg) * a.q_head;
+            const int wr = w * 128 + (warp & 3) * 32, lr = lane / NU, u = lane % NU;
             float c = a.scale_log2;
-            {
-                uint4 x[NU];
-                uint32_t top = 0;
+#pragma unroll 1
+            for (int s0 = 0; s0 < kSteps; s0 += kBatch) {
+                uint4 x[kBatch];
 #pragma unroll
-                for (int i = 0; i < NU; i++) {
-                    x[i] = live ? reinterpret_cast<const uint4 *>(qp)[i] : make_uint4(0u, 0u, 0u, 0u);
-                    const uint32_t e[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
-#pragma unroll
-                    for (int y = 0; y < 4; y++) top = max(top, max(e[y] & 0x7fffu, (e[y] >> 16) & 0x7fffu));
-                }
-                float up = 1.f;
-                if constexpr (I4) {
-                    // as in the few-row kernel: the largest |q| of the row to [2^14, 2^15)
-                    const int ex = (int)(top >> 7), sh = ex == 255 ? 0 : min(14 + 127 - ex, 100);
-                    up = __uint_as_float((uint32_t)(sh + 127) << 23);
-                    c = fmaxf(c * __uint_as_float((uint32_t)(127 - sh) << 23), 1.17549435e-38f);   // -inf * c stays -inf
+                for (int s = 0; s < kBatch; s++) {
+                    const int row = (s0 + s) * kRows + lr;
+                    const long long off = __shfl_sync(0xffffffffu, q_off, row);
+                    x[s] = wr + row < rows ? *reinterpret_cast<const uint4 *>(a.q + off + 8 * u) : make_uint4(0u, 0u, 0u, 0u);
                 }
 #pragma unroll
-                for (int i = 0; i < NU; i++) {
+                for (int s = 0; s < kBatch; s++) {
                     if constexpr (I4) {
-                        const uint32_t e[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+                        // as in the few-row kernel: the largest |q| of the row to [2^14, 2^15)
+                        const uint32_t e[4] = {x[s].x, x[s].y, x[s].z, x[s].w};
+                        uint32_t top = 0;
+#pragma unroll
+                        for (int y = 0; y < 4; y++) top = max(top, max(e[y] & 0x7fffu, (e[y] >> 16) & 0x7fffu));
+#pragma unroll
+                        for (int y = 1; y < NU; y <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, y));
+                        const int ex = (int)(top >> 7), sh = ex == 255 ? 0 : min(14 + 127 - ex, 100);
+                        const float up = __uint_as_float((uint32_t)(sh + 127) << 23);
                         float f[8];
 #pragma unroll
                         for (int y = 0; y < 4; y++) {
                             f[2 * y] = __uint_as_float(e[y] << 16) * up;
                             f[2 * y + 1] = __uint_as_float(e[y] & 0xffff0000u) * up;
                         }
-                        x[i] = make_uint4(h2_bits(__floats2half2_rn(f[0], f[4])), h2_bits(__floats2half2_rn(f[1], f[5])),
+                        x[s] = make_uint4(h2_bits(__floats2half2_rn(f[0], f[4])), h2_bits(__floats2half2_rn(f[1], f[5])),
                                           h2_bits(__floats2half2_rn(f[2], f[6])), h2_bits(__floats2half2_rn(f[3], f[7])));
+                        const int osh = __shfl_sync(0xffffffffu, sh, (lane % kRows) * NU);
+                        if (lane / kRows == s0 + s) c *= __uint_as_float((uint32_t)(127 - osh) << 23);
                     }
-                    *reinterpret_cast<uint4 *>(sQ + w * C::kTile + tile_unit(r, i)) = x[i];
+                    *reinterpret_cast<uint4 *>(sQ + w * C::kTile + tile_unit((warp & 3) * 32 + (s0 + s) * kRows + lr, u)) = x[s];
                 }
             }
+            c = fmaxf(c, 1.17549435e-38f);   // -inf * c stays -inf
             fence_proxy_async_smem();
             mbar_arrive(q_full + w);
             const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
@@ -1227,8 +1279,8 @@ __global__ void __launch_bounds__(512, 1) kv_attend_many_kernel(const __grid_con
                 float2 sum[2];
                 while (true) {
                     float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-                    const float mu = m == -INFINITY ? 0.f : m;
-                    const float2 c2 = make_float2(c, c), mu2 = make_float2(-mu, -mu);
+                    const float mref = m == -INFINITY ? 0.f : m;
+                    const float2 c2 = make_float2(c, c), mu2 = make_float2(-mref, -mref);
                     sum[0] = sum[1] = make_float2(0.f, 0.f);
 #pragma unroll
                     for (int x = 0; x < 2; x++)
@@ -1272,8 +1324,8 @@ __global__ void __launch_bounds__(512, 1) kv_attend_many_kernel(const __grid_con
             const int last = halves - 1;   // its product follows all others into O
             if (ok && wait_all(pv_done + 2 * w + (last & 1), (last >> 1) & 1, DEVERR_TIMEOUT_EPILOGUE)) {
                 tc_fence_after();
-                bf16 *op = a.out + (long long)(row0 + tok) * a.o_row + (long long)(head * G + hg) * a.o_head;
-                float *wp = a.ws + (((long long)unit * a.splits + split) * 256 + rr) * (D + 2);
+                float *wp = many_part<D>(a, unit, split);
+                uint8_t *sO = sQ + w * C::kTile;   // Q is dead: O's rows on their way to whole-row stores
                 const float inv = 1.0f / l;   // l = 0: every score was -inf, and 0 * inf is the formula's NaN
                 bool bad = false;
 #pragma unroll 1
@@ -1288,34 +1340,49 @@ __global__ void __launch_bounds__(512, 1) kv_attend_many_kernel(const __grid_con
                             v[unit_dim(I4, i)] = o[8 * y + i];
                             bad |= o[8 * y + i] != o[8 * y + i];
                         }
-                        if (!live) continue;
-                        if (parts == 1)
-                            *reinterpret_cast<uint4 *>(op + x + 8 * y) =
+                        if (parts == 1) {
+                            *reinterpret_cast<uint4 *>(sO + tile_unit(r, x / 8 + y)) =
                                 make_uint4(pack_bf16x2(v[0] * inv, v[1] * inv), pack_bf16x2(v[2] * inv, v[3] * inv),
                                            pack_bf16x2(v[4] * inv, v[5] * inv), pack_bf16x2(v[6] * inv, v[7] * inv));
-                        else
-#pragma unroll
-                            for (int i = 0; i < 4; i++)
-                                reinterpret_cast<float2 *>(wp + x + 8 * y)[i] = make_float2(v[2 * i], v[2 * i + 1]);
+                        } else {
+                            float4 *dst = reinterpret_cast<float4 *>(wp) + (x / 4 + 2 * y) * 256 + rr;
+                            dst[0] = make_float4(v[0], v[1], v[2], v[3]);
+                            dst[256] = make_float4(v[4], v[5], v[6], v[7]);
+                        }
                     }
                 }
-                if (live && parts > 1) {
-                    wp[D] = m;
-                    wp[D + 1] = l;
+                if (parts > 1) {
+                    wp[256 * D + rr] = m;
+                    wp[256 * (D + 1) + rr] = l;
+                } else {
+                    __syncwarp();
+                    const long long o_off = (long long)(row0 + tok) * a.o_row + (long long)(head * G + hg) * a.o_head;
+#pragma unroll 4
+                    for (int s = 0; s < kSteps; s++) {
+                        const int row = s * kRows + lr;
+                        const long long off = __shfl_sync(0xffffffffu, o_off, row);
+                        if (wr + row < rows)
+                            *reinterpret_cast<uint4 *>(a.out + off + 8 * u) =
+                                *reinterpret_cast<const uint4 *>(sO + tile_unit((warp & 3) * 32 + row, u));
+                    }
+                    __syncwarp();
                 }
                 // a NaN: recompute the row so that key rows it cannot see do not reach it
                 for (unsigned todo = __ballot_sync(0xffffffffu, bad && live); todo; todo &= todo - 1) {
-                    const int x = __ffs(todo) - 1, xr = base + w * 128 + (warp & 3) * 32 + x, xt = xr / G, xh = xr % G;
+                    const int x = __ffs(todo) - 1, xr = wr + x, xt = (base + xr) / G, xh = (base + xr) % G;
                     float mm, ll, oo[D / 32];
                     kv_row_plain<D>(a, trow, head, a.q + (long long)(row0 + xt) * a.q_row + (long long)(head * G + xh) * a.q_head,
                                     i0 + xt, KT, kt, c0, c1, mm, ll, oo);
-                    float *xw = a.ws + (((long long)unit * a.splits + split) * 256 + xr - base) * (D + 2);
                     bf16 *xo = a.out + (long long)(row0 + xt) * a.o_row + (long long)(head * G + xh) * a.o_head;
                     for (int i = 0; i < D / 32; i++) {
-                        if (parts == 1) xo[lane + 32 * i] = __float2bfloat16_rn(oo[i] / ll);
-                        else xw[lane + 32 * i] = oo[i];
+                        const int d = lane + 32 * i;
+                        if (parts == 1) xo[d] = __float2bfloat16_rn(oo[i] / ll);
+                        else wp[((d >> 2) * 256 + xr) * 4 + (d & 3)] = oo[i];
                     }
-                    if (parts > 1 && lane == 0) { xw[D] = mm; xw[D + 1] = ll; }
+                    if (parts > 1 && lane == 0) {
+                        wp[256 * D + xr] = mm;
+                        wp[256 * (D + 1) + xr] = ll;
+                    }
                     __syncwarp();
                 }
             }
@@ -1327,17 +1394,15 @@ __global__ void __launch_bounds__(512, 1) kv_attend_many_kernel(const __grid_con
         tc_fence_after();
         tmem_dealloc(tbase, 512);
     }
-    if (parts > 1 && warp < 8 && kv_last_part<C::kSoftmax>(a.cnt + unit, parts, flag))
-        kv_join_parts<D, C::kSoftmax>(a.ws + (long long)unit * a.splits * 256 * (D + 2), 256ll * (D + 2), parts, rows, [&](int r) {
-            const int x = base + r;
-            return a.out + (long long)(row0 + x / G) * a.o_row + (long long)(head * G + x % G) * a.o_head;
-        });
 }
 
 template <int D, bool I4>
 cudaError_t launch_many(const KvAttendArgs &a, int pairs, cudaStream_t s) {
-    return launch_k(pdl_enabled() ? kLaunchPdl : 0u, kv_attend_many_kernel<D, I4>, dim3((unsigned)a.n_seq * a.g.H * pairs * a.splits),
-                    dim3(ManyCfg<D, I4>::kThreads), ManyCfg<D, I4>::kSmem, s, a, pairs);
+    const unsigned flags = pdl_enabled() ? kLaunchPdl : 0u, units = (unsigned)a.n_seq * a.g.H * pairs;
+    cudaError_t e = launch_k(flags, kv_attend_many_kernel<D, I4>, dim3(units * a.splits), dim3(ManyCfg<D, I4>::kThreads),
+                             ManyCfg<D, I4>::kSmem, s, a, pairs);
+    if (e != cudaSuccess || a.splits == 1) return e;
+    return launch_k(flags, kv_join_many_kernel<D>, dim3(units, D / 16), dim3(256), 0, s, a, pairs);
 }
 
 template <int D, bool I4, int NT>
