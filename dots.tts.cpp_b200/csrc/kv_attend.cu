@@ -4,6 +4,7 @@
 // over the rows j <= i with window = 0, or j > i - window, or j < sinks.
 #include "kv.cuh"
 
+#include <algorithm>
 #include <cmath>
 #include <type_traits>
 
@@ -27,6 +28,12 @@ struct KeyTiles {
     }
     DTTS_DEV int tile(int v) const { return v < sink_tiles ? v : win0 + v - sink_tiles; }
 };
+
+// Where part s of n tiles in `parts` parts begins: parts differ by a tile at most.
+DTTS_DEV int part_start(int n, int parts, int s) {
+    const int q = n / parts;
+    return s * q + min(s, n - parts * q);
+}
 
 DTTS_DEV float kv_elem(const KvGeom &g, const uint8_t *seg, bool is_v, int r, int d) {
     if (g.i4) {
@@ -253,7 +260,7 @@ __global__ void __launch_bounds__(FewCfg<D, I4>::kThreads, NT == 1 ? 3 : 1) kv_a
     const KeyTiles kt(KT, i0, len, a.window, a.sinks);
     const int parts = min(a.splits, max(1, (kt.n + a.tiles_per_split - 1) / a.tiles_per_split));
     if (split >= parts) return;
-    const int c0 = (int)((long long)kt.n * split / parts), c1 = (int)((long long)kt.n * (split + 1) / parts);
+    const int c0 = part_start(kt.n, parts, split), c1 = part_start(kt.n, parts, split + 1);
 
     uint8_t *ring = smem + warp * C::kStages * C::kStage;
     uint64_t *bar = bars + warp * C::kStages;
@@ -703,17 +710,33 @@ __global__ void __launch_bounds__(FewCfg<D, I4>::kThreads, NT == 1 ? 3 : 1) kv_a
 }
 
 // ---------------------------------------------------------------- many rows
-// tcgen05 pieces that only this kernel uses: A operand from TMEM, 32-column
-// stores, and the MN-major descriptor of a [keys][dims] tile of 64-dim chunks
-// (rows of 128 bytes, 128-byte swizzle): 8-key groups 1024 bytes apart, chunks
-// kChunk bytes apart.
+// tcgen05 pieces that only this kernel uses.  Its operand tiles are rows of 128 bytes in 64-element chunks with the
+// 128-byte swizzle, 8-row groups 1024 bytes apart, so the upper word of every descriptor is the same (stride,
+// version, layout: see sdesc_k128) and is put in beside each instruction; the lower one holds the address and,
+// for the MN-major V tile, the distance of its chunks.  (A 64-bit descriptor kept across the kernel's loops came out
+// of the compiler with its upper word lost.)
 constexpr int kChunk = 128 * 128;   // 128 rows x 64 elements of 2 bytes
-DTTS_DEV void tc_mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+DTTS_DEV uint32_t desc_k(uint32_t saddr) { return ((saddr >> 4) & 0x3fffu) | (1u << 16); }
+DTTS_DEV uint32_t desc_mn(uint32_t saddr) { return ((saddr >> 4) & 0x3fffu) | ((uint32_t)(kChunk >> 4) << 16); }
+// D (tmem) (+)= A (smem) B^T (smem)
+DTTS_DEV void tc_mma_ss(uint32_t d_tmem, uint32_t adesc, uint32_t bdesc, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\t"
+        "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\t"
         "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d_tmem),
-        "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate)
+        "mov.b64 a, {%1, 0x40004040};\n\t"
+        "mov.b64 b, {%2, 0x40004040};\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n\t}\n" ::"r"(d_tmem),
+        "r"(adesc), "r"(bdesc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+// D (tmem) (+)= A (tmem) B (smem, MN-major)
+DTTS_DEV void tc_mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint32_t bdesc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t.reg .b64 b;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "mov.b64 b, {%2, 0x40004040};\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %3, p;\n\t}\n" ::"r"(d_tmem),
+        "r"(a_tmem), "r"(bdesc), "r"(idesc), "r"(accumulate)
         : "memory");
 }
 // 32 columns on their way to r; r may be used after tmem_ld_wait(r), which waits
@@ -760,9 +783,6 @@ DTTS_DEV void tmem_ld16(uint32_t taddr, float (&v)[16]) {
     for (int i = 0; i < 16; i++) v[i] = __uint_as_float(r[i]);
 }
 DTTS_DEV void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-DTTS_DEV uint64_t sdesc_mn128(uint32_t saddr) {
-    return (sdesc_k128(saddr) & ~(0x3fffull << 16)) | ((uint64_t)(kChunk >> 4) << 16);
-}
 // byte offset of 16-byte unit u (8 elements) of row r in a tile of 64-element chunks
 DTTS_DEV int tile_unit(int r, int u) { return (u >> 3) * kChunk + r * 128 + (((u & 7) ^ (r & 7)) << 4); }
 
@@ -778,6 +798,22 @@ struct ManyUnit {
           kt(kKvManyKeyTile, i0 + base / a.G, i_last + 1, a.window, a.sinks) {
         on = (long long)cnt * a.G > kKvFewRows && rows > 0 && (long long)row0 + cnt <= a.total_rows;
         parts = min(a.splits, max(1, (kt.n + a.tiles_per_split - 1) / a.tiles_per_split));
+    }
+};
+// A part of a unit's keys: what a CTA takes at a time.  Items are numbered from the longest key ranges down.
+struct ManyItem : ManyUnit {
+    int unit, split, c0, n, halves, tiles;   // first key block, key blocks, half blocks of 64 keys, row tiles
+    DTTS_DEV ManyItem(const KvAttendArgs &a, int pairs, int index)
+        : ManyUnit(a, index / a.splits % (a.n_seq * a.g.H), pairs - 1 - index / a.splits / (a.n_seq * a.g.H)),
+          split(index % a.splits) {
+        const int u = index / a.splits;
+        unit = u % (a.n_seq * a.g.H) * pairs + pairs - 1 - u / (a.n_seq * a.g.H);
+        on = on && split < parts;
+        c0 = part_start(kt.n, parts, split);
+        n = part_start(kt.n, parts, split + 1) - c0;
+        // the last half stays out where no row sees it
+        halves = 2 * n - (kt.tile(c0 + n - 1) * kKvManyKeyTile + 64 > i_last ? 1 : 0);
+        tiles = rows > 128 ? 2 : 1;
     }
 };
 // A part's result: O as [D / 4][256 rows][4], then m [256], l [256], so that a warp's rows are contiguous.
@@ -827,7 +863,7 @@ __global__ void __launch_bounds__(256) kv_join_many_kernel(const __grid_constant
 template <int D, bool I4>
 struct ManyCfg {
     static constexpr int KT = kKvManyKeyTile, kTile = D / 64 * kChunk;   // one operand tile of 128 rows
-    static constexpr int kSoftmax = 256, kProducerWarps = 6, kThreads = 512;
+    static constexpr int kProducerWarps = 6, kThreads = 512;   // beside 8 softmax and 2 issuing warps
     // registers a thread: 128 at launch (512 x 128 = 65536), then 256 x (176 + 80) = 65536
     static constexpr int kSoftmaxRegs = 176, kOtherRegs = 80;
     static constexpr int kSmem = 6 * kTile + 256 + 1024;      // Q x 2, K x 2, V x 2, barriers
@@ -911,6 +947,39 @@ DTTS_DEV bool kv_wait(uint64_t *bar, uint32_t parity, volatile int *abort_flag, 
     }
 }
 
+// Recomputes the rows of this warp (of eight) of an item that came out with a NaN, so that key rows that a query
+// cannot see do not reach it.
+template <int D>
+__device__ __noinline__ void many_repair(const KvAttendArgs &a, int pairs, int index) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const ManyItem m(a, pairs, index);
+    float *wp = many_part<D>(a, m.unit, m.split);
+    for (int r = warp * 32; r < min(m.rows, warp * 32 + 32); r++) {
+        const int tok = (m.base + r) / a.G, hq = m.head * a.G + (m.base + r) % a.G;
+        bf16 *o = a.out + (long long)(m.row0 + tok) * a.o_row + (long long)hq * a.o_head;
+        bool bad = false;
+        for (int i = 0; i < D / 32; i++) {
+            const int d = lane + 32 * i;
+            const float v = m.parts == 1 ? __bfloat162float(o[d]) : wp[((d >> 2) * 256 + r) * 4 + (d & 3)];
+            bad |= v != v;
+        }
+        if (!__any_sync(0xffffffffu, bad)) continue;
+        float mm, ll, oo[D / 32];
+        kv_row_plain<D>(a, a.m.table + (long long)a.m.seq[m.b] * a.g.max_pages, m.head,
+                        a.q + (long long)(m.row0 + tok) * a.q_row + (long long)hq * a.q_head, m.i0 + tok, kKvManyKeyTile, m.kt,
+                        m.c0, m.c0 + m.n, mm, ll, oo);
+        for (int i = 0; i < D / 32; i++) {
+            const int d = lane + 32 * i;
+            if (m.parts == 1) o[d] = __float2bfloat16_rn(oo[i] / ll);
+            else wp[((d >> 2) * 256 + r) * 4 + (d & 3)] = oo[i];
+        }
+        if (m.parts > 1 && lane == 0) {
+            wp[256 * D + r] = mm;
+            wp[256 * (D + 1) + r] = ll;
+        }
+    }
+}
+
 // Attention of up to 256 rows (new token x query head of one kv head, two tiles of
 // 128) of one sequence over a part of its keys, in blocks of 128 keys.
 //   warps 0-3, 4-7: softmax of tile 0, 1, one row a thread, half a block (64 keys) at
@@ -931,7 +1000,7 @@ DTTS_DEV bool kv_wait(uint64_t *bar, uint32_t parity, volatile int *abort_flag, 
 // of |v|, the size of the output's own rounding): a second term would cost half as
 // much tensor time again.
 template <int D, bool I4>
-__global__ void __launch_bounds__(512, 1) kv_attend_many_kernel(const __grid_constant__ KvAttendArgs a, int pairs) {
+__global__ void __launch_bounds__(512, 1) kv_attend_many_kernel(const __grid_constant__ KvAttendArgs a, int pairs, int items) {
     using C = ManyCfg<D, I4>;
     constexpr int KT = C::KT, NU = D / 8;   // 16-byte units a row
     extern __shared__ uint8_t smem_raw[];
@@ -941,23 +1010,11 @@ __global__ void __launch_bounds__(512, 1) kv_attend_many_kernel(const __grid_con
     // s_full, p_full, pv_done: [tile][half]
     uint64_t *q_full = bars, *s_full = bars + 2, *p_full = bars + 6, *pv_done = bars + 10;
     uint64_t *k_full = bars + 14, *k_empty = bars + 16, *v_full = bars + 18, *v_empty = bars + 20, *drain = bars + 22;
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 24);
-    volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
+    uint64_t *item_full = bars + 24, *item_empty = bars + 26;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 28);
+    volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1), *ring = abort_flag + 1;   // ring [2]
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     pdl_wait();
-
-    const int split = blockIdx.x % a.splits, u = blockIdx.x / a.splits;
-    const int bh = u % (a.n_seq * a.g.H), pair = pairs - 1 - u / (a.n_seq * a.g.H);   // longest key ranges first
-    const int unit = bh * pairs + pair;
-    const ManyUnit mu(a, bh, pair);
-    if (!mu.on || split >= mu.parts) return;
-    const int head = mu.head, len = mu.len, row0 = mu.row0, G = a.G, base = mu.base, rows = mu.rows, parts = mu.parts;
-    const int tiles = rows > 128 ? 2 : 1, i0 = mu.i0, i_last = mu.i_last;
-    const KeyTiles &kt = mu.kt;
-    const int *trow = a.m.table + (long long)a.m.seq[mu.b] * a.g.max_pages;
-    const int c0 = (int)((long long)kt.n * split / parts), c1 = (int)((long long)kt.n * (split + 1) / parts), n = c1 - c0;
-    // half blocks of 64 keys; the last one stays out where no row sees it
-    const int halves = 2 * n - (kt.tile(c1 - 1) * KT + 64 > i_last ? 1 : 0);
 
     if (tid == 0) {
         for (int w = 0; w < 2; w++) {
@@ -968,10 +1025,12 @@ __global__ void __launch_bounds__(512, 1) kv_attend_many_kernel(const __grid_con
                 mbar_init(pv_done + 2 * w + h, 1);
             }
             mbar_init(k_full + w, 8);
-            mbar_init(k_empty + w, tiles);
+            mbar_init(k_empty + w, 2);
             mbar_init(v_full + w, 8);
-            mbar_init(v_empty + w, tiles);
+            mbar_init(v_empty + w, 2);
             mbar_init(drain + w, 1);
+            mbar_init(item_full + w, 1);
+            mbar_init(item_empty + w, C::kThreads / 32);
         }
         *abort_flag = 0;
         fence_mbar_init();
@@ -987,218 +1046,297 @@ __global__ void __launch_bounds__(512, 1) kv_attend_many_kernel(const __grid_con
     // only now: the next kernel's CTAs may take TMEM before they wait for this grid
     pdl_trigger();
 
-    if (warp >= 8) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kOtherRegs));
-    else asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::kSoftmaxRegs));
     // the same answer in all lanes of the warp
     auto wait_all = [&](uint64_t *bar, uint32_t parity, int code) {
         return __all_sync(0xffffffffu, kv_wait(bar, parity, abort_flag, a.err, code)) != 0;
     };
-    if (warp >= 14) {
-        const int w = warp - 14;
-        // The whole warp runs the loop, so that addresses and descriptors stay uniform; one elected lane issues.
-        const bool lead = elect_one();
-        constexpr uint64_t kTileD = C::kTile >> 4;   // descriptor units of 16 bytes
-        constexpr uint64_t kHalfD = (64 * 128) >> 4;
-        const uint64_t qd = sdesc_k128(smem_u32(sQ)) + w * kTileD, kd = sdesc_k128(smem_u32(sK)), vd = sdesc_mn128(smem_u32(sV));
-        uint64_t *sf = s_full + 2 * w, *pf = p_full + 2 * w, *pd = pv_done + 2 * w;
-        auto scores = [&](int i) {   // of half block i: Q K^T, 64 keys
-            const uint64_t kw = kd + ((i >> 1) & 1) * kTileD + (i & 1) * kHalfD;
-            const uint32_t d = tbase + w * 128 + (i & 1) * 64;
-            if (lead) {
-#pragma unroll
-                for (int x = 0; x < D / 16; x++) {
-                    const uint64_t off = ((x >> 2) * kChunk + (x & 3) * 32) >> 4;
-                    tc_mma_bf16(d, qd + off, kw + off, C::idesc(64), x ? 1u : 0u);
-                }
-                tc_commit(sf + (i & 1));
-            }
-            __syncwarp();
-        };
-        if (w < tiles) {
-            bool ok = wait_all(k_full, 0, DEVERR_TIMEOUT_MMA) && wait_all(q_full + w, 0, DEVERR_TIMEOUT_MMA);
-            if (ok) {
+    // Items are drawn from a counter (a CTA's first one is its own number): producer warp 8 draws the next one when it
+    // has requested all of the last one's rows, and hands it to every warp through a ring of two.  Barrier phases
+    // run on from item to item, so loading and scores of the next item begin behind the last one's.
+    auto take = [&](int seq) {   // item number `seq` of this CTA; >= items: no more
+        if (!wait_all(item_full + (seq & 1), (seq >> 1) & 1, DEVERR_TIMEOUT_PRODUCER)) return items;
+        const int index = ring[seq & 1];
+        __syncwarp();
+        if (lane == 0) mbar_arrive(item_empty + (seq & 1));
+        return index;
+    };
+    // the register split stands in the branch that it is for: behind a join the smaller share would hold for both
+    if (warp >= 8) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kOtherRegs));
+        if (warp >= 14) {
+            const int w = warp - 14;
+            // The whole warp runs the loop, so that addresses and descriptors stay uniform; one elected lane issues.
+            const bool lead = elect_one();
+            constexpr uint32_t kTileD = C::kTile >> 4, kHalfD = (64 * 128) >> 4;   // descriptor units of 16 bytes
+            const uint32_t qd = desc_k(smem_u32(sQ)) + w * kTileD, kd = desc_k(smem_u32(sK)), vd = desc_mn(smem_u32(sV));
+            uint64_t *sf = s_full + 2 * w, *pf = p_full + 2 * w, *pd = pv_done + 2 * w;
+            // kb: key blocks of the items before; hb: half blocks of this tile before.  Half g = hb + i of the tile has
+            // score buffer g & 1.
+            int kb = 0, hb = 0, qn = 0;
+            bool ok = true;
+            auto scores = [&](int i) {   // Q K^T of half block i of the item, 64 keys, into buffer (hb + i) & 1
+                const int g = hb + i;
+                // whose columns P of half g - 2 was read from
+                if (g >= 2 && !wait_all(pd + (g & 1), ((g - 2) >> 1) & 1, DEVERR_TIMEOUT_MMA)) return false;
                 tc_fence_after();
-                scores(0);
-            }
-            for (int i = 0; i < halves && ok; i++) {
-                const int k = i >> 1, h = i & 1;
-                if (i + 1 < halves) {
-                    // the next half's scores take the columns that P of the half before this one is read from
-                    if (h == 1) ok = wait_all(k_full + ((k + 1) & 1), ((k + 1) >> 1) & 1, DEVERR_TIMEOUT_MMA);
-                    if (ok && i >= 1) ok = wait_all(pd + (h ^ 1), ((i - 1) >> 1) & 1, DEVERR_TIMEOUT_MMA);
-                    if (!ok) break;
-                    tc_fence_after();
-                    scores(i + 1);
-                }
-                if (h == 0) {
-                    if (lead) tc_commit(k_empty + (k & 1));   // both halves' scores are issued
-                    __syncwarp();
-                    ok = wait_all(v_full + (k & 1), (k >> 1) & 1, DEVERR_TIMEOUT_MMA);
-                }
-                ok = ok && wait_all(pf + h, k & 1, DEVERR_TIMEOUT_MMA);
-                if (!ok) break;
-                tc_fence_after();
-                const uint64_t vw = vd + (k & 1) * kTileD + h * kHalfD;
-                const uint32_t d = tbase + 256 + w * 128, p = tbase + w * 128 + h * 64;
+                const uint32_t kw = kd + ((kb + (i >> 1)) & 1) * kTileD + (i & 1) * kHalfD;
+                const uint32_t d = tbase + w * 128 + (g & 1) * 64;
                 if (lead) {
 #pragma unroll
-                    for (int x = 0; x < 4; x++)
-                        tc_mma_ts(d, p + 8 * x, vw + x * (2048 >> 4), C::idesc(D) | (1u << 16), i || x ? 1u : 0u);
-                    tc_commit(pd + h);
-                    if (h == 1) tc_commit(v_empty + (k & 1));
+                    for (int x = 0; x < D / 16; x++) {
+                        const uint32_t off = ((x >> 2) * kChunk + (x & 3) * 32) >> 4;
+                        tc_mma_ss(d, qd + off, kw + off, C::idesc(64), x ? 1u : 0u);
+                    }
+                    tc_commit(sf + (g & 1));
                 }
                 __syncwarp();
+                return true;
+            };
+            for (int it = 0; ok; it++) {
+                const int index = take(it);
+                if (index >= items) break;
+                const ManyItem m(a, pairs, index);
+                if (w >= m.tiles) {   // no second tile: only release the blocks
+                    for (int k = kb; k < kb + m.n && ok; k++) {
+                        ok = wait_all(k_full + (k & 1), (k >> 1) & 1, DEVERR_TIMEOUT_MMA);
+                        if (ok && lane == 0) mbar_arrive(k_empty + (k & 1));
+                        ok = ok && wait_all(v_full + (k & 1), (k >> 1) & 1, DEVERR_TIMEOUT_MMA);
+                        if (ok && lane == 0) mbar_arrive(v_empty + (k & 1));
+                    }
+                    kb += m.n;
+                    continue;
+                }
+                ok = wait_all(k_full + (kb & 1), (kb >> 1) & 1, DEVERR_TIMEOUT_MMA) &&
+                     wait_all(q_full + w, qn & 1, DEVERR_TIMEOUT_MMA) && scores(0);
+                qn++;
+                for (int i = 0; i < m.halves && ok; i++) {
+                    const int k = kb + (i >> 1), g = hb + i;
+                    if (i + 1 < m.halves) {
+                        if (i & 1) ok = wait_all(k_full + ((k + 1) & 1), ((k + 1) >> 1) & 1, DEVERR_TIMEOUT_MMA);
+                        if (!ok || !(ok = scores(i + 1))) break;
+                    }
+                    if (!(i & 1)) {
+                        if (lead) tc_commit(k_empty + (k & 1));   // both halves' scores are issued
+                        __syncwarp();
+                        ok = wait_all(v_full + (k & 1), (k >> 1) & 1, DEVERR_TIMEOUT_MMA);
+                    }
+                    ok = ok && wait_all(pf + (g & 1), (g >> 1) & 1, DEVERR_TIMEOUT_MMA);
+                    if (!ok) break;
+                    tc_fence_after();
+                    const uint32_t vw = vd + (k & 1) * kTileD + (i & 1) * kHalfD;
+                    const uint32_t d = tbase + 256 + w * 128, p = tbase + w * 128 + (g & 1) * 64;
+                    if (lead) {
+#pragma unroll
+                        for (int x = 0; x < 4; x++)
+                            tc_mma_ts(d, p + 8 * x, vw + x * (2048 >> 4), C::idesc(D) | (1u << 16), i || x ? 1u : 0u);
+                        tc_commit(pd + (g & 1));
+                        if ((i & 1) || i + 1 == m.halves) tc_commit(v_empty + (k & 1));
+                    }
+                    __syncwarp();
+                }
+                kb += m.n;
+                hb += m.halves;
             }
-        }
-        // every product done before TMEM is given back (also after an abort)
-        if (lead) tc_commit(drain + w);
-        __syncwarp();
-        const unsigned long long t0 = globaltimer_ns();
-        while (!mbar_try_wait(drain + w, 0) && globaltimer_ns() - t0 < kWaitLimitNs) {}
-        __syncwarp();
-    } else if (warp >= 8) {
-        // ---- pages -> tiles.  A job is 16 rows of K or V, one block of a page: jobs K0 .. K7, V0 .. V7
-        // of key block 0, then of block 1, ...; producer warp pw takes jobs pw, pw + 7, ...  A job's page
-        // number is loaded two jobs ahead, its rows one job ahead.
-        const int P = a.g.P, lg = a.g.lgP, jobs = 16 * n;
-        const uint8_t *head_pool = a.pool + kv_seg_off(a.g, 0, 0, head);
-        auto row_of = [&](int job) { return kt.tile(c0 + (job >> 4)) * KT + (job & 7) * 16; };
-        auto page_of = [&](int job) {   // -1: nothing to load
-            if (job >= jobs) return -1;
-            const int j = row_of(job);
-            return j < len ? trow[j >> lg] : -1;
-        };
-        // the job's block of 16 rows and how many of them exist
-        auto block_of = [&](int job, int page, int &live) -> const uint8_t * {
-            const int j = row_of(job);
-            live = (unsigned)page < (unsigned)a.g.n_pages ? len - j : 0;
-            return head_pool + (live > 0 ? page : 0) * a.g.page_stride + ((j & (P - 1)) >> 4) * (32 * (C::RB + C::SB));
-        };
-        auto wait_empty = [&](int job) {
-            const int k = job >> 4;
-            return k < 2 || wait_all((job & 8 ? v_empty : k_empty) + (k & 1), ((k >> 1) - 1) & 1, DEVERR_TIMEOUT_PRODUCER);
-        };
-        auto announce = [&](int job) {
-            fence_proxy_async_smem();
+            // every product done before TMEM is given back (also after an abort)
+            if (lead) tc_commit(drain + w);
             __syncwarp();
-            if (lane == 0) mbar_arrive((job & 8 ? v_full : k_full) + ((job >> 4) & 1));
-        };
-        constexpr int kStep = C::kProducerWarps;
-        int job = warp - 8;
-        if constexpr (I4) {
-            // A lane takes unit un = lane / 8 of rows lane % 8 and lane % 8 + 8: a quarter warp then stores eight
-            // rows of one unit, which the tile's swizzle spreads over all banks.  K: the words of dims 32 j +
-            // 8 un of all groups j; V: the dims of group un (D = 64: two groups a row, row by un / 2).
-            const NibbleMasks nib;
-            constexpr int kV = D / 64;   // V units a lane
-            const int lr = lane & 7, un = lane >> 3, vr = D == 128 ? lr : lr + 8 * (un >> 1), vu = D == 128 ? un : un & 1;
-            const uint32_t k_at = lr * C::RB + un * (D / 8), ks_at = 32 * C::RB + lr * C::SB;
-            const uint32_t v_at = (16 + vr) * C::RB + 16 * (vu ^ kv_swz_v(true, D, vr));
-            const uint32_t vs_at = 32 * C::RB + (16 + vr) * C::SB + 2 * vu;
-            const uint32_t k_to = lr * 128 + ((un ^ lr) << 4);                                        // + j: see below
-            const uint32_t v_to = (vu >> 1) * kChunk + vr * 128 + (((4 * (vu & 1)) ^ lr) << 4);       // vr % 8 = lr
-            struct Raw {
-                uint4 w[2];
-                uint2 s[2];
-            };
-            auto load = [&](int jb, int page, Raw &raw) {
-                int live;
-                const uint8_t *blk = block_of(jb, page, live);
-                if (jb & 8) {
-#pragma unroll
-                    for (int x = 0; x < kV; x++) {
-                        raw.w[x] = make_uint4(0u, 0u, 0u, 0u);
-                        raw.s[x].x = 0u;
-                        if (vr + 8 * x >= live) continue;
-                        raw.w[x] = *reinterpret_cast<const uint4 *>(blk + v_at + 8 * x * C::RB);   // 8 rows on: the same swap
-                        raw.s[x].x = *reinterpret_cast<const uint16_t *>(blk + vs_at + 8 * x * C::SB);
-                    }
-                } else {
-#pragma unroll
-                    for (int x = 0; x < 2; x++) {
-                        raw.w[x] = make_uint4(0u, 0u, 0u, 0u);
-                        raw.s[x] = make_uint2(0u, 0u);
-                        if (lr + 8 * x >= live) continue;
-                        if constexpr (D == 128) {
-                            raw.w[x] = *reinterpret_cast<const uint4 *>(blk + k_at + 8 * x * C::RB);
-                            raw.s[x] = *reinterpret_cast<const uint2 *>(blk + ks_at + 8 * x * C::SB);
-                        } else {
-                            const uint2 y = *reinterpret_cast<const uint2 *>(blk + k_at + 8 * x * C::RB);
-                            raw.w[x].x = y.x;
-                            raw.w[x].y = y.y;
-                            raw.s[x].x = *reinterpret_cast<const uint32_t *>(blk + ks_at + 8 * x * C::SB);
-                        }
-                    }
-                }
-            };
-            auto store = [&](int jb, const Raw &raw) {
-                uint8_t *dst = (jb & 8 ? sV : sK) + ((jb >> 4) & 1) * C::kTile + (jb & 7) * (16 * 128);
-                if (jb & 8) {
-#pragma unroll
-                    for (int x = 0; x < kV; x++) {
-                        const uint32_t e[4] = {raw.w[x].x, raw.w[x].y, raw.w[x].z, raw.w[x].w};
-                        const __half2 sc = bits_h2(__byte_perm(raw.s[x].x, 0u, 0x1010));
-#pragma unroll
-                        for (int q = 0; q < 4; q++)
-                            *reinterpret_cast<uint4 *>(dst + x * 1024 + (v_to ^ (q << 4))) = dequant_unit(e[q], nib, sc);
-                    }
-                } else {
-#pragma unroll
-                    for (int x = 0; x < 2; x++) {
-                        const uint32_t e[4] = {raw.w[x].x, raw.w[x].y, raw.w[x].z, raw.w[x].w};
-#pragma unroll
-                        for (int j = 0; j < D / 32; j++) {   // unit 4 j + un: chunk j / 2, place (4 (j % 2) + un) ^ row
-                            const __half2 sc = bits_h2(__byte_perm((j >> 1) ? raw.s[x].y : raw.s[x].x, 0u, j & 1 ? 0x3232 : 0x1010));
-                            *reinterpret_cast<uint4 *>(dst + (j >> 1) * kChunk + x * 1024 + (k_to ^ ((j & 1) << 6))) =
-                                dequant_unit(e[j], nib, sc);
-                        }
-                    }
-                }
-            };
-            Raw ra, rb;   // this job's rows and the next one's, in turn
-            load(job, page_of(job), ra);
-            int page = page_of(job + kStep);
-            auto one = [&](Raw &cur, Raw &next) {
-                if (job + kStep < jobs) load(job + kStep, page, next);
-                page = page_of(job + 2 * kStep);
-                if (!wait_empty(job)) return false;
-                store(job, cur);
-                announce(job);
-                job += kStep;
-                return job < jobs;
-            };
-            while (one(ra, rb) && one(rb, ra)) {}
+            const unsigned long long t0 = globaltimer_ns();
+            while (!mbar_try_wait(drain + w, 0) && globaltimer_ns() - t0 < kWaitLimitNs) {}
+            __syncwarp();
         } else {
-            // a job is announced when the second one behind it has been requested
-            int issued = 0, page = page_of(job);
-            for (; job < jobs; job += kStep, issued++) {
-                int live;
-                const uint8_t *blk = block_of(job, page, live);
-                page = page_of(job + kStep);
-                if (!wait_empty(job)) break;
-                const int is_v = (job >> 3) & 1, r0 = (job & 7) * 16;
-                const uint32_t dst = smem_u32((is_v ? sV : sK) + ((job >> 4) & 1) * C::kTile);
-#pragma unroll
-                for (int x = 0; x < 16 * NU / 32; x++) {
-                    const int it = lane + 32 * x, r = it / NU, u = it % NU;
-                    const int su = u ^ (is_v ? kv_swz_v(false, D, r) : kv_swz_k(false, r));
-                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + tile_unit(r0 + r, u)),
-                                 "l"(blk + (is_v * 16 + r) * C::RB + su * 16), "r"(r < live ? 16 : 0)
-                                 : "memory");
+            // ---- pages -> tiles.  A job is 16 rows of K or V, one block of a page: jobs K0 .. K7, V0 .. V7
+            // of key block 0, then of block 1, ...; producer warp pw takes jobs pw, pw + 6, ... of an item.  A job's
+            // page number is loaded two jobs ahead, its rows one job ahead.
+            const int P = a.g.P, lg = a.g.lgP;
+            int kb = 0, jobs = 0, c0 = 0, len = 0;   // key blocks of the items before; this item
+            const uint8_t *head_pool = nullptr;
+            const int *trow = nullptr;
+            KeyTiles kt(KT, 0, 0, 0, 0);
+            auto row_of = [&](int job) { return kt.tile(c0 + (job >> 4)) * KT + (job & 7) * 16; };
+            auto page_of = [&](int job) {   // -1: nothing to load
+                if (job >= jobs) return -1;
+                const int j = row_of(job);
+                return j < len ? trow[j >> lg] : -1;
+            };
+            // the job's block of 16 rows and how many of them exist
+            auto block_of = [&](int job, int page, int &live) -> const uint8_t * {
+                const int j = row_of(job);
+                live = (unsigned)page < (unsigned)a.g.n_pages ? len - j : 0;
+                return head_pool + (live > 0 ? page : 0) * a.g.page_stride + ((j & (P - 1)) >> 4) * (32 * (C::RB + C::SB));
+            };
+            auto wait_empty = [&](int job) {
+                const int k = kb + (job >> 4);
+                return k < 2 || wait_all((job & 8 ? v_empty : k_empty) + (k & 1), ((k >> 1) - 1) & 1, DEVERR_TIMEOUT_PRODUCER);
+            };
+            auto stage_of = [&](int job) { return ((job & 8 ? sV : sK) + ((kb + (job >> 4)) & 1) * C::kTile); };
+            auto announce = [&](int job) {
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive((job & 8 ? v_full : k_full) + ((kb + (job >> 4)) & 1));
+            };
+            constexpr int kStep = C::kProducerWarps;
+            int job = 0;
+            // the next item's jobs for this warp; false: no more items
+            int it = -1;
+            auto next_item = [&]() {
+                kb += jobs >> 4;
+                it++;
+                if (warp == 8) {
+                    // the ring's place is free once every warp has read the item before last
+                    if (it >= 2 && !wait_all(item_empty + (it & 1), ((it >> 1) - 1) & 1, DEVERR_TIMEOUT_PRODUCER)) return false;
+                    if (lane == 0) {
+                        int index = blockIdx.x;
+                        if (it > 0) index = gridDim.x + atomicAdd(a.ticket, 1);
+                        while (index < items && !ManyItem(a, pairs, index).on) index = gridDim.x + atomicAdd(a.ticket, 1);
+                        ring[it & 1] = index;
+                        mbar_arrive(item_full + (it & 1));
+                    }
+                    __syncwarp();
                 }
-                asm volatile("cp.async.commit_group;" ::: "memory");
-                if (issued >= 2) {
-                    asm volatile("cp.async.wait_group 2;" ::: "memory");
-                    announce(job - 2 * kStep);
+                const int index = take(it);
+                if (index >= items) return false;
+                const ManyItem m(a, pairs, index);
+                jobs = 16 * m.n;
+                c0 = m.c0;
+                len = m.len;
+                kt = m.kt;
+                head_pool = a.pool + kv_seg_off(a.g, 0, 0, m.head);
+                trow = a.m.table + (long long)a.m.seq[m.b] * a.g.max_pages;
+                job = warp - 8;
+                return true;
+            };
+            if constexpr (I4) {
+                // A lane takes unit un = lane / 8 of rows lane % 8 and lane % 8 + 8: a quarter warp then stores eight
+                // rows of one unit, which the tile's swizzle spreads over all banks.  K: the words of dims 32 j +
+                // 8 un of all groups j; V: the dims of group un (D = 64: two groups a row, row by un / 2).
+                const NibbleMasks nib;
+                constexpr int kV = D / 64;   // V units a lane
+                const int lr = lane & 7, un = lane >> 3, vr = D == 128 ? lr : lr + 8 * (un >> 1), vu = D == 128 ? un : un & 1;
+                const uint32_t k_at = lr * C::RB + un * (D / 8), ks_at = 32 * C::RB + lr * C::SB;
+                const uint32_t v_at = (16 + vr) * C::RB + 16 * (vu ^ kv_swz_v(true, D, vr));
+                const uint32_t vs_at = 32 * C::RB + (16 + vr) * C::SB + 2 * vu;
+                const uint32_t k_to = lr * 128 + ((un ^ lr) << 4);                                        // + j: see below
+                const uint32_t v_to = (vu >> 1) * kChunk + vr * 128 + (((4 * (vu & 1)) ^ lr) << 4);       // vr % 8 = lr
+                struct Raw {
+                    uint4 w[2];
+                    uint2 s[2];
+                };
+                auto load = [&](int jb, int page, Raw &raw) {
+                    int live;
+                    const uint8_t *blk = block_of(jb, page, live);
+                    if (jb & 8) {
+#pragma unroll
+                        for (int x = 0; x < kV; x++) {
+                            raw.w[x] = make_uint4(0u, 0u, 0u, 0u);
+                            raw.s[x].x = 0u;
+                            if (vr + 8 * x >= live) continue;
+                            raw.w[x] = *reinterpret_cast<const uint4 *>(blk + v_at + 8 * x * C::RB);   // 8 rows on: the same swap
+                            raw.s[x].x = *reinterpret_cast<const uint16_t *>(blk + vs_at + 8 * x * C::SB);
+                        }
+                    } else {
+#pragma unroll
+                        for (int x = 0; x < 2; x++) {
+                            raw.w[x] = make_uint4(0u, 0u, 0u, 0u);
+                            raw.s[x] = make_uint2(0u, 0u);
+                            if (lr + 8 * x >= live) continue;
+                            if constexpr (D == 128) {
+                                raw.w[x] = *reinterpret_cast<const uint4 *>(blk + k_at + 8 * x * C::RB);
+                                raw.s[x] = *reinterpret_cast<const uint2 *>(blk + ks_at + 8 * x * C::SB);
+                            } else {
+                                const uint2 y = *reinterpret_cast<const uint2 *>(blk + k_at + 8 * x * C::RB);
+                                raw.w[x].x = y.x;
+                                raw.w[x].y = y.y;
+                                raw.s[x].x = *reinterpret_cast<const uint32_t *>(blk + ks_at + 8 * x * C::SB);
+                            }
+                        }
+                    }
+                };
+                auto store = [&](int jb, const Raw &raw) {
+                    uint8_t *dst = stage_of(jb) + (jb & 7) * (16 * 128);
+                    if (jb & 8) {
+#pragma unroll
+                        for (int x = 0; x < kV; x++) {
+                            const uint32_t e[4] = {raw.w[x].x, raw.w[x].y, raw.w[x].z, raw.w[x].w};
+                            const __half2 sc = bits_h2(__byte_perm(raw.s[x].x, 0u, 0x1010));
+#pragma unroll
+                            for (int q = 0; q < 4; q++)
+                                *reinterpret_cast<uint4 *>(dst + x * 1024 + (v_to ^ (q << 4))) = dequant_unit(e[q], nib, sc);
+                        }
+                    } else {
+#pragma unroll
+                        for (int x = 0; x < 2; x++) {
+                            const uint32_t e[4] = {raw.w[x].x, raw.w[x].y, raw.w[x].z, raw.w[x].w};
+#pragma unroll
+                            for (int j = 0; j < D / 32; j++) {   // unit 4 j + un: chunk j / 2, place (4 (j % 2) + un) ^ row
+                                const __half2 sc = bits_h2(__byte_perm((j >> 1) ? raw.s[x].y : raw.s[x].x, 0u, j & 1 ? 0x3232 : 0x1010));
+                                *reinterpret_cast<uint4 *>(dst + (j >> 1) * kChunk + x * 1024 + (k_to ^ ((j & 1) << 6))) =
+                                    dequant_unit(e[j], nib, sc);
+                            }
+                        }
+                    }
+                };
+                Raw ra, rb;   // this job's rows and the next one's, in turn
+                int page = -1;
+                bool ok = true;
+                auto one = [&](Raw &cur, Raw &next) {
+                    if (job + kStep < jobs) load(job + kStep, page, next);
+                    page = page_of(job + 2 * kStep);
+                    if (!(ok = wait_empty(job))) return false;
+                    store(job, cur);
+                    announce(job);
+                    job += kStep;
+                    return job < jobs;
+                };
+                while (ok && next_item()) {
+                    load(job, page_of(job), ra);
+                    page = page_of(job + kStep);
+                    while (one(ra, rb) && one(rb, ra)) {}
+                }
+            } else {
+                // a job is announced when the second one behind it has been requested
+                bool ok = true;
+                while (ok && next_item()) {
+                    int issued = 0, page = page_of(job);
+                    for (; job < jobs; job += kStep, issued++) {
+                        int live;
+                        const uint8_t *blk = block_of(job, page, live);
+                        page = page_of(job + kStep);
+                        if (!(ok = wait_empty(job))) break;
+                        const int is_v = (job >> 3) & 1, r0 = (job & 7) * 16;
+                        const uint32_t dst = smem_u32(stage_of(job));
+#pragma unroll
+                        for (int x = 0; x < 16 * NU / 32; x++) {
+                            const int it2 = lane + 32 * x, r = it2 / NU, u = it2 % NU;
+                            const int su = u ^ (is_v ? kv_swz_v(false, D, r) : kv_swz_k(false, r));
+                            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + tile_unit(r0 + r, u)),
+                                         "l"(blk + (is_v * 16 + r) * C::RB + su * 16), "r"(r < live ? 16 : 0)
+                                         : "memory");
+                        }
+                        asm volatile("cp.async.commit_group;" ::: "memory");
+                        if (issued >= 2) {
+                            asm volatile("cp.async.wait_group 2;" ::: "memory");
+                            announce(job - 2 * kStep);
+                        }
+                    }
+                    asm volatile("cp.async.wait_all;" ::: "memory");
+                    for (int i = min(issued, 2); i > 0; i--) announce(job - i * kStep);
                 }
             }
-            asm volatile("cp.async.wait_all;" ::: "memory");
-            for (int i = min(issued, 2); i > 0; i--) announce(job - i * kStep);
         }
     } else {
         // ---- softmax, a row a thread
-        const int w = warp >> 2, r = tid & 127, rr = w * 128 + r;
-        if (w < tiles) {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::kSoftmaxRegs));
+        const int w = warp >> 2, r = tid & 127, rr = w * 128 + r, G = a.G;
+        int hb = 0;   // half blocks of this tile in the items before
+        bool ok = true;
+        for (int it = 0; ok; it++) {
+            const int index = take(it);
+            if (index >= items) break;
+            const ManyItem mi(a, pairs, index);
+            if (w >= mi.tiles) continue;
+            const int head = mi.head, row0 = mi.row0, base = mi.base, rows = mi.rows, parts = mi.parts, i0 = mi.i0;
+            const int halves = mi.halves, c0 = mi.c0;
+            const KeyTiles &kt = mi.kt;
             const bool live = rr < rows;
             const int tok = (base + (live ? rr : 0)) / G, hg = (base + (live ? rr : 0)) % G, qi = live ? i0 + tok : -1;
             // Q: the warp loads its 32 rows two (D = 64: four) at a time, 16 bytes a lane; row offsets and scale
@@ -1250,11 +1388,10 @@ __global__ void __launch_bounds__(512, 1) kv_attend_many_kernel(const __grid_con
             const int q_min = i0 + (base + w * 128) / G, q_max = i0 + (base + min(rows, w * 128 + 128) - 1) / G;
             const int qlo = a.window ? qi - a.window : -1;   // the last row before the window
             float m = -INFINITY, l = 0.f;
-            bool ok = true;
             for (int i = 0; i < halves; i++) {
-                const int h = i & 1, j0 = kt.tile(c0 + (i >> 1)) * KT + 64 * h;
+                const int g = hb + i, h = g & 1, j0 = kt.tile(c0 + (i >> 1)) * KT + 64 * (i & 1);
                 const uint32_t ti = ts + 64 * h;
-                ok = wait_all(s_full + 2 * w + h, (i >> 1) & 1, DEVERR_TIMEOUT_EPILOGUE);
+                ok = wait_all(s_full + 2 * w + h, (g >> 1) & 1, DEVERR_TIMEOUT_EPILOGUE);
                 if (!ok) break;
                 tc_fence_after();
                 const bool all = j0 + 63 <= q_min && (a.window == 0 || j0 > q_max - a.window || j0 + 63 < a.sinks);
@@ -1297,7 +1434,7 @@ __global__ void __launch_bounds__(512, 1) kv_attend_many_kernel(const __grid_con
                     if (!__any_sync(0xffffffffu, top > m + 8.f)) break;
                     const float mn = fmaxf(m, top), corr = mn == -INFINITY ? 1.f : exp2f(m - mn);
                     if (i > 0) {
-                        ok = wait_all(pv_done + 2 * w + (h ^ 1), ((i - 1) >> 1) & 1, DEVERR_TIMEOUT_EPILOGUE);
+                        ok = wait_all(pv_done + 2 * w + (h ^ 1), ((g - 1) >> 1) & 1, DEVERR_TIMEOUT_EPILOGUE);
                         if (!ok) break;
                         tc_fence_after();
 #pragma unroll 1
@@ -1321,10 +1458,11 @@ __global__ void __launch_bounds__(512, 1) kv_attend_many_kernel(const __grid_con
                 tc_fence_before();
                 mbar_arrive(p_full + 2 * w + h);
             }
-            const int last = halves - 1;   // its product follows all others into O
+            hb += halves;
+            const int last = hb - 1;   // its product follows all others into O
             if (ok && wait_all(pv_done + 2 * w + (last & 1), (last >> 1) & 1, DEVERR_TIMEOUT_EPILOGUE)) {
                 tc_fence_after();
-                float *wp = many_part<D>(a, unit, split);
+                float *wp = many_part<D>(a, mi.unit, mi.split);
                 uint8_t *sO = sQ + w * C::kTile;   // Q is dead: O's rows on their way to whole-row stores
                 const float inv = 1.0f / l;   // l = 0: every score was -inf, and 0 * inf is the formula's NaN
                 bool bad = false;
@@ -1367,29 +1505,14 @@ __global__ void __launch_bounds__(512, 1) kv_attend_many_kernel(const __grid_con
                     }
                     __syncwarp();
                 }
-                // a NaN: recompute the row so that key rows it cannot see do not reach it
-                for (unsigned todo = __ballot_sync(0xffffffffu, bad && live); todo; todo &= todo - 1) {
-                    const int x = __ffs(todo) - 1, xr = wr + x, xt = (base + xr) / G, xh = (base + xr) % G;
-                    float mm, ll, oo[D / 32];
-                    kv_row_plain<D>(a, trow, head, a.q + (long long)(row0 + xt) * a.q_row + (long long)(head * G + xh) * a.q_head,
-                                    i0 + xt, KT, kt, c0, c1, mm, ll, oo);
-                    bf16 *xo = a.out + (long long)(row0 + xt) * a.o_row + (long long)(head * G + xh) * a.o_head;
-                    for (int i = 0; i < D / 32; i++) {
-                        const int d = lane + 32 * i;
-                        if (parts == 1) xo[d] = __float2bfloat16_rn(oo[i] / ll);
-                        else wp[((d >> 2) * 256 + xr) * 4 + (d & 3)] = oo[i];
-                    }
-                    if (parts > 1 && lane == 0) {
-                        wp[256 * D + xr] = mm;
-                        wp[256 * (D + 1) + xr] = ll;
-                    }
-                    __syncwarp();
-                }
+                if (__any_sync(0xffffffffu, bad && live)) many_repair<D>(a, pairs, index);
             }
         }
     }
     tc_fence_before();
     __syncthreads();
+    // the last CTA leaves the counters at zero for the next launch
+    if (tid == 0 && atomicAdd(a.ticket + 1, 1) == (int)gridDim.x - 1) a.ticket[0] = a.ticket[1] = 0;
     if (warp == 15) {
         tc_fence_after();
         tmem_dealloc(tbase, 512);
@@ -1397,10 +1520,10 @@ __global__ void __launch_bounds__(512, 1) kv_attend_many_kernel(const __grid_con
 }
 
 template <int D, bool I4>
-cudaError_t launch_many(const KvAttendArgs &a, int pairs, cudaStream_t s) {
+cudaError_t launch_many(const KvAttendArgs &a, int pairs, int num_sms, cudaStream_t s) {
     const unsigned flags = pdl_enabled() ? kLaunchPdl : 0u, units = (unsigned)a.n_seq * a.g.H * pairs;
-    cudaError_t e = launch_k(flags, kv_attend_many_kernel<D, I4>, dim3(units * a.splits), dim3(ManyCfg<D, I4>::kThreads),
-                             ManyCfg<D, I4>::kSmem, s, a, pairs);
+    cudaError_t e = launch_k(flags, kv_attend_many_kernel<D, I4>, dim3(std::min(units * a.splits, (unsigned)num_sms)),
+                             dim3(ManyCfg<D, I4>::kThreads), ManyCfg<D, I4>::kSmem, s, a, pairs, (int)(units * a.splits));
     if (e != cudaSuccess || a.splits == 1) return e;
     return launch_k(flags, kv_join_many_kernel<D>, dim3(units, D / 16), dim3(256), 0, s, a, pairs);
 }
@@ -1438,10 +1561,10 @@ cudaError_t kv_attend_prepare(const KvGeom &g, KvShapes *k) {
     return g.D == 128 ? prepare<128, false>(k) : prepare<64, false>(k);
 }
 
-cudaError_t launch_kv_attend(const KvAttendArgs &a, bool many, int rows_or_pairs, cudaStream_t s) {
+cudaError_t launch_kv_attend(const KvAttendArgs &a, bool many, int rows_or_pairs, int num_sms, cudaStream_t s) {
     if (many) {
-        if (a.g.i4) return a.g.D == 128 ? launch_many<128, true>(a, rows_or_pairs, s) : launch_many<64, true>(a, rows_or_pairs, s);
-        return a.g.D == 128 ? launch_many<128, false>(a, rows_or_pairs, s) : launch_many<64, false>(a, rows_or_pairs, s);
+        if (a.g.i4) return a.g.D == 128 ? launch_many<128, true>(a, rows_or_pairs, num_sms, s) : launch_many<64, true>(a, rows_or_pairs, num_sms, s);
+        return a.g.D == 128 ? launch_many<128, false>(a, rows_or_pairs, num_sms, s) : launch_many<64, false>(a, rows_or_pairs, num_sms, s);
     }
     if (a.g.i4) return a.g.D == 128 ? launch_few<128, true>(a, rows_or_pairs, s) : launch_few<64, true>(a, rows_or_pairs, s);
     return a.g.D == 128 ? launch_few<128, false>(a, rows_or_pairs, s) : launch_few<64, false>(a, rows_or_pairs, s);
