@@ -171,7 +171,6 @@ struct KvAttendArgs {
     int splits, tiles_per_split;              // parts of a long key range, key tiles a part should hold
     float *ws;                                // partial results
     int *cnt;                                 // arrivals per split unit, zero between calls
-    int *ticket;                              // [2] items drawn, CTAs done; zero between calls
     int *err;
 };
 // What sizes the launches of a cache's attention kernels.
@@ -184,7 +183,7 @@ constexpr int kKvManyKeyTile = 128;
 cudaError_t kv_attend_prepare(const KvGeom &g, KvShapes *k);
 // many: sequences of more than kKvFewRows rows, in rows_or_pairs pairs of row tiles
 // (256 rows) at most; otherwise sequences of up to that many, rows_or_pairs at most
-cudaError_t launch_kv_attend(const KvAttendArgs &a, bool many, int rows_or_pairs, int num_sms, cudaStream_t s);
+cudaError_t launch_kv_attend(const KvAttendArgs &a, bool many, int rows_or_pairs, cudaStream_t s);
 // rows (new tokens x query heads per kv head) that the few-row kernel takes
 constexpr int kKvFewRows = 16;
 

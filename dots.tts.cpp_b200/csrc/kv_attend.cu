@@ -4,7 +4,6 @@
 // over the rows j <= i with window = 0, or j > i - window, or j < sinks.
 #include "kv.cuh"
 
-#include <algorithm>
 #include <cmath>
 #include <type_traits>
 
@@ -35,50 +34,61 @@ DTTS_DEV int part_start(int n, int parts, int s) {
     return s * q + min(s, n - parts * q);
 }
 
-DTTS_DEV float kv_elem(const KvGeom &g, const uint8_t *seg, bool is_v, int r, int d) {
-    if (g.i4) {
-        const int w = d >> 3;
-        const uint8_t *row = seg + kv_row_off(g, is_v, r);
-        const uint32_t q = *reinterpret_cast<const uint32_t *>(row + (is_v ? kv_word_v(g.D, w, r) : kv_word_k(g.D, w)));
-        const float s = __half2float(*reinterpret_cast<const __half *>(
-            seg + kv_scale_off(g, is_v, r) + (d >> 5) * 2));
-        return kv_nibble(q, d & 7) * s;
-    }
-    const int u = (d >> 3) ^ (is_v ? kv_swz_v(false, g.D, r) : kv_swz_k(false, r));
-    return __bfloat162float(*reinterpret_cast<const bf16 *>(seg + kv_row_off(g, is_v, r) + u * 16 + (d & 7) * 2));
-}
-
 // One query row against key tiles [v0, v1) by one warp in plain arithmetic: only
 // visible rows are touched, so a non-finite value in a row that this query cannot
 // see has no effect on it.  The fast kernels multiply such a row's V by zero and
-// come here when that has left a NaN.  o[c]: dim lane + 32 c.
+// come here when that has left a NaN.  32 keys at a time: a lane scores one of
+// them, then holds dims D / 32 lane .. of the sum over them.
 template <int D>
 __device__ __noinline__ void kv_row_plain(const KvAttendArgs &a, const int *trow, int head, const bf16 *q, int i, int KT,
                                           const KeyTiles &kt, int v0, int v1, float &m, float &l, float (&o)[D / 32]) {
     const int lane = threadIdx.x & 31;
+    constexpr int C = D / 32;
     m = -INFINITY;
     l = 0.f;
-    for (int c = 0; c < D / 32; c++) o[c] = 0.f;
-    for (int v = v0; v < v1; v++) {
-        const int j0 = kt.tile(v) * KT;
-        for (int jj = 0; jj < KT; jj++) {
-            const int j = j0 + jj;
-            if (!kv_visible(j, i, a.window, a.sinks)) continue;
-            const int page = trow[j >> a.g.lgP];
-            if (page < 0 || page >= a.g.n_pages) continue;
-            const uint8_t *seg = a.pool + kv_seg_off(a.g, page, 0, head);
+    for (int c = 0; c < C; c++) o[c] = 0.f;
+    for (int v = v0; v < v1; v++)
+        for (int jj = 0; jj < KT; jj += 32) {
+            const int j = kt.tile(v) * KT + jj + lane;
+            const bool in = jj + lane < KT && kv_visible(j, i, a.window, a.sinks);   // KT may be 16
+            const int page = in ? trow[j >> a.g.lgP] : -1;
+            const bool on = (unsigned)page < (unsigned)a.g.n_pages;
+            const uint8_t *seg = a.pool + kv_seg_off(a.g, on ? page : 0, 0, head);
             const int r = j & (a.g.P - 1);
             float s = 0.f;
-            for (int c = 0; c < D / 32; c++)
-                s = fmaf(__bfloat162float(q[lane + 32 * c]), kv_elem(a.g, seg, false, r, lane + 32 * c), s);
-            s = warp_sum(s) * a.scale_log2;
-            const float mn = fmaxf(m, s), mu = mn == -INFINITY ? 0.f : mn;
-            const float corr = exp2f(m - mu), p = exp2f(s - mu);
-            l = l * corr + p;
-            for (int c = 0; c < D / 32; c++) o[c] = o[c] * corr + p * kv_elem(a.g, seg, true, r, lane + 32 * c);
+            if (on) {
+#pragma unroll 4
+                for (int w = 0; w < D / 8; w++) {
+                    float x[8];
+                    kv_load8(a.g, seg, false, r, w, x);
+#pragma unroll
+                    for (int d = 0; d < 8; d++) s = fmaf(__bfloat162float(q[8 * w + d]), x[d], s);
+                }
+            }
+            s = on ? s * a.scale_log2 : -INFINITY;
+            const float mn = fmaxf(m, warp_max(s)), mu = mn == -INFINITY ? 0.f : mn;   // fmaxf drops a NaN; p keeps it
+            const float corr = exp2f(m - mu), p = on ? exp2f(s - mu) : 0.f;
+            l = l * corr + warp_sum(p);
+            for (int c = 0; c < C; c++) o[c] *= corr;
+            const unsigned live = __ballot_sync(0xffffffffu, on);
+#pragma unroll 4
+            for (int k = 0; k < 32; k++) {
+                const float pk = __shfl_sync(0xffffffffu, p, k);
+                const long long off = __shfl_sync(0xffffffffu, (long long)(seg - a.pool), k);
+                const int rk = __shfl_sync(0xffffffffu, r, k);
+                if (!((live >> k) & 1u)) continue;
+                float x[8];
+                kv_load8(a.g, a.pool + off, true, rk, lane * C / 8, x);
+#pragma unroll
+                for (int c = 0; c < C; c++) {
+                    float xc = 0.f;   // x[lane * C % 8 + c], with a constant index
+#pragma unroll
+                    for (int d = c; d < 8; d += C) xc = lane * C % 8 + c == d ? x[d] : xc;
+                    o[c] += pk * xc;
+                }
+            }
             m = mn;
         }
-    }
 }
 
 DTTS_DEV float merge_weight(float m, float top) { return m == -INFINITY ? 0.f : exp2f(m - top); }
@@ -667,7 +677,7 @@ __global__ void __launch_bounds__(FewCfg<D, I4>::kThreads, NT == 1 ? 3 : 1) kv_a
                             i0 + r / G, KT, kt, c0, c1, mm, ll, oo);
             for (int w = 0; w < C::kWarps; w++) {
                 float *dst = res + w * WS + r * RS;
-                for (int c = 0; c < D / 32; c++) dst[lane + 32 * c] = w ? 0.f : oo[c];
+                for (int c = 0; c < D / 32; c++) dst[D / 32 * lane + c] = w ? 0.f : oo[c];
                 if (lane == 0) { dst[D] = w ? -INFINITY : mm; dst[D + 1] = w ? 0.f : ll; }
             }
         }
@@ -800,22 +810,6 @@ struct ManyUnit {
         parts = min(a.splits, max(1, (kt.n + a.tiles_per_split - 1) / a.tiles_per_split));
     }
 };
-// A part of a unit's keys: what a CTA takes at a time.  Items are numbered from the longest key ranges down.
-struct ManyItem : ManyUnit {
-    int unit, split, c0, n, halves, tiles;   // first key block, key blocks, half blocks of 64 keys, row tiles
-    DTTS_DEV ManyItem(const KvAttendArgs &a, int pairs, int index)
-        : ManyUnit(a, index / a.splits % (a.n_seq * a.g.H), pairs - 1 - index / a.splits / (a.n_seq * a.g.H)),
-          split(index % a.splits) {
-        const int u = index / a.splits;
-        unit = u % (a.n_seq * a.g.H) * pairs + pairs - 1 - u / (a.n_seq * a.g.H);
-        on = on && split < parts;
-        c0 = part_start(kt.n, parts, split);
-        n = part_start(kt.n, parts, split + 1) - c0;
-        // the last half stays out where no row sees it
-        halves = 2 * n - (kt.tile(c0 + n - 1) * kKvManyKeyTile + 64 > i_last ? 1 : 0);
-        tiles = rows > 128 ? 2 : 1;
-    }
-};
 // A part's result: O as [D / 4][256 rows][4], then m [256], l [256], so that a warp's rows are contiguous.
 template <int D>
 DTTS_DEV float *many_part(const KvAttendArgs &a, int unit, int split) {
@@ -913,7 +907,8 @@ DTTS_DEV bool elect_one() {
 }
 
 // Waits like mbar_wait, asleep in the barrier for up to a microsecond a try, so that
-// a waiting role leaves the issue slots to the working ones.
+// a waiting role leaves the issue slots to the working ones; five times as long, for
+// a CTA may have to wait for TMEM until another one has recomputed rows.
 DTTS_DEV bool kv_wait(uint64_t *bar, uint32_t parity, volatile int *abort_flag, int *err, int code) {
     const uint32_t addr = smem_u32(bar);
     uint32_t done;
@@ -939,43 +934,10 @@ DTTS_DEV bool kv_wait(uint64_t *bar, uint32_t parity, volatile int *abort_flag, 
         if (*abort_flag) return false;
         const unsigned long long t = globaltimer_ns();
         if (t0 == 0) t0 = t;
-        if (t - t0 > kWaitLimitNs) {
+        if (t - t0 > 5 * kWaitLimitNs) {
             if (err) atomicCAS(err, 0, code);
             *abort_flag = 1;
             return false;
-        }
-    }
-}
-
-// Recomputes the rows of this warp (of eight) of an item that came out with a NaN, so that key rows that a query
-// cannot see do not reach it.
-template <int D>
-__device__ __noinline__ void many_repair(const KvAttendArgs &a, int pairs, int index) {
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const ManyItem m(a, pairs, index);
-    float *wp = many_part<D>(a, m.unit, m.split);
-    for (int r = warp * 32; r < min(m.rows, warp * 32 + 32); r++) {
-        const int tok = (m.base + r) / a.G, hq = m.head * a.G + (m.base + r) % a.G;
-        bf16 *o = a.out + (long long)(m.row0 + tok) * a.o_row + (long long)hq * a.o_head;
-        bool bad = false;
-        for (int i = 0; i < D / 32; i++) {
-            const int d = lane + 32 * i;
-            const float v = m.parts == 1 ? __bfloat162float(o[d]) : wp[((d >> 2) * 256 + r) * 4 + (d & 3)];
-            bad |= v != v;
-        }
-        if (!__any_sync(0xffffffffu, bad)) continue;
-        float mm, ll, oo[D / 32];
-        kv_row_plain<D>(a, a.m.table + (long long)a.m.seq[m.b] * a.g.max_pages, m.head,
-                        a.q + (long long)(m.row0 + tok) * a.q_row + (long long)hq * a.q_head, m.i0 + tok, kKvManyKeyTile, m.kt,
-                        m.c0, m.c0 + m.n, mm, ll, oo);
-        for (int i = 0; i < D / 32; i++) {
-            const int d = lane + 32 * i;
-            if (m.parts == 1) o[d] = __float2bfloat16_rn(oo[i] / ll);
-            else wp[((d >> 2) * 256 + r) * 4 + (d & 3)] = oo[i];
-        }
-        if (m.parts > 1 && lane == 0) {
-            wp[256 * D + r] = mm;
-            wp[256 * (D + 1) + r] = ll;
         }
     }
 }
@@ -1000,7 +962,7 @@ __device__ __noinline__ void many_repair(const KvAttendArgs &a, int pairs, int i
 // of |v|, the size of the output's own rounding): a second term would cost half as
 // much tensor time again.
 template <int D, bool I4>
-__global__ void __launch_bounds__(512, 1) kv_attend_many_kernel(const __grid_constant__ KvAttendArgs a, int pairs, int items) {
+__global__ void __launch_bounds__(512, 1) kv_attend_many_kernel(const __grid_constant__ KvAttendArgs a, int pairs) {
     using C = ManyCfg<D, I4>;
     constexpr int KT = C::KT, NU = D / 8;   // 16-byte units a row
     extern __shared__ uint8_t smem_raw[];
@@ -1010,11 +972,23 @@ __global__ void __launch_bounds__(512, 1) kv_attend_many_kernel(const __grid_con
     // s_full, p_full, pv_done: [tile][half]
     uint64_t *q_full = bars, *s_full = bars + 2, *p_full = bars + 6, *pv_done = bars + 10;
     uint64_t *k_full = bars + 14, *k_empty = bars + 16, *v_full = bars + 18, *v_empty = bars + 20, *drain = bars + 22;
-    uint64_t *item_full = bars + 24, *item_empty = bars + 26;
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 28);
-    volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1), *ring = abort_flag + 1;   // ring [2]
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 24);
+    volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     pdl_wait();
+
+    const int split = blockIdx.x % a.splits, u = blockIdx.x / a.splits;
+    const int bh = u % (a.n_seq * a.g.H), pair = pairs - 1 - u / (a.n_seq * a.g.H);   // longest key ranges first
+    const int unit = bh * pairs + pair;
+    const ManyUnit mu(a, bh, pair);
+    if (!mu.on || split >= mu.parts) return;
+    const int head = mu.head, len = mu.len, row0 = mu.row0, G = a.G, base = mu.base, rows = mu.rows, parts = mu.parts;
+    const int tiles = rows > 128 ? 2 : 1, i0 = mu.i0, i_last = mu.i_last;
+    const KeyTiles &kt = mu.kt;
+    const int *trow = a.m.table + (long long)a.m.seq[mu.b] * a.g.max_pages;
+    const int c0 = part_start(kt.n, parts, split), c1 = part_start(kt.n, parts, split + 1), n = c1 - c0;
+    // half blocks of 64 keys; the last one stays out where no row sees it
+    const int halves = 2 * n - (kt.tile(c1 - 1) * KT + 64 > i_last ? 1 : 0);
 
     if (tid == 0) {
         for (int w = 0; w < 2; w++) {
@@ -1025,12 +999,10 @@ __global__ void __launch_bounds__(512, 1) kv_attend_many_kernel(const __grid_con
                 mbar_init(pv_done + 2 * w + h, 1);
             }
             mbar_init(k_full + w, 8);
-            mbar_init(k_empty + w, 2);
+            mbar_init(k_empty + w, tiles);
             mbar_init(v_full + w, 8);
-            mbar_init(v_empty + w, 2);
+            mbar_init(v_empty + w, tiles);
             mbar_init(drain + w, 1);
-            mbar_init(item_full + w, 1);
-            mbar_init(item_empty + w, C::kThreads / 32);
         }
         *abort_flag = 0;
         fence_mbar_init();
@@ -1050,16 +1022,6 @@ __global__ void __launch_bounds__(512, 1) kv_attend_many_kernel(const __grid_con
     auto wait_all = [&](uint64_t *bar, uint32_t parity, int code) {
         return __all_sync(0xffffffffu, kv_wait(bar, parity, abort_flag, a.err, code)) != 0;
     };
-    // Items are drawn from a counter (a CTA's first one is its own number): producer warp 8 draws the next one when it
-    // has requested all of the last one's rows, and hands it to every warp through a ring of two.  Barrier phases
-    // run on from item to item, so loading and scores of the next item begin behind the last one's.
-    auto take = [&](int seq) {   // item number `seq` of this CTA; >= items: no more
-        if (!wait_all(item_full + (seq & 1), (seq >> 1) & 1, DEVERR_TIMEOUT_PRODUCER)) return items;
-        const int index = ring[seq & 1];
-        __syncwarp();
-        if (lane == 0) mbar_arrive(item_empty + (seq & 1));
-        return index;
-    };
     // the register split stands in the branch that it is for: behind a join the smaller share would hold for both
     if (warp >= 8) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kOtherRegs));
@@ -1070,72 +1032,54 @@ __global__ void __launch_bounds__(512, 1) kv_attend_many_kernel(const __grid_con
             constexpr uint32_t kTileD = C::kTile >> 4, kHalfD = (64 * 128) >> 4;   // descriptor units of 16 bytes
             const uint32_t qd = desc_k(smem_u32(sQ)) + w * kTileD, kd = desc_k(smem_u32(sK)), vd = desc_mn(smem_u32(sV));
             uint64_t *sf = s_full + 2 * w, *pf = p_full + 2 * w, *pd = pv_done + 2 * w;
-            // kb: key blocks of the items before; hb: half blocks of this tile before.  Half g = hb + i of the tile has
-            // score buffer g & 1.
-            int kb = 0, hb = 0, qn = 0;
-            bool ok = true;
-            auto scores = [&](int i) {   // Q K^T of half block i of the item, 64 keys, into buffer (hb + i) & 1
-                const int g = hb + i;
-                // whose columns P of half g - 2 was read from
-                if (g >= 2 && !wait_all(pd + (g & 1), ((g - 2) >> 1) & 1, DEVERR_TIMEOUT_MMA)) return false;
-                tc_fence_after();
-                const uint32_t kw = kd + ((kb + (i >> 1)) & 1) * kTileD + (i & 1) * kHalfD;
-                const uint32_t d = tbase + w * 128 + (g & 1) * 64;
+            auto scores = [&](int i) {   // of half block i: Q K^T, 64 keys
+                const uint32_t kw = kd + ((i >> 1) & 1) * kTileD + (i & 1) * kHalfD;
+                const uint32_t d = tbase + w * 128 + (i & 1) * 64;
                 if (lead) {
 #pragma unroll
                     for (int x = 0; x < D / 16; x++) {
                         const uint32_t off = ((x >> 2) * kChunk + (x & 3) * 32) >> 4;
                         tc_mma_ss(d, qd + off, kw + off, C::idesc(64), x ? 1u : 0u);
                     }
-                    tc_commit(sf + (g & 1));
+                    tc_commit(sf + (i & 1));
                 }
                 __syncwarp();
-                return true;
             };
-            for (int it = 0; ok; it++) {
-                const int index = take(it);
-                if (index >= items) break;
-                const ManyItem m(a, pairs, index);
-                if (w >= m.tiles) {   // no second tile: only release the blocks
-                    for (int k = kb; k < kb + m.n && ok; k++) {
-                        ok = wait_all(k_full + (k & 1), (k >> 1) & 1, DEVERR_TIMEOUT_MMA);
-                        if (ok && lane == 0) mbar_arrive(k_empty + (k & 1));
-                        ok = ok && wait_all(v_full + (k & 1), (k >> 1) & 1, DEVERR_TIMEOUT_MMA);
-                        if (ok && lane == 0) mbar_arrive(v_empty + (k & 1));
-                    }
-                    kb += m.n;
-                    continue;
+            if (w < tiles) {
+                bool ok = wait_all(k_full, 0, DEVERR_TIMEOUT_MMA) && wait_all(q_full + w, 0, DEVERR_TIMEOUT_MMA);
+                if (ok) {
+                    tc_fence_after();
+                    scores(0);
                 }
-                ok = wait_all(k_full + (kb & 1), (kb >> 1) & 1, DEVERR_TIMEOUT_MMA) &&
-                     wait_all(q_full + w, qn & 1, DEVERR_TIMEOUT_MMA) && scores(0);
-                qn++;
-                for (int i = 0; i < m.halves && ok; i++) {
-                    const int k = kb + (i >> 1), g = hb + i;
-                    if (i + 1 < m.halves) {
-                        if (i & 1) ok = wait_all(k_full + ((k + 1) & 1), ((k + 1) >> 1) & 1, DEVERR_TIMEOUT_MMA);
-                        if (!ok || !(ok = scores(i + 1))) break;
+                for (int i = 0; i < halves && ok; i++) {
+                    const int k = i >> 1, h = i & 1;
+                    if (i + 1 < halves) {
+                        // the next half's scores take the columns that P of the half before this one is read from
+                        if (h == 1) ok = wait_all(k_full + ((k + 1) & 1), ((k + 1) >> 1) & 1, DEVERR_TIMEOUT_MMA);
+                        if (ok && i >= 1) ok = wait_all(pd + (h ^ 1), ((i - 1) >> 1) & 1, DEVERR_TIMEOUT_MMA);
+                        if (!ok) break;
+                        tc_fence_after();
+                        scores(i + 1);
                     }
-                    if (!(i & 1)) {
+                    if (h == 0) {
                         if (lead) tc_commit(k_empty + (k & 1));   // both halves' scores are issued
                         __syncwarp();
                         ok = wait_all(v_full + (k & 1), (k >> 1) & 1, DEVERR_TIMEOUT_MMA);
                     }
-                    ok = ok && wait_all(pf + (g & 1), (g >> 1) & 1, DEVERR_TIMEOUT_MMA);
+                    ok = ok && wait_all(pf + h, k & 1, DEVERR_TIMEOUT_MMA);
                     if (!ok) break;
                     tc_fence_after();
-                    const uint32_t vw = vd + (k & 1) * kTileD + (i & 1) * kHalfD;
-                    const uint32_t d = tbase + 256 + w * 128, p = tbase + w * 128 + (g & 1) * 64;
+                    const uint32_t vw = vd + (k & 1) * kTileD + h * kHalfD;
+                    const uint32_t d = tbase + 256 + w * 128, p = tbase + w * 128 + h * 64;
                     if (lead) {
 #pragma unroll
                         for (int x = 0; x < 4; x++)
                             tc_mma_ts(d, p + 8 * x, vw + x * (2048 >> 4), C::idesc(D) | (1u << 16), i || x ? 1u : 0u);
-                        tc_commit(pd + (g & 1));
-                        if ((i & 1) || i + 1 == m.halves) tc_commit(v_empty + (k & 1));
+                        tc_commit(pd + h);
+                        if (h == 1) tc_commit(v_empty + (k & 1));
                     }
                     __syncwarp();
                 }
-                kb += m.n;
-                hb += m.halves;
             }
             // every product done before TMEM is given back (also after an abort)
             if (lead) tc_commit(drain + w);
@@ -1145,13 +1089,10 @@ __global__ void __launch_bounds__(512, 1) kv_attend_many_kernel(const __grid_con
             __syncwarp();
         } else {
             // ---- pages -> tiles.  A job is 16 rows of K or V, one block of a page: jobs K0 .. K7, V0 .. V7
-            // of key block 0, then of block 1, ...; producer warp pw takes jobs pw, pw + 6, ... of an item.  A job's
-            // page number is loaded two jobs ahead, its rows one job ahead.
-            const int P = a.g.P, lg = a.g.lgP;
-            int kb = 0, jobs = 0, c0 = 0, len = 0;   // key blocks of the items before; this item
-            const uint8_t *head_pool = nullptr;
-            const int *trow = nullptr;
-            KeyTiles kt(KT, 0, 0, 0, 0);
+            // of key block 0, then of block 1, ...; producer warp pw takes jobs pw, pw + 7, ...  A job's page
+            // number is loaded two jobs ahead, its rows one job ahead.
+            const int P = a.g.P, lg = a.g.lgP, jobs = 16 * n;
+            const uint8_t *head_pool = a.pool + kv_seg_off(a.g, 0, 0, head);
             auto row_of = [&](int job) { return kt.tile(c0 + (job >> 4)) * KT + (job & 7) * 16; };
             auto page_of = [&](int job) {   // -1: nothing to load
                 if (job >= jobs) return -1;
@@ -1165,46 +1106,16 @@ __global__ void __launch_bounds__(512, 1) kv_attend_many_kernel(const __grid_con
                 return head_pool + (live > 0 ? page : 0) * a.g.page_stride + ((j & (P - 1)) >> 4) * (32 * (C::RB + C::SB));
             };
             auto wait_empty = [&](int job) {
-                const int k = kb + (job >> 4);
+                const int k = job >> 4;
                 return k < 2 || wait_all((job & 8 ? v_empty : k_empty) + (k & 1), ((k >> 1) - 1) & 1, DEVERR_TIMEOUT_PRODUCER);
             };
-            auto stage_of = [&](int job) { return ((job & 8 ? sV : sK) + ((kb + (job >> 4)) & 1) * C::kTile); };
             auto announce = [&](int job) {
                 fence_proxy_async_smem();
                 __syncwarp();
-                if (lane == 0) mbar_arrive((job & 8 ? v_full : k_full) + ((kb + (job >> 4)) & 1));
+                if (lane == 0) mbar_arrive((job & 8 ? v_full : k_full) + ((job >> 4) & 1));
             };
             constexpr int kStep = C::kProducerWarps;
-            int job = 0;
-            // the next item's jobs for this warp; false: no more items
-            int it = -1;
-            auto next_item = [&]() {
-                kb += jobs >> 4;
-                it++;
-                if (warp == 8) {
-                    // the ring's place is free once every warp has read the item before last
-                    if (it >= 2 && !wait_all(item_empty + (it & 1), ((it >> 1) - 1) & 1, DEVERR_TIMEOUT_PRODUCER)) return false;
-                    if (lane == 0) {
-                        int index = blockIdx.x;
-                        if (it > 0) index = gridDim.x + atomicAdd(a.ticket, 1);
-                        while (index < items && !ManyItem(a, pairs, index).on) index = gridDim.x + atomicAdd(a.ticket, 1);
-                        ring[it & 1] = index;
-                        mbar_arrive(item_full + (it & 1));
-                    }
-                    __syncwarp();
-                }
-                const int index = take(it);
-                if (index >= items) return false;
-                const ManyItem m(a, pairs, index);
-                jobs = 16 * m.n;
-                c0 = m.c0;
-                len = m.len;
-                kt = m.kt;
-                head_pool = a.pool + kv_seg_off(a.g, 0, 0, m.head);
-                trow = a.m.table + (long long)a.m.seq[m.b] * a.g.max_pages;
-                job = warp - 8;
-                return true;
-            };
+            int job = warp - 8;
             if constexpr (I4) {
                 // A lane takes unit un = lane / 8 of rows lane % 8 and lane % 8 + 8: a quarter warp then stores eight
                 // rows of one unit, which the tile's swizzle spreads over all banks.  K: the words of dims 32 j +
@@ -1252,7 +1163,7 @@ __global__ void __launch_bounds__(512, 1) kv_attend_many_kernel(const __grid_con
                     }
                 };
                 auto store = [&](int jb, const Raw &raw) {
-                    uint8_t *dst = stage_of(jb) + (jb & 7) * (16 * 128);
+                    uint8_t *dst = (jb & 8 ? sV : sK) + ((jb >> 4) & 1) * C::kTile + (jb & 7) * (16 * 128);
                     if (jb & 8) {
 #pragma unroll
                         for (int x = 0; x < kV; x++) {
@@ -1276,67 +1187,51 @@ __global__ void __launch_bounds__(512, 1) kv_attend_many_kernel(const __grid_con
                     }
                 };
                 Raw ra, rb;   // this job's rows and the next one's, in turn
-                int page = -1;
-                bool ok = true;
+                load(job, page_of(job), ra);
+                int page = page_of(job + kStep);
                 auto one = [&](Raw &cur, Raw &next) {
                     if (job + kStep < jobs) load(job + kStep, page, next);
                     page = page_of(job + 2 * kStep);
-                    if (!(ok = wait_empty(job))) return false;
+                    if (!wait_empty(job)) return false;
                     store(job, cur);
                     announce(job);
                     job += kStep;
                     return job < jobs;
                 };
-                while (ok && next_item()) {
-                    load(job, page_of(job), ra);
-                    page = page_of(job + kStep);
-                    while (one(ra, rb) && one(rb, ra)) {}
-                }
+                while (one(ra, rb) && one(rb, ra)) {}
             } else {
                 // a job is announced when the second one behind it has been requested
-                bool ok = true;
-                while (ok && next_item()) {
-                    int issued = 0, page = page_of(job);
-                    for (; job < jobs; job += kStep, issued++) {
-                        int live;
-                        const uint8_t *blk = block_of(job, page, live);
-                        page = page_of(job + kStep);
-                        if (!(ok = wait_empty(job))) break;
-                        const int is_v = (job >> 3) & 1, r0 = (job & 7) * 16;
-                        const uint32_t dst = smem_u32(stage_of(job));
+                int issued = 0, page = page_of(job);
+                for (; job < jobs; job += kStep, issued++) {
+                    int live;
+                    const uint8_t *blk = block_of(job, page, live);
+                    page = page_of(job + kStep);
+                    if (!wait_empty(job)) break;
+                    const int is_v = (job >> 3) & 1, r0 = (job & 7) * 16;
+                    const uint32_t dst = smem_u32((is_v ? sV : sK) + ((job >> 4) & 1) * C::kTile);
 #pragma unroll
-                        for (int x = 0; x < 16 * NU / 32; x++) {
-                            const int it2 = lane + 32 * x, r = it2 / NU, u = it2 % NU;
-                            const int su = u ^ (is_v ? kv_swz_v(false, D, r) : kv_swz_k(false, r));
-                            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + tile_unit(r0 + r, u)),
-                                         "l"(blk + (is_v * 16 + r) * C::RB + su * 16), "r"(r < live ? 16 : 0)
-                                         : "memory");
-                        }
-                        asm volatile("cp.async.commit_group;" ::: "memory");
-                        if (issued >= 2) {
-                            asm volatile("cp.async.wait_group 2;" ::: "memory");
-                            announce(job - 2 * kStep);
-                        }
+                    for (int x = 0; x < 16 * NU / 32; x++) {
+                        const int it = lane + 32 * x, r = it / NU, u = it % NU;
+                        const int su = u ^ (is_v ? kv_swz_v(false, D, r) : kv_swz_k(false, r));
+                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + tile_unit(r0 + r, u)),
+                                     "l"(blk + (is_v * 16 + r) * C::RB + su * 16), "r"(r < live ? 16 : 0)
+                                     : "memory");
                     }
-                    asm volatile("cp.async.wait_all;" ::: "memory");
-                    for (int i = min(issued, 2); i > 0; i--) announce(job - i * kStep);
+                    asm volatile("cp.async.commit_group;" ::: "memory");
+                    if (issued >= 2) {
+                        asm volatile("cp.async.wait_group 2;" ::: "memory");
+                        announce(job - 2 * kStep);
+                    }
                 }
+                asm volatile("cp.async.wait_all;" ::: "memory");
+                for (int i = min(issued, 2); i > 0; i--) announce(job - i * kStep);
             }
         }
     } else {
         // ---- softmax, a row a thread
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::kSoftmaxRegs));
-        const int w = warp >> 2, r = tid & 127, rr = w * 128 + r, G = a.G;
-        int hb = 0;   // half blocks of this tile in the items before
-        bool ok = true;
-        for (int it = 0; ok; it++) {
-            const int index = take(it);
-            if (index >= items) break;
-            const ManyItem mi(a, pairs, index);
-            if (w >= mi.tiles) continue;
-            const int head = mi.head, row0 = mi.row0, base = mi.base, rows = mi.rows, parts = mi.parts, i0 = mi.i0;
-            const int halves = mi.halves, c0 = mi.c0;
-            const KeyTiles &kt = mi.kt;
+        const int w = warp >> 2, r = tid & 127, rr = w * 128 + r;
+        if (w < tiles) {
             const bool live = rr < rows;
             const int tok = (base + (live ? rr : 0)) / G, hg = (base + (live ? rr : 0)) % G, qi = live ? i0 + tok : -1;
             // Q: the warp loads its 32 rows two (D = 64: four) at a time, 16 bytes a lane; row offsets and scale
@@ -1388,10 +1283,11 @@ __global__ void __launch_bounds__(512, 1) kv_attend_many_kernel(const __grid_con
             const int q_min = i0 + (base + w * 128) / G, q_max = i0 + (base + min(rows, w * 128 + 128) - 1) / G;
             const int qlo = a.window ? qi - a.window : -1;   // the last row before the window
             float m = -INFINITY, l = 0.f;
+            bool ok = true;
             for (int i = 0; i < halves; i++) {
-                const int g = hb + i, h = g & 1, j0 = kt.tile(c0 + (i >> 1)) * KT + 64 * (i & 1);
+                const int h = i & 1, j0 = kt.tile(c0 + (i >> 1)) * KT + 64 * h;
                 const uint32_t ti = ts + 64 * h;
-                ok = wait_all(s_full + 2 * w + h, (g >> 1) & 1, DEVERR_TIMEOUT_EPILOGUE);
+                ok = wait_all(s_full + 2 * w + h, (i >> 1) & 1, DEVERR_TIMEOUT_EPILOGUE);
                 if (!ok) break;
                 tc_fence_after();
                 const bool all = j0 + 63 <= q_min && (a.window == 0 || j0 > q_max - a.window || j0 + 63 < a.sinks);
@@ -1434,7 +1330,7 @@ __global__ void __launch_bounds__(512, 1) kv_attend_many_kernel(const __grid_con
                     if (!__any_sync(0xffffffffu, top > m + 8.f)) break;
                     const float mn = fmaxf(m, top), corr = mn == -INFINITY ? 1.f : exp2f(m - mn);
                     if (i > 0) {
-                        ok = wait_all(pv_done + 2 * w + (h ^ 1), ((g - 1) >> 1) & 1, DEVERR_TIMEOUT_EPILOGUE);
+                        ok = wait_all(pv_done + 2 * w + (h ^ 1), ((i - 1) >> 1) & 1, DEVERR_TIMEOUT_EPILOGUE);
                         if (!ok) break;
                         tc_fence_after();
 #pragma unroll 1
@@ -1458,11 +1354,10 @@ __global__ void __launch_bounds__(512, 1) kv_attend_many_kernel(const __grid_con
                 tc_fence_before();
                 mbar_arrive(p_full + 2 * w + h);
             }
-            hb += halves;
-            const int last = hb - 1;   // its product follows all others into O
+            const int last = halves - 1;   // its product follows all others into O
             if (ok && wait_all(pv_done + 2 * w + (last & 1), (last >> 1) & 1, DEVERR_TIMEOUT_EPILOGUE)) {
                 tc_fence_after();
-                float *wp = many_part<D>(a, mi.unit, mi.split);
+                float *wp = many_part<D>(a, unit, split);
                 uint8_t *sO = sQ + w * C::kTile;   // Q is dead: O's rows on their way to whole-row stores
                 const float inv = 1.0f / l;   // l = 0: every score was -inf, and 0 * inf is the formula's NaN
                 bool bad = false;
@@ -1505,14 +1400,29 @@ __global__ void __launch_bounds__(512, 1) kv_attend_many_kernel(const __grid_con
                     }
                     __syncwarp();
                 }
-                if (__any_sync(0xffffffffu, bad && live)) many_repair<D>(a, pairs, index);
+                // a NaN: recompute the row so that key rows it cannot see do not reach it
+                for (unsigned todo = __ballot_sync(0xffffffffu, bad && live); todo; todo &= todo - 1) {
+                    const int x = __ffs(todo) - 1, xr = wr + x, xt = (base + xr) / G, xh = (base + xr) % G;
+                    float mm, ll, oo[D / 32];
+                    kv_row_plain<D>(a, trow, head, a.q + (long long)(row0 + xt) * a.q_row + (long long)(head * G + xh) * a.q_head,
+                                    i0 + xt, KT, kt, c0, c1, mm, ll, oo);
+                    bf16 *xo = a.out + (long long)(row0 + xt) * a.o_row + (long long)(head * G + xh) * a.o_head;
+                    for (int i = 0; i < D / 32; i++) {
+                        const int d = D / 32 * lane + i;
+                        if (parts == 1) xo[d] = __float2bfloat16_rn(oo[i] / ll);
+                        else wp[((d >> 2) * 256 + xr) * 4 + (d & 3)] = oo[i];
+                    }
+                    if (parts > 1 && lane == 0) {
+                        wp[256 * D + xr] = mm;
+                        wp[256 * (D + 1) + xr] = ll;
+                    }
+                    __syncwarp();
+                }
             }
         }
     }
     tc_fence_before();
     __syncthreads();
-    // the last CTA leaves the counters at zero for the next launch
-    if (tid == 0 && atomicAdd(a.ticket + 1, 1) == (int)gridDim.x - 1) a.ticket[0] = a.ticket[1] = 0;
     if (warp == 15) {
         tc_fence_after();
         tmem_dealloc(tbase, 512);
@@ -1520,10 +1430,10 @@ __global__ void __launch_bounds__(512, 1) kv_attend_many_kernel(const __grid_con
 }
 
 template <int D, bool I4>
-cudaError_t launch_many(const KvAttendArgs &a, int pairs, int num_sms, cudaStream_t s) {
+cudaError_t launch_many(const KvAttendArgs &a, int pairs, cudaStream_t s) {
     const unsigned flags = pdl_enabled() ? kLaunchPdl : 0u, units = (unsigned)a.n_seq * a.g.H * pairs;
-    cudaError_t e = launch_k(flags, kv_attend_many_kernel<D, I4>, dim3(std::min(units * a.splits, (unsigned)num_sms)),
-                             dim3(ManyCfg<D, I4>::kThreads), ManyCfg<D, I4>::kSmem, s, a, pairs, (int)(units * a.splits));
+    cudaError_t e = launch_k(flags, kv_attend_many_kernel<D, I4>, dim3(units * a.splits), dim3(ManyCfg<D, I4>::kThreads),
+                             ManyCfg<D, I4>::kSmem, s, a, pairs);
     if (e != cudaSuccess || a.splits == 1) return e;
     return launch_k(flags, kv_join_many_kernel<D>, dim3(units, D / 16), dim3(256), 0, s, a, pairs);
 }
@@ -1561,10 +1471,10 @@ cudaError_t kv_attend_prepare(const KvGeom &g, KvShapes *k) {
     return g.D == 128 ? prepare<128, false>(k) : prepare<64, false>(k);
 }
 
-cudaError_t launch_kv_attend(const KvAttendArgs &a, bool many, int rows_or_pairs, int num_sms, cudaStream_t s) {
+cudaError_t launch_kv_attend(const KvAttendArgs &a, bool many, int rows_or_pairs, cudaStream_t s) {
     if (many) {
-        if (a.g.i4) return a.g.D == 128 ? launch_many<128, true>(a, rows_or_pairs, num_sms, s) : launch_many<64, true>(a, rows_or_pairs, num_sms, s);
-        return a.g.D == 128 ? launch_many<128, false>(a, rows_or_pairs, num_sms, s) : launch_many<64, false>(a, rows_or_pairs, num_sms, s);
+        if (a.g.i4) return a.g.D == 128 ? launch_many<128, true>(a, rows_or_pairs, s) : launch_many<64, true>(a, rows_or_pairs, s);
+        return a.g.D == 128 ? launch_many<128, false>(a, rows_or_pairs, s) : launch_many<64, false>(a, rows_or_pairs, s);
     }
     if (a.g.i4) return a.g.D == 128 ? launch_few<128, true>(a, rows_or_pairs, s) : launch_few<64, true>(a, rows_or_pairs, s);
     return a.g.D == 128 ? launch_few<128, false>(a, rows_or_pairs, s) : launch_few<64, false>(a, rows_or_pairs, s);

@@ -365,7 +365,7 @@ int dtts_kv::plan_attend(const dtts_kv_attend_args &a, KvAttendPlan *plan) const
     p.n_seq = n_seq; p.G = G; p.total_rows = b_rows;
     p.scale_log2 = a.scale * 1.4426950408889634f;
     p.window = a.window; p.sinks = a.sinks;
-    p.ws = ws; p.cnt = cnt; p.ticket = cnt + kMaxUnits; p.err = d_err;
+    p.ws = ws; p.cnt = cnt; p.err = d_err;
     std::vector<std::pair<long long, long long>> parts;
     // both kernels run where a batch mixes steps and prompts; each takes its own sequences
     for (int many = 0; many < 2; many++) {
@@ -420,7 +420,7 @@ int dtts_kv::attend(const KvAttendPlan &plan, int layer) {
         if (!plan.rows_or_pairs[many]) continue;
         KvAttendArgs p = plan.args[many];
         p.pool += (long long)layer * g.H * g.seg;
-        DTTS_CUDA(launch_kv_attend(p, many == 1, plan.rows_or_pairs[many], num_sms, stream));
+        DTTS_CUDA(launch_kv_attend(p, many == 1, plan.rows_or_pairs[many], stream));
     }
     return DTTS_OK;
 }
@@ -480,7 +480,7 @@ int dtts_kv_create(const dtts_kv_config *c, int device, dtts_kv **out) try {
     kv->pool = (uint8_t *)kv->mem.alloc(pool_bytes);
     kv->meta = (int *)kv->mem.alloc((size_t)ints * 4);
     kv->keep = (int *)kv->mem.alloc((size_t)c->max_tokens * 4);
-    kv->cnt = (int *)kv->mem.alloc((size_t)(kMaxUnits + 2) * 4);
+    kv->cnt = (int *)kv->mem.alloc((size_t)kMaxUnits * 4);
     kv->d_err = (int *)kv->mem.alloc(4);
     kv->ws = (float *)kv->mem.alloc((size_t)kWsFloats * 4);
     if (!kv->pool || !kv->meta || !kv->keep || !kv->cnt || !kv->d_err || !kv->ws) {
@@ -491,7 +491,7 @@ int dtts_kv_create(const dtts_kv_config *c, int device, dtts_kv **out) try {
     kv->meta_h.assign((size_t)ints, 0);
     DTTS_CUDA(cudaMemsetAsync(kv->pool, 0, pool_bytes, kv->stream));
     DTTS_CUDA(cudaMemsetAsync(kv->meta, 0, (size_t)ints * 4, kv->stream));
-    DTTS_CUDA(cudaMemsetAsync(kv->cnt, 0, (size_t)(kMaxUnits + 2) * 4, kv->stream));
+    DTTS_CUDA(cudaMemsetAsync(kv->cnt, 0, (size_t)kMaxUnits * 4, kv->stream));
     DTTS_CUDA(cudaMemsetAsync(kv->d_err, 0, 4, kv->stream));
     DTTS_CUDA(cudaStreamSynchronize(kv->stream));
     kv->seqs.resize(g.max_seqs);
