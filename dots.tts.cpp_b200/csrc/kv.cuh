@@ -100,14 +100,19 @@ DTTS_DEV uint32_t kv_encode8(const float (&x)[8], __half *s16) {
     float s = __bfloat162float(__float2bfloat16_rn(__fdiv_rn(a, 7.0f)));
     s = fminf(fmaxf(s, kKvScaleMin), kKvScaleMax);
     *s16 = bad ? __ushort_as_half(0x7e00) : __float2half_rn(s);
+    // c = rint(x / s) without a division a value.  x and s have 8 significant bits, so x / s lies on a rounding
+    // border n + 1/2 exactly or at least 2^-9.2 away from it (numerator of the difference over 2 s).  x * (1 / s)
+    // in one rounding to multiples of 2^-16 (an fma onto 192) is off by 2^-17 + 2^-21 at most: on a border it comes
+    // out as the border, elsewhere on the right side of it.
+    const float rs = __frcp_rn(s);
     uint32_t w = 0;
 #pragma unroll
     for (int i = 0; i < 8; i++) {
-        // IEEE division: x / s is on a rounding border only when the quotient is exact
-        const float c = fminf(fmaxf(rintf(__fdiv_rn(x[i], s)), -7.f), 7.f);
-        w |= (uint32_t)((bad ? 0 : (int)c) + 8) << (4 * i);
+        const float q = fminf(fmaxf(fmaf(x[i], rs, 192.f) - 192.f, -7.f), 7.f);
+        // + 1.5 * 2^23 rounds to the nearest even integer and leaves it, plus 8, in the low bits
+        w |= (__float_as_uint(q + 12582920.f) & 15u) << (4 * i);
     }
-    return w;
+    return bad ? 0x88888888u : w;
 }
 
 DTTS_DEV float kv_nibble(uint32_t w, int i) { return (float)((int)((w >> (4 * i)) & 15u) - 8); }

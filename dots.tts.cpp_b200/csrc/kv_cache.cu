@@ -12,6 +12,7 @@
 #include <cstring>
 #include <memory>
 #include <new>
+#include <type_traits>
 
 using namespace dtts;
 
@@ -27,12 +28,16 @@ constexpr int kWsFloats = 9 * 1024 * 1024;     // 36 MB of partial results
 constexpr int kMaxUnits = 1 << 16;             // split units with an arrival counter
 
 // ---------------------------------------------------------------- metadata
-constexpr int kPokes = 500;
+// Lists travel in kernel parameters.  A launch with 4 KB of parameters costs the host 4 us more than one with
+// half a KB, so every list has a short form beside the long one.
+template <int N>
 struct Pokes {
+    static constexpr int kMax = N;
     int n;
-    int index[kPokes], value[kPokes];
+    int index[N], value[N];
 };
-__global__ void kv_poke_kernel(int *__restrict__ meta, const __grid_constant__ Pokes p) {
+template <int N>
+__global__ void kv_poke_kernel(int *__restrict__ meta, const __grid_constant__ Pokes<N> p) {
     pdl_wait();
     pdl_trigger();
     for (int i = threadIdx.x; i < p.n; i += blockDim.x) meta[p.index[i]] = p.value[i];
@@ -49,13 +54,15 @@ __global__ void kv_put_kernel(int *__restrict__ dst, const __grid_constant__ Put
     for (int i = threadIdx.x; i < p.n; i += blockDim.x) dst[i] = p.value[i];
 }
 
-constexpr int kForks = 900;
+template <int N>
 struct Forks {
+    static constexpr int kMax = N;
     int n, src, pages;
-    int dst[kForks];
+    int dst[N];
 };
 // one block per new table row
-__global__ void kv_fork_tables_kernel(int *__restrict__ table, int max_pages, const __grid_constant__ Forks f) {
+template <int N>
+__global__ void kv_fork_tables_kernel(int *__restrict__ table, int max_pages, const __grid_constant__ Forks<N> f) {
     pdl_wait();
     pdl_trigger();
     for (int i = threadIdx.x; i < f.pages; i += blockDim.x)
@@ -64,8 +71,11 @@ __global__ void kv_fork_tables_kernel(int *__restrict__ table, int max_pages, co
 
 // ---------------------------------------------------------------- rows
 // A lane handles 8 dims of K or of V; D / 4 lanes take one (row, head): K by the
-// first half of them, V by the second.  The rows' places come from the batch.
-// Bound by memory: 4 D bytes read and 2 (RB + SB) written a row and head.
+// first half of them, V by the second.  The rows' places come from the batch; a
+// warp takes kWriteItems times 128 / D of them, whose loads are all in flight
+// before the first is encoded.  Bound by memory: 4 D bytes read and 2 (RB + SB)
+// written a row and head.
+constexpr int kWriteItems = 4;
 __global__ void __launch_bounds__(256) kv_write_kernel(const __grid_constant__ KvGeom g, const __grid_constant__ KvMeta m,
                                                        uint8_t *__restrict__ pool, int n_seq, int rows,
                                                        const bf16 *__restrict__ k, const bf16 *__restrict__ v,
@@ -73,71 +83,113 @@ __global__ void __launch_bounds__(256) kv_write_kernel(const __grid_constant__ K
                                                        long long v_head) {
     pdl_wait();
     pdl_trigger();
-    const int lpr = g.D / 4;   // lanes a (row, head): 32 or 16
-    const long long id = ((long long)blockIdx.x * blockDim.x + threadIdx.x) / lpr;
-    const int l = threadIdx.x % lpr, w = l % (lpr / 2);
+    const int lpr = g.D / 4, step = 32 / lpr;   // lanes a (row, head): 32 or 16; items a warp and turn
+    const int lane = threadIdx.x & 31, l = lane % lpr, w = l % (lpr / 2);
     const bool is_v = l >= lpr / 2;
-    bool on = id < (long long)rows * g.H;
-    const int row = on ? (int)(id / g.H) : 0, head = on ? (int)(id % g.H) : 0;
-    const int b = kv_find_entry(m.start, n_seq, row);
-    const int off = row - m.start[b];
-    on = on && off < m.cnt[b];
-    const int tok = on ? m.len[b] - m.cnt[b] + off : 0;
-    const int page = on ? m.table[(long long)m.seq[b] * g.max_pages + (tok >> g.lgP)] : -1;
-    on = on && page >= 0 && page < g.n_pages;
-    uint4 q = make_uint4(0u, 0u, 0u, 0u);
-    if (on)
-        q = is_v ? *reinterpret_cast<const uint4 *>(v + row * v_row + head * v_head + 8 * w)
-                 : *reinterpret_cast<const uint4 *>(k + row * k_row + head * k_head + 8 * w);
-    kv_store8(g, pool + kv_seg_off(g, on ? page : 0, 0, head), is_v, tok & (g.P - 1), w, q, on);
+    const long long first = ((long long)blockIdx.x * 8 + (threadIdx.x >> 5)) * (kWriteItems * step) + lane / lpr;
+    int row = (int)min(first / g.H, (long long)INT32_MAX), head = (int)(first % g.H);
+    int b = 0, start = 0, end = -1, tok0 = 0;   // entry of the batch: its rows [start, end)
+    const int *trow = m.table;
+    uint4 q[kWriteItems];
+    uint8_t *seg[kWriteItems];
+    int place[kWriteItems];                     // row within the page; -1: nothing to store
+#pragma unroll
+    for (int x = 0; x < kWriteItems; x++) {
+        q[x] = make_uint4(0u, 0u, 0u, 0u);
+        seg[x] = pool;
+        place[x] = -1;
+        if (row < rows) {
+            if (row >= end) {
+                b = kv_find_entry(m.start, n_seq, row);
+                start = m.start[b];
+                end = start + m.cnt[b];
+                tok0 = m.len[b] - m.cnt[b] - start;
+                trow = m.table + (long long)m.seq[b] * g.max_pages;
+            }
+            const int tok = tok0 + row, page = row < end ? trow[tok >> g.lgP] : -1;
+            if ((unsigned)page < (unsigned)g.n_pages) {
+                q[x] = is_v ? *reinterpret_cast<const uint4 *>(v + row * v_row + head * v_head + 8 * w)
+                            : *reinterpret_cast<const uint4 *>(k + row * k_row + head * k_head + 8 * w);
+                seg[x] = pool + kv_seg_off(g, page, 0, head);
+                place[x] = tok & (g.P - 1);
+            }
+        }
+        for (head += step; head >= g.H; head -= g.H) row++;
+    }
+#pragma unroll
+    for (int x = 0; x < kWriteItems; x++) kv_store8(g, seg[x], is_v, max(place[x], 0), w, q[x], place[x] >= 0);
 }
 
 // Rows [first, first + count) of the listed sequences, for n_layers layers, as
 // [layer][row][head][D] fp32 or bf16.  Same lane split as the write.
-constexpr int kReads = 320;
+template <int N>
 struct Reads {
+    static constexpr int kMax = N;
     int n, rows, n_layers;            // entries, rows a layer (of all entries of the call)
-    int seq[kReads], first[kReads], start[kReads + 1];   // start: first output row, start[n]: end
+    int seq[N], first[N], start[N + 1];   // start: first output row, start[n]: end
 };
-template <bool F32>
+constexpr int kReadItems = 4;
+template <bool F32, int N>
 __global__ void __launch_bounds__(256) kv_read_kernel(const __grid_constant__ KvGeom g, const int *__restrict__ table,
-                                                      const uint8_t *__restrict__ pool, const __grid_constant__ Reads r,
+                                                      const uint8_t *__restrict__ pool, const __grid_constant__ Reads<N> r,
                                                       void *__restrict__ k, void *__restrict__ v) {
     pdl_wait();
     pdl_trigger();
-    const int lpr = g.D / 4;
-    const long long id = ((long long)blockIdx.x * blockDim.x + threadIdx.x) / lpr;
-    const int l = threadIdx.x % lpr, w = l % (lpr / 2), n_rows = r.start[r.n] - r.start[0];
+    const int lpr = g.D / 4, step = 32 / lpr;
+    const int lane = threadIdx.x & 31, l = lane % lpr, w = l % (lpr / 2), layer = blockIdx.y;
     const bool is_v = l >= lpr / 2;
-    if (id >= (long long)n_rows * g.H) return;
-    const int row = r.start[0] + (int)(id / g.H), head = (int)(id % g.H), layer = blockIdx.y;
-    const int e = kv_find_entry(r.start, r.n, row);
-    const int tok = r.first[e] + row - r.start[e];
-    const int page = table[(long long)r.seq[e] * g.max_pages + (tok >> g.lgP)];
-    if (page < 0 || page >= g.n_pages) return;
-    float x[8];
-    kv_load8(g, pool + kv_seg_off(g, page, layer, head), is_v, tok & (g.P - 1), w, x);
-    const long long at = (((long long)layer * r.rows + row) * g.H + head) * g.D + 8 * w;
+    const long long item = ((long long)blockIdx.x * 8 + (threadIdx.x >> 5)) * (kReadItems * step) + lane / lpr;
+    const int row_end = r.start[r.n];
+    int row = (int)min(r.start[0] + item / g.H, (long long)row_end), head = (int)(item % g.H);
+    int e = 0, end = -1, shift = 0;
+    const int *trow = table;
+    float x[kReadItems][8];
+    long long at[kReadItems];   // output element; -1: none
+#pragma unroll
+    for (int i = 0; i < kReadItems; i++) {
+        at[i] = -1;
+        if (row < row_end) {
+            if (row >= end) {
+                e = kv_find_entry(r.start, r.n, row);
+                end = r.start[e + 1];
+                shift = r.first[e] - r.start[e];
+                trow = table + (long long)r.seq[e] * g.max_pages;
+            }
+            const int tok = row + shift, page = trow[tok >> g.lgP];
+            if ((unsigned)page < (unsigned)g.n_pages) {
+                kv_load8(g, pool + kv_seg_off(g, page, layer, head), is_v, tok & (g.P - 1), w, x[i]);
+                at[i] = (((long long)layer * r.rows + row) * g.H + head) * g.D + 8 * w;
+            }
+        }
+        for (head += step; head >= g.H; head -= g.H) row++;
+    }
     void *dst = is_v ? v : k;
-    if (F32) {
-        float4 *o = reinterpret_cast<float4 *>(static_cast<float *>(dst) + at);
-        o[0] = make_float4(x[0], x[1], x[2], x[3]);
-        o[1] = make_float4(x[4], x[5], x[6], x[7]);
-    } else {
-        *reinterpret_cast<uint4 *>(static_cast<bf16 *>(dst) + at) =
-            make_uint4(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), pack_bf16x2(x[4], x[5]), pack_bf16x2(x[6], x[7]));
+#pragma unroll
+    for (int i = 0; i < kReadItems; i++) {
+        if (at[i] < 0) continue;
+        if (F32) {
+            float4 *o = reinterpret_cast<float4 *>(static_cast<float *>(dst) + at[i]);
+            o[0] = make_float4(x[i][0], x[i][1], x[i][2], x[i][3]);
+            o[1] = make_float4(x[i][4], x[i][5], x[i][6], x[i][7]);
+        } else {
+            *reinterpret_cast<uint4 *>(static_cast<bf16 *>(dst) + at[i]) =
+                make_uint4(pack_bf16x2(x[i][0], x[i][1]), pack_bf16x2(x[i][2], x[i][3]), pack_bf16x2(x[i][4], x[i][5]),
+                           pack_bf16x2(x[i][6], x[i][7]));
+        }
     }
 }
 
 // The first `rows` rows of pages src to pages dst, all layers and heads: whole
 // 16-row blocks, one contiguous run a segment.
-constexpr int kCopies = 320;
+template <int N>
 struct Copies {
+    static constexpr int kMax = N;
     int n;
-    int src[kCopies], dst[kCopies], rows[kCopies];
+    int src[N], dst[N], rows[N];
 };
+template <int N>
 __global__ void __launch_bounds__(256) kv_copy_pages_kernel(const __grid_constant__ KvGeom g, uint8_t *__restrict__ pool,
-                                                            const __grid_constant__ Copies c) {
+                                                            const __grid_constant__ Copies<N> c) {
     pdl_wait();
     pdl_trigger();
     const int e = blockIdx.y, n = c.rows[e];
@@ -149,39 +201,54 @@ __global__ void __launch_bounds__(256) kv_copy_pages_kernel(const __grid_constan
 }
 
 // Rows keep[j] of table row src to rows j0 + j of table row dst (j < n), all
-// layers and heads.  A thread moves one 16-byte unit; units change their place
-// within the row as the row's number does.  Then the scales, a row at a time.
+// layers and heads (blockIdx.y).  kLanes lanes move a row: a 16-byte unit of K or V
+// each, or a row's K or V scales; units change their place within the row as the
+// row's number does.  A warp has kGatherRows turns of rows in flight.
+constexpr int kGatherRows = 4;
+template <bool I4, int D>
 __global__ void __launch_bounds__(256) kv_gather_kernel(const __grid_constant__ KvGeom g, const int *__restrict__ table,
                                                         uint8_t *__restrict__ pool, const int *__restrict__ keep, int n,
                                                         int j0, int src, int dst) {
     pdl_wait();
     pdl_trigger();
-    const int u_row = g.RB / 16, per = 2 * u_row + (g.i4 ? 2 : 0);   // units of K, of V; scales of K, of V
-    const long long base = (long long)blockIdx.y * g.seg;            // (layer, head)
-    for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < (long long)n * per;
-         i += (long long)gridDim.x * blockDim.x) {
-        const int j = (int)(i / per), u = (int)(i % per);
-        const int a = keep[j], b = j0 + j;
-        const int pa = table[(long long)src * g.max_pages + (a >> g.lgP)];
-        const int pb = table[(long long)dst * g.max_pages + (b >> g.lgP)];
-        if (pa < 0 || pa >= g.n_pages || pb < 0 || pb >= g.n_pages) continue;
-        const uint8_t *sa = pool + (long long)pa * g.page_stride + base;
-        uint8_t *sb = pool + (long long)pb * g.page_stride + base;
+    constexpr int kUnits = I4 ? D / 32 : D / 8;                  // of K, of V
+    constexpr int kLanes = 2 * kUnits + (I4 ? 2 : 0) > 16 ? 32 : 16, kStep = 32 / kLanes;
+    const int lane = threadIdx.x & 31, u = lane % kLanes;
+    const uint8_t *from = pool + (long long)blockIdx.y * g.seg;   // (layer, head)
+    uint8_t *to = pool + (long long)blockIdx.y * g.seg;
+    const int *tsrc = table + (long long)src * g.max_pages, *tdst = table + (long long)dst * g.max_pages;
+    int j = (blockIdx.x * 8 + (threadIdx.x >> 5)) * (kGatherRows * kStep) + lane / kLanes;
+    uint4 x[kGatherRows];
+    uint8_t *at[kGatherRows];
+#pragma unroll
+    for (int i = 0; i < kGatherRows; i++, j += kStep) {
+        at[i] = nullptr;
+        if (j >= n || u >= 2 * kUnits + (I4 ? 2 : 0)) continue;
+        const int a = keep[j], b = j0 + j, pa = tsrc[a >> g.lgP], pb = tdst[b >> g.lgP];
+        if ((unsigned)pa >= (unsigned)g.n_pages || (unsigned)pb >= (unsigned)g.n_pages) continue;
         const int ra = a & (g.P - 1), rb = b & (g.P - 1);
-        if (u < 2 * u_row) {
-            const bool is_v = u >= u_row;
-            const int w = is_v ? u - u_row : u;
-            const int ua = w ^ (is_v ? kv_swz_v(g.i4, g.D, ra) : kv_swz_k(g.i4, ra));
-            const int ub = w ^ (is_v ? kv_swz_v(g.i4, g.D, rb) : kv_swz_k(g.i4, rb));
-            *reinterpret_cast<uint4 *>(sb + kv_row_off(g, is_v, rb) + ub * 16) =
-                *reinterpret_cast<const uint4 *>(sa + kv_row_off(g, is_v, ra) + ua * 16);
+        const uint8_t *sa = from + (long long)pa * g.page_stride;
+        at[i] = to + (long long)pb * g.page_stride;
+        if (u < 2 * kUnits) {
+            const bool is_v = u >= kUnits;
+            const int w = is_v ? u - kUnits : u;
+            const int ua = w ^ (is_v ? kv_swz_v(I4, D, ra) : kv_swz_k(I4, ra)), ub = w ^ (is_v ? kv_swz_v(I4, D, rb) : kv_swz_k(I4, rb));
+            x[i] = *reinterpret_cast<const uint4 *>(sa + kv_row_off(g, is_v, ra) + ua * 16);
+            at[i] += kv_row_off(g, is_v, rb) + ub * 16;
         } else {
-            const bool is_v = u > 2 * u_row;
+            const bool is_v = u > 2 * kUnits;
             sa += kv_scale_off(g, is_v, ra);
-            sb += kv_scale_off(g, is_v, rb);
-            if (g.SB == 8) *reinterpret_cast<uint2 *>(sb) = *reinterpret_cast<const uint2 *>(sa);
-            else *reinterpret_cast<uint32_t *>(sb) = *reinterpret_cast<const uint32_t *>(sa);
+            at[i] += kv_scale_off(g, is_v, rb);
+            x[i].x = *reinterpret_cast<const uint32_t *>(sa);
+            if (D == 128) x[i].y = *reinterpret_cast<const uint32_t *>(sa + 4);
         }
+    }
+#pragma unroll
+    for (int i = 0; i < kGatherRows; i++) {
+        if (!at[i]) continue;
+        if (u < 2 * kUnits) *reinterpret_cast<uint4 *>(at[i]) = x[i];
+        else if (D == 128) *reinterpret_cast<uint2 *>(at[i]) = make_uint2(x[i].x, x[i].y);
+        else *reinterpret_cast<uint32_t *>(at[i]) = x[i].x;
     }
 }
 
@@ -209,14 +276,21 @@ KvMeta dtts_kv::kv_meta() const {
 }
 
 int dtts_kv::flush() {
-    for (size_t i = 0; i < pokes.size(); i += kPokes) {
-        Pokes p;
-        p.n = (int)std::min<size_t>(kPokes, pokes.size() - i);
+    auto send = [&](auto &p, size_t i) -> int {
+        constexpr int kMax = std::remove_reference_t<decltype(p)>::kMax;
+        p.n = (int)std::min<size_t>(kMax, pokes.size() - i);
         for (int j = 0; j < p.n; j++) {
             p.index[j] = pokes[i + j];
             p.value[j] = meta_h[pokes[i + j]];   // an index listed twice gets its last value both times
         }
-        DTTS_CUDA(launch_k(kv_pdl(), kv_poke_kernel, dim3(1), dim3(256), 0, stream, meta, p));
+        DTTS_CUDA(launch_k(kv_pdl(), kv_poke_kernel<kMax>, dim3(1), dim3(256), 0, stream, meta, p));
+        return DTTS_OK;
+    };
+    Pokes<60> few;
+    Pokes<500> many;
+    for (size_t i = 0; i < pokes.size(); i += pokes.size() <= 60 ? 60 : 500) {
+        int st = pokes.size() <= 60 ? send(few, i) : send(many, i);
+        if (st) return st;
     }
     pokes.clear();
     return DTTS_OK;
@@ -268,9 +342,10 @@ int dtts_kv::extend(int n_seq, const int *sq, const int *n_new) {
     DTTS_CHECK(rows <= INT32_MAX / 2, DTTS_ERR_ARG, "%lld new rows in one batch", rows);
     DTTS_CHECK(need <= (long long)free_pages.size(), DTTS_ERR_OOM, "%lld pages needed, %zu free", need,
                free_pages.size());
-    Copies c;
-    c.n = 0;
-    std::vector<Copies> copies;
+    struct Copy {
+        int src, dst, rows;
+    };
+    std::vector<Copy> copies;
     b_seq.assign(sq, sq + n_seq);
     b_cnt.assign(n_new, n_new + n_seq);
     b_len.resize(n_seq);
@@ -283,10 +358,7 @@ int dtts_kv::extend(int n_seq, const int *sq, const int *n_new) {
             refs[from]--;   // shared: never the last user here
             s.pages.back() = to;
             poke(table_at(sq[b], (int)s.pages.size() - 1), to);
-            c.src[c.n] = from;
-            c.dst[c.n] = to;
-            c.rows[c.n] = s.len & (g.P - 1);
-            if (++c.n == kCopies) { copies.push_back(c); c.n = 0; }
+            copies.push_back({from, to, s.len & (g.P - 1)});
         }
         const int pos = s.pos;
         s.len += n_new[b];
@@ -308,9 +380,21 @@ int dtts_kv::extend(int n_seq, const int *sq, const int *n_new) {
         poke(g.max_seqs + b, start);
         poke(2 * g.max_seqs + b, 0);
     }
-    if (c.n) copies.push_back(c);
-    for (const Copies &cc : copies)
-        DTTS_CUDA(launch_k(kv_pdl(), kv_copy_pages_kernel, dim3(g.L * g.H, cc.n), dim3(256), 0, stream, g, pool, cc));
+    auto send = [&](auto &c, size_t i) -> int {
+        constexpr int kMax = std::remove_reference_t<decltype(c)>::kMax;
+        c.n = (int)std::min<size_t>(kMax, copies.size() - i);
+        for (int j = 0; j < c.n; j++) {
+            c.src[j] = copies[i + j].src;
+            c.dst[j] = copies[i + j].dst;
+            c.rows[j] = copies[i + j].rows;
+        }
+        DTTS_CUDA(launch_k(kv_pdl(), kv_copy_pages_kernel<kMax>, dim3(g.L * g.H, c.n), dim3(256), 0, stream, g, pool, c));
+        return DTTS_OK;
+    };
+    Copies<40> few;
+    Copies<320> many;
+    for (size_t i = 0; i < copies.size(); i += copies.size() <= 40 ? 40 : 320)
+        if ((st = copies.size() <= 40 ? send(few, i) : send(many, i))) return st;
     return flush();
 }
 
@@ -588,15 +672,20 @@ int dtts_kv_fork(dtts_kv *kv, int src, int n, int *dst) try {
     DTTS_CHECK((int)to.size() == n, DTTS_ERR_OOM, "%d sequences wanted, %zu free", n, to.size());
     if ((st = kv->flush())) return st;   // the source's row on the device is current
     const int pages = (int)kv->seqs[src].pages.size();
-    for (int i = 0; i < n && pages; i += kForks) {
-        Forks f;
-        f.n = std::min(kForks, n - i);
+    auto send = [&](auto &f, int i) -> int {
+        constexpr int kMax = std::remove_reference_t<decltype(f)>::kMax;
+        f.n = std::min(kMax, n - i);
         f.src = src;
         f.pages = pages;
         for (int j = 0; j < f.n; j++) f.dst[j] = to[i + j];
-        DTTS_CUDA(launch_k(kv_pdl(), kv_fork_tables_kernel, dim3(f.n), dim3(128), 0, kv->stream,
+        DTTS_CUDA(launch_k(kv_pdl(), kv_fork_tables_kernel<kMax>, dim3(f.n), dim3(128), 0, kv->stream,
                            kv->meta + 5 * kv->g.max_seqs, kv->g.max_pages, f));
-    }
+        return DTTS_OK;
+    };
+    Forks<60> few;
+    Forks<900> many;
+    for (int i = 0; i < n && pages; i += n <= 60 ? 60 : 900)
+        if ((st = n <= 60 ? send(few, i) : send(many, i))) return st;
     for (int s : to) {
         kv->seqs[s] = kv->seqs[src];
         for (int p = 0; p < pages; p++) {
@@ -699,10 +788,15 @@ int dtts_kv_compact(dtts_kv *kv, int seq, int n_keep, const int *keep) try {
             std::memcpy(p.value, keep + j0 + i, (size_t)p.n * 4);
             DTTS_CUDA(launch_k(kv_pdl(), kv_put_kernel, dim3(1), dim3(256), 0, kv->stream, kv->keep + i, p));
         }
-        const long long units = (long long)n * (2 * g.RB / 16 + (g.i4 ? 2 : 0));
-        const int gx = (int)std::min<long long>((units + 255) / 256, 1024);
-        DTTS_CUDA(launch_k(kv_pdl(), kv_gather_kernel, dim3(gx, g.L * g.H), dim3(256), 0, kv->stream, g,
-                           (const int *)(kv->meta + 5 * g.max_seqs), kv->pool, (const int *)kv->keep, n, j0, seq, scratch));
+        auto gather = [&](auto kernel, int rows_a_warp) {
+            return launch_k(kv_pdl(), kernel, dim3((n + 8 * rows_a_warp - 1) / (8 * rows_a_warp), g.L * g.H), dim3(256), 0,
+                            kv->stream, g, (const int *)(kv->meta + 5 * g.max_seqs), kv->pool, (const int *)kv->keep, n, j0,
+                            seq, scratch);
+        };
+        DTTS_CUDA(g.i4 ? (g.D == 128 ? gather(kv_gather_kernel<true, 128>, 2 * kGatherRows)
+                                     : gather(kv_gather_kernel<true, 64>, 2 * kGatherRows))
+                       : (g.D == 128 ? gather(kv_gather_kernel<false, 128>, kGatherRows)
+                                     : gather(kv_gather_kernel<false, 64>, 2 * kGatherRows)));
     }
     for (int p = 0; p < total; p++) kv->poke(kv->table_at(seq, p), pages[p]);
     if ((st = kv->flush())) return st;
@@ -756,7 +850,7 @@ int dtts_kv_write(dtts_kv *kv, int layer, const void *k, const void *v, long lon
     DeviceGuard dg(kv->device);
     int st = kv->flush();
     if (st) return st;
-    const int per_block = 256 / (g.D / 4);
+    const int per_block = 256 / (g.D / 4) * kWriteItems;
     const long long items = (long long)kv->b_rows * g.H;
     DTTS_CHECK((items + per_block - 1) / per_block <= INT32_MAX, DTTS_ERR_ARG, "%d rows in one batch", kv->b_rows);
     DTTS_CUDA(launch_k(kv_pdl(), kv_write_kernel, dim3((unsigned)((items + per_block - 1) / per_block)), dim3(256), 0,
@@ -790,11 +884,11 @@ int dtts_kv_read(dtts_kv *kv, int layer, int n_layers, int n, const int *seqs, c
     DeviceGuard dg(kv->device);
     int st = kv->flush();
     if (st) return st;
-    const int per_block = 256 / (g.D / 4);
+    const int per_block = 256 / (g.D / 4) * kReadItems;
     int start = 0;
-    for (int i = 0; i < n; i += kReads) {
-        Reads r;
-        r.n = std::min(kReads, n - i);
+    auto send = [&](auto &r, int i) -> int {
+        constexpr int kMax = std::remove_reference_t<decltype(r)>::kMax;
+        r.n = std::min(kMax, n - i);
         r.rows = (int)rows;
         r.n_layers = n_layers;
         for (int j = 0; j < r.n; j++) {
@@ -805,15 +899,20 @@ int dtts_kv_read(dtts_kv *kv, int layer, int n_layers, int n, const int *seqs, c
         }
         r.start[r.n] = start;
         const long long items = (long long)(start - r.start[0]) * g.H;
-        if (!items) continue;
+        if (!items) return DTTS_OK;
         const dim3 grid((unsigned)((items + per_block - 1) / per_block), n_layers);
         const uint8_t *pool = kv->pool + (long long)layer * g.H * g.seg;
         const int *table = kv->meta + 5 * g.max_seqs;
         if (dtype == DTTS_DTYPE_F32)
-            DTTS_CUDA(launch_k(kv_pdl(), kv_read_kernel<true>, grid, dim3(256), 0, kv->stream, g, table, pool, r, k, v));
+            DTTS_CUDA(launch_k(kv_pdl(), kv_read_kernel<true, kMax>, grid, dim3(256), 0, kv->stream, g, table, pool, r, k, v));
         else
-            DTTS_CUDA(launch_k(kv_pdl(), kv_read_kernel<false>, grid, dim3(256), 0, kv->stream, g, table, pool, r, k, v));
-    }
+            DTTS_CUDA(launch_k(kv_pdl(), kv_read_kernel<false, kMax>, grid, dim3(256), 0, kv->stream, g, table, pool, r, k, v));
+        return DTTS_OK;
+    };
+    Reads<40> few;
+    Reads<320> many;
+    for (int i = 0; i < n; i += n <= 40 ? 40 : 320)
+        if ((st = n <= 40 ? send(few, i) : send(many, i))) return st;
     return DTTS_OK;
 } catch (const std::bad_alloc &) {
     set_error("out of host memory");

@@ -527,6 +527,9 @@ class KVAttendArgs(C.Structure):
 
 def _ints(a):
     """Sequence or int32 array -> (keep-alive, address, length)."""
+    if isinstance(a, (list, tuple)) and len(a) <= 256:      # short lists: twice as fast as through numpy
+        c = (C.c_int * len(a))(*a)
+        return c, C.addressof(c), len(a)
     a = np.ascontiguousarray(a, np.int32).ravel()
     return a, a.ctypes.data, a.size
 
@@ -547,6 +550,8 @@ class KVCache:
         self.h, self._lib = h, lib()
         self.n_layers, self.n_kv_heads, self.head_dim = n_layers, n_kv_heads, head_dim
         self._args = KVAttendArgs()
+        self._args_ref = C.byref(self._args)
+        self._scale = head_dim ** -0.5
 
     def close(self):
         if getattr(self, "h", None):
@@ -575,9 +580,9 @@ class KVCache:
         check(self._lib.dtts_kv_close(self.h, n, p))
 
     def fork(self, seq, n=1):
-        out = np.zeros(max(n, 0), np.int32)
-        check(self._lib.dtts_kv_fork(self.h, seq, n, out.ctypes.data))
-        return out.tolist()
+        out = (C.c_int * max(n, 0))()
+        check(self._lib.dtts_kv_fork(self.h, seq, n, out))
+        return list(out)
 
     def truncate(self, seq, n_tokens):
         check(self._lib.dtts_kv_truncate(self.h, seq, n_tokens))
@@ -612,11 +617,10 @@ class KVCache:
         check(self._lib.dtts_kv_extend(self.h, n, p, q))
 
     def _strides(self, x, heads, what):
-        shape = tuple(x.shape)
-        if len(shape) != 3 or shape[1] != heads or shape[2] != self.head_dim or x.element_size() != 2 or \
-                (shape[2] > 1 and x.stride(2) != 1):
+        shape, st = x.shape, x.stride()
+        if len(shape) != 3 or shape[1] != heads or shape[2] != self.head_dim or st[2] != 1 or x.element_size() != 2:
             raise ValueError(f"{what}: bf16 [rows][{heads}][{self.head_dim}] with a dense last dimension expected")
-        return x.stride(0), x.stride(1)
+        return st[0], st[1]
 
     def write(self, layer, k, v):
         kr, kh = self._strides(k, self.n_kv_heads, "k")
@@ -629,9 +633,9 @@ class KVCache:
         a.q, a.out = q.data_ptr(), out.data_ptr()
         a.q_row, a.q_head = self._strides(q, a.n_heads, "q")
         a.out_row, a.out_head = self._strides(out, a.n_heads, "out")
-        a.scale = self.head_dim ** -0.5 if scale is None else scale
+        a.scale = self._scale if scale is None else scale
         a.window, a.sinks = window, sinks
-        check(self._lib.dtts_kv_attend(self.h, layer, C.byref(a)))
+        check(self._lib.dtts_kv_attend(self.h, layer, self._args_ref))
         return out
 
     def read(self, layer, seqs, first, count, k, v, n_layers=1):
@@ -639,7 +643,7 @@ class KVCache:
         s, ps, n = _ints(seqs)
         f, pf, nf = _ints(first)
         c, pc, nc = _ints(count)
-        size = n_layers * int(c.sum()) * self.n_kv_heads * self.head_dim
+        size = n_layers * int(sum(c)) * self.n_kv_heads * self.head_dim
         if not n == nf == nc:
             raise ValueError("seqs, first and count differ in length")
         if k.element_size() != v.element_size() or not (k.is_contiguous() and v.is_contiguous()) or \
@@ -737,8 +741,9 @@ class LLM:
         if mem == MEM_HOST:
             emb = _f32(emb)
             out = np.zeros_like(emb) if out is None else out
-        if tuple(emb.shape) != (int(c.sum()), 1536) or tuple(out.shape) != tuple(emb.shape):
-            raise ValueError(f"emb and out: [{int(c.sum())}][1536] expected")
+        rows = int(sum(c))
+        if tuple(emb.shape) != (rows, 1536) or tuple(out.shape) != (rows, 1536):
+            raise ValueError(f"emb and out: [{rows}][1536] expected")
         check(lib().dtts_llm_extend(self.h, kv.h, n, ps, pc, _addr(emb), window, sinks, _addr(out), mem))
         return out
 
