@@ -70,20 +70,33 @@ __global__ void kv_fork_tables_kernel(int *__restrict__ table, int max_pages, co
 }
 
 // ---------------------------------------------------------------- rows
+// the geometry with what the instance fixes as constants
+template <bool I4, int D>
+DTTS_DEV KvGeom fixed_geom(const KvGeom &g) {
+    KvGeom c = g;
+    c.i4 = I4;
+    c.D = D;
+    c.RB = I4 ? D / 2 : 2 * D;
+    c.SB = I4 ? D / 16 : 0;
+    return c;
+}
+
 // A lane handles 8 dims of K or of V; D / 4 lanes take one (row, head): K by the
 // first half of them, V by the second.  The rows' places come from the batch; a
 // warp takes kWriteItems times 128 / D of them, whose loads are all in flight
 // before the first is encoded.  Bound by memory: 4 D bytes read and 2 (RB + SB)
 // written a row and head.
 constexpr int kWriteItems = 4;
-__global__ void __launch_bounds__(256) kv_write_kernel(const __grid_constant__ KvGeom g, const __grid_constant__ KvMeta m,
+template <bool I4, int D>
+__global__ void __launch_bounds__(256) kv_write_kernel(const __grid_constant__ KvGeom geom, const __grid_constant__ KvMeta m,
                                                        uint8_t *__restrict__ pool, int n_seq, int rows,
                                                        const bf16 *__restrict__ k, const bf16 *__restrict__ v,
                                                        long long k_row, long long k_head, long long v_row,
                                                        long long v_head) {
     pdl_wait();
     pdl_trigger();
-    const int lpr = g.D / 4, step = 32 / lpr;   // lanes a (row, head): 32 or 16; items a warp and turn
+    const KvGeom g = fixed_geom<I4, D>(geom);
+    constexpr int lpr = D / 4, step = 32 / lpr;   // lanes a (row, head): 32 or 16; items a warp and turn
     const int lane = threadIdx.x & 31, l = lane % lpr, w = l % (lpr / 2);
     const bool is_v = l >= lpr / 2;
     const long long first = ((long long)blockIdx.x * 8 + (threadIdx.x >> 5)) * (kWriteItems * step) + lane / lpr;
@@ -122,6 +135,17 @@ __global__ void __launch_bounds__(256) kv_write_kernel(const __grid_constant__ K
 
 // Rows [first, first + count) of the listed sequences, for n_layers layers, as
 // [layer][row][head][D] fp32 or bf16.  Same lane split as the write.
+// 8 floats to 32-byte (wide) or 16-byte aligned memory: whole 32-byte sectors in one instruction where possible
+DTTS_DEV void store8_f32(float *p, const float (&x)[8], bool wide) {
+    if (wide) {
+        asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "f"(x[0]), "f"(x[1]), "f"(x[2]),
+                     "f"(x[3]), "f"(x[4]), "f"(x[5]), "f"(x[6]), "f"(x[7])
+                     : "memory");
+    } else {
+        reinterpret_cast<float4 *>(p)[0] = make_float4(x[0], x[1], x[2], x[3]);
+        reinterpret_cast<float4 *>(p)[1] = make_float4(x[4], x[5], x[6], x[7]);
+    }
+}
 template <int N>
 struct Reads {
     static constexpr int kMax = N;
@@ -129,13 +153,14 @@ struct Reads {
     int seq[N], first[N], start[N + 1];   // start: first output row, start[n]: end
 };
 constexpr int kReadItems = 4;
-template <bool F32, int N>
-__global__ void __launch_bounds__(256) kv_read_kernel(const __grid_constant__ KvGeom g, const int *__restrict__ table,
+template <bool I4, int D, bool F32, int N>
+__global__ void __launch_bounds__(256) kv_read_kernel(const __grid_constant__ KvGeom geom, const int *__restrict__ table,
                                                       const uint8_t *__restrict__ pool, const __grid_constant__ Reads<N> r,
                                                       void *__restrict__ k, void *__restrict__ v) {
     pdl_wait();
     pdl_trigger();
-    const int lpr = g.D / 4, step = 32 / lpr;
+    const KvGeom g = fixed_geom<I4, D>(geom);
+    constexpr int lpr = D / 4, step = 32 / lpr;
     const int lane = threadIdx.x & 31, l = lane % lpr, w = l % (lpr / 2), layer = blockIdx.y;
     const bool is_v = l >= lpr / 2;
     const long long item = ((long long)blockIdx.x * 8 + (threadIdx.x >> 5)) * (kReadItems * step) + lane / lpr;
@@ -164,13 +189,12 @@ __global__ void __launch_bounds__(256) kv_read_kernel(const __grid_constant__ Kv
         for (head += step; head >= g.H; head -= g.H) row++;
     }
     void *dst = is_v ? v : k;
+    const bool wide = (reinterpret_cast<uintptr_t>(dst) & 31u) == 0;
 #pragma unroll
     for (int i = 0; i < kReadItems; i++) {
         if (at[i] < 0) continue;
         if (F32) {
-            float4 *o = reinterpret_cast<float4 *>(static_cast<float *>(dst) + at[i]);
-            o[0] = make_float4(x[i][0], x[i][1], x[i][2], x[i][3]);
-            o[1] = make_float4(x[i][4], x[i][5], x[i][6], x[i][7]);
+            store8_f32(static_cast<float *>(dst) + at[i], x[i], wide);
         } else {
             *reinterpret_cast<uint4 *>(static_cast<bf16 *>(dst) + at[i]) =
                 make_uint4(pack_bf16x2(x[i][0], x[i][1]), pack_bf16x2(x[i][2], x[i][3]), pack_bf16x2(x[i][4], x[i][5]),
@@ -853,9 +877,13 @@ int dtts_kv_write(dtts_kv *kv, int layer, const void *k, const void *v, long lon
     const int per_block = 256 / (g.D / 4) * kWriteItems;
     const long long items = (long long)kv->b_rows * g.H;
     DTTS_CHECK((items + per_block - 1) / per_block <= INT32_MAX, DTTS_ERR_ARG, "%d rows in one batch", kv->b_rows);
-    DTTS_CUDA(launch_k(kv_pdl(), kv_write_kernel, dim3((unsigned)((items + per_block - 1) / per_block)), dim3(256), 0,
-                       kv->stream, g, kv->kv_meta(), kv->pool + (long long)layer * g.H * g.seg, (int)kv->b_seq.size(),
-                       kv->b_rows, (const bf16 *)k, (const bf16 *)v, k_row, k_head, v_row, v_head));
+    auto write = [&](auto kernel) {
+        return launch_k(kv_pdl(), kernel, dim3((unsigned)((items + per_block - 1) / per_block)), dim3(256), 0, kv->stream, g,
+                        kv->kv_meta(), kv->pool + (long long)layer * g.H * g.seg, (int)kv->b_seq.size(), kv->b_rows,
+                        (const bf16 *)k, (const bf16 *)v, k_row, k_head, v_row, v_head);
+    };
+    DTTS_CUDA(g.i4 ? (g.D == 128 ? write(kv_write_kernel<true, 128>) : write(kv_write_kernel<true, 64>))
+                   : (g.D == 128 ? write(kv_write_kernel<false, 128>) : write(kv_write_kernel<false, 64>)));
     return DTTS_OK;
 }
 
@@ -903,10 +931,13 @@ int dtts_kv_read(dtts_kv *kv, int layer, int n_layers, int n, const int *seqs, c
         const dim3 grid((unsigned)((items + per_block - 1) / per_block), n_layers);
         const uint8_t *pool = kv->pool + (long long)layer * g.H * g.seg;
         const int *table = kv->meta + 5 * g.max_seqs;
-        if (dtype == DTTS_DTYPE_F32)
-            DTTS_CUDA(launch_k(kv_pdl(), kv_read_kernel<true, kMax>, grid, dim3(256), 0, kv->stream, g, table, pool, r, k, v));
-        else
-            DTTS_CUDA(launch_k(kv_pdl(), kv_read_kernel<false, kMax>, grid, dim3(256), 0, kv->stream, g, table, pool, r, k, v));
+        auto read = [&](auto f32, auto b16) {
+            return launch_k(kv_pdl(), dtype == DTTS_DTYPE_F32 ? f32 : b16, grid, dim3(256), 0, kv->stream, g, table, pool, r, k, v);
+        };
+        DTTS_CUDA(g.i4 ? (g.D == 128 ? read(kv_read_kernel<true, 128, true, kMax>, kv_read_kernel<true, 128, false, kMax>)
+                                     : read(kv_read_kernel<true, 64, true, kMax>, kv_read_kernel<true, 64, false, kMax>))
+                       : (g.D == 128 ? read(kv_read_kernel<false, 128, true, kMax>, kv_read_kernel<false, 128, false, kMax>)
+                                     : read(kv_read_kernel<false, 64, true, kMax>, kv_read_kernel<false, 64, false, kMax>)));
         return DTTS_OK;
     };
     Reads<40> few;
