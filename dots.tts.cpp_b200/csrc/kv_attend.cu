@@ -1089,7 +1089,7 @@ __global__ void __launch_bounds__(512, 1) kv_attend_many_kernel(const __grid_con
             __syncwarp();
         } else {
             // ---- pages -> tiles.  A job is 16 rows of K or V, one block of a page: jobs K0 .. K7, V0 .. V7
-            // of key block 0, then of block 1, ...; producer warp pw takes jobs pw, pw + 7, ...  A job's page
+            // of key block 0, then of block 1, ...; producer warp pw takes jobs pw, pw + 6, ...  A job's page
             // number is loaded two jobs ahead, its rows one job ahead.
             const int P = a.g.P, lg = a.g.lgP, jobs = 16 * n;
             const uint8_t *head_pool = a.pool + kv_seg_off(a.g, 0, 0, head);

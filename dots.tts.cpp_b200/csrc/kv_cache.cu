@@ -133,8 +133,6 @@ __global__ void __launch_bounds__(256) kv_write_kernel(const __grid_constant__ K
     for (int x = 0; x < kWriteItems; x++) kv_store8(g, seg[x], is_v, max(place[x], 0), w, q[x], place[x] >= 0);
 }
 
-// Rows [first, first + count) of the listed sequences, for n_layers layers, as
-// [layer][row][head][D] fp32 or bf16.  Same lane split as the write.
 // 8 floats to 32-byte (wide) or 16-byte aligned memory: whole 32-byte sectors in one instruction where possible
 DTTS_DEV void store8_f32(float *p, const float (&x)[8], bool wide) {
     if (wide) {
@@ -152,6 +150,8 @@ struct Reads {
     int n, rows, n_layers;            // entries, rows a layer (of all entries of the call)
     int seq[N], first[N], start[N + 1];   // start: first output row, start[n]: end
 };
+// Rows [first, first + count) of the listed sequences, for n_layers layers, as
+// [layer][row][head][D] fp32 or bf16.  Same lane split as the write.
 constexpr int kReadItems = 4;
 template <bool I4, int D, bool F32, int N>
 __global__ void __launch_bounds__(256) kv_read_kernel(const __grid_constant__ KvGeom geom, const int *__restrict__ table,
@@ -300,6 +300,13 @@ KvMeta dtts_kv::kv_meta() const {
 }
 
 int dtts_kv::flush() {
+    if (pokes.empty()) return DTTS_OK;
+    // While the stream is capturing, a trim's marks may be pending (the calls that add pages send theirs): they stay so.
+    // No call may reach the rows that they concern, and in a graph every replay would set them again, over the tables
+    // of that time.
+    cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
+    DTTS_CUDA(cudaStreamIsCapturing(stream, &cap));
+    if (cap != cudaStreamCaptureStatusNone) return DTTS_OK;
     auto send = [&](auto &p, size_t i) -> int {
         constexpr int kMax = std::remove_reference_t<decltype(p)>::kMax;
         p.n = (int)std::min<size_t>(kMax, pokes.size() - i);
@@ -472,7 +479,9 @@ int dtts_kv::plan_attend(const dtts_kv_attend_args &a, KvAttendPlan *plan) const
     p.q_row = a.q_row; p.q_head = a.q_head; p.o_row = a.out_row; p.o_head = a.out_head;
     p.n_seq = n_seq; p.G = G; p.total_rows = b_rows;
     p.scale_log2 = a.scale * 1.4426950408889634f;
-    p.window = a.window; p.sinks = a.sinks;
+    // what no sequence reaches, cut so that row numbers minus or plus them stay in 32 bits
+    p.window = a.window >= max_tokens ? 0 : a.window;
+    p.sinks = (int)std::min<long long>(a.sinks, max_tokens);
     p.ws = ws; p.cnt = cnt; p.err = d_err;
     std::vector<std::pair<long long, long long>> parts;
     // both kernels run where a batch mixes steps and prompts; each takes its own sequences
@@ -495,7 +504,7 @@ int dtts_kv::plan_attend(const dtts_kv_attend_args &a, KvAttendPlan *plan) const
         if (!max_rows) continue;
         const int rt = many ? (max_rows + 255) / 256 : 1;
         const long long units = (long long)n_seq * g.H * rt;
-        DTTS_CHECK(units <= INT32_MAX / 256, DTTS_ERR_ARG, "%lld row tiles in one batch", units);
+        DTTS_CHECK(units <= INT32_MAX, DTTS_ERR_ARG, "%lld row tiles in one batch", units);
         // Parts of the key ranges: as short as they may be with all CTAs resident at once, but not
         // shorter than what hides a CTA's start and the join.
         const long long resident = (long long)(many ? 1 : std::max(1, shapes.few_ctas[max_rows > 8])) * num_sms;
@@ -745,7 +754,7 @@ int dtts_kv_truncate(dtts_kv *kv, int seq, int n_tokens) {
     return DTTS_OK;
 }
 
-int dtts_kv_trim(dtts_kv *kv, int seq, int window, int sinks) {
+int dtts_kv_trim(dtts_kv *kv, int seq, int window, int sinks) try {
     DTTS_CHECK(kv, DTTS_ERR_ARG, "null cache");
     DTTS_CHECK(seq_ok(kv, seq), DTTS_ERR_ARG, "sequence %d is not open", seq);
     DTTS_CHECK(window >= 1 && sinks >= 0, DTTS_ERR_ARG, "window %d, sinks %d", window, sinks);
@@ -774,6 +783,9 @@ int dtts_kv_trim(dtts_kv *kv, int seq, int window, int sinks) {
     for (int e : kv->b_seq)
         if (e == seq) { kv->drop_batch(); break; }
     return DTTS_OK;
+} catch (const std::bad_alloc &) {
+    set_error("out of host memory");
+    return DTTS_ERR_OOM;
 }
 
 int dtts_kv_compact(dtts_kv *kv, int seq, int n_keep, const int *keep) try {

@@ -535,19 +535,20 @@ def _ints(a):
 
 
 class KVCache:
-    """The paged K/V cache (dtts_kv_*).  k, v, q and out are bf16 device tensors
-    [rows][heads][head_dim] (anything with data_ptr(), stride(), element_size()
-    and is_contiguous()) whose last dimension is dense; calls only enqueue."""
+    """The paged K/V cache (dtts_kv_*).  k, v, q and out are bf16 torch tensors on the cache's
+    device, [rows][heads][head_dim] with a dense last dimension and at least the current
+    batch's rows; calls only enqueue."""
 
     def __init__(self, n_layers, n_kv_heads, head_dim, n_pages, max_seqs, max_tokens, page_tokens=64,
                  dtype=DTYPE_BF16, device=0):
         c = KVConfig(n_layers, n_kv_heads, head_dim, page_tokens, n_pages, max_seqs, max_tokens, dtype)
         h = _vp()
         check(lib().dtts_kv_create(C.byref(c), device, C.byref(h)))
-        self._init(h, n_layers, n_kv_heads, head_dim)
+        self._init(h, n_layers, n_kv_heads, head_dim, device)
 
-    def _init(self, h, n_layers, n_kv_heads, head_dim):
-        self.h, self._lib = h, lib()
+    def _init(self, h, n_layers, n_kv_heads, head_dim, device):
+        self.h, self._lib, self.device = h, lib(), device
+        self._rows = 0    # of the current batch
         self.n_layers, self.n_kv_heads, self.head_dim = n_layers, n_kv_heads, head_dim
         self._args = KVAttendArgs()
         self._args_ref = C.byref(self._args)
@@ -615,11 +616,16 @@ class KVCache:
         if n != m:
             raise ValueError(f"{n} sequences, {m} counts")
         check(self._lib.dtts_kv_extend(self.h, n, p, q))
+        self._rows = int(sum(c))
 
     def _strides(self, x, heads, what):
         shape, st = x.shape, x.stride()
-        if len(shape) != 3 or shape[1] != heads or shape[2] != self.head_dim or st[2] != 1 or x.element_size() != 2:
-            raise ValueError(f"{what}: bf16 [rows][{heads}][{self.head_dim}] with a dense last dimension expected")
+        if len(shape) != 3 or shape[1] != heads or shape[2] != self.head_dim or st[2] != 1 or \
+                x.get_device() != self.device or str(x.dtype) != "torch.bfloat16":
+            raise ValueError(f"{what}: bf16 [rows][{heads}][{self.head_dim}] on device {self.device} with a dense last "
+                             "dimension expected")
+        if shape[0] < self._rows:
+            raise DttsError(ERR_ARG, f"{what}: {shape[0]} rows, the current batch has {self._rows}")
         return st[0], st[1]
 
     def write(self, layer, k, v):
@@ -646,10 +652,10 @@ class KVCache:
         size = n_layers * int(sum(c)) * self.n_kv_heads * self.head_dim
         if not n == nf == nc:
             raise ValueError("seqs, first and count differ in length")
-        if k.element_size() != v.element_size() or not (k.is_contiguous() and v.is_contiguous()) or \
-                k.numel() != size or v.numel() != size:
-            raise ValueError(f"k and v: dense, {size} elements of one type expected")
-        dtype = DTYPE_F32 if k.element_size() == 4 else DTYPE_BF16
+        dtype = {"torch.float32": DTYPE_F32, "torch.bfloat16": DTYPE_BF16}.get(str(k.dtype))
+        if dtype is None or k.dtype != v.dtype or not (k.is_contiguous() and v.is_contiguous()) or \
+                k.numel() != size or v.numel() != size or k.get_device() != self.device or v.get_device() != self.device:
+            raise ValueError(f"k and v: dense, {size} elements of one type (fp32 or bf16) on device {self.device} expected")
         check(self._lib.dtts_kv_read(self.h, layer, n_layers, n, ps, pf, pc, k.data_ptr(), v.data_ptr(), dtype))
 
 
@@ -687,7 +693,7 @@ class LLM:
         s = LLMW(n_layers, arr, _ptr(fn))
         h = _vp()
         check(lib().dtts_llm_create(C.byref(s), device, max_batch, max_seq, C.byref(h)))
-        self.h = h
+        self.h, self.device = h, device
         self.n_layers = n_layers
 
     def close(self):
@@ -729,7 +735,7 @@ class LLM:
         h = _vp()
         check(lib().dtts_llm_kv_create(self.h, n_pages, max_seqs, page_tokens, dtype, C.byref(h)))
         kv = KVCache.__new__(KVCache)
-        kv._init(h, self.n_layers, 2, 128)
+        kv._init(h, self.n_layers, 2, 128, self.device)
         return kv
 
     def extend(self, kv, seqs, n_new, emb, out=None, window=0, sinks=0, mem=MEM_HOST):
@@ -744,7 +750,9 @@ class LLM:
         rows = int(sum(c))
         if tuple(emb.shape) != (rows, 1536) or tuple(out.shape) != (rows, 1536):
             raise ValueError(f"emb and out: [{rows}][1536] expected")
+        kv._rows = max(kv._rows, rows)   # an error may leave either batch
         check(lib().dtts_llm_extend(self.h, kv.h, n, ps, pc, _addr(emb), window, sinks, _addr(out), mem))
+        kv._rows = rows
         return out
 
 

@@ -557,3 +557,93 @@ def test_pool_beyond_32_bits():
     got, _ = read(kv, f, 0, n - 5, layer=L - 1)
     assert torch.equal(got[0].double(), k[5:].double())
     kv.close()
+
+
+@pytest.mark.parametrize("dtype", [BF, I4])
+@pytest.mark.parametrize("window,sinks", [(2 ** 31 - 1, 0), (2 ** 31 - 1, 2 ** 31 - 1), (0, 2 ** 31 - 1), (5, 2 ** 31 - 1),
+                                          (2 ** 31 - 200, 3)])
+def test_windows_and_sinks_beyond_every_row(dtype, window, sinks):
+    """Row numbers minus such a window do not fit 32 bits."""
+    attend_case(dtype, 128, 12, 2, 64, [90, 333, 200], [90, 150, 1], window, sinks)
+
+
+def test_a_pending_trim_stays_out_of_a_captured_graph():
+    """A trim's marks that were pending at a capture do not come back with every replay of the graph."""
+    g = rng(21)
+    kv = make(page=16, n_pages=40)
+    a, b = kv.open(), kv.open()
+    ka, va = rand(g, 40, 2, 128), rand(g, 40, 2, 128)
+    fill(kv, [a, b], [(ka[:20], va[:20]), (rand(g, 90, 2, 128), rand(g, 90, 2, 128))])
+    kn, vn = ka[20:21].cuda(), va[20:21].cuda()
+    q = rand(g, 1, 12, 128).cuda()
+    out = torch.empty_like(q)
+    kv.extend([a], [1])
+    kv.write(0, kn, vn)
+    kv.attend(0, q, out)
+    kv.trim(b, 8)
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=torch.cuda.current_stream()):
+        kv.write(0, kn, vn)
+        kv.attend(0, q, out)
+    kv.close_seqs([b])
+    c = kv.open()
+    assert c == b                                  # the same table row, other pages
+    kc, vc = rand(g, 90, 2, 128), rand(g, 90, 2, 128)
+    fill(kv, [c], [(kc, vc)])
+    for i in range(21, 24):
+        kv.extend([a], [1])
+        kn.copy_(ka[i:i + 1])
+        vn.copy_(va[i:i + 1])
+        graph.replay()
+        want, tol = R.attend(q.cpu(), R.held(ka[:i + 1], True), R.held(va[:i + 1], True), i, 0, 0, None, True)
+        torch.cuda.synchronize()
+        R.assert_close(out, want, tol, f"replay at row {i}")
+        k, v = read(kv, c, 0, 90)
+        assert torch.equal(k[0].double(), R.held(kc, True)) and torch.equal(v[0].double(), R.held(vc, True))
+    qc = rand(g, 1, 12, 128)
+    kv.extend([c], [1])
+    kv.write(0, kc[:1].cuda(), vc[:1].cuda())
+    oc = torch.empty(1, 12, 128, dtype=torch.bfloat16, device="cuda")
+    kv.attend(0, qc.cuda(), oc)
+    torch.cuda.synchronize()
+    kk, vv = torch.cat([kc, kc[:1]]), torch.cat([vc, vc[:1]])
+    want, tol = R.attend(qc, R.held(kk, True), R.held(vv, True), 90, 0, 0, None, True)
+    R.assert_close(oc, want, tol, "the reopened sequence")
+    kv.sync()
+    kv.close()
+
+
+def test_tensors_that_do_not_fit_the_batch_are_refused():
+    kv = make(page=16, n_pages=8)
+    s = kv.open()
+    kv.extend([s], [3])
+    ok = torch.zeros(3, 2, 128, dtype=torch.bfloat16, device="cuda")
+    q = torch.zeros(3, 12, 128, dtype=torch.bfloat16, device="cuda")
+    for rows in (ok[:2], ok[:0]):
+        for call in (lambda: kv.write(0, rows, ok), lambda: kv.write(0, ok, rows)):
+            with pytest.raises(dtts.DttsError) as e:
+                call()
+            assert e.value.status == dtts.ERR_ARG
+    for bad in (ok.half(), ok.cpu(), ok[:, :1], ok[:, :, ::2], ok.float()):
+        with pytest.raises(ValueError):
+            kv.write(0, bad, ok)
+        with pytest.raises(ValueError):
+            kv.write(0, ok, bad)
+    for call in (lambda: kv.attend(0, q[:2], torch.empty_like(q)), lambda: kv.attend(0, q, q[:2])):
+        with pytest.raises(dtts.DttsError) as e:
+            call()
+        assert e.value.status == dtts.ERR_ARG
+    for bad in (q.half(), q.cpu(), q[:, :, :64]):
+        with pytest.raises(ValueError):
+            kv.attend(0, bad, torch.empty_like(q))
+        with pytest.raises(ValueError):
+            kv.attend(0, q, bad)
+    kv.write(0, ok, ok)
+    out = torch.empty(1, 3, 2, 128, device="cuda")
+    for bad in (out.half(), out.int(), out.cpu(), out[:, :2], out.bfloat16()):
+        with pytest.raises(ValueError):
+            kv.read(0, [s], [0], [3], out, bad)
+    kv.read(0, [s], [0], [3], out, out.clone())
+    torch.cuda.synchronize()
+    kv.close()

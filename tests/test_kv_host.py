@@ -66,3 +66,19 @@ def test_four_bit_rows_are_within_half_a_step():
     assert (err <= s * (0.5 + 7 * 2.0 ** -8)).all()
     # every value is exact in half
     assert torch.equal(R.held(x, True).to(torch.float16).double(), R.held(x, True))
+
+
+def test_host_tensors_and_other_types_are_refused():
+    """The Python calls look at shapes, types and devices before the library sees an address."""
+    kv = dtts.KVCache.__new__(dtts.KVCache)
+    kv._init(None, 1, 2, 64, 0)
+    kv._rows = 2
+    host = torch.zeros(2, 2, 64, dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="on device 0"):
+        kv.write(0, host, host)
+    with pytest.raises(ValueError, match="on device 0"):
+        kv.attend(0, host, host)
+    with pytest.raises(ValueError, match="on device 0"):
+        kv.read(0, [0], [0], [2], torch.zeros(1, 2, 2, 64), torch.zeros(1, 2, 2, 64))
+    with pytest.raises(ValueError):
+        kv.extend([0, 1], [1])
