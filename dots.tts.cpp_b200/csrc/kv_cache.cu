@@ -204,7 +204,8 @@ __global__ void __launch_bounds__(256) kv_read_kernel(const __grid_constant__ Kv
 }
 
 // The first `rows` rows of pages src to pages dst, all layers and heads: whole
-// 16-row blocks, one contiguous run a segment.
+// 16-row blocks, one contiguous run a segment.  The first block also applies the
+// metadata updates p, which saves a growing fork a launch.
 template <int N>
 struct Copies {
     static constexpr int kMax = N;
@@ -213,9 +214,12 @@ struct Copies {
 };
 template <int N>
 __global__ void __launch_bounds__(256) kv_copy_pages_kernel(const __grid_constant__ KvGeom g, uint8_t *__restrict__ pool,
-                                                            const __grid_constant__ Copies<N> c) {
+                                                            const __grid_constant__ Copies<N> c, int *__restrict__ meta,
+                                                            const __grid_constant__ Pokes<60> p) {
     pdl_wait();
     pdl_trigger();
+    if (blockIdx.x == 0 && blockIdx.y == 0)
+        for (int i = threadIdx.x; i < p.n; i += blockDim.x) meta[p.index[i]] = p.value[i];
     const int e = blockIdx.y, n = c.rows[e];
     const uint8_t *src = pool + (long long)c.src[e] * g.page_stride + (long long)blockIdx.x * g.seg;
     uint8_t *dst = pool + (long long)c.dst[e] * g.page_stride + (long long)blockIdx.x * g.seg;
@@ -299,6 +303,16 @@ KvMeta dtts_kv::kv_meta() const {
     return m;
 }
 
+// the next pending updates from i on, as many as fit
+template <typename P>
+void dtts_kv::take_pokes(P &p, size_t i) const {
+    p.n = (int)std::min<size_t>(P::kMax, pokes.size() - i);
+    for (int j = 0; j < p.n; j++) {
+        p.index[j] = pokes[i + j];
+        p.value[j] = meta_h[pokes[i + j]];   // an index listed twice gets its last value both times
+    }
+}
+
 int dtts_kv::flush() {
     if (pokes.empty()) return DTTS_OK;
     // While the stream is capturing, a trim's marks may be pending (the calls that add pages send theirs): they stay so.
@@ -309,11 +323,7 @@ int dtts_kv::flush() {
     if (cap != cudaStreamCaptureStatusNone) return DTTS_OK;
     auto send = [&](auto &p, size_t i) -> int {
         constexpr int kMax = std::remove_reference_t<decltype(p)>::kMax;
-        p.n = (int)std::min<size_t>(kMax, pokes.size() - i);
-        for (int j = 0; j < p.n; j++) {
-            p.index[j] = pokes[i + j];
-            p.value[j] = meta_h[pokes[i + j]];   // an index listed twice gets its last value both times
-        }
+        take_pokes(p, i);
         DTTS_CUDA(launch_k(kv_pdl(), kv_poke_kernel<kMax>, dim3(1), dim3(256), 0, stream, meta, p));
         return DTTS_OK;
     };
@@ -411,6 +421,9 @@ int dtts_kv::extend(int n_seq, const int *sq, const int *n_new) {
         poke(g.max_seqs + b, start);
         poke(2 * g.max_seqs + b, 0);
     }
+    Pokes<60> own;   // sent with the first copies
+    own.n = 0;
+    if (!copies.empty() && pokes.size() <= 60) take_pokes(own, 0);
     auto send = [&](auto &c, size_t i) -> int {
         constexpr int kMax = std::remove_reference_t<decltype(c)>::kMax;
         c.n = (int)std::min<size_t>(kMax, copies.size() - i);
@@ -419,13 +432,14 @@ int dtts_kv::extend(int n_seq, const int *sq, const int *n_new) {
             c.dst[j] = copies[i + j].dst;
             c.rows[j] = copies[i + j].rows;
         }
-        DTTS_CUDA(launch_k(kv_pdl(), kv_copy_pages_kernel<kMax>, dim3(g.L * g.H, c.n), dim3(256), 0, stream, g, pool, c));
+        DTTS_CUDA(launch_k(kv_pdl(), kv_copy_pages_kernel<kMax>, dim3(g.L * g.H, c.n), dim3(256), 0, stream, g, pool, c, meta, own));
         return DTTS_OK;
     };
     Copies<40> few;
-    Copies<320> many;
-    for (size_t i = 0; i < copies.size(); i += copies.size() <= 40 ? 40 : 320)
+    Copies<240> many;
+    for (size_t i = 0; i < copies.size(); i += copies.size() <= 40 ? 40 : 240)
         if ((st = copies.size() <= 40 ? send(few, i) : send(many, i))) return st;
+    if (own.n) pokes.clear();
     return flush();
 }
 

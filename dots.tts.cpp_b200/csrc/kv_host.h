@@ -52,6 +52,8 @@ struct dtts_kv {
         meta_h[index] = value;
         pokes.push_back(index);
     }
+    template <typename P>
+    void take_pokes(P &p, size_t i) const;
     int flush();                          // enqueues the pending metadata updates
     int take_page() {
         const int p = free_pages.top();

@@ -7,6 +7,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+from array import array
 
 import numpy as np
 
@@ -527,9 +528,9 @@ class KVAttendArgs(C.Structure):
 
 def _ints(a):
     """Sequence or int32 array -> (keep-alive, address, length)."""
-    if isinstance(a, (list, tuple)) and len(a) <= 256:      # short lists: twice as fast as through numpy
-        c = (C.c_int * len(a))(*a)
-        return c, C.addressof(c), len(a)
+    if isinstance(a, (list, tuple)):      # 16 entries: a third of the time of a ctypes array, a half of numpy's
+        c = array("i", a)
+        return (c, *c.buffer_info())
     a = np.ascontiguousarray(a, np.int32).ravel()
     return a, a.ctypes.data, a.size
 
