@@ -117,25 +117,38 @@ DTTS_DEV uint32_t kv_encode8(const float (&x)[8], __half *s16) {
 
 DTTS_DEV float kv_nibble(uint32_t w, int i) { return (float)((int)((w >> (4 * i)) & 15u) - 8); }
 
-// dims 8 w .. 8 w + 7 of row r of a segment (r within the page), as floats
-DTTS_DEV void kv_load8(const KvGeom &g, const uint8_t *seg, bool is_v, int r, int w, float (&x)[8]) {
+// dims 8 w .. 8 w + 7 of row r of a segment (r within the page): what is held, and as floats
+struct KvRaw8 {
+    uint4 q;      // 4-bit rows: the word in q.x
+    __half s;
+};
+DTTS_DEV KvRaw8 kv_raw8(const KvGeom &g, const uint8_t *seg, bool is_v, int r, int w) {
+    KvRaw8 a;
     if (g.i4) {
-        const uint8_t *row = seg + kv_row_off(g, is_v, r);
-        const uint32_t q = *reinterpret_cast<const uint32_t *>(row + (is_v ? kv_word_v(g.D, w, r) : kv_word_k(g.D, w)));
-        const float s = __half2float(*reinterpret_cast<const __half *>(
-            seg + kv_scale_off(g, is_v, r) + (w >> 2) * 2));
-#pragma unroll
-        for (int i = 0; i < 8; i++) x[i] = kv_nibble(q, i) * s;
+        a.q.x = *reinterpret_cast<const uint32_t *>(seg + kv_row_off(g, is_v, r) + (is_v ? kv_word_v(g.D, w, r) : kv_word_k(g.D, w)));
+        a.s = *reinterpret_cast<const __half *>(seg + kv_scale_off(g, is_v, r) + (w >> 2) * 2);
     } else {
         const int u = w ^ (is_v ? kv_swz_v(false, g.D, r) : kv_swz_k(false, r));
-        const uint4 q = *reinterpret_cast<const uint4 *>(seg + kv_row_off(g, is_v, r) + u * 16);
-        const uint32_t e[4] = {q.x, q.y, q.z, q.w};
+        a.q = *reinterpret_cast<const uint4 *>(seg + kv_row_off(g, is_v, r) + u * 16);
+    }
+    return a;
+}
+DTTS_DEV void kv_values8(const KvGeom &g, const KvRaw8 &a, float (&x)[8]) {
+    if (g.i4) {
+        const float s = __half2float(a.s);
+#pragma unroll
+        for (int i = 0; i < 8; i++) x[i] = kv_nibble(a.q.x, i) * s;
+    } else {
+        const uint32_t e[4] = {a.q.x, a.q.y, a.q.z, a.q.w};
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             x[2 * i] = __uint_as_float(e[i] << 16);
             x[2 * i + 1] = __uint_as_float(e[i] & 0xffff0000u);
         }
     }
+}
+DTTS_DEV void kv_load8(const KvGeom &g, const uint8_t *seg, bool is_v, int r, int w, float (&x)[8]) {
+    kv_values8(g, kv_raw8(g, seg, is_v, r, w), x);
 }
 
 // Stores 8 bf16 values (packed in q) as dims 8 w .. of row r; all lanes of the

@@ -168,11 +168,14 @@ __global__ void __launch_bounds__(256) kv_read_kernel(const __grid_constant__ Kv
     int row = (int)min(r.start[0] + item / g.H, (long long)row_end), head = (int)(item % g.H);
     int e = 0, end = -1, shift = 0;
     const int *trow = table;
-    float x[kReadItems][8];
+    // rows, then their pages, then what is held, each for all items before the next depends on it
+    int tok[kReadItems], page[kReadItems], hd[kReadItems];
     long long at[kReadItems];   // output element; -1: none
 #pragma unroll
     for (int i = 0; i < kReadItems; i++) {
         at[i] = -1;
+        tok[i] = 0;
+        hd[i] = head;
         if (row < row_end) {
             if (row >= end) {
                 e = kv_find_entry(r.start, r.n, row);
@@ -180,26 +183,35 @@ __global__ void __launch_bounds__(256) kv_read_kernel(const __grid_constant__ Kv
                 shift = r.first[e] - r.start[e];
                 trow = table + (long long)r.seq[e] * g.max_pages;
             }
-            const int tok = row + shift, page = trow[tok >> g.lgP];
-            if ((unsigned)page < (unsigned)g.n_pages) {
-                kv_load8(g, pool + kv_seg_off(g, page, layer, head), is_v, tok & (g.P - 1), w, x[i]);
-                at[i] = (((long long)layer * r.rows + row) * g.H + head) * g.D + 8 * w;
-            }
+            tok[i] = row + shift;
+            at[i] = (((long long)layer * r.rows + row) * g.H + head) * g.D + 8 * w;
         }
+        page[i] = trow[tok[i] >> g.lgP];
         for (head += step; head >= g.H; head -= g.H) row++;
+    }
+    KvRaw8 raw[kReadItems];
+#pragma unroll
+    for (int i = 0; i < kReadItems; i++) {
+        if ((unsigned)page[i] >= (unsigned)g.n_pages) {
+            page[i] = 0;
+            at[i] = -1;
+        }
+        raw[i] = kv_raw8(g, pool + kv_seg_off(g, page[i], layer, hd[i]), is_v, tok[i] & (g.P - 1), w);
     }
     void *dst = is_v ? v : k;
     const bool wide = (reinterpret_cast<uintptr_t>(dst) & 31u) == 0;
 #pragma unroll
     for (int i = 0; i < kReadItems; i++) {
         if (at[i] < 0) continue;
-        if (F32) {
-            store8_f32(static_cast<float *>(dst) + at[i], x[i], wide);
-        } else {
+        float x[8];
+        kv_values8(g, raw[i], x);
+        if (F32)
+            store8_f32(static_cast<float *>(dst) + at[i], x, wide);
+        else if (I4)
             *reinterpret_cast<uint4 *>(static_cast<bf16 *>(dst) + at[i]) =
-                make_uint4(pack_bf16x2(x[i][0], x[i][1]), pack_bf16x2(x[i][2], x[i][3]), pack_bf16x2(x[i][4], x[i][5]),
-                           pack_bf16x2(x[i][6], x[i][7]));
-        }
+                make_uint4(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), pack_bf16x2(x[4], x[5]), pack_bf16x2(x[6], x[7]));
+        else
+            *reinterpret_cast<uint4 *>(static_cast<bf16 *>(dst) + at[i]) = raw[i].q;
     }
 }
 
