@@ -103,14 +103,16 @@ __global__ void __launch_bounds__(256) kv_write_kernel(const __grid_constant__ K
     int row = (int)min(first / g.H, (long long)INT32_MAX), head = (int)(first % g.H);
     int b = 0, start = 0, end = -1, tok0 = 0;   // entry of the batch: its rows [start, end)
     const int *trow = m.table;
+    const bf16 *src = (is_v ? v : k) + 8 * w;
+    const long long src_row = is_v ? v_row : k_row, src_head = is_v ? v_head : k_head;
     uint4 q[kWriteItems];
-    uint8_t *seg[kWriteItems];
-    int place[kWriteItems];                     // row within the page; -1: nothing to store
+    int page[kWriteItems], place[kWriteItems], hd[kWriteItems];   // place: row within the page
 #pragma unroll
     for (int x = 0; x < kWriteItems; x++) {
         q[x] = make_uint4(0u, 0u, 0u, 0u);
-        seg[x] = pool;
-        place[x] = -1;
+        page[x] = -1;                           // nothing to store
+        place[x] = 0;
+        hd[x] = head;
         if (row < rows) {
             if (row >= end) {
                 b = kv_find_entry(m.start, n_seq, row);
@@ -119,18 +121,18 @@ __global__ void __launch_bounds__(256) kv_write_kernel(const __grid_constant__ K
                 tok0 = m.len[b] - m.cnt[b] - start;
                 trow = m.table + (long long)m.seq[b] * g.max_pages;
             }
-            const int tok = tok0 + row, page = row < end ? trow[tok >> g.lgP] : -1;
-            if ((unsigned)page < (unsigned)g.n_pages) {
-                q[x] = is_v ? *reinterpret_cast<const uint4 *>(v + row * v_row + head * v_head + 8 * w)
-                            : *reinterpret_cast<const uint4 *>(k + row * k_row + head * k_head + 8 * w);
-                seg[x] = pool + kv_seg_off(g, page, 0, head);
-                place[x] = tok & (g.P - 1);
-            }
+            const int tok = tok0 + row;
+            place[x] = tok & (g.P - 1);
+            if (row < end) page[x] = trow[tok >> g.lgP];
+            q[x] = *reinterpret_cast<const uint4 *>(src + row * src_row + head * src_head);
         }
         for (head += step; head >= g.H; head -= g.H) row++;
     }
 #pragma unroll
-    for (int x = 0; x < kWriteItems; x++) kv_store8(g, seg[x], is_v, max(place[x], 0), w, q[x], place[x] >= 0);
+    for (int x = 0; x < kWriteItems; x++) {
+        const bool on = (unsigned)page[x] < (unsigned)g.n_pages;
+        kv_store8(g, pool + kv_seg_off(g, on ? page[x] : 0, 0, hd[x]), is_v, place[x], w, q[x], on);
+    }
 }
 
 // 8 floats to 32-byte (wide) or 16-byte aligned memory: whole 32-byte sectors in one instruction where possible
@@ -246,49 +248,50 @@ __global__ void __launch_bounds__(256) kv_copy_pages_kernel(const __grid_constan
 // row's number does.  A warp has kGatherRows turns of rows in flight.
 constexpr int kGatherRows = 4;
 template <bool I4, int D>
-__global__ void __launch_bounds__(256) kv_gather_kernel(const __grid_constant__ KvGeom g, const int *__restrict__ table,
+__global__ void __launch_bounds__(256) kv_gather_kernel(const __grid_constant__ KvGeom geom, const int *__restrict__ table,
                                                         uint8_t *__restrict__ pool, const int *__restrict__ keep, int n,
                                                         int j0, int src, int dst) {
     pdl_wait();
     pdl_trigger();
+    const KvGeom g = fixed_geom<I4, D>(geom);
     constexpr int kUnits = I4 ? D / 32 : D / 8;                  // of K, of V
     constexpr int kLanes = 2 * kUnits + (I4 ? 2 : 0) > 16 ? 32 : 16, kStep = 32 / kLanes;
     const int lane = threadIdx.x & 31, u = lane % kLanes;
-    const uint8_t *from = pool + (long long)blockIdx.y * g.seg;   // (layer, head)
-    uint8_t *to = pool + (long long)blockIdx.y * g.seg;
+    const bool unit = u < 2 * kUnits, mine = u < 2 * kUnits + (I4 ? 2 : 0);
+    const bool is_v = unit ? u >= kUnits : u > 2 * kUnits;
+    const int w = unit ? u - (is_v ? kUnits : 0) : 0;
+    uint8_t *seg = pool + (long long)blockIdx.y * g.seg;   // (layer, head)
     const int *tsrc = table + (long long)src * g.max_pages, *tdst = table + (long long)dst * g.max_pages;
-    int j = (blockIdx.x * 8 + (threadIdx.x >> 5)) * (kGatherRows * kStep) + lane / kLanes;
-    uint4 x[kGatherRows];
-    uint8_t *at[kGatherRows];
+    const int j = (blockIdx.x * 8 + (threadIdx.x >> 5)) * (kGatherRows * kStep) + lane / kLanes;
+    // row numbers, pages and values, each for all rows before the next depends on it
+    int ra[kGatherRows], pa[kGatherRows], pb[kGatherRows];
 #pragma unroll
-    for (int i = 0; i < kGatherRows; i++, j += kStep) {
-        at[i] = nullptr;
-        if (j >= n || u >= 2 * kUnits + (I4 ? 2 : 0)) continue;
-        const int a = keep[j], b = j0 + j, pa = tsrc[a >> g.lgP], pb = tdst[b >> g.lgP];
-        if ((unsigned)pa >= (unsigned)g.n_pages || (unsigned)pb >= (unsigned)g.n_pages) continue;
-        const int ra = a & (g.P - 1), rb = b & (g.P - 1);
-        const uint8_t *sa = from + (long long)pa * g.page_stride;
-        at[i] = to + (long long)pb * g.page_stride;
-        if (u < 2 * kUnits) {
-            const bool is_v = u >= kUnits;
-            const int w = is_v ? u - kUnits : u;
-            const int ua = w ^ (is_v ? kv_swz_v(I4, D, ra) : kv_swz_k(I4, ra)), ub = w ^ (is_v ? kv_swz_v(I4, D, rb) : kv_swz_k(I4, rb));
-            x[i] = *reinterpret_cast<const uint4 *>(sa + kv_row_off(g, is_v, ra) + ua * 16);
-            at[i] += kv_row_off(g, is_v, rb) + ub * 16;
-        } else {
-            const bool is_v = u > 2 * kUnits;
-            sa += kv_scale_off(g, is_v, ra);
-            at[i] += kv_scale_off(g, is_v, rb);
-            x[i].x = *reinterpret_cast<const uint32_t *>(sa);
-            if (D == 128) x[i].y = *reinterpret_cast<const uint32_t *>(sa + 4);
-        }
+    for (int i = 0; i < kGatherRows; i++) ra[i] = keep[min(j + i * kStep, n - 1)];
+#pragma unroll
+    for (int i = 0; i < kGatherRows; i++) {
+        pa[i] = tsrc[ra[i] >> g.lgP];
+        pb[i] = tdst[(j0 + min(j + i * kStep, n - 1)) >> g.lgP];
+    }
+    // where u's part of row r stands in a page
+    auto place = [&](int r) {
+        return unit ? kv_row_off(g, is_v, r) + (w ^ (is_v ? kv_swz_v(I4, D, r) : kv_swz_k(I4, r))) * 16 : kv_scale_off(g, is_v, r);
+    };
+    uint4 x[kGatherRows];
+#pragma unroll
+    for (int i = 0; i < kGatherRows; i++) {
+        const uint8_t *at = seg + ((unsigned)pa[i] < (unsigned)g.n_pages ? pa[i] : 0) * g.page_stride + place(ra[i] & (g.P - 1));
+        x[i] = make_uint4(0u, 0u, 0u, 0u);
+        if (unit) x[i] = *reinterpret_cast<const uint4 *>(at);
+        else if (mine && D == 128) *reinterpret_cast<uint2 *>(&x[i]) = *reinterpret_cast<const uint2 *>(at);
+        else if (mine) x[i].x = *reinterpret_cast<const uint32_t *>(at);
     }
 #pragma unroll
     for (int i = 0; i < kGatherRows; i++) {
-        if (!at[i]) continue;
-        if (u < 2 * kUnits) *reinterpret_cast<uint4 *>(at[i]) = x[i];
-        else if (D == 128) *reinterpret_cast<uint2 *>(at[i]) = make_uint2(x[i].x, x[i].y);
-        else *reinterpret_cast<uint32_t *>(at[i]) = x[i].x;
+        if (j + i * kStep >= n || (unsigned)pa[i] >= (unsigned)g.n_pages || (unsigned)pb[i] >= (unsigned)g.n_pages) continue;
+        uint8_t *at = seg + pb[i] * g.page_stride + place((j0 + j + i * kStep) & (g.P - 1));
+        if (unit) *reinterpret_cast<uint4 *>(at) = x[i];
+        else if (mine && D == 128) *reinterpret_cast<uint2 *>(at) = make_uint2(x[i].x, x[i].y);
+        else if (mine) *reinterpret_cast<uint32_t *>(at) = x[i].x;
     }
 }
 
