@@ -43,15 +43,35 @@ __global__ void kv_poke_kernel(int *__restrict__ meta, const __grid_constant__ P
     for (int i = threadIdx.x; i < p.n; i += blockDim.x) meta[p.index[i]] = p.value[i];
 }
 
-constexpr int kPuts = 1000;
-struct Puts {
-    int n;
-    int value[kPuts];
+// Kept rows as bits (bit i of word x: row 32 (first + x) + i), to their ascending list from dst[base] on; the
+// updates p beside them.  A row costs a bit of parameters, so thousands of rows are one launch.
+template <int N>
+struct KeepBits {
+    static constexpr int kMax = N;
+    int n, first, base;
+    uint32_t word[N];
 };
-__global__ void kv_put_kernel(int *__restrict__ dst, const __grid_constant__ Puts p) {
+template <int N>
+__global__ void __launch_bounds__(1024) kv_keep_kernel(int *__restrict__ dst, const __grid_constant__ KeepBits<N> k,
+                                                       int *__restrict__ meta, const __grid_constant__ Pokes<60> p) {
+    static_assert(N <= 1024, "a thread a word");
+    __shared__ int total[32];
     pdl_wait();
     pdl_trigger();
-    for (int i = threadIdx.x; i < p.n; i += blockDim.x) dst[i] = p.value[i];
+    const int t = threadIdx.x, lane = t & 31;
+    for (int i = t; i < p.n; i += blockDim.x) meta[p.index[i]] = p.value[i];
+    uint32_t w = t < k.n ? k.word[t] : 0u;
+    int at = __popc(w);   // inclusive sum over the warp, then over the warps before
+#pragma unroll
+    for (int x = 1; x < 32; x <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, at, x);
+        if (lane >= x) at += y;
+    }
+    if (lane == 31) total[t >> 5] = at;
+    __syncthreads();
+    at += k.base - __popc(w);
+    for (int x = 0; x < t >> 5; x++) at += total[x];
+    for (; w; w &= w - 1) dst[at++] = 32 * (k.first + t) + __ffs(w) - 1;
 }
 
 template <int N>
@@ -845,14 +865,37 @@ int dtts_kv_compact(dtts_kv *kv, int seq, int n_keep, const int *keep) try {
         pages.push_back(kv->take_page());
         kv->poke(kv->table_at(scratch, p), pages.back());
     }
-    if ((st = kv->flush())) return st;
+    Pokes<60> own;   // the new pages' entries travel with the first rows
+    own.n = 0;
+    const bool beside = n > 0 && kv->pokes.size() <= 60;
+    if (beside)
+        kv->take_pokes(own, 0);
+    else if ((st = kv->flush()))
+        return st;
     if (n > 0) {
-        for (int i = 0; i < n; i += kPuts) {
-            Puts p;
-            p.n = std::min(kPuts, n - i);
-            std::memcpy(p.value, keep + j0 + i, (size_t)p.n * 4);
-            DTTS_CUDA(launch_k(kv_pdl(), kv_put_kernel, dim3(1), dim3(256), 0, kv->stream, kv->keep + i, p));
-        }
+        const int first = keep[j0] >> 5, words = (keep[n_keep - 1] >> 5) - first + 1;
+        std::vector<uint32_t> bits((size_t)words, 0u);
+        for (int j = j0; j < n_keep; j++) bits[(keep[j] >> 5) - first] |= 1u << (keep[j] & 31);
+        int base = 0;
+        auto send = [&](auto &k, int i) -> int {
+            constexpr int kMax = std::remove_reference_t<decltype(k)>::kMax;
+            k.n = std::min(kMax, words - i);
+            k.first = first + i;
+            k.base = base;
+            for (int x = 0; x < k.n; x++) {
+                k.word[x] = bits[i + x];
+                base += __builtin_popcount(k.word[x]);
+            }
+            if (base == k.base) return DTTS_OK;   // none kept here; the first words hold a row
+            DTTS_CUDA(launch_k(kv_pdl(), kv_keep_kernel<kMax>, dim3(1), dim3((k.n + 31) / 32 * 32), 0, kv->stream, kv->keep, k,
+                               kv->meta, own));
+            return DTTS_OK;
+        };
+        KeepBits<224> few;
+        KeepBits<768> many;
+        for (int i = 0; i < words; i += words <= 224 ? 224 : 768)
+            if ((st = words <= 224 ? send(few, i) : send(many, i))) return st;
+        if (beside) kv->pokes.clear();
         auto gather = [&](auto kernel, int rows_a_warp) {
             return launch_k(kv_pdl(), kernel, dim3((n + 8 * rows_a_warp - 1) / (8 * rows_a_warp), g.L * g.H), dim3(256), 0,
                             kv->stream, g, (const int *)(kv->meta + 5 * g.max_seqs), kv->pool, (const int *)kv->keep, n, j0,

@@ -647,3 +647,21 @@ def test_tensors_that_do_not_fit_the_batch_are_refused():
     kv.read(0, [s], [0], [3], out, out.clone())
     torch.cuda.synchronize()
     kv.close()
+
+
+@pytest.mark.parametrize("n", [7168, 7200, 24600, 60000])
+def test_compact_long_sequences(n):
+    """Row lists of one launch and of several, runs and single rows far apart."""
+    g = rng(31)
+    kv = make(H=1, D=64, page=128, n_pages=1000, max_tokens=60000)
+    s = kv.open()
+    fill(kv, [s], [(rand(g, n, 1, 64), rand(g, n, 1, 64))])
+    k, v = read(kv, s, 0, n)
+    half = (torch.rand(n, generator=g) < 0.5).nonzero().flatten().tolist()
+    for keep in (half, [5, n - 1], [0, 31, 32, 63, 64, 4097] + list(range(n - 70, n)), list(range(1, n))):
+        (f,) = kv.fork(s)
+        kv.compact(f, keep)
+        gk, gv = read(kv, f, 0, len(keep))
+        assert torch.equal(gk, k[:, keep]) and torch.equal(gv, v[:, keep])
+        kv.close_seqs([f])
+    kv.close()
