@@ -80,39 +80,48 @@ DTTS_DEV int kv_find_entry(const int *start, int n, int row) {
     return lo;
 }
 
-// Quantises 8 bf16 values (a quarter of a group whose four lanes are neighbours)
-// to one word of nibbles; returns the group's scale through s16.  All lanes of
-// the warp take part.
-DTTS_DEV uint32_t kv_encode8(const float (&x)[8], __half *s16) {
-    float a = 0.f;
-    int bad = 0;
-#pragma unroll
-    for (int i = 0; i < 8; i++) {
-        const float m = fabsf(x[i]);
-        bad |= !(m <= 3.402823466e38f);   // fmaxf drops NaN
-        a = fmaxf(a, m);
-    }
-#pragma unroll
-    for (int o = 1; o < 4; o <<= 1) {
-        a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, o));
-        bad |= __shfl_xor_sync(0xffffffffu, bad, o);
-    }
-    float s = __bfloat162float(__float2bfloat16_rn(__fdiv_rn(a, 7.0f)));
+// Quantises 8 packed bf16 values (a quarter of a group whose four lanes are
+// neighbours) to one word of nibbles; returns the group's scale through s16.  All
+// lanes of the warp take part.
+DTTS_DEV uint32_t kv_encode8(uint4 q, __half *s16) {
+    const uint32_t e[4] = {q.x, q.y, q.z, q.w};
+    // the largest |x|: magnitudes compare as integers, infinity and NaN above all others
+    uint32_t top = __vmaxu2(__vmaxu2(e[0] & 0x7fff7fffu, e[1] & 0x7fff7fffu), __vmaxu2(e[2] & 0x7fff7fffu, e[3] & 0x7fff7fffu));
+    top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    top = max(top & 0xffffu, top >> 16);
+    const bool bad = top >= 0x7f80u;
+    const float a = __uint_as_float(top << 16);
+    // bf16(a / 7) from a product: a / 7 is never nearer than 1 / 14 of the last place (2^-11.8 relative) to a rounding
+    // border (2 a 2^t - 14 k - 7 is odd for integers a 2^t and k), and the product is off by 2^-23
+    float s = __bfloat162float(__float2bfloat16_rn(a * (1.0f / 7.0f)));
     s = fminf(fmaxf(s, kKvScaleMin), kKvScaleMax);
     *s16 = bad ? __ushort_as_half(0x7e00) : __float2half_rn(s);
+    float x[8];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        x[2 * i] = __uint_as_float(e[i] << 16);
+        x[2 * i + 1] = __uint_as_float(e[i] & 0xffff0000u);
+    }
+    // up to there |x / s| <= 7 (1 + 2^-8), which rounds to 7 at most
+    if (a > 7.f * kKvScaleMax)
+#pragma unroll
+        for (int i = 0; i < 8; i++) x[i] = fminf(fmaxf(x[i], -7.f * kKvScaleMax), 7.f * kKvScaleMax);
     // c = rint(x / s) without a division a value.  x and s have 8 significant bits, so x / s lies on a rounding
     // border n + 1/2 exactly or at least 2^-9.2 away from it (numerator of the difference over 2 s).  x * (1 / s)
-    // in one rounding to multiples of 2^-16 (an fma onto 192) is off by 2^-17 + 2^-21 at most: on a border it comes
-    // out as the border, elsewhere on the right side of it.
-    const float rs = __frcp_rn(s);
+    // in one rounding to multiples of 2^-16 (an fma onto 192; 1 / s is good to 2^-23) is off by 2^-17 + 2^-20 at
+    // most: on a border it comes out as the border, elsewhere on the right side of it.
+    float rs;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(rs) : "f"(s));
     uint32_t w = 0;
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
-        const float q = fminf(fmaxf(fmaf(x[i], rs, 192.f) - 192.f, -7.f), 7.f);
-        // + 1.5 * 2^23 rounds to the nearest even integer and leaves it, plus 8, in the low bits
-        w |= (__float_as_uint(q + 12582920.f) & 15u) << (4 * i);
+    for (int i = 7; i >= 0; i--) {
+        // with the 192 this adds 1.5 * 2^23 + 8: rounds to the nearest even integer and leaves it, plus 8, in the low
+        // bits, below 0x4b400000, which adds up to a constant over the word
+        w = (w << 4) + __float_as_uint(fmaf(x[i], rs, 192.f) + 12582728.f);
     }
-    return bad ? 0x88888888u : w;
+    constexpr uint32_t kAbove = (uint32_t)(0x4b400000ull * 0x11111111ull);
+    return bad ? 0x88888888u : w - kAbove;
 }
 
 DTTS_DEV float kv_nibble(uint32_t w, int i) { return (float)((int)((w >> (4 * i)) & 15u) - 8); }
@@ -155,15 +164,8 @@ DTTS_DEV void kv_load8(const KvGeom &g, const uint8_t *seg, bool is_v, int r, in
 // warp call it, four neighbouring lanes hold one group; on: this lane stores.
 DTTS_DEV void kv_store8(const KvGeom &g, uint8_t *seg, bool is_v, int r, int w, uint4 q, bool on) {
     if (g.i4) {
-        const uint32_t e[4] = {q.x, q.y, q.z, q.w};
-        float x[8];
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            x[2 * i] = __uint_as_float(e[i] << 16);
-            x[2 * i + 1] = __uint_as_float(e[i] & 0xffff0000u);
-        }
         __half s;
-        const uint32_t c = kv_encode8(x, &s);
+        const uint32_t c = kv_encode8(q, &s);
         if (!on) return;
         uint8_t *row = seg + kv_row_off(g, is_v, r);
         *reinterpret_cast<uint32_t *>(row + (is_v ? kv_word_v(g.D, w, r) : kv_word_k(g.D, w))) = c;

@@ -665,3 +665,25 @@ def test_compact_long_sequences(n):
         assert torch.equal(gk, k[:, keep]) and torch.equal(gv, v[:, keep])
         kv.close_seqs([f])
     kv.close()
+
+
+def test_int4_every_pair_of_significands():
+    """Each group's largest value against every bf16 value from a 32nd of it up: all quotients a code is rounded from."""
+    top, rest = [], []
+    for a in range(128, 256):
+        x = torch.cat([torch.arange(128, 256) * 2.0 ** -e for e in range(6)])
+        x = x[x <= a]
+        x = torch.cat([x, x[:-len(x) % 31]]) if len(x) % 31 else x
+        x = x.view(-1, 31) * torch.where(torch.arange(31) % 2 == 0, 1.0, -1.0)
+        rest.append(x)
+        top.append(torch.full((len(x), 1), float(a)))
+    rows = torch.cat([torch.cat(top), torch.cat(rest)], 1)
+    rows = torch.cat([rows, rows[:-len(rows) % 8]]).view(-1, 2, 128) / 64
+    k = rows.to(torch.bfloat16)
+    assert torch.equal(k.float(), rows)
+    kv = make(n_pages=20)
+    s = kv.open()
+    fill(kv, [s], [(k, -k)])
+    got_k, got_v = read(kv, s, 0, len(k))
+    assert torch.equal(got_k[0].double(), R.held(k, True)) and torch.equal(got_v[0].double(), R.held(-k, True))
+    kv.close()
