@@ -239,6 +239,10 @@ struct FewCfg {
 // bf16 terms (2^-17).
 // The running maximum m of a column is raised only when a score passes it by 2^8
 // (P <= 2^8 is as exact as P <= 1), so most tiles need no exchange between lanes.
+// Measured (12 query heads over 2 of 128): 32 sequences of 4097 .. 32768 4-bit rows 47.9 us, 3.55 TB/s of rows, bound
+// by unpacking (52% of the issue slots, integer and half pipes at their rate); 64 of 1000 .. 8191 bf16 rows 54.5 us,
+// 5.5 TB/s, bound by DRAM; one of 48 rows 5.9 us, bound by latency.  4 warps of 64-key tiles and three CTAs an SM
+// hide the most: 8 warps of 32 keys and two CTAs measured 53.2 us for the first of these, 12 of 64 and one 49.7.
 template <int D, bool I4, int NT>
 __global__ void __launch_bounds__(FewCfg<D, I4>::kThreads, NT == 1 ? 3 : 1) kv_attend_few_kernel(const __grid_constant__ KvAttendArgs a) {
     using C = FewCfg<D, I4>;
@@ -816,7 +820,9 @@ DTTS_DEV float *many_part(const KvAttendArgs &a, int unit, int split) {
     return a.ws + ((long long)unit * a.splits + split) * 256 * (D + 2);
 }
 
-// Joins the parts of a unit, a row a thread, 16 dims a block (blockIdx.y).
+// Joins the parts of a unit, a row a thread, 16 dims a block (blockIdx.y).  Bound by latency: 8.5 us alone, caches
+// cold, for two chunks of 512 tokens in 3 parts.  A kernel of its own, since one CTA a unit that joins after its
+// attention is too few: with whole-row loads of Q beside it, this took the two chunks from 79 to 44 us.
 template <int D>
 __global__ void __launch_bounds__(256) kv_join_many_kernel(const __grid_constant__ KvAttendArgs a, int pairs) {
     pdl_wait();
@@ -961,6 +967,9 @@ DTTS_DEV bool kv_wait(uint64_t *bar, uint32_t parity, volatile int *abort_flag, 
 // rounded by 2^-11.  bf16 rows: P is rounded to bf16 (2^-8 of the P-weighted mean
 // of |v|, the size of the output's own rounding): a second term would cost half as
 // much tensor time again.
+// Measured: four prompts of 1501 .. 2047 tokens (12 query heads over 2 of 128, 4 bits) 74 us, 530 TFLOP/s; chunks of
+// 512 tokens behind windows of 4096 (bf16) 45 us, 582 TFLOP/s.  A CTA per row-tile pair, longest first: resident CTAs
+// that draw their pairs from a counter measured 81 and 45 us.
 template <int D, bool I4>
 __global__ void __launch_bounds__(512, 1) kv_attend_many_kernel(const __grid_constant__ KvAttendArgs a, int pairs) {
     using C = ManyCfg<D, I4>;
