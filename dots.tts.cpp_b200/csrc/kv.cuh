@@ -195,8 +195,11 @@ struct KvAttendArgs {
 };
 // What sizes the launches of a cache's attention kernels.
 struct KvShapes {
-    int few_key_tile, few_min_tiles;   // rows of a key tile; fewest tiles a part is given
-    int few_ctas[2];                   // resident CTAs per SM: up to 8, up to 16 query rows
+    int few_key_tile, few_warps;   // rows of a key tile; warps of a CTA, which take them in turn
+    int few_ctas[2];               // resident CTAs per SM: up to 8, up to 16 query rows
+    // microseconds a tile of a warp takes with 1, 2, 3 CTAs on an SM, divided by their number; what a launch of so
+    // many takes beside (measured, see kv_attend_prepare)
+    float few_tile_us[2][3], few_start_us[3];
 };
 constexpr int kKvManyKeyTile = 128;
 // Sets the kernels' attributes on the current device.

@@ -1458,7 +1458,17 @@ cudaError_t prepare_few(int *ctas) {
 template <int D, bool I4>
 cudaError_t prepare(KvShapes *k) {
     k->few_key_tile = FewCfg<D, I4>::KT;
-    k->few_min_tiles = 2 * FewCfg<D, I4>::kWarps;
+    k->few_warps = FewCfg<D, I4>::kWarps;
+    // 64 sequences of 300 .. 32768 rows, 12 query heads over 2 of 128: 6.3 + 1.46 x, 8 + 1.45 x, 10 + 1.02 x us for x
+    // tiles a warp, with 1, 2, 3 CTAs on an SM (4 bits), 4 + 0.8 x, 0.72 x, 0.68 x (bf16).  Tiles of other shapes by
+    // their size; 9 .. 16 query rows measured 2.2 x, 1.8 x.
+    constexpr float size = I4 ? D / 128.f : FewCfg<D, I4>::KT * D / 2048.f;
+    const float one[3] = {I4 ? 1.46f : 0.8f, I4 ? 1.45f : 0.72f, I4 ? 1.02f : 0.68f}, start[3] = {0.f, I4 ? 1.5f : 0.5f, I4 ? 3.5f : 1.f};
+    for (int c = 0; c < 3; c++) {
+        k->few_tile_us[0][c] = one[c] * size;
+        k->few_tile_us[1][c] = (I4 ? (c ? 1.8f : 2.2f) : one[c]) * size;
+        k->few_start_us[c] = start[c];
+    }
     cudaError_t e = prepare_few<D, I4, 1>(&k->few_ctas[0]);
     if (e == cudaSuccess) e = prepare_few<D, I4, 2>(&k->few_ctas[1]);
     if (e != cudaSuccess) return e;

@@ -538,13 +538,14 @@ int dtts_kv::plan_attend(const dtts_kv_attend_args &a, KvAttendPlan *plan) const
     p.window = a.window >= max_tokens ? 0 : a.window;
     p.sinks = (int)std::min<long long>(a.sinks, max_tokens);
     p.ws = ws; p.cnt = cnt; p.err = d_err;
-    std::vector<std::pair<long long, long long>> parts;
+    std::vector<std::pair<int, int>> parts;
     // both kernels run where a batch mixes steps and prompts; each takes its own sequences
     for (int many = 0; many < 2; many++) {
         const int kt = many ? kKvManyKeyTile : shapes.few_key_tile;
         long long tiles = 0, max_tiles = 0;
         int max_rows = 0;
         parts.clear();   // (key tiles, row tiles) of this kernel's sequences
+        int same[32] = {};   // sequences of so few key tiles are counted, not listed
         for (int b = 0; b < n_seq; b++) {
             const long long rows = (long long)b_cnt[b] * G;
             if (rows == 0 || (rows > kKvFewRows) != (many == 1)) continue;
@@ -554,31 +555,64 @@ int dtts_kv::plan_attend(const dtts_kv_attend_args &a, KvAttendPlan *plan) const
             tiles += nt * rt * g.H;
             max_tiles = std::max(max_tiles, nt);
             max_rows = (int)std::min<long long>(INT32_MAX / 2, std::max<long long>(max_rows, rows));
-            parts.emplace_back(nt, rt);
+            if (nt < 32) same[nt] += (int)rt;
+            else parts.emplace_back((int)nt, (int)rt);
         }
+        for (int nt = 1; nt < 32; nt++)
+            if (same[nt]) parts.emplace_back(nt, same[nt]);
         if (!max_rows) continue;
         const int rt = many ? (max_rows + 255) / 256 : 1;
         const long long units = (long long)n_seq * g.H * rt;
         DTTS_CHECK(units <= INT32_MAX, DTTS_ERR_ARG, "%lld row tiles in one batch", units);
-        // Parts of the key ranges: as short as they may be with all CTAs resident at once, but not
-        // shorter than what hides a CTA's start and the join.
-        const long long resident = (long long)(many ? 1 : std::max(1, shapes.few_ctas[max_rows > 8])) * num_sms;
-        const long long min_tiles = many ? 2 : shapes.few_min_tiles;
         auto ctas = [&](long long per) {
+            const int len = (int)per;
             long long n = 0;
-            for (auto &x : parts) n += (x.first + per - 1) / per * x.second * g.H;
-            return n;
+            for (auto &x : parts) n += (long long)((x.first + len - 1) / len) * x.second;
+            return n * g.H;
         };
-        long long per = std::max(min_tiles, (tiles + resident - 1) / resident), hi = std::max(per, max_tiles);
-        while (per < hi) {   // the smallest part length with at most `resident` CTAs, or no split at all
-            const long long mid = (per + hi) / 2;
-            if (ctas(mid) <= resident) hi = mid; else per = mid + 1;
+        const long long slots = kWsFloats / (many ? 256ll : (long long)kKvFewRows) / (g.D + 2);
+        const long long most = units > kMaxUnits ? 1 : std::max(1ll, slots / units);   // parts that the workspace has room for
+        long long per = max_tiles;
+        if (many) {
+            // Parts of the key ranges: as short as they may be with all CTAs resident at once, or no split at all
+            long long hi = per;
+            per = std::min(hi, std::max(2ll, (tiles + num_sms - 1) / num_sms));
+            while (per < hi) {
+                const long long mid = (per + hi) / 2;
+                if (ctas(mid) <= num_sms) hi = mid; else per = mid + 1;
+            }
+        } else {
+            // The number of parts of the longest range with the least time for all: the tiles of the warps that share
+            // an SM, and the join, 0.5 us and 0.28 more a part.  No split beats two halves for 64 sequences of 1000
+            // rows (12.0 against 14.7 us); one of 16000 takes 16.8 us in 16 parts, 18.5 in 32.
+            const int wide = max_rows > 8, resident = std::min(3, std::max(1, shapes.few_ctas[wide]));
+            float best = INFINITY;
+            // whether parts of len tiles fit on the SMs at once; they are kept where they take the least time so far
+            auto fits = [&](long long len) {
+                const long long n = (max_tiles + len - 1) / len, c = (ctas(len) + num_sms - 1) / num_sms;
+                if (n > 1 && c > resident) return false;
+                const int at = (int)std::min<long long>(c, resident) - 1;
+                const int w = shapes.few_warps;   // few tiles: the warp with one more counts
+                const float turns = len < 8 * w ? (float)((len + w - 1) / w) : (float)len / w;
+                const float us = turns * (float)c * shapes.few_tile_us[wide][at] +
+                                 shapes.few_start_us[at] + (n > 1 ? 0.5f + 0.28f * (float)n : 0.f);
+                if (us < best) {
+                    best = us;
+                    per = len;
+                }
+                return true;
+            };
+            long long hi = max_tiles, lo = 0;   // the shortest parts that fit, the longest that do not
+            for (long long n = 1; n <= std::min(most, max_tiles) && !lo; n += 1 + n / 16) {
+                const long long len = (max_tiles + n - 1) / n;
+                if (fits(len)) hi = len; else lo = len;
+            }
+            while (lo && hi - lo > 1) {
+                const long long mid = (lo + hi) / 2;
+                if (fits(mid)) hi = mid; else lo = mid;
+            }
         }
-        long long splits = (max_tiles + per - 1) / per;
-        const int slot_rows = many ? 256 : kKvFewRows;
-        const long long slots = kWsFloats / ((long long)slot_rows * (g.D + 2));
-        if (units > kMaxUnits) splits = 1;
-        splits = std::max(1ll, std::min(splits, slots / units));
+        const long long splits = std::max(1ll, std::min((max_tiles + per - 1) / per, most));
         p.splits = (int)splits;
         p.tiles_per_split = (int)per;
         plan->args[many] = p;

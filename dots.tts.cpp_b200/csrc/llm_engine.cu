@@ -519,7 +519,7 @@ struct dtts_llm {
     // The new tokens of a ragged batch over a paged cache.  A step (one token for
     // every sequence) is a graph: its kernels read lengths and tables on the device,
     // so one graph serves every step with the same batch size and split of the
-    // attention (rounded up to a power of two; a part then holds at least 4 tiles).
+    // attention (rounded down to a power of two; a part holds at least 4 tiles).
     int extend(dtts_kv *kv, int n_seq, const int *seqs, const int *n_new, const float *emb, int window, int sinks,
                float *hidden, int mem) {
         long long M = 0;
@@ -560,7 +560,7 @@ struct dtts_llm {
         if (step) {
             KvAttendArgs &p = plan.args[0];
             int pow2 = 1;
-            while (pow2 < p.splits) pow2 *= 2;
+            while (2 * pow2 <= p.splits) pow2 *= 2;
             const int splits = std::min(pow2, kv->max_splits(n_seq));
             cudaGraphExec_t exec = nullptr;
             for (Graph &g : graphs)
