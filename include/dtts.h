@@ -346,7 +346,8 @@ int dtts_pe_stream_length(dtts_pe *p, int *tokens);
  * waits and reports device errors) and must be serialised by the caller, like an engine's.
  * dtts_kv_write, dtts_kv_attend and dtts_kv_read may be captured into a CUDA graph; a replay acts on
  * the batch that is current on the stream then (same number of sequences and new tokens as at the
- * capture, any lengths).  All work of a cache shares its workspace: replays of graphs captured from one
+ * capture, any lengths; the split of long key ranges over the GPU stays as it was sized at the
+ * capture, so capture again when the sequences have grown much).  All work of a cache shares its workspace: replays of graphs captured from one
  * cache must not overlap with each other or with its calls.  The calls that change tables
  * (extend, fork, compact) return DTTS_ERR_UNSUPPORTED while the stream is capturing.
  *
