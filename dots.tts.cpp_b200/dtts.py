@@ -582,9 +582,9 @@ class KVCache:
         check(self._lib.dtts_kv_close(self.h, n, p))
 
     def fork(self, seq, n=1):
-        out = (C.c_int * max(n, 0))()
-        check(self._lib.dtts_kv_fork(self.h, seq, n, out))
-        return list(out)
+        out = array("i", bytes(4 * max(n, 0)))
+        check(self._lib.dtts_kv_fork(self.h, seq, n, out.buffer_info()[0]))
+        return out.tolist()
 
     def truncate(self, seq, n_tokens):
         check(self._lib.dtts_kv_truncate(self.h, seq, n_tokens))

@@ -374,7 +374,8 @@ int dtts_kv_sync(dtts_kv *kv);
 int dtts_kv_open(dtts_kv *kv, int *seq);                       /* a new, empty sequence           */
 int dtts_kv_close(dtts_kv *kv, int n, const int *seqs);        /* frees sequences and their pages */
 /* n new sequences with the rows of src.  Pages are shared; a shared, partly filled last page is
- * copied when a sequence that shares it grows. */
+ * copied when a sequence that shares it grows.  Where src is in the current batch, rows written
+ * after the fork are the new sequences' rows too. */
 int dtts_kv_fork(dtts_kv *kv, int src, int n, int *dst);
 int dtts_kv_truncate(dtts_kv *kv, int seq, int n_tokens);      /* drops the rows behind n_tokens  */
 /* Frees the pages that no later token sees through a window of `window` tokens with `sinks` first

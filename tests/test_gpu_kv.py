@@ -687,3 +687,31 @@ def test_int4_every_pair_of_significands():
     got_k, got_v = read(kv, s, 0, len(k))
     assert torch.equal(got_k[0].double(), R.held(k, True)) and torch.equal(got_v[0].double(), R.held(-k, True))
     kv.close()
+
+
+@pytest.mark.parametrize("dtype", [BF, I4])
+def test_rows_written_after_a_fork_are_shared(dtype):
+    """A fork of a sequence of the current batch sees the batch's rows; a grown one keeps its own copy."""
+    g = rng(41)
+    kv = make(page=32, dtype=dtype)
+    s = kv.open()
+    k, v = rand(g, 45, 2, 128), rand(g, 45, 2, 128)
+    fill(kv, [s], [(k[:40], v[:40])])
+    kv.extend([s], [5])
+    f, h = kv.fork(s, 2)
+    kv.write(0, k[40:].cuda(), v[40:].cuda())
+    k2, v2 = rand(g, 3, 2, 128), rand(g, 3, 2, 128)
+    fill(kv, [f], [(k2, v2)])
+    for seq, wk, wv in ((s, k, v), (h, k, v), (f, torch.cat([k, k2]), torch.cat([v, v2]))):
+        gk, gv = read(kv, seq, 0, len(wk))
+        assert torch.equal(gk[0].double(), R.held(wk, dtype == I4)) and torch.equal(gv[0].double(), R.held(wv, dtype == I4))
+    kv.close()
+
+
+@pytest.mark.parametrize("dtype", [BF, I4])
+@pytest.mark.parametrize("D,Hq,H,page", [(128, 12, 2, 64), (64, 16, 16, 16), (128, 32, 2, 128)])
+def test_step_lengths_around_the_choice_of_parts(dtype, D, Hq, H, page):
+    """One part, two, and as many as fit, for one stream and for many."""
+    attend_case(dtype, D, Hq, H, page, [1100], [1])
+    attend_case(dtype, D, Hq, H, page, [9000], [1])
+    attend_case(dtype, D, Hq, H, page, [100 + 31 * i for i in range(40)], [1] * 40)
