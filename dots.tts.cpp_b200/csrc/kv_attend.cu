@@ -95,29 +95,48 @@ DTTS_DEV float merge_weight(float m, float top) { return m == -INFINITY ? 0.f : 
 
 // Joins the parts of `rows` rows (row stride D + 2 floats: O, m, l; part stride
 // `part` floats) and stores rows r -> out_of(r).  Parts are taken in order, so
-// the result does not depend on which CTA arrived last.
+// the result does not depend on which CTA arrived last.  Plain loads, which the fence
+// behind the counter orders, eight parts in flight at a time (one after another, a part
+// cost 0.28 us); eight dims a thread, so that 8 rows of 128 are one pass of 128 threads.
 template <int D, int N, typename OutOf>
 DTTS_DEV void kv_join_parts(const float *ws, long long part, int parts, int rows, OutOf out_of) {
+    constexpr int kBatch = 8;   // parts in flight at a time
     for (int e = threadIdx.x; e < rows * (D / 8); e += N) {
         const int r = e / (D / 8), c = e % (D / 8);
         const float *w = ws + (long long)r * (D + 2);
         float top = -INFINITY;
-        for (int s = 0; s < parts; s++) top = fmaxf(top, __ldcg(w + s * part + D));
+        for (int s0 = 0; s0 < parts; s0 += kBatch) {
+            float m[kBatch];
+#pragma unroll
+            for (int i = 0; i < kBatch; i++) m[i] = w[min(s0 + i, parts - 1) * part + D];
+#pragma unroll
+            for (int i = 0; i < kBatch; i++) top = fmaxf(top, m[i]);
+        }
         float l = 0.f, o[8];
 #pragma unroll
         for (int i = 0; i < 8; i++) o[i] = 0.f;
-        for (int s = 0; s < parts; s++) {
-            const float f = merge_weight(__ldcg(w + s * part + D), top);
-            l += f * __ldcg(w + s * part + D + 1);
+        for (int s0 = 0; s0 < parts; s0 += kBatch) {
+            float2 ml[kBatch], x[kBatch][4];
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const float2 x = __ldcg(reinterpret_cast<const float2 *>(w + s * part + 8 * c) + i);
-                o[2 * i] += f * x.x;
-                o[2 * i + 1] += f * x.y;
+            for (int i = 0; i < kBatch; i++) {
+                const float *p = w + min(s0 + i, parts - 1) * part;
+                ml[i] = *reinterpret_cast<const float2 *>(p + D);
+#pragma unroll
+                for (int j = 0; j < 4; j++) x[i][j] = reinterpret_cast<const float2 *>(p + 8 * c)[j];
             }
+#pragma unroll
+            for (int i = 0; i < kBatch; i++)
+                if (s0 + i < parts) {
+                    const float f = merge_weight(ml[i].x, top);
+                    l += f * ml[i].y;
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        o[2 * j] += f * x[i][j].x;
+                        o[2 * j + 1] += f * x[i][j].y;
+                    }
+                }
         }
         bf16 *dst = out_of(r);
-        if (!dst) continue;
         const float inv = 1.0f / l;   // l = 0: every score was -inf, and 0 * inf is the formula's NaN
         *reinterpret_cast<uint4 *>(dst + 8 * c) =
             make_uint4(pack_bf16x2(o[0] * inv, o[1] * inv), pack_bf16x2(o[2] * inv, o[3] * inv),
@@ -239,10 +258,11 @@ struct FewCfg {
 // bf16 terms (2^-17).
 // The running maximum m of a column is raised only when a score passes it by 2^8
 // (P <= 2^8 is as exact as P <= 1), so most tiles need no exchange between lanes.
-// Measured (12 query heads over 2 of 128): 32 sequences of 4097 .. 32768 4-bit rows 47.9 us, 3.55 TB/s of rows, bound
+// Measured (12 query heads over 2 of 128): 32 sequences of 4097 .. 32768 4-bit rows 45.8 us, 3.7 TB/s of rows, bound
 // by unpacking (52% of the issue slots, integer and half pipes at their rate); 64 of 1000 .. 8191 bf16 rows 54.5 us,
 // 5.5 TB/s, bound by DRAM; one of 48 rows 5.9 us, bound by latency.  4 warps of 64-key tiles and three CTAs an SM
-// hide the most: 8 warps of 32 keys and two CTAs measured 53.2 us for the first of these, 12 of 64 and one 49.7.
+// hide the most: 8 warps of 32 keys and two CTAs measured 53.2 us for the first of these, 12 of 64 and
+// one 49.7, when these took 47.9.
 template <int D, bool I4, int NT>
 __global__ void __launch_bounds__(FewCfg<D, I4>::kThreads, NT == 1 ? 3 : 1) kv_attend_few_kernel(const __grid_constant__ KvAttendArgs a) {
     using C = FewCfg<D, I4>;

@@ -583,8 +583,8 @@ int dtts_kv::plan_attend(const dtts_kv_attend_args &a, KvAttendPlan *plan) const
             }
         } else {
             // The number of parts of the longest range with the least time for all: the tiles of the warps that share
-            // an SM, and the join, 0.5 us and 0.28 more a part.  No split beats two halves for 64 sequences of 1000
-            // rows (12.0 against 14.7 us); one of 16000 takes 16.8 us in 16 parts, 18.5 in 32.
+            // an SM, and the join, 1.2 us and 0.16 more a part.  No split beats two halves for 64 sequences of 1000
+            // 4-bit rows (12.0 against 14.7 us); as many parts as fit take 37 us for one of 16000 bf16 rows, this 15.
             const int wide = max_rows > 8, resident = std::min(3, std::max(1, shapes.few_ctas[wide]));
             float best = INFINITY;
             // whether parts of len tiles fit on the SMs at once; they are kept where they take the least time so far
@@ -595,7 +595,7 @@ int dtts_kv::plan_attend(const dtts_kv_attend_args &a, KvAttendPlan *plan) const
                 const int w = shapes.few_warps;   // few tiles: the warp with one more counts
                 const float turns = len < 8 * w ? (float)((len + w - 1) / w) : (float)len / w;
                 const float us = turns * (float)c * shapes.few_tile_us[wide][at] +
-                                 shapes.few_start_us[at] + (n > 1 ? 0.5f + 0.28f * (float)n : 0.f);
+                                 shapes.few_start_us[at] + (n > 1 ? 1.2f + 0.16f * (float)n : 0.f);
                 if (us < best) {
                     best = us;
                     per = len;
