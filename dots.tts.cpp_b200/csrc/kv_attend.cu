@@ -253,9 +253,9 @@ struct FewCfg {
 // partial sums.  Pairs 1 and 3 of a word enter as 64 + n (1024 + 16 n against q /
 // 16), and the products' accumulators start at -72 sum of those q: the products
 // are exact and a group's sums stay within 80 s sum |q|.  V enters as the exact half
-// values c s; Q as half after an exact scaling by a power of two.  P is half (2^-12
-// relative, against 2^-9 of the bf16 output); with bf16 rows P is split into two
-// bf16 terms (2^-17).
+// values c s; Q as half after an exact scaling by a power of two.  P is half (2^-11
+// relative, against 2^-8 of the bf16 output); with bf16 rows P is split into two
+// bf16 terms (2^-16).
 // The running maximum m of a column is raised only when a score passes it by 2^8
 // (P <= 2^8 is as exact as P <= 1), so most tiles need no exchange between lanes.
 // Measured (12 query heads over 2 of 128): 32 sequences of 4097 .. 32768 4-bit rows 45.8 us, 3.7 TB/s of rows, bound
