@@ -533,14 +533,15 @@ struct dtts_llm {
         }
         DTTS_CHECK(M <= (1 << 24), DTTS_ERR_ARG, "%lld tokens in one call", M);
         DeviceGuard g(device);
+        int st = kv->not_capturing("extend");   // the cache's stream; the engine's below
+        if (st) return st;
         // the cache works on the engine's stream during the call; its own stream waits for what is enqueued here
         struct Streams {
             dtts_kv *kv;
             cudaStream_t back;
             ~Streams() { dtts_kv_set_stream(kv, back); }
         } streams{kv, kv->stream};
-        int st = dtts_kv_set_stream(kv, stream);
-        if (st || (st = kv->not_capturing("extend"))) return st;
+        if ((st = dtts_kv_set_stream(kv, stream)) || (st = kv->not_capturing("extend"))) return st;
         if ((st = ensure(M + 1))) return st;
         dtts_kv_attend_args aa;
         std::memset(&aa, 0, sizeof(aa));

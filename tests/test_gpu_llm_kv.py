@@ -172,3 +172,31 @@ def test_refusals_change_nothing(llm):
     assert kv.length(s) == 40
     assert np.isfinite(llm.extend(kv, [s], [1], x[:1], window=4)).all()
     kv.close()
+
+
+def test_capturing_streams_are_refused(weights):
+    """A call while the cache's stream or the engine's is capturing changes nothing."""
+    e = dtts.LLM(weights, n_layers=LAYERS, max_batch=1, max_seq=64)
+    kv = e.kv_cache(8, 2, 16)
+    s = kv.open()
+    x = emb_of("capture", 4, 1536)
+    e.extend(kv, [s], [2], x[:2])
+    st = torch.cuda.Stream()
+    y = torch.zeros(8, device="cuda")
+    for mine in (kv, e):
+        mine.set_stream(st.cuda_stream)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.stream(st):
+            with torch.cuda.graph(graph, stream=st, capture_error_mode="thread_local"):
+                y.add_(1)
+                with pytest.raises(dtts.DttsError) as err:
+                    e.extend(kv, [s], [1], x[2:3])
+        assert err.value.status == dtts.ERR_UNSUPPORTED and kv.length(s) == 2
+        graph.replay()
+        torch.cuda.synchronize()
+        mine.set_stream(None)
+    want = decoder(weights, x)
+    assert_bf16_close(e.extend(kv, [s], [2], x[2:]), want[2:], "after the refusals")
+    kv.close()
+    e.close()
