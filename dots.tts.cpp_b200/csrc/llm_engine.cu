@@ -519,7 +519,7 @@ struct dtts_llm {
     // The new tokens of a ragged batch over a paged cache.  A step (one token for
     // every sequence) is a graph: its kernels read lengths and tables on the device,
     // so one graph serves every step with the same batch size and split of the
-    // attention (rounded down to a power of two; a part holds at least 4 tiles).
+    // attention (rounded down to 2^n or 3 * 2^n; a part holds at least 4 tiles).
     int extend(dtts_kv *kv, int n_seq, const int *seqs, const int *n_new, const float *emb, int window, int sinks,
                float *hidden, int mem) {
         long long M = 0;
@@ -560,9 +560,10 @@ struct dtts_llm {
                                   mem == DTTS_MEM_HOST ? cudaMemcpyHostToDevice : cudaMemcpyDeviceToDevice, stream));
         if (step) {
             KvAttendArgs &p = plan.args[0];
-            int pow2 = 1;
-            while (2 * pow2 <= p.splits) pow2 *= 2;
-            const int splits = std::min(pow2, kv->max_splits(n_seq));
+            int round = 1;   // 1, 2, 3, 4, 6, 8, 12, ...
+            while (2 * round <= p.splits) round *= 2;
+            if (round / 2 * 3 <= p.splits && round > 1) round = round / 2 * 3;
+            const int splits = std::min(round, kv->max_splits(n_seq));
             cudaGraphExec_t exec = nullptr;
             for (Graph &g : graphs)
                 if (g.B == n_seq && g.uid == kv->uid && g.window == window && g.sinks == sinks && g.splits == splits)
