@@ -80,6 +80,13 @@ DTTS_DEV int kv_find_entry(const int *start, int n, int row) {
     return lo;
 }
 
+// Whether the batch has rows or entries beyond those that a launch was sized for (a
+// replayed graph meets the batch that is current then).
+DTTS_DEV bool kv_batch_over(const KvGeom &g, const KvMeta &m, int n_seq, int rows) {
+    const int beyond = n_seq < g.max_seqs ? m.cnt[n_seq] : 0;   // entries behind the batch hold no rows
+    return m.start[n_seq - 1] + m.cnt[n_seq - 1] > rows || beyond > 0;
+}
+
 // Quantises 8 packed bf16 values (a quarter of a group whose four lanes are
 // neighbours) to one word of nibbles; returns the group's scale through s16.  All
 // lanes of the warp take part.
@@ -189,6 +196,7 @@ struct KvAttendArgs {
     float scale_log2;                         // scale * log2(e)
     int window, sinks;
     int splits, tiles_per_split;              // parts of a long key range, key tiles a part should hold
+    int both;                                 // the other kernel (few rows, many rows) is launched too
     float *ws;                                // partial results
     int *cnt;                                 // arrivals per split unit, zero between calls
     int *err;

@@ -287,9 +287,13 @@ __global__ void __launch_bounds__(FewCfg<D, I4>::kThreads, NT == 1 ? 3 : 1) kv_a
     const int cnt = a.m.cnt[b], len = a.m.len[b], row0 = a.m.start[b], G = a.G;
     const int *trow = a.m.table + (long long)a.m.seq[b] * a.g.max_pages;
     const long long rows_ll = (long long)cnt * G;
-    if (rows_ll < 1 || rows_ll > kKvFewRows) return;   // none, or the other kernel's
-    const int rows = min((int)rows_ll, 8 * NT);
-    if ((long long)row0 + cnt > a.total_rows) return;
+    if (blockIdx.x == 0 && threadIdx.x == 0 && kv_batch_over(a.g, a.m, a.n_seq, a.total_rows)) atomicCAS(a.err, 0, DEVERR_BATCH);
+    // none, or the other kernel's; or rows that a replayed graph was not captured for
+    if (rows_ll < 1 || rows_ll > 8 * NT || (long long)row0 + cnt > a.total_rows) {
+        if (rows_ll > 8 * NT && !(a.both && rows_ll > kKvFewRows) && threadIdx.x == 0) atomicCAS(a.err, 0, DEVERR_BATCH);
+        return;
+    }
+    const int rows = (int)rows_ll;
     const int i0 = len - cnt;
     const KeyTiles kt(KT, i0, len, a.window, a.sinks);
     const int parts = min(a.splits, max(1, (kt.n + a.tiles_per_split - 1) / a.tiles_per_split));
@@ -1010,6 +1014,12 @@ __global__ void __launch_bounds__(512, 1) kv_attend_many_kernel(const __grid_con
     const int bh = u % (a.n_seq * a.g.H), pair = pairs - 1 - u / (a.n_seq * a.g.H);   // longest key ranges first
     const int unit = bh * pairs + pair;
     const ManyUnit mu(a, bh, pair);
+    if (split == 0 && pair == 0 && tid == 0) {   // rows that a replayed graph was not captured for
+        const long long all = (long long)mu.cnt * a.G;
+        if (all > 256ll * pairs || (all > 0 && all <= kKvFewRows && !a.both) ||
+            (bh == 0 && kv_batch_over(a.g, a.m, a.n_seq, a.total_rows)))
+            atomicCAS(a.err, 0, DEVERR_BATCH);
+    }
     if (!mu.on || split >= mu.parts) return;
     const int head = mu.head, len = mu.len, row0 = mu.row0, G = a.G, base = mu.base, rows = mu.rows, parts = mu.parts;
     const int tiles = rows > 128 ? 2 : 1, i0 = mu.i0, i_last = mu.i_last;

@@ -113,9 +113,10 @@ __global__ void __launch_bounds__(256) kv_write_kernel(const __grid_constant__ K
                                                        uint8_t *__restrict__ pool, int n_seq, int rows,
                                                        const bf16 *__restrict__ k, const bf16 *__restrict__ v,
                                                        long long k_row, long long k_head, long long v_row,
-                                                       long long v_head) {
+                                                       long long v_head, int *__restrict__ err) {
     pdl_wait();
     pdl_trigger();
+    if (blockIdx.x == gridDim.x - 1 && threadIdx.x == 0 && kv_batch_over(geom, m, n_seq, rows)) atomicCAS(err, 0, DEVERR_BATCH);
     const KvGeom g = fixed_geom<I4, D>(geom);
     constexpr int lpr = D / 4, step = 32 / lpr;   // lanes a (row, head): 32 or 16; items a warp and turn
     const int lane = threadIdx.x & 31, l = lane % lpr, w = l % (lpr / 2);
@@ -457,7 +458,8 @@ int dtts_kv::extend(int n_seq, const int *sq, const int *n_new) {
         poke(4 * g.max_seqs + b, pos);
         start += n_new[b];
     }
-    // entries behind the batch hold no rows (a graph captured for a larger batch finds nothing to do there)
+    // entries behind the batch hold no rows: row lookups of a graph captured for more entries stay in range, and
+    // kv_batch_over tells by them that there are more entries than at a capture
     for (int b = n_seq; b < g.max_seqs; b++) {
         poke(g.max_seqs + b, start);
         poke(2 * g.max_seqs + b, 0);
@@ -521,6 +523,7 @@ int dtts_kv::plan_attend(const dtts_kv_attend_args &a, KvAttendPlan *plan) const
             return DTTS_ERR_ARG;
         }
     plan->rows_or_pairs[0] = plan->rows_or_pairs[1] = 0;
+    plan->args[0].both = plan->args[1].both = 0;
     if (b_rows == 0) return DTTS_OK;
     DTTS_CHECK(a.q && a.out, DTTS_ERR_ARG, "null argument");
     DTTS_CHECK(aligned16(a.q) && aligned16(a.out) && !((a.q_row | a.q_head | a.out_row | a.out_head) & 7), DTTS_ERR_ARG,
@@ -618,6 +621,7 @@ int dtts_kv::plan_attend(const dtts_kv_attend_args &a, KvAttendPlan *plan) const
         plan->args[many] = p;
         plan->rows_or_pairs[many] = many ? rt : max_rows;
     }
+    plan->args[0].both = plan->args[1].both = plan->rows_or_pairs[0] && plan->rows_or_pairs[1];
     return DTTS_OK;
 }
 
@@ -744,6 +748,8 @@ int dtts_kv_sync(dtts_kv *kv) {
     DTTS_CUDA(cudaMemcpy(&err, kv->d_err, 4, cudaMemcpyDeviceToHost));
     if (err) {
         cudaMemset(kv->d_err, 0, 4);
+        DTTS_CHECK(err != DEVERR_BATCH, DTTS_ERR_ARG,
+                   "a replayed graph met a batch whose sequences have other numbers of new tokens than at its capture");
         set_error("device wait limit reached (code %d)", err);
         return DTTS_ERR_TIMEOUT;
     }
@@ -1004,7 +1010,7 @@ int dtts_kv_write(dtts_kv *kv, int layer, const void *k, const void *v, long lon
     auto write = [&](auto kernel) {
         return launch_k(kv_pdl(), kernel, dim3((unsigned)((items + per_block - 1) / per_block)), dim3(256), 0, kv->stream, g,
                         kv->kv_meta(), kv->pool + (long long)layer * g.H * g.seg, (int)kv->b_seq.size(), kv->b_rows,
-                        (const bf16 *)k, (const bf16 *)v, k_row, k_head, v_row, v_head);
+                        (const bf16 *)k, (const bf16 *)v, k_row, k_head, v_row, v_head, kv->d_err);
     };
     DTTS_CUDA(g.i4 ? (g.D == 128 ? write(kv_write_kernel<true, 128>) : write(kv_write_kernel<true, 64>))
                    : (g.D == 128 ? write(kv_write_kernel<false, 128>) : write(kv_write_kernel<false, 64>)));

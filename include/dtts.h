@@ -345,10 +345,13 @@ int dtts_pe_stream_length(dtts_pe *p, int *tokens);
  * projection) or come in any order.  Calls only enqueue work on the cache's stream (dtts_kv_sync
  * waits and reports device errors) and must be serialised by the caller, like an engine's.
  * dtts_kv_write, dtts_kv_attend and dtts_kv_read may be captured into a CUDA graph; a replay acts on
- * the batch that is current on the stream then (same number of sequences and new tokens as at the
- * capture, any lengths; the split of long key ranges over the GPU stays as it was sized at the
- * capture, so capture again when the sequences have grown much).  All work of a cache shares its workspace: replays of graphs captured from one
- * cache must not overlap with each other or with its calls.  The calls that change tables
+ * the batch that is current on the stream then: as many sequences as at the capture, each with as many
+ * new tokens as the one in its place had, of any lengths.  Rows that the captured launches do not reach
+ * (one sequence has more new tokens, or there are more sequences) are left as they were, and
+ * the next dtts_kv_sync returns DTTS_ERR_ARG.  Do not replay a graph after its batch has ended until the next
+ * dtts_kv_extend.  The split of long key ranges over the GPU stays as it was sized at the
+ * capture, so capture again when the sequences have grown much.  All work of a cache shares its
+ * workspace: replays of graphs captured from one cache must not overlap with each other or with its calls.  The calls that change tables
  * (extend, fork, compact) return DTTS_ERR_UNSUPPORTED while the stream is capturing.
  *
  * 4-bit rows (DTTS_DTYPE_INT4): for every 32 consecutive values x of a row (a token's head) one

@@ -715,3 +715,75 @@ def test_step_lengths_around_the_choice_of_parts(dtype, D, Hq, H, page):
     attend_case(dtype, D, Hq, H, page, [1100], [1])
     attend_case(dtype, D, Hq, H, page, [9000], [1])
     attend_case(dtype, D, Hq, H, page, [100 + 31 * i for i in range(40)], [1] * 40)
+
+
+def replay_of(kv, captured, then, dtype, seed):
+    """A graph of write + attend captured for a batch of `captured` new tokens a sequence, replayed for `then`; returns
+    what was stored and attended then."""
+    g = rng(seed)
+    seqs = [kv.open() for _ in range(max(len(captured), len(then)))]
+    base = [(rand(g, 20 + 7 * b, 2, 128), rand(g, 20 + 7 * b, 2, 128)) for b in range(len(seqs))]
+    fill(kv, seqs, base)
+    rows = max(sum(captured), sum(then))
+    k, v, q = rand(g, rows, 2, 128), rand(g, rows, 2, 128), rand(g, rows, 12, 128)
+    kd, vd, qd = k.cuda(), v.cuda(), q.cuda()
+    out = torch.full_like(qd, 7.0)
+    kv.extend(seqs[:len(captured)], captured)
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=torch.cuda.current_stream()):
+        kv.write(0, kd, vd)
+        kv.attend(0, qd, out)
+    for s, n in zip(seqs, base):
+        kv.truncate(s, len(n[0]))
+    kv.extend(seqs[:len(then)], then)
+    graph.replay()
+    torch.cuda.synchronize()
+    return seqs, base, k, v, q, out, graph
+
+
+@pytest.mark.parametrize("dtype", [BF, I4])
+@pytest.mark.parametrize("captured,then", [
+    ([1, 1, 1], [2, 1, 0]),       # 12 rows a key head where 6 were captured
+    ([15, 16], [1, 30]),          # a sequence of few rows where only long ones were
+    ([1, 2, 2], [5, 0, 0]),       # and the other way round
+    ([40, 40], [60, 20]),         # 360 rows where 256 were
+    ([1, 40], [30, 50]),          # more rows than the graph knows
+    ([1, 1], [1, 1, 1]), ([40], [40, 1]), ([3, 3], [3, 3, 3])])    # more sequences
+def test_a_replay_that_does_not_reach_its_batch_is_reported(dtype, captured, then):
+    """Rows that the captured launches do not cover are an error at the next sync, not old output; the cache works on."""
+    kv = make(dtype=dtype, n_pages=40)
+    seqs, base, k, v, q, out, graph = replay_of(kv, captured, then, dtype, 51)
+    with pytest.raises(dtts.DttsError) as e:
+        kv.sync()
+    assert e.value.status == dtts.ERR_ARG, e.value
+    kv.sync()                                          # reported once
+    kv.write(0, k.cuda(), v.cuda())                    # the batch is current still: eager calls serve it
+    kv.attend(0, q.cuda(), out)
+    kv.sync()
+    at = 0
+    for b, t in enumerate(then):
+        n = len(base[b][0]) + t
+        kk, vv = torch.cat([base[b][0], k[at:at + t]]), torch.cat([base[b][1], v[at:at + t]])
+        want, tol = R.attend(q[at:at + t], R.held(kk, dtype == I4), R.held(vv, dtype == I4), n - t, int4=dtype == I4)
+        R.assert_close(out[at:at + t], want, tol, f"sequence {b}")
+        at += t
+    del graph
+    kv.close()
+
+
+@pytest.mark.parametrize("dtype", [BF, I4])
+@pytest.mark.parametrize("news", [[1, 1, 1], [2, 1, 0], [40, 1, 2], [60], [43, 50]])
+def test_a_replay_of_the_same_counts_is_served(dtype, news):
+    kv = make(dtype=dtype, n_pages=40)
+    seqs, base, k, v, q, out, graph = replay_of(kv, news, news, dtype, 52)
+    kv.sync()
+    at = 0
+    for b, t in enumerate(news):
+        n = len(base[b][0]) + t
+        kk, vv = torch.cat([base[b][0], k[at:at + t]]), torch.cat([base[b][1], v[at:at + t]])
+        want, tol = R.attend(q[at:at + t], R.held(kk, dtype == I4), R.held(vv, dtype == I4), n - t, int4=dtype == I4)
+        R.assert_close(out[at:at + t], want, tol, f"sequence {b}")
+        at += t
+    del graph
+    kv.close()
