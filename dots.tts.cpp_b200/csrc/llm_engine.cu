@@ -354,8 +354,8 @@ struct dtts_llm {
         DTTS_CUDA(cudaStreamSynchronize(stream));
         drop_graphs();
         ws.free_all();
-        cap_tok = std::max<long long>(tok, 64);
-        const size_t T = (size_t)cap_tok;
+        cap_tok = 0;   // until all of it is there
+        const size_t T = (size_t)std::max<long long>(tok, 64);
         h = (float *)ws.alloc(T * kLH * 4);
         qkv = (float *)ws.alloc(T * kLQKV * 4);
         q = (float *)ws.alloc(T * kLH * 4);
@@ -363,11 +363,16 @@ struct dtts_llm {
         act = (bf16 *)ws.alloc(T * kLH * 2);
         ao = (bf16 *)ws.alloc(T * kLH * 2);
         ffn = (bf16 *)ws.alloc(T * kLF * 2);
-        DTTS_CHECK(h && qkv && q && gu && act && ao && ffn, DTTS_ERR_OOM, "LLM workspace allocation failed");
+        if (!(h && qkv && q && gu && act && ao && ffn)) {
+            ws.free_all();
+            set_error("LLM workspace allocation failed (%lld tokens)", tok);
+            return DTTS_ERR_OOM;
+        }
         bool ok = make_tmap_bf16(&t_act, act, T, kLH, 128) && make_tmap_bf16(&t_ao, ao, T, kLH, 128) &&
                   make_tmap_bf16(&t_ffn, ffn, T, kLF, 128) && make_tmap_f32_resid(&t_h, h, T, kLH) &&
                   make_tmap_f32_resid(&t_qkv_r, qkv, T, kLQKV) && make_tmap_f32_resid(&t_gu_r, gu, T, 2 * kLF);
         DTTS_CHECK(ok, DTTS_ERR_CUDA, "tensor map (LLM workspace)");
+        cap_tok = (long long)T;
         return DTTS_OK;
     }
 

@@ -52,7 +52,10 @@ struct DeviceArena {
     void *alloc(size_t n) {
         void *p = nullptr;
         if (n == 0) n = 16;
-        if (cudaMalloc(&p, n) != cudaSuccess) return nullptr;
+        if (cudaMalloc(&p, n) != cudaSuccess) {
+            cudaGetLastError();   // the caller reports it; it must not surface in a later call
+            return nullptr;
+        }
         ptrs.push_back(p);
         bytes += n;
         return p;

@@ -200,3 +200,31 @@ def test_capturing_streams_are_refused(weights):
     assert_bf16_close(e.extend(kv, [s], [2], x[2:]), want[2:], "after the refusals")
     kv.close()
     e.close()
+
+
+@pytest.mark.parametrize("dense", [False, True])
+def test_a_workspace_that_does_not_fit_leaves_the_engine_usable(weights, dense):
+    """1.7 million tokens need 198 GB of workspace (116224 bytes each), more than the device has, beside pages for
+    all of them; the next calls, above and below 256 tokens, work on a workspace of their own."""
+    n, rows = 416, 4096
+    e = dtts.LLM(weights, n_layers=LAYERS, max_batch=n if dense else 1, max_seq=rows)
+    kv = e.kv_cache(n * rows // 128, n, 128)
+    x = emb_of("fit", 303, 1536)
+    s = kv.open()
+    e.extend(kv, [s], [2], x[:2])                          # a small workspace is there before
+    seqs = [s] + [kv.open() for _ in range(n - 1)]
+    free, small = kv.free_pages(), torch.zeros(16, device="cuda")
+    counts = [rows - 2] + [rows] * (n - 1)
+    ps, pc = dtts._ints(seqs), dtts._ints(counts)
+    if dense:
+        st = dtts.lib().dtts_llm_prefill(e.h, small.data_ptr(), n, rows, small.data_ptr(), dtts.MEM_DEVICE)
+    else:
+        st = dtts.lib().dtts_llm_extend(e.h, kv.h, n, ps[1], pc[1], small.data_ptr(), 0, 0, small.data_ptr(), dtts.MEM_DEVICE)
+    assert st == dtts.ERR_OOM
+    assert [kv.length(q) for q in seqs] == [2] + [0] * (n - 1) and kv.free_pages() == free
+    want = decoder(weights, x)
+    assert_bf16_close(e.extend(kv, [s], [1], x[2:3]), want[2:3], "a step")
+    assert_bf16_close(e.extend(kv, [s], [299], x[3:302]), want[3:302], "a prompt")
+    assert_bf16_close(e.extend(kv, [s], [1], x[302:]), want[302:], "the next step")
+    kv.close()
+    e.close()
