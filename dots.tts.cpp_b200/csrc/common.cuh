@@ -154,6 +154,12 @@ DTTS_DEV bool mbar_wait(uint64_t *bar, uint32_t parity, volatile int *abort_flag
     }
 }
 
+// The same by a whole warp, one answer for all its lanes: near the limit, or when another role gives up, the lanes'
+// own answers differ, and lanes that went on alone would run warp-wide instructions without the others.
+DTTS_DEV bool mbar_wait_warp(uint64_t *bar, uint32_t parity, volatile int *abort_flag, int *err, int code) {
+    return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, err, code)) != 0;
+}
+
 // --------------------------------------------------------------------- TMA
 // 2-D tiled load of box (x = inner/K coordinate, y = row) into shared memory,
 // completing on `bar`.  x is always a multiple of 64 bf16 (128 bytes).

@@ -643,7 +643,7 @@ __global__ void __launch_bounds__(FewCfg<D, I4>::kThreads, NT == 1 ? 3 : 1) kv_a
     };
     for (int it = 0, stage = 0, ph = 0; it < n_mine; it++) {
         const int j0 = tile_row(it);
-        if (!mbar_wait(bar + stage, ph, abort_flag, a.err, DEVERR_TIMEOUT_PRODUCER)) break;
+        if (!mbar_wait_warp(bar + stage, ph, abort_flag, a.err, DEVERR_TIMEOUT_PRODUCER)) break;
         const uint8_t *sT = ring + stage * C::kStage;
         if (j0 + KT - 1 <= i0 && (a.window == 0 || j0 > len - 1 - a.window || j0 + KT - 1 < a.sinks))
             tile(std::true_type{}, sT, j0);
@@ -657,13 +657,14 @@ __global__ void __launch_bounds__(FewCfg<D, I4>::kThreads, NT == 1 ? 3 : 1) kv_a
         if (++stage == C::kStages) { stage = 0; ph ^= 1; }
     }
     // a wait that ran out: let this warp's copies land before the rings are reused
-    if (*abort_flag) {
+    if (__any_sync(0xffffffffu, *abort_flag != 0)) {
         const unsigned long long t0 = globaltimer_ns();
         for (int s = 0; s < C::kStages && s < n_mine; s++) {
             const int last = (n_mine - 1 - s) / C::kStages;   // phases of this stage, if all were issued
             for (int ph = 0; ph <= last; ph++)
                 while (!mbar_try_wait(bar + s, ph & 1) && globaltimer_ns() - t0 < kWaitLimitNs / 4) {}
         }
+        __syncwarp();
     }
 
     // ---- join the warps: rows of D + 2 floats (O, m, l) a warp

@@ -30,6 +30,35 @@ __global__ void wait_limit_selftest_kernel(int *err) {
     if (threadIdx.x == 0) (void)mbar_wait(&bar, 0, &abort_flag, err, DEVERR_TIMEOUT_PRODUCER);
     __syncthreads();
 }
+
+// A warp whose lanes' own waits end differently: the even lanes' barrier has completed its first phase, the odd
+// lanes' has not (open) or has too, and another role has given up.  answers: the lanes for which the warp's wait, then
+// the lane's own, succeeded; sum: of the lane numbers, over all lanes behind the wait.
+__global__ void warp_wait_selftest_kernel(int open, unsigned *answers, int *sum, int *err) {
+    __shared__ uint64_t bars[2];
+    __shared__ int abort_flag;
+    const int lane = threadIdx.x;
+    if (lane == 0) {
+        mbar_init(bars, 1);
+        mbar_init(bars + 1, 1);
+        abort_flag = 1;
+        fence_mbar_init();
+        mbar_arrive(bars);
+        if (!open) mbar_arrive(bars + 1);
+    }
+    __syncwarp();
+    const bool own = mbar_wait(bars + (lane & 1), 0, &abort_flag, err, DEVERR_TIMEOUT_PRODUCER);
+    __syncwarp();
+    const bool all = mbar_wait_warp(bars + (lane & 1), 0, &abort_flag, err, DEVERR_TIMEOUT_PRODUCER);
+    const unsigned a = __ballot_sync(0xffffffffu, all), o = __ballot_sync(0xffffffffu, own);
+    int x = lane;
+    for (int d = 16; d; d >>= 1) x += __shfl_xor_sync(0xffffffffu, x, d);
+    if (lane == 0) {
+        answers[0] = a;
+        answers[1] = o;
+        *sum = x;
+    }
+}
 }  // namespace
 
 extern "C" {
@@ -234,6 +263,25 @@ int dtts_selftest_wait_limit(int device, int *code) {
         set_error("device wait limit reached (code %d)", *code);
         return DTTS_ERR_TIMEOUT;
     }
+    return DTTS_OK;
+}
+
+int dtts_selftest_warp_wait(int open, unsigned *warp_lanes, unsigned *own_lanes, int device) {
+    DTTS_CHECK(warp_lanes && own_lanes, DTTS_ERR_ARG, "null argument");
+    int nsm = 0, st = check_device(device, &nsm);
+    if (st) return st;
+    DeviceGuard g(device);
+    Scratch s;
+    int *d = (int *)s.a.alloc(16), h[4] = {0, 0, 0, 0};
+    DTTS_CHECK(d, DTTS_ERR_OOM, "cudaMalloc failed");
+    DTTS_CUDA(cudaMemset(d, 0, 16));
+    warp_wait_selftest_kernel<<<1, 32>>>(open, (unsigned *)d, d + 2, d + 3);
+    DTTS_CUDA(cudaGetLastError());
+    if ((st = stream_wait(0, 30.0))) return st;
+    DTTS_CUDA(cudaMemcpy(h, d, 16, cudaMemcpyDeviceToHost));
+    DTTS_CHECK(h[2] == 496 && h[3] == 0, DTTS_ERR_CUDA, "lanes sum to %d, error word %d", h[2], h[3]);
+    *warp_lanes = (unsigned)h[0];
+    *own_lanes = (unsigned)h[1];
     return DTTS_OK;
 }
 

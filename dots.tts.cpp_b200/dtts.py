@@ -119,7 +119,7 @@ EXPORTS = [
     "dtts_kv_fork", "dtts_kv_truncate", "dtts_kv_trim", "dtts_kv_compact", "dtts_kv_length", "dtts_kv_free_pages",
     "dtts_kv_extend", "dtts_kv_write", "dtts_kv_attend", "dtts_kv_read",
     "dtts_voc_create", "dtts_voc_destroy", "dtts_voc_set_stream", "dtts_voc_decode", "dtts_voc_aa_filter",
-    "dtts_selftest_voc_activation", "dtts_selftest_wait_limit", "dtts_selftest_conv", "dtts_attn_create", "dtts_attn_destroy", "dtts_attn_forward",
+    "dtts_selftest_voc_activation", "dtts_selftest_wait_limit", "dtts_selftest_warp_wait", "dtts_selftest_conv", "dtts_attn_create", "dtts_attn_destroy", "dtts_attn_forward",
     "dtts_attn_profile_core", "dtts_attn_forward_f32_noalloc", "dtts_pe_create", "dtts_pe_create_from_safetensors", "dtts_pe_destroy",
     "dtts_pe_set_stream", "dtts_pe_sync", "dtts_pe_forward", "dtts_pe_stream_reset", "dtts_pe_decode",
     "dtts_pe_stream_length", "dtts_selftest_gemm", "dtts_selftest_attention", "dtts_selftest_e4m3",
@@ -257,6 +257,7 @@ def lib(path: str = LIB_PATH):
     L.dtts_voc_aa_filter.argtypes = [_fp]
     L.dtts_selftest_voc_activation.argtypes = [_fp, C.c_int, C.c_int, _fp, _fp, _fp, _fp, C.c_int, _fp]
     L.dtts_selftest_wait_limit.argtypes = [C.c_int, C.POINTER(C.c_int)]
+    L.dtts_selftest_warp_wait.argtypes = [C.c_int, C.POINTER(C.c_uint), C.POINTER(C.c_uint), C.c_int]
     L.dtts_selftest_conv.argtypes = [_fp, C.c_int, C.c_int, _fp, _fp, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int,
                                      _fp, C.c_int]
     L.dtts_selftest_e4m3.argtypes = [_fp, _u8p, C.c_int, C.c_int]
@@ -834,6 +835,13 @@ def selftest_wait_limit(device=0):
     code = C.c_int()
     st = lib().dtts_selftest_wait_limit(device, C.byref(code))
     return st, code.value
+
+
+def selftest_warp_wait(open, device=0):
+    """(lanes the warp's bounded wait succeeds for, lanes whose own does), as bits."""
+    w, o = C.c_uint(), C.c_uint()
+    check(lib().dtts_selftest_warp_wait(int(open), C.byref(w), C.byref(o), device))
+    return w.value, o.value
 
 
 def selftest_conv(x, w, bias=None, dil=1, pad_left=None, bn=64, device=0):

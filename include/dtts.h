@@ -499,6 +499,10 @@ int dtts_selftest_voc_activation(const float *x, int len, int ch, const float *a
  * %globaltimer); it must give up, leave its code in *code (1: producer wait) and
  * return DTTS_ERR_TIMEOUT with the context still usable. */
 int dtts_selftest_wait_limit(int device, int *code);
+/* The bounded wait of a whole warp, while another role has given up: the even lanes wait on a barrier that is
+ * complete, the odd lanes on one that is (open = 0) or is not.  *own_lanes: the lanes whose own wait succeeds,
+ * *warp_lanes: those for which the warp's does; all or none. */
+int dtts_selftest_warp_wait(int open, unsigned *warp_lanes, unsigned *own_lanes, int device);
 /* A time convolution through the tcgen05 GEMM over taps, as the vocoder runs it:
  * out[t][o] = bias[o] + sum_k sum_c x[t + k dil - pad_left][c] w[o][c][k] (zero outside
  * [0, T)); x [T][C], w [N][C][K], inputs rounded to bf16; C % 64 == 0, bn | N. */

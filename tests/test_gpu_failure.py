@@ -26,3 +26,12 @@ def test_device_wait_limit_reports_and_context_survives():
     got = dtts.selftest_gemm(A, B)
     want = bf16(A).astype(np.float64) @ bf16(B).astype(np.float64).T
     assert rel(got, want) <= 1e-5
+
+
+def test_a_warp_gives_up_as_one():
+    """Where some lanes of a warp see their barrier complete and others see that the kernel has given up, all of them
+    get the same answer: lanes that went on alone would run warp-wide instructions without the rest."""
+    warp, own = dtts.selftest_warp_wait(open=True)
+    assert own == 0x55555555 and warp == 0
+    warp, own = dtts.selftest_warp_wait(open=False)
+    assert own == warp == 0xffffffff
