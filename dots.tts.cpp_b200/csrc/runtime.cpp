@@ -26,6 +26,7 @@ void set_error(const char *fmt, ...) {
 const char *last_error() { return g_err; }
 
 int cuda_status(cudaError_t e, const char *what) {
+    cudaGetLastError();   // reported here; a later call's check must not find it again
     set_error("%s: %s (%s)", what, cudaGetErrorName(e), cudaGetErrorString(e));
     if (e == cudaErrorMemoryAllocation) return DTTS_ERR_OOM;
     if (e == cudaErrorNoDevice || e == cudaErrorInvalidDevice || e == cudaErrorInsufficientDriver)

@@ -5,6 +5,7 @@ weights, several sequences prefilled together and stepped together; bf16 bar
 on the final-normed hidden states."""
 import numpy as np
 import pytest
+import torch
 
 import dtts
 import synth
@@ -51,4 +52,21 @@ def test_cache_capacity_is_checked(weights):
     llm.prefill(synth.normal(7, "llm.c", (1, 4, 1536), 1.0))
     with pytest.raises(dtts.DttsError):
         llm.step(synth.normal(7, "llm.c2", (1, 1536), 1.0))
+    llm.close()
+
+
+def test_an_error_is_reported_once(weights):
+    """The legacy default stream (handle 1) cannot be captured, so a step on it is an error; the next calls work."""
+    prompts = synth.normal(6, "llm.p3", (2, 6, 1536), 1.0)
+    llm = dtts.LLM(weights, n_layers=2, max_batch=2, max_seq=32)
+    full = llm.prefill(prompts)
+    llm.prefill(prompts[:, :4])
+    llm.set_stream(1)
+    with pytest.raises(dtts.DttsError) as e:
+        llm.step(prompts[:, 4])
+    assert e.value.status == dtts.ERR_CUDA and llm.length() == 4
+    torch.cuda.synchronize()
+    llm.set_stream(None)
+    for i in (4, 5):
+        assert_bf16_close(llm.step(prompts[:, i]), full[:, i], f"token {i}")
     llm.close()
