@@ -394,17 +394,14 @@ int dtts_kv::not_capturing(const char *what) const {
     return DTTS_OK;
 }
 
-// Grows the sequences and makes them the current batch.  Nothing changes unless
-// everything fits.
-int dtts_kv::extend(int n_seq, const int *sq, const int *n_new) {
-    int st = not_capturing("extend");
-    if (st) return st;
+int dtts_kv::fits(int n_seq, const int *sq, const int *n_new, long long *pages) {
     std::vector<int> listed(sq, sq + n_seq);
     std::sort(listed.begin(), listed.end());
     DTTS_CHECK(std::adjacent_find(listed.begin(), listed.end()) == listed.end(), DTTS_ERR_ARG,
                "a sequence is listed twice");
     long long need = 0, rows = 0;
     std::vector<int> lowered;   // shared tail pages counted as copied
+    lowered.reserve(n_seq);
     for (int b = 0; b < n_seq; b++) {
         const Seq &s = seqs[sq[b]];
         const long long len = (long long)s.len + n_new[b];
@@ -425,24 +422,63 @@ int dtts_kv::extend(int n_seq, const int *sq, const int *n_new) {
     DTTS_CHECK(rows <= INT32_MAX / 2, DTTS_ERR_ARG, "%lld new rows in one batch", rows);
     DTTS_CHECK(need <= (long long)free_pages.size(), DTTS_ERR_OOM, "%lld pages needed, %zu free", need,
                free_pages.size());
-    struct Copy {
-        int src, dst, rows;
-    };
+    *pages = need;
+    return DTTS_OK;
+}
+
+void dtts_kv::take_back() {
+    for (auto x = grown.rbegin(); x != grown.rend(); ++x) {
+        Seq &s = seqs[x->seq];
+        for (; (int)s.pages.size() > x->pages; s.pages.pop_back()) drop_page(s.pages.back());
+        if (x->tail >= 0) {
+            drop_page(s.pages.back());
+            s.pages.back() = x->tail;
+            refs[x->tail]++;
+            poke(table_at(x->seq, x->pages - 1), x->tail);
+        }
+        s.len = x->len;
+        s.pos = x->pos;
+    }
+    grown.clear();
+    drop_batch();
+}
+
+// Grows the sequences and makes them the current batch.  Nothing changes unless
+// everything fits and every launch succeeds.
+int dtts_kv::extend(int n_seq, const int *sq, const int *n_new) {
+    long long need = 0;
+    int st = not_capturing("extend");
+    if (st || (st = fits(n_seq, sq, n_new, &need))) return st;
+    // room for all that is listed below first: from the first change on, nothing throws
     std::vector<Copy> copies;
+    copies.reserve(n_seq);
+    grown.clear();
+    grown.reserve(n_seq);
+    pokes.reserve(pokes.size() + (size_t)need + 5 * (size_t)g.max_seqs + 2 * (size_t)n_seq);   // also take_back's
+    for (int b = 0; b < n_seq; b++) {
+        Seq &s = seqs[sq[b]];
+        const size_t pages = (size_t)((s.len + (long long)n_new[b] + g.P - 1) / g.P);
+        if (pages > s.pages.capacity()) s.pages.reserve(std::max(pages, 2 * s.pages.size()));
+    }
+    b_seq.reserve(n_seq);
+    b_cnt.reserve(n_seq);
+    b_len.reserve(n_seq);
     b_seq.assign(sq, sq + n_seq);
     b_cnt.assign(n_new, n_new + n_seq);
     b_len.resize(n_seq);
-    b_rows = (int)rows;
     int start = 0;
     for (int b = 0; b < n_seq; b++) {
         Seq &s = seqs[sq[b]];
+        Growth was = {sq[b], s.len, s.pos, (int)s.pages.size(), -1};
         if (n_new[b] > 0 && (s.len & (g.P - 1)) && refs[s.pages.back()] > 1) {
             const int from = s.pages.back(), to = take_page();
             refs[from]--;   // shared: never the last user here
             s.pages.back() = to;
+            was.tail = from;
             poke(table_at(sq[b], (int)s.pages.size() - 1), to);
             copies.push_back({from, to, s.len & (g.P - 1)});
         }
+        grown.push_back(was);
         const int pos = s.pos;
         s.len += n_new[b];
         s.pos += n_new[b];
@@ -458,12 +494,20 @@ int dtts_kv::extend(int n_seq, const int *sq, const int *n_new) {
         poke(4 * g.max_seqs + b, pos);
         start += n_new[b];
     }
+    b_rows = start;
     // entries behind the batch hold no rows: row lookups of a graph captured for more entries stay in range, and
     // kv_batch_over tells by them that there are more entries than at a capture
     for (int b = n_seq; b < g.max_seqs; b++) {
         poke(g.max_seqs + b, start);
         poke(2 * g.max_seqs + b, 0);
     }
+    if ((st = send_growth(copies))) take_back();
+    return st;
+}
+
+// Enqueues the copies of shared last pages and the pending metadata updates.
+int dtts_kv::send_growth(const std::vector<Copy> &copies) {
+    int st = DTTS_OK;
     Pokes<60> own;   // sent with the first copies
     own.n = 0;
     if (!copies.empty() && pokes.size() <= 60) take_pokes(own, 0);

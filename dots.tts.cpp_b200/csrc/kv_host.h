@@ -55,6 +55,10 @@ struct dtts_kv {
     template <typename P>
     void take_pokes(P &p, size_t i) const;
     int flush();                          // enqueues the pending metadata updates
+    struct Copy {
+        int src, dst, rows;               // pages, rows in use
+    };
+    int send_growth(const std::vector<Copy> &copies);
     int take_page() {
         const int p = free_pages.top();
         free_pages.pop();
@@ -67,7 +71,15 @@ struct dtts_kv {
     void drop_batch();
     int not_capturing(const char *what) const;
     int check_batch(int n_seq, const int *sq, const int *n_new) const;
+    // What the last extend() changed of a sequence: its state before, and the shared last page that a copy replaced
+    struct Growth {
+        int seq, len, pos, pages, tail;   // tail: -1 where none was replaced
+    };
+    std::vector<Growth> grown;
+    // Whether extend() would find everything it needs; *pages: how many it takes. Changes nothing.
+    int fits(int n_seq, const int *sq, const int *n_new, long long *pages);
     int extend(int n_seq, const int *sq, const int *n_new);
+    void take_back();                     // undoes the last extend(), before any other change; the batch ends
     // Whether attention of n_new[b] further tokens would reach rows that a trim freed.
     int check_window(int n_seq, const int *sq, const int *n_new, int window, int sinks) const;
     int max_splits(int n_seq) const;      // of the few-row kernel, for the workspace

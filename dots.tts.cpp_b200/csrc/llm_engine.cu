@@ -547,7 +547,27 @@ struct dtts_llm {
             ~Streams() { dtts_kv_set_stream(kv, back); }
         } streams{kv, kv->stream};
         if ((st = dtts_kv_set_stream(kv, stream)) || (st = kv->not_capturing("extend"))) return st;
+        // what can be refused first: neither the workspace nor the cache changes for a request that does not fit
+        long long pages = 0;
+        if ((st = kv->check_window(n_seq, seqs, n_new, window, sinks))) return st;
+        if ((st = kv->fits(n_seq, seqs, n_new, &pages))) return st;
         if ((st = ensure(M + 1))) return st;
+        if ((st = kv->extend(n_seq, seqs, n_new))) return st;
+        if (M == 0) return DTTS_OK;
+        try {
+            st = forward(kv, n_seq, emb, window, sinks, hidden, mem, step);
+        } catch (const std::bad_alloc &) {
+            kv->take_back();
+            throw;
+        }
+        if (st) kv->take_back();
+        return st;
+    }
+
+    // The decoder on the batch that kv->extend has just made.
+    int forward(dtts_kv *kv, int n_seq, const float *emb, int window, int sinks, float *hidden, int mem, bool step) {
+        int st;
+        const long long M = kv->b_rows;
         dtts_kv_attend_args aa;
         std::memset(&aa, 0, sizeof(aa));
         aa.q = q; aa.q_row = kLH; aa.q_head = kLHD;
@@ -555,9 +575,6 @@ struct dtts_llm {
         aa.n_heads = kLNH;
         aa.scale = 1.0f / sqrtf((float)kLHD);
         aa.window = window; aa.sinks = sinks;
-        if ((st = kv->check_window(n_seq, seqs, n_new, window, sinks))) return st;
-        if ((st = kv->extend(n_seq, seqs, n_new))) return st;
-        if (M == 0) return DTTS_OK;
         KvAttendPlan plan;
         if ((st = kv->plan_attend(aa, &plan))) return st;
         float *outd = qkv;
@@ -580,6 +597,7 @@ struct dtts_llm {
                     DTTS_CUDA(cudaStreamSynchronize(stream));
                     drop_graphs();
                 }
+                graphs.reserve(graphs.size() + 1);
                 if ((st = capture(&exec, [&] { return enqueue(n_seq, 1, 0, false, outd, kv, &plan); }))) return st;
                 graphs.push_back({n_seq, kv->uid, window, sinks, splits, exec});
             }

@@ -449,7 +449,8 @@ int dtts_llm_length(dtts_llm *e, int *tokens);
  * sinks of dtts_kv_attend_args; token positions continue from the sequence's position.  K and V are rounded
  * to bf16 (and then, in a 4-bit cache, to 4 bits), q to bf16.  dtts_llm_kv_create makes a cache of the
  * engine's geometry for sequences of up to max_seq tokens; the call works on the engine's stream, before which
- * the work already enqueued on the cache's stream comes, and the cache's stream waits for it. */
+ * the work already enqueued on the cache's stream comes, and the cache's stream waits for it.  An error leaves the
+ * sequences and pages as they were; where it comes up behind the checks of the request, the cache's batch has ended. */
 int dtts_llm_kv_create(dtts_llm *e, int n_pages, int max_seqs, int page_tokens, int dtype, dtts_kv **out);
 int dtts_llm_extend(dtts_llm *e, dtts_kv *kv, int n_seq, const int *seqs, const int *n_new, const float *emb,
                     int window, int sinks, float *hidden, int mem);

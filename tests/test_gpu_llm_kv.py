@@ -228,3 +228,37 @@ def test_a_workspace_that_does_not_fit_leaves_the_engine_usable(weights, dense):
     assert_bf16_close(e.extend(kv, [s], [1], x[302:]), want[302:], "the next step")
     kv.close()
     e.close()
+
+
+def test_an_error_behind_the_growth_takes_it_back(weights):
+    """A step on the legacy default stream fails where it would be captured: lengths, positions, pages (a fork's shared
+    one among them) and the rows are as they were, and the batch is over."""
+    e = dtts.LLM(weights, n_layers=LAYERS, max_batch=1, max_seq=128)
+    kv = e.kv_cache(12, 4, 16)
+    x, y = emb_of("back", 45, 1536), emb_of("back2", 45, 1536)
+    a, b = kv.open(), kv.open()
+    e.extend(kv, [a, b], [40, 16], np.concatenate([x[:40], y[:16]]))
+    (f,) = kv.fork(a)
+    free = kv.free_pages()
+    assert free == 12 - 4
+    for _ in range(2):
+        torch.cuda.synchronize()
+        e.set_stream(1)
+        with pytest.raises(dtts.DttsError) as err:
+            e.extend(kv, [f, b, a], [1, 1, 1], np.stack([x[40], y[16], x[40]]))
+        torch.cuda.synchronize()
+        e.set_stream(None)
+        assert err.value.status == dtts.ERR_CUDA
+        assert [kv.length(s) for s in (a, b, f)] == [kv.position(s) for s in (a, b, f)] == [40, 16, 40]
+        assert kv.free_pages() == free
+        with pytest.raises(dtts.DttsError):        # no batch is current
+            kv.write(0, torch.zeros(3, 2, 128, dtype=torch.bfloat16, device="cuda"),
+                     torch.zeros(3, 2, 128, dtype=torch.bfloat16, device="cuda"))
+    out = [e.extend(kv, [f, b, a], [1, 1, 1], np.stack([y[i - 24], y[i - 24], x[i]])) for i in (40, 41, 42)]
+    assert_bf16_close(np.stack([o[2] for o in out]), decoder(weights, x[:43])[40:], "the source")
+    assert_bf16_close(np.stack([o[1] for o in out]), decoder(weights, y[:19])[16:], "the other stream")
+    assert_bf16_close(np.stack([o[0] for o in out]), decoder(weights, np.concatenate([x[:40], y[16:19]]))[40:], "the fork")
+    kv.close_seqs([a, b, f])
+    assert kv.free_pages() == 12
+    kv.close()
+    e.close()
