@@ -224,6 +224,10 @@ DTTS_DEV void unpack_nibbles(uint32_t w, const NibbleMasks &k, __half2 (&h)[4]) 
     h[3] = __hfma2(h[3], sixteenth, k72);
 }
 
+// The largest exponent of the scaling of queries against 4-bit rows: 2^126 and 2^-126 are both normal.  It holds for
+// rows below 2^-111; a bf16 number is a multiple of 2^-133, so their values become multiples of 2^-7, as halves exact.
+constexpr int kMaxUp = 126;
+
 // Row of a 16-row block that row k of a fragment stands for: adjacent k have rows
 // of different parity, and {k = 0, 2, 4, 6}, {1, 3, 5, 7} all four residues mod 4.
 __host__ __device__ constexpr int frag_row(int k) { return (k & 8) | ((k & 7) < 4 ? (k & 7) : (k & 7) ^ 1); }
@@ -369,7 +373,7 @@ __global__ void __launch_bounds__(FewCfg<D, I4>::kThreads, NT == 1 ? 3 : 1) kv_a
             top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
             top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
             const int ex = (int)(top >> 7);   // biased exponent; 0: zeros and subnormals, 255: inf or NaN
-            const int sh = ex == 255 ? 0 : min(14 + 127 - ex, 100);
+            const int sh = ex == 255 ? 0 : min(14 + 127 - ex, kMaxUp);
             const float up = __uint_as_float((uint32_t)(sh + 127) << 23);
 #pragma unroll
             for (int j = 0; j < NG; j++) {
@@ -1299,7 +1303,7 @@ __global__ void __launch_bounds__(512, 1) kv_attend_many_kernel(const __grid_con
                         for (int y = 0; y < 4; y++) top = max(top, max(e[y] & 0x7fffu, (e[y] >> 16) & 0x7fffu));
 #pragma unroll
                         for (int y = 1; y < NU; y <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, y));
-                        const int ex = (int)(top >> 7), sh = ex == 255 ? 0 : min(14 + 127 - ex, 100);
+                        const int ex = (int)(top >> 7), sh = ex == 255 ? 0 : min(14 + 127 - ex, kMaxUp);
                         const float up = __uint_as_float((uint32_t)(sh + 127) << 23);
                         float f[8];
 #pragma unroll

@@ -787,3 +787,28 @@ def test_a_replay_of_the_same_counts_is_served(dtype, news):
         at += t
     del graph
     kv.close()
+
+
+@pytest.mark.parametrize("t", [1, 30])
+@pytest.mark.parametrize("exponent", [-126, -122, -118, -112, -100])
+def test_tiny_queries_with_a_large_scale(t, exponent):
+    """Queries near the smallest bf16 numbers, brought back by the scale: 4-bit rows take them as halves after an exact
+    scaling, which has to reach half's normal range.  All dims pull the same way, so a rounding of q shows."""
+    g = rng(61)
+    n = 300
+    kv = make(dtype=I4)
+    s = kv.open()
+    sign = torch.where(torch.rand(2, 128, generator=g) < 0.5, -1.0, 1.0)
+    k = (sign * (torch.rand(n, 2, 1, generator=g) * 2 - 1) * 2.0 ** 15).to(torch.bfloat16)
+    v = rand(g, n, 2, 128)
+    size = 1.0 + torch.randint(0, 128, (t, 12, 1), generator=g) / 128     # 8 significant bits
+    q = (sign.repeat_interleave(6, 0) * size * 2.0 ** exponent).to(torch.bfloat16)
+    scale = float(np.float32(min(1e30, 2.0 ** (-exponent - 22))))           # scores up to 2 or so
+    fill(kv, [s], [(k[:n - t], v[:n - t])])
+    fill(kv, [s], [(k[n - t:], v[n - t:])])
+    out = torch.empty(t, 12, 128, dtype=torch.bfloat16, device="cuda")
+    kv.attend(0, q.cuda(), out, scale=scale)
+    kv.sync()
+    want, tol = R.attend(q, R.held(k, True), R.held(v, True), n - t, scale=scale)
+    R.assert_close(out, want, tol)
+    kv.close()
