@@ -532,8 +532,24 @@ def _ints(a):
     if isinstance(a, (list, tuple)):      # 16 entries: a third of the time of a ctypes array, a half of numpy's
         c = array("i", a)
         return (c, *c.buffer_info())
+    a = np.asarray(a)
+    if a.size and (a.dtype.kind not in "iu" or a.min() < -2 ** 31 or a.max() >= 2 ** 31):
+        raise ValueError("32-bit integers expected")
     a = np.ascontiguousarray(a, np.int32).ravel()
     return a, a.ctypes.data, a.size
+
+
+def _rows_f32(a, shape, device, what):
+    """Checks a dense fp32 buffer: of the device with this number, or host memory (None)."""
+    if tuple(a.shape) != shape:
+        raise ValueError(f"{what}: {list(shape)} expected, not {list(a.shape)}")
+    if hasattr(a, "data_ptr"):
+        ok = str(a.dtype) == "torch.float32" and a.is_contiguous() and \
+            (a.device.type == "cpu" if device is None else a.is_cuda and a.get_device() == device)
+    else:
+        ok = device is None and a.dtype == np.float32 and a.flags.c_contiguous and a.flags.writeable
+    if not ok:
+        raise ValueError(f"{what}: dense fp32 " + ("host memory" if device is None else f"on device {device}") + " expected")
 
 
 class KVCache:
@@ -750,8 +766,8 @@ class LLM:
             emb = _f32(emb)
             out = np.zeros_like(emb) if out is None else out
         rows = int(sum(c))
-        if tuple(emb.shape) != (rows, 1536) or tuple(out.shape) != (rows, 1536):
-            raise ValueError(f"emb and out: [{rows}][1536] expected")
+        for x, what in ((emb, "emb"), (out, "out")):
+            _rows_f32(x, (rows, 1536), self.device if mem == MEM_DEVICE else None, what)
         kv._rows = max(kv._rows, rows)   # an error may leave either batch
         check(lib().dtts_llm_extend(self.h, kv.h, n, ps, pc, _addr(emb), window, sinks, _addr(out), mem))
         kv._rows = rows

@@ -2,6 +2,7 @@
 definition of 4-bit rows the GPU tests rely on."""
 import ctypes as C
 
+import numpy as np
 import pytest
 import torch
 
@@ -82,3 +83,48 @@ def test_host_tensors_and_other_types_are_refused():
         kv.read(0, [0], [0], [2], torch.zeros(1, 2, 2, 64), torch.zeros(1, 2, 2, 64))
     with pytest.raises(ValueError):
         kv.extend([0, 1], [1])
+
+
+def _llm_and_cache():
+    kv = dtts.KVCache.__new__(dtts.KVCache)
+    kv._init(None, 1, 2, 128, 0)
+    e = dtts.LLM.__new__(dtts.LLM)
+    e.h, e.device, e.n_layers = None, 0, 1
+    return e, kv
+
+
+@pytest.mark.parametrize("mem", [dtts.MEM_HOST, dtts.MEM_DEVICE])
+def test_decoder_buffers_of_another_kind_are_refused(dtts_mod, mem):
+    """The library writes rows x 1536 floats to out: a buffer that does not hold them is refused before the call."""
+    e, kv = _llm_and_cache()
+    emb = np.zeros((3, 1536), np.float32)
+    frozen = np.zeros((3, 1536), np.float32)
+    frozen.flags.writeable = False
+    bad = [np.zeros((3, 1536), t) for t in (np.float16, np.float64, np.int8)]
+    bad += [np.zeros((2, 1536), np.float32), np.zeros((1536, 3), np.float32), np.zeros((1536, 3), np.float32).T,
+            np.zeros((6, 1536), np.float32)[::2], frozen, torch.zeros(3, 1536, dtype=torch.bfloat16),
+            torch.zeros(1536, 3).T, torch.zeros(3, 1536, device="meta")]
+    for out in bad:
+        with pytest.raises(ValueError, match="out|emb"):
+            e.extend(kv, [0], [3], emb, out=out, mem=mem)
+    if mem == dtts.MEM_DEVICE:          # host memory in place of the device's
+        for x in (emb, torch.zeros(3, 1536)):
+            with pytest.raises(ValueError, match="on device 0"):
+                e.extend(kv, [0], [3], x, out=x, mem=mem)
+    else:
+        for out in (None, np.zeros((3, 1536), np.float32), torch.zeros(3, 1536)):
+            with pytest.raises(dtts.DttsError):        # as far as the library, which has no engine here
+                e.extend(kv, [0], [3], emb, out=out, mem=mem)
+
+
+@pytest.mark.parametrize("bad", [np.array([0.5]), np.array([2 ** 32 + 1]), np.array([-2 ** 31 - 1]), np.array([True]),
+                                 np.array([2 ** 63], np.uint64), np.array(["1"]), range(2 ** 31, 2 ** 31 + 1)])
+def test_numbers_that_are_not_32_bit_integers_are_refused(dtts_mod, bad):
+    """None of them becomes another sequence or count on the way."""
+    kv = dtts.KVCache.__new__(dtts.KVCache)
+    kv._init(None, 1, 2, 64, 0)
+    for call in (lambda: kv.extend(bad, [1]), lambda: kv.extend([1], bad), lambda: kv.close_seqs(bad), lambda: kv.compact(0, bad)):
+        with pytest.raises(ValueError):
+            call()
+    for good in (np.array([1]), np.array([1], np.uint8), range(1, 2), torch.tensor([1])):
+        assert dtts._ints(good)[0].tolist() == [1] and dtts._ints(good)[2] == 1
