@@ -323,7 +323,9 @@ struct dtts_llm {
     int *d_len = nullptr;                // cache length on the device (graph-captured steps)
     int *d_err = nullptr;
     // step graphs, one per batch size; dropped when the workspace moves
-    // (paged: also the cache, the window and the split of its attention; uid 0: the dense cache)
+    // (paged: also the cache, the window and the split of its attention; uid 0: the dense cache); the least recently
+    // used first.  Of the paged ones, kPagedGraphs are kept.
+    static constexpr int kPagedGraphs = 64;
     struct Graph {
         int B;
         long long uid;
@@ -587,15 +589,21 @@ struct dtts_llm {
             if (round / 2 * 3 <= p.splits && round > 1) round = round / 2 * 3;
             const int splits = std::min(round, kv->max_splits(n_seq));
             cudaGraphExec_t exec = nullptr;
-            for (Graph &g : graphs)
-                if (g.B == n_seq && g.uid == kv->uid && g.window == window && g.sinks == sinks && g.splits == splits)
-                    exec = g.exec;
-            if (!exec) {
+            const auto used = std::find_if(graphs.begin(), graphs.end(), [&](const Graph &g) {
+                return g.B == n_seq && g.uid == kv->uid && g.window == window && g.sinks == sinks && g.splits == splits;
+            });
+            if (used != graphs.end()) {
+                exec = used->exec;
+                std::rotate(used, used + 1, graphs.end());
+            } else {
                 p.splits = splits;
                 p.tiles_per_split = 4;
-                if (graphs.size() >= 64) {
-                    DTTS_CUDA(cudaStreamSynchronize(stream));
-                    drop_graphs();
+                auto paged = [](const Graph &g) { return g.uid != 0; };
+                if (std::count_if(graphs.begin(), graphs.end(), paged) >= kPagedGraphs) {
+                    DTTS_CUDA(cudaStreamSynchronize(stream));   // it may be running
+                    const auto oldest = std::find_if(graphs.begin(), graphs.end(), paged);
+                    cudaGraphExecDestroy(oldest->exec);
+                    graphs.erase(oldest);
                 }
                 graphs.reserve(graphs.size() + 1);
                 if ((st = capture(&exec, [&] { return enqueue(n_seq, 1, 0, false, outd, kv, &plan); }))) return st;

@@ -185,3 +185,41 @@ def test_more_step_graphs_than_are_kept(wide, llm):
     for b in range(2):
         check(wide, np.stack([o[b] for o in steps]), dense[b, :39], causal(39), BF, 4, f"dense sequence {b}")
     kv.close()
+
+
+def test_step_graphs_in_use_outlive_the_others(wide, weights):
+    """Over 64 windows take the place of the least recently used paged graph only.  The legacy default stream (handle 1)
+    runs a graph but captures none, so a step on it works where its graph is there."""
+    llm = dtts.LLM(weights, n_layers=LAYERS, max_batch=2, max_seq=256)
+    kv = llm.kv_cache(32, 2, 16)
+    s = kv.open()
+    x = emb_of("kept", 200, 1536)
+    dense = emb_of("keptdense", 2, 6, 1536)
+    llm.prefill(dense[:, :4])
+    last = llm.step(dense[:, 4])
+    got, windows = [llm.extend(kv, [s], [20], x[:20])], []
+    for i in range(70):
+        for w in (4, 5 + i):
+            n = 20 + len(windows)
+            got.append(llm.extend(kv, [s], [1], x[n:n + 1], window=w))
+            windows.append(w)
+    torch.cuda.synchronize()
+    llm.set_stream(1)
+    n = 20 + len(windows)
+    last2 = llm.step(dense[:, 5])                                    # the dense step's
+    got.append(llm.extend(kv, [s], [1], x[n:n + 1], window=4))       # the one of every other step
+    got.append(llm.extend(kv, [s], [1], x[n + 1:n + 2], window=74))  # the newest
+    with pytest.raises(dtts.DttsError):
+        llm.extend(kv, [s], [1], x[n + 2:n + 3], window=5)           # the oldest
+    windows += [4, 74]
+    torch.cuda.synchronize()
+    llm.set_stream(None)
+    assert kv.length(s) == n + 2
+    sees = causal(n + 2)
+    for i, w in enumerate(windows):
+        sees[20 + i] = R.visible(n + 2, 20 + i, w, 0)
+    check(wide, np.concatenate(got), x[:n + 2], sees, BF, 0, "windows")
+    for b in range(2):
+        check(wide, np.stack([last[b], last2[b]]), dense[b], causal(6), BF, 4, f"dense sequence {b}")
+    kv.close()
+    llm.close()
