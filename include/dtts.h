@@ -354,6 +354,11 @@ int dtts_pe_stream_length(dtts_pe *p, int *tokens);
  * workspace: replays of graphs captured from one cache must not overlap with each other or with its calls.  The calls that change tables
  * (extend, fork, compact) return DTTS_ERR_UNSUPPORTED while the stream is capturing.
  *
+ * Attention keeps scores, softmax sums and weighted sums of values in fp32 and rounds the output to bf16.  The softmax's
+ * numerators enter the products with the values rounded: to half against 4-bit rows; against bf16 rows to
+ * two bf16 terms where a sequence has up to 16 rows of queries a key head (new tokens x query heads per key
+ * head), to one, 2^-8, where it has more.  Queries enter the products with 4-bit rows as halves, scaled by a power of two.
+ *
  * 4-bit rows (DTTS_DTYPE_INT4): for every 32 consecutive values x of a row (a token's head) one
  * scale s = clamp(bf16(max|x| / 7), 2^-14, 9344), held in half, and integers
  * c = clamp(round_half_even(x / s), -7, 7); the value held is c s.  4.5 bits a value.  Magnitudes
@@ -380,12 +385,16 @@ int dtts_kv_close(dtts_kv *kv, int n, const int *seqs);        /* frees sequence
  * copied when a sequence that shares it grows.  Where src is in the current batch, rows written
  * after the fork are the new sequences' rows too. */
 int dtts_kv_fork(dtts_kv *kv, int src, int n, int *dst);
-int dtts_kv_truncate(dtts_kv *kv, int seq, int n_tokens);      /* drops the rows behind n_tokens  */
+/* Drops the rows behind n_tokens.  The position of the next token goes back by as many, also where a
+ * compaction has left gaps between the positions of the rows kept or dropped. */
+int dtts_kv_truncate(dtts_kv *kv, int seq, int n_tokens);
 /* Frees the pages that no later token sees through a window of `window` tokens with `sinks` first
  * rows visible.  Row numbers stay; calls that would reach a freed row are refused. */
 int dtts_kv_trim(dtts_kv *kv, int seq, int window, int sinks);
 /* Keeps the n_keep listed rows (ascending) and repacks them densely; the position of the next token
- * stays.  Needs free pages for the repacked part while it runs. */
+ * stays.  Row numbers (windows, sinks, truncations, reads, later compactions) count the rows held from then on, not
+ * positions: a window of 100 is the last 100 rows that were kept or added since.  Needs free
+ * pages for the repacked part while it runs. */
 int dtts_kv_compact(dtts_kv *kv, int seq, int n_keep, const int *keep);
 /* rows held, and position of the next token (they differ after a compaction); either may be NULL */
 int dtts_kv_length(dtts_kv *kv, int seq, int *tokens, int *position);
@@ -446,8 +455,9 @@ int dtts_llm_length(dtts_llm *e, int *tokens);
 /* The same decoder over a paged cache (dtts_kv_*), for streams that start, fork and end on their own:
  * appends n_new[b] >= 0 tokens to each of the n_seq sequences, prompts and steps mixed freely; emb and
  * hidden are [sum of n_new][1536] in the order of seqs.  Row i of a sequence attends with the window and
- * sinks of dtts_kv_attend_args; token positions continue from the sequence's position.  K and V are rounded
- * to bf16 (and then, in a 4-bit cache, to 4 bits), q to bf16.  dtts_llm_kv_create makes a cache of the
+ * sinks of dtts_kv_attend_args, which count rows; token positions continue from the sequence's position (after a
+ * compaction the two differ).  K and V are rounded
+ * to bf16 (and then, in a 4-bit cache, to 4 bits), q to bf16, where dtts_llm_step keeps q in fp32.  dtts_llm_kv_create makes a cache of the
  * engine's geometry for sequences of up to max_seq tokens; the call works on the engine's stream, before which
  * the work already enqueued on the cache's stream comes, and the cache's stream waits for it.  An error leaves the
  * sequences and pages as they were; where it comes up behind the checks of the request, the cache's batch has ended. */

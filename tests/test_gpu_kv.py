@@ -812,3 +812,19 @@ def test_tiny_queries_with_a_large_scale(t, exponent):
     want, tol = R.attend(q, R.held(k, True), R.held(v, True), n - t, scale=scale)
     R.assert_close(out, want, tol)
     kv.close()
+
+
+def test_positions_after_a_compaction_and_truncations():
+    kv = make(page=16, n_pages=20)
+    s = kv.open()
+    kv.extend([s], [100])
+    kv.compact(s, list(range(10)) + list(range(80, 100)))
+    assert (kv.length(s), kv.position(s)) == (30, 100)
+    kv.extend([s], [5])
+    kv.truncate(s, 32)                     # two of the new tokens are left
+    assert (kv.length(s), kv.position(s)) == (32, 102)
+    kv.truncate(s, 5)                      # 27 rows fewer, whichever positions they had
+    assert (kv.length(s), kv.position(s)) == (5, 75)
+    kv.extend([s], [1])
+    assert (kv.length(s), kv.position(s)) == (6, 76)
+    kv.close()
