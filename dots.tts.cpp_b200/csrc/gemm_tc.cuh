@@ -485,7 +485,7 @@ __global__ void __launch_bounds__(GemmCfg<BN, NW, EPI, F8>::THREADS, 1)
         for (int u = blockIdx.x; u < num_units; u += gridDim.x, it++) {
             const int acc = it & 1;
             const uint32_t acc_phase = (it >> 1) & 1;
-            if (!mbar_wait(&tfull[acc], acc_phase, abort_flag, ep.err, DEVERR_TIMEOUT_EPILOGUE)) break;
+            if (!mbar_wait_warp(&tfull[acc], acc_phase, abort_flag, ep.err, DEVERR_TIMEOUT_EPILOGUE)) break;
             tc_fence_after();
             const int tile = u % num_tiles, split = u / num_tiles;
             int mb, nb;
@@ -737,7 +737,7 @@ __global__ void __launch_bounds__(GemmCfg<BN, NW, EPI, F8>::THREADS, 1)
                     __syncwarp();
                     st.mr = mr;
                 }
-                if (!mbar_wait(&ln_bar[ew], lphase, abort_flag, ep.err, DEVERR_TIMEOUT_EPILOGUE)) { ok = false; break; }
+                if (!mbar_wait_warp(&ln_bar[ew], lphase, abort_flag, ep.err, DEVERR_TIMEOUT_EPILOGUE)) { ok = false; break; }
                 pending = false;
                 lphase ^= 1u;
                 ln_rows_smem<rows_w, F8 != 0>(rows_s, nrows, r_lo, ep.ln, st, lane);
