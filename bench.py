@@ -66,10 +66,13 @@ def parse():
     ap.add_argument("--max-batch", type=int, default=128,
                     help="utterances per solve in the global_solve line (throughput peaks at 64-128)")
     ap.add_argument("--global-steps", type=int, default=2, help="timed passes over the global workload")
-    ap.add_argument("--part", choices=["all", "dit", "pe", "llm", "voc", "attn"], default="all",
+    ap.add_argument("--part", choices=["all", "dit", "pe", "llm", "llm_kv", "voc", "attn"], default="all",
                     help="run one part alone and print its JSON object (profiling drivers): dit = the DiT solve "
                          "(bf16 unless --dtype fp8), pe = PatchEncoder prefill + decode, llm = LLM steps, "
+                         "llm_kv = LLM prompts and steps over the paged cache, "
                          "voc = BigVGAN decode, attn = the attention sublayer")
+    ap.add_argument("--kv-rows", type=int, nargs="+", default=[64, 1000, 4000],
+                    help="rows a stream of --part llm_kv holds before its steps (4000 at most)")
     ap.add_argument("--pe-steps", type=int, default=125, help="PatchEncoder decode steps per pass")
     ap.add_argument("--sweep", action="store_true",
                     help="per-GPU sweep instead of the benchmark line: batch 16..256 at L = 64 and L = 16/64/256 "
@@ -698,6 +701,54 @@ def measure_llm(args, local_rank, cpu_sample=False):
     return res
 
 
+def measure_llm_kv(args, local_rank):
+    """The LLM decoder over the paged cache (not part of the benchmark line): 28 layers, 64 streams, in bf16 and 4-bit
+    rows.  For each number of rows: the prompts, 64 streams a call up to 1000 tokens each and 16 above, then 16 untimed
+    and 64 timed steps of one token for every stream (device-resident inputs, CUDA events on the engine's stream; the
+    second of two passes, so that the step graphs are there).  A step reads more than L2 holds (3 GB of weights)."""
+    import torch
+    import dtts
+    import synth
+    dev = torch.device("cuda", local_rank)
+    B, warm, steps, layers, page = args.n_utt, 16, 64, 28, 64
+    llm = dtts.LLM(synth.llm_weights(3, n_layers=layers), n_layers=layers, max_batch=1, max_seq=4096, device=local_rank)
+    stream = torch.cuda.Stream(device=dev)
+    llm.set_stream(stream.cuda_stream)
+    res = {"workload": f"LLM decoder over the paged cache, {layers} layers, {B} streams: prompts, then {warm} untimed and {steps} timed steps",
+           "rows": {}}
+    gen = torch.Generator(device=dev)
+    gen.manual_seed(4)
+    ev = [torch.cuda.Event(enable_timing=True) for _ in range(4)]
+    for rows in args.kv_rows:
+        call = B if rows <= 1000 else min(B, 16)
+        emb = torch.randn(call * rows, 1536, device=dev, generator=gen)
+        tok = torch.randn(B, 1536, device=dev, generator=gen)
+        out, out_tok = torch.empty_like(emb), torch.empty_like(tok)
+        res["rows"][rows] = {}
+        for name, dtype in (("bf16", dtts.DTYPE_BF16), ("int4", dtts.DTYPE_INT4)):
+            kv = llm.kv_cache(B * ((rows + warm + steps) // page + 1), B, page, dtype)
+            with torch.cuda.stream(stream):
+                for rep in range(2):
+                    seqs = [kv.open() for _ in range(B)]
+                    ev[0].record(stream)
+                    for b in range(0, B, call):
+                        n = min(call, B - b)
+                        llm.extend(kv, seqs[b:b + n], [rows] * n, emb[:n * rows], out=out[:n * rows], mem=dtts.MEM_DEVICE)
+                    ev[1].record(stream)
+                    for i in range(warm + steps):
+                        if i == warm:
+                            ev[2].record(stream)
+                        llm.extend(kv, seqs, [1] * B, tok, out=out_tok, mem=dtts.MEM_DEVICE)
+                    ev[3].record(stream)
+                    torch.cuda.synchronize()
+                    kv.sync()
+                    kv.close_seqs(seqs)
+            res["rows"][rows][name] = {"prompt_ms": ev[0].elapsed_time(ev[1]), "step_ms": ev[2].elapsed_time(ev[3]) / steps}
+            kv.close()
+    llm.close()
+    return res
+
+
 def measure_voc(args, local_rank, cpu_sample):
     """BigVGAN decoder on one utterance of 250 latent frames (20 s of 24 kHz
     audio): device-resident latents, CUDA events on the engine stream, 2
@@ -819,6 +870,8 @@ def run_part(args, local_rank):
         r = measure_pe(args, local_rank, cpu)
     elif args.part == "llm":
         r = measure_llm(args, local_rank, cpu)
+    elif args.part == "llm_kv":
+        r = measure_llm_kv(args, local_rank)
     elif args.part == "voc":
         r = measure_voc(args, local_rank, cpu)
     else:
