@@ -25,6 +25,7 @@ enum DeviceError : int {
     DEVERR_NONFINITE = 4,
     DEVERR_TIMEOUT_BARRIER = 5,   // a grid barrier between CTAs of one kernel
     DEVERR_BATCH = 6,             // a replayed graph's launches do not reach all rows of the current batch
+    DEVERR_FREED = 7,             // a replayed graph reaches rows whose page was freed
 };
 
 // Every spin on an mbarrier gives up after this long (globaltimer ns).

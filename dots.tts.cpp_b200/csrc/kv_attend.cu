@@ -312,6 +312,10 @@ __global__ void __launch_bounds__(FewCfg<D, I4>::kThreads, NT == 1 ? 3 : 1) kv_a
     auto tile_row = [&](int it) { return kt.tile(c0 + warp + it * C::kWarps) * KT; };
     // the page of the tile's first rows, loaded one issue ahead; -1: no tile, or freed
     auto page_of = [&](int it) { return it < n_mine ? trow[tile_row(it) >> a.g.lgP] : -1; };
+    // a page that is not there: only a replayed graph can meet one that a query sees
+    auto freed = [&](int j) {
+        if (j + chunk > (a.window ? i0 - a.window + 1 : 0) || j < a.sinks) atomicCAS(a.err, 0, DEVERR_FREED);
+    };
     // one lane requests the tile: a copy per page it touches
     auto issue = [&](int it, int stage, int page) {
         if (lane != 0) return;
@@ -322,11 +326,16 @@ __global__ void __launch_bounds__(FewCfg<D, I4>::kThreads, NT == 1 ? 3 : 1) kv_a
             mbar_arrive_expect_tx(bar + stage, bytes);
             if (bytes)
                 bulk_load_1d(dst, head_pool + page * a.g.page_stride + ((j0 & (P - 1)) >> 4) * C::kBlock, bytes, bar + stage);
+            else
+                freed(j0);
             return;
         }
         for (int r = 0; r < rows_in; r += chunk) {   // whole pages
             if (r) page = trow[(j0 + r) >> a.g.lgP];
-            if ((unsigned)page >= (unsigned)a.g.n_pages) continue;
+            if ((unsigned)page >= (unsigned)a.g.n_pages) {
+                freed(j0 + r);
+                continue;
+            }
             // the phase completes with the arrival behind the last piece; the pieces only add bytes
             const uint32_t bytes = ((min(rows_in - r, chunk) + 15) >> 4) * C::kBlock;
             mbar_expect_tx(bar + stage, bytes);
@@ -1123,6 +1132,15 @@ __global__ void __launch_bounds__(512, 1) kv_attend_many_kernel(const __grid_con
                         if (h == 1) tc_commit(v_empty + (k & 1));
                     }
                     __syncwarp();
+                }
+            }
+            // Pages that are not there, while the last softmax runs: only a replayed graph can meet one that a query sees
+            // (in the loop of the unpacking warps this cost the prompts 2%).
+            if (w == 1) {
+                const int step = min(a.g.P, KT), lo = a.window ? i0 + base / G - a.window + 1 : 0;
+                for (int x = lane * step; x < n * KT; x += 32 * step) {
+                    const int j = kt.tile(c0 + x / KT) * KT + x % KT;
+                    if (j <= i_last && (j + step > lo || j < a.sinks) && trow[j >> a.g.lgP] < 0) atomicCAS(a.err, 0, DEVERR_FREED);
                 }
             }
             // every product done before TMEM is given back (also after an abort)

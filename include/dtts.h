@@ -348,7 +348,7 @@ int dtts_pe_stream_length(dtts_pe *p, int *tokens);
  * the batch that is current on the stream then: as many sequences as at the capture, each with as many
  * new tokens as the one in its place had, of any lengths.  Rows that the captured launches do not reach
  * (one sequence has more new tokens, or there are more sequences) are left as they were, and
- * the next dtts_kv_sync returns DTTS_ERR_ARG.  Do not replay a graph after its batch has ended until the next
+ * the next dtts_kv_sync returns DTTS_ERR_ARG; so it does where a replay reaches rows that a trim has freed since.  Do not replay a graph after its batch has ended until the next
  * dtts_kv_extend.  The split of long key ranges over the GPU stays as it was sized at the
  * capture, so capture again when the sequences have grown much.  All work of a cache shares its
  * workspace: replays of graphs captured from one cache must not overlap with each other or with its calls.  The calls that change tables
