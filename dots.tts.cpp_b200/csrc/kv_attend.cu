@@ -262,11 +262,14 @@ struct FewCfg {
 // bf16 terms (2^-16).
 // The running maximum m of a column is raised only when a score passes it by 2^8
 // (P <= 2^8 is as exact as P <= 1), so most tiles need no exchange between lanes.
-// Measured (12 query heads over 2 of 128): 32 sequences of 4097 .. 32768 4-bit rows 45.8 us, 3.7 TB/s of rows, bound
-// by unpacking (52% of the issue slots, integer and half pipes at their rate); 64 of 1000 .. 8191 bf16 rows 54.5 us,
-// 5.5 TB/s, bound by DRAM; one of 48 rows 5.9 us, bound by latency.  4 warps of 64-key tiles and three CTAs an SM
-// hide the most: 8 warps of 32 keys and two CTAs measured 53.2 us for the first of these, 12 of 64 and
-// one 49.7, when these took 47.9.
+// Measured (12 query heads over 2 of 128): 32 sequences of 4097 .. 32768 4-bit rows 46.2 us, 3.7 TB/s of rows; the
+// counters (53% of the issue slots, integer pipe 41% and its neighbour for fp32 and half 41% active, tensor pipe 21%,
+// DRAM at half its rate) show no unit at its limit: three warps a scheduler do not cover the chains of instructions
+// that turn words into products.  64 of 1000 .. 8191 bf16 rows 52.7 us, 5.7 TB/s, bound by DRAM; one of 48 rows 5.6 us, bound by
+// latency.  4 warps of 64-key tiles and three CTAs an SM are best for long ranges: 8 warps of 32 keys and two CTAs
+// measured 53.2 us for the first of these and 59.8 for the second, 12 of 64 and one 49.7 and 56.0, when these took
+// 47.2 and 53.8.  Short ranges pay for it: 64 sequences of 65 .. 512 4-bit rows took 9.3 us against 8.3 with 8 warps of 32, 64 behind
+// windows of 1024 16.1 against 13.5 with 12 of 64 and 15.4 with 8 of 32.  One shape serves all.
 template <int D, bool I4, int NT>
 __global__ void __launch_bounds__(FewCfg<D, I4>::kThreads, NT == 1 ? 3 : 1) kv_attend_few_kernel(const __grid_constant__ KvAttendArgs a) {
     using C = FewCfg<D, I4>;
@@ -998,15 +1001,17 @@ DTTS_DEV bool kv_wait(uint64_t *bar, uint32_t parity, volatile int *abort_flag, 
 //                   MN-major); while one warp waits, the other's products run.
 // A tile has two score buffers of 64 columns: the scores of the next half are
 // computed while the softmax of this one runs and P V of the one before, so no role
-// waits for a round trip.  Bound by the softmax's exponentials (128 x 128 a block
-// and tile at 16 a clock and SM) and by the operands' shared memory reads, which take
+// waits for a round trip.  Bound by the chain of a half block (scores from TMEM,
+// exponentials, P back) with two softmax warps a scheduler beside the unpacking ones: the
+// tensor pipe is active 29% of the time, the unit of the exponentials 33%, half the
+// issue slots are used.  The operands' shared memory reads would be next; they take
 // longer than the products themselves (S: 128 x 64 x 16 a step reads 6 KB in 32 clocks).
 // 4-bit rows: all operands half, Q after an exact power-of-two scaling of the row, P
 // rounded by 2^-11.  bf16 rows: P is rounded to bf16 (2^-8 of the P-weighted mean
 // of |v|, the size of the output's own rounding): a second term would cost half as
 // much tensor time again.
 // Measured: four prompts of 1501 .. 2047 tokens (12 query heads over 2 of 128, 4 bits) 74 us, 530 TFLOP/s; chunks of
-// 512 tokens behind windows of 4096 (bf16) 45 us, 582 TFLOP/s.  A CTA per row-tile pair, longest first: resident CTAs
+// 512 tokens behind windows of 4096 (bf16) 44.5 us, 589 TFLOP/s.  A CTA per row-tile pair, longest first: resident CTAs
 // that draw their pairs from a counter measured 81 and 45 us.
 template <int D, bool I4>
 __global__ void __launch_bounds__(512, 1) kv_attend_many_kernel(const __grid_constant__ KvAttendArgs a, int pairs) {
@@ -1513,8 +1518,9 @@ cudaError_t prepare(KvShapes *k) {
     k->few_key_tile = FewCfg<D, I4>::KT;
     k->few_warps = FewCfg<D, I4>::kWarps;
     // 64 sequences of 300 .. 32768 rows, 12 query heads over 2 of 128: 6.3 + 1.46 x, 8 + 1.45 x, 10 + 1.02 x us for x
-    // tiles a warp, with 1, 2, 3 CTAs on an SM (4 bits), 4 + 0.8 x, 0.72 x, 0.68 x (bf16).  Tiles of other shapes by
-    // their size; 9 .. 16 query rows measured 2.2 x, 1.8 x.
+    // tiles a warp, with 1, 2, 3 CTAs on an SM (4 bits; why a second CTA adds nothing is not known), 4 + 0.8 x, 0.72 x,
+    // 0.68 x (bf16).  9 .. 16 query rows measured 2.2 x, 1.8 x against 4-bit rows.  Not measured: tiles of heads of 64, taken by
+    // their size, and 9 .. 16 query rows against bf16 rows, taken like 8.
     constexpr float size = I4 ? D / 128.f : FewCfg<D, I4>::KT * D / 2048.f;
     const float one[3] = {I4 ? 1.46f : 0.8f, I4 ? 1.45f : 0.72f, I4 ? 1.02f : 0.68f}, start[3] = {0.f, I4 ? 1.5f : 0.5f, I4 ? 3.5f : 1.f};
     for (int c = 0; c < 3; c++) {
