@@ -1011,7 +1011,7 @@ DTTS_DEV bool kv_wait(uint64_t *bar, uint32_t parity, volatile int *abort_flag, 
 // of |v|, the size of the output's own rounding): a second term would cost half as
 // much tensor time again.
 // Measured: four prompts of 1501 .. 2047 tokens (12 query heads over 2 of 128, 4 bits) 74 us, 530 TFLOP/s; chunks of
-// 512 tokens behind windows of 4096 (bf16) 44.5 us, 589 TFLOP/s.  A CTA per row-tile pair, longest first: resident CTAs
+// 512 tokens behind windows of 4096 (bf16) 44.9 us, 584 TFLOP/s.  A CTA per row-tile pair, longest first: resident CTAs
 // that draw their pairs from a counter measured 81 and 45 us.
 template <int D, bool I4>
 __global__ void __launch_bounds__(512, 1) kv_attend_many_kernel(const __grid_constant__ KvAttendArgs a, int pairs) {
@@ -1454,8 +1454,29 @@ __global__ void __launch_bounds__(512, 1) kv_attend_many_kernel(const __grid_con
                 if (parts > 1) {
                     wp[256 * D + rr] = m;
                     wp[256 * (D + 1) + rr] = l;
-                } else {
+                }
+                __syncwarp();
+                // a NaN: recompute the row so that key rows it cannot see do not reach it, before anything is stored
+                // over q, which out may be
+                for (unsigned todo = __ballot_sync(0xffffffffu, bad && live); todo; todo &= todo - 1) {
+                    const int x = __ffs(todo) - 1, xr = wr + x, xt = (base + xr) / G, xh = (base + xr) % G;
+                    float mm, ll, oo[D / 32];
+                    kv_row_plain<D>(a, trow, head, a.q + (long long)(row0 + xt) * a.q_row + (long long)(head * G + xh) * a.q_head,
+                                    i0 + xt, KT, kt, c0, c1, mm, ll, oo);
+                    for (int i = 0; i < D / 32; i++) {
+                        const int d = D / 32 * lane + i;
+                        if (parts == 1)
+                            reinterpret_cast<bf16 *>(sO + tile_unit((warp & 3) * 32 + x, d >> 3))[d & 7] = __float2bfloat16_rn(oo[i] / ll);
+                        else
+                            wp[((d >> 2) * 256 + xr) * 4 + (d & 3)] = oo[i];
+                    }
+                    if (parts > 1 && lane == 0) {
+                        wp[256 * D + xr] = mm;
+                        wp[256 * (D + 1) + xr] = ll;
+                    }
                     __syncwarp();
+                }
+                if (parts == 1) {
                     const long long o_off = (long long)(row0 + tok) * a.o_row + (long long)(head * G + hg) * a.o_head;
 #pragma unroll 4
                     for (int s = 0; s < kSteps; s++) {
@@ -1465,25 +1486,6 @@ __global__ void __launch_bounds__(512, 1) kv_attend_many_kernel(const __grid_con
                             *reinterpret_cast<uint4 *>(a.out + off + 8 * u) =
                                 *reinterpret_cast<const uint4 *>(sO + tile_unit((warp & 3) * 32 + row, u));
                     }
-                    __syncwarp();
-                }
-                // a NaN: recompute the row so that key rows it cannot see do not reach it
-                for (unsigned todo = __ballot_sync(0xffffffffu, bad && live); todo; todo &= todo - 1) {
-                    const int x = __ffs(todo) - 1, xr = wr + x, xt = (base + xr) / G, xh = (base + xr) % G;
-                    float mm, ll, oo[D / 32];
-                    kv_row_plain<D>(a, trow, head, a.q + (long long)(row0 + xt) * a.q_row + (long long)(head * G + xh) * a.q_head,
-                                    i0 + xt, KT, kt, c0, c1, mm, ll, oo);
-                    bf16 *xo = a.out + (long long)(row0 + xt) * a.o_row + (long long)(head * G + xh) * a.o_head;
-                    for (int i = 0; i < D / 32; i++) {
-                        const int d = D / 32 * lane + i;
-                        if (parts == 1) xo[d] = __float2bfloat16_rn(oo[i] / ll);
-                        else wp[((d >> 2) * 256 + xr) * 4 + (d & 3)] = oo[i];
-                    }
-                    if (parts > 1 && lane == 0) {
-                        wp[256 * D + xr] = mm;
-                        wp[256 * (D + 1) + xr] = ll;
-                    }
-                    __syncwarp();
                 }
             }
         }

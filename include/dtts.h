@@ -407,7 +407,7 @@ int dtts_kv_write(dtts_kv *kv, int layer, const void *k, const void *v, long lon
 typedef struct dtts_kv_attend_args {
     const void *q;                    /* [rows][n_heads][head_dim]                          */
     long long q_row, q_head;          /* strides in elements                                */
-    void *out;                        /* like q                                             */
+    void *out;                        /* like q; may be q itself, with its strides          */
     long long out_row, out_head;
     int n_heads;                      /* a multiple of n_kv_heads; query head h reads key head
                                          h / (n_heads / n_kv_heads)                         */

@@ -1,5 +1,5 @@
 """The paged K/V cache (dtts_kv_*) at the edges of what its calls allow: replays over rows that a trim has freed, chunks
-behind trimmed pages, large groups of query heads, very many sequences."""
+behind trimmed pages, queries and outputs in one buffer, large groups of query heads, very many sequences."""
 import pytest
 import torch
 
@@ -105,6 +105,35 @@ def test_chunks_behind_trimmed_pages(dtype, page, window, sinks):
         n += t
         want, tol = R.attend(q, R.held(k[:n], dtype == I4), R.held(v[:n], dtype == I4), n - t, window, sinks, int4=dtype == I4)
         R.assert_close(out, want, tol, f"{t} tokens at {n - t}")
+    kv.close()
+
+
+@pytest.mark.parametrize("dtype", [BF, I4])
+@pytest.mark.parametrize("D,Hq,H", [(128, 12, 2), (64, 4, 2)])
+def test_outputs_in_place_of_queries(dtype, D, Hq, H):
+    """out may be q: steps in one part and in many, prompts, with rows that are recomputed for a NaN they do not see."""
+    g = rng(74)
+    lens, news = [3000, 40, 200, 70], [1, 2, 150, 70]
+    kv = make(H=H, D=D, dtype=dtype, n_pages=80)
+    seqs = [kv.open() for _ in lens]
+    rows = [(rand(g, n, H, D), rand(g, n, H, D)) for n in lens]
+    for b, j in ((0, 5), (2, 120), (3, 69)):
+        rows[b][0][j, 0, 3] = rows[b][1][j, :, 7] = float("nan")
+    fill(kv, seqs, [(k[:n - t], v[:n - t]) for (k, v), n, t in zip(rows, lens, news)])
+    fill(kv, seqs, [(k[n - t:], v[n - t:]) for (k, v), n, t in zip(rows, lens, news)])
+    q = rand(g, sum(news), Hq, D)
+    x = q.cuda()
+    kv.attend(0, x, x, window=2000, sinks=0)
+    kv.sync()
+    row = 0
+    for b, (n, t) in enumerate(zip(lens, news)):
+        want, tol = R.attend(q[row:row + t], R.held(rows[b][0], dtype == I4), R.held(rows[b][1], dtype == I4), n - t, 2000, 0,
+                             int4=dtype == I4)
+        got = x[row:row + t].cpu()
+        assert torch.equal(torch.isnan(got), torch.isnan(want)), f"sequence {b}"
+        ok = torch.isfinite(want)
+        R.assert_close(torch.where(ok, got.double(), 0), torch.where(ok, want, 0), torch.where(ok, tol, 1e-30), f"sequence {b}")
+        row += t
     kv.close()
 
 
