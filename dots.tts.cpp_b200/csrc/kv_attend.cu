@@ -901,6 +901,44 @@ __global__ void __launch_bounds__(256) kv_join_many_kernel(const __grid_constant
                             pack_bf16x2(o[8 * i + 4] * inv, o[8 * i + 5] * inv), pack_bf16x2(o[8 * i + 6] * inv, o[8 * i + 7] * inv));
 }
 
+// Where this CTA of the many-row kernel stands: its part, its (sequence, key head), its pair of row tiles
+struct ManyPlace {
+    int split, bh, pair;
+    DTTS_DEV ManyPlace(const KvAttendArgs &a, int pairs, unsigned block) {
+        const int u = block / a.splits;
+        split = block % a.splits;
+        bh = u % (a.n_seq * a.g.H);
+        pair = pairs - 1 - u / (a.n_seq * a.g.H);   // longest key ranges first
+    }
+};
+
+// Sets the error word where the unit has rows that a replayed graph was not captured for: its first CTA calls it.
+DTTS_DEV void many_check_batch(const KvAttendArgs &a, int pairs, const ManyPlace &at, const ManyUnit &n) {
+    if (at.split || at.pair) return;
+    const long long all = (long long)n.cnt * a.G;
+    if (all > 256ll * pairs || (all > 0 && all <= kKvFewRows && !a.both) ||
+        (at.bh == 0 && kv_batch_over(a.g, a.m, a.n_seq, a.total_rows)))
+        atomicCAS(a.err, 0, DEVERR_BATCH);
+}
+
+// That, and the error word where a row that the CTA's queries see stands on a page that is not there; a warp calls it.
+// Works out its place again: kept live for it, the CTA's variables cost the kernel spilled registers (chunks 1% slower).
+DTTS_DEV void many_check(const KvAttendArgs &a, int pairs) {
+    constexpr int KT = kKvManyKeyTile;
+    unsigned block;   // a blockIdx.x that is not known to be the one from the start
+    asm volatile("mov.u32 %0, %%ctaid.x;" : "=r"(block));
+    const ManyPlace at(a, pairs, block);
+    const ManyUnit n(a, at.bh, at.pair);
+    if ((threadIdx.x & 31) == 0) many_check_batch(a, pairs, at, n);
+    const int *trow = a.m.table + (long long)a.m.seq[n.b] * a.g.max_pages;
+    const int step = min(a.g.P, KT), first = n.i0 + n.base / a.G, lo = a.window ? first - a.window + 1 : 0;
+    const int v0 = part_start(n.kt.n, n.parts, at.split), v1 = part_start(n.kt.n, n.parts, at.split + 1);
+    for (int x = v0 * KT + (threadIdx.x & 31) * step; x < v1 * KT; x += 32 * step) {
+        const int j = n.kt.tile(x / KT) * KT + x % KT;
+        if (j <= n.i_last && (j + step > lo || j < a.sinks) && trow[j >> a.g.lgP] < 0) atomicCAS(a.err, 0, DEVERR_FREED);
+    }
+}
+
 template <int D, bool I4>
 struct ManyCfg {
     static constexpr int KT = kKvManyKeyTile, kTile = D / 64 * kChunk;   // one operand tile of 128 rows
@@ -1010,8 +1048,8 @@ DTTS_DEV bool kv_wait(uint64_t *bar, uint32_t parity, volatile int *abort_flag, 
 // rounded by 2^-11.  bf16 rows: P is rounded to bf16 (2^-8 of the P-weighted mean
 // of |v|, the size of the output's own rounding): a second term would cost half as
 // much tensor time again.
-// Measured: four prompts of 1501 .. 2047 tokens (12 query heads over 2 of 128, 4 bits) 74 us, 530 TFLOP/s; chunks of
-// 512 tokens behind windows of 4096 (bf16) 44.9 us, 584 TFLOP/s.  A CTA per row-tile pair, longest first: resident CTAs
+// Measured: four prompts of 1501 .. 2047 tokens (12 query heads over 2 of 128, 4 bits) 75 us, 525 TFLOP/s; chunks of
+// 512 tokens behind windows of 4096 (bf16) 44.7 us, 586 TFLOP/s.  A CTA per row-tile pair, longest first: resident CTAs
 // that draw their pairs from a counter measured 81 and 45 us.
 template <int D, bool I4>
 __global__ void __launch_bounds__(512, 1) kv_attend_many_kernel(const __grid_constant__ KvAttendArgs a, int pairs) {
@@ -1029,17 +1067,13 @@ __global__ void __launch_bounds__(512, 1) kv_attend_many_kernel(const __grid_con
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     pdl_wait();
 
-    const int split = blockIdx.x % a.splits, u = blockIdx.x / a.splits;
-    const int bh = u % (a.n_seq * a.g.H), pair = pairs - 1 - u / (a.n_seq * a.g.H);   // longest key ranges first
-    const int unit = bh * pairs + pair;
+    const ManyPlace at(a, pairs, blockIdx.x);
+    const int split = at.split, bh = at.bh, pair = at.pair, unit = bh * pairs + pair;
     const ManyUnit mu(a, bh, pair);
-    if (split == 0 && pair == 0 && tid == 0) {   // rows that a replayed graph was not captured for
-        const long long all = (long long)mu.cnt * a.G;
-        if (all > 256ll * pairs || (all > 0 && all <= kKvFewRows && !a.both) ||
-            (bh == 0 && kv_batch_over(a.g, a.m, a.n_seq, a.total_rows)))
-            atomicCAS(a.err, 0, DEVERR_BATCH);
+    if (!mu.on || split >= mu.parts) {
+        if (tid == 0) many_check_batch(a, pairs, at, mu);
+        return;
     }
-    if (!mu.on || split >= mu.parts) return;
     const int head = mu.head, len = mu.len, row0 = mu.row0, G = a.G, base = mu.base, rows = mu.rows, parts = mu.parts;
     const int tiles = rows > 128 ? 2 : 1, i0 = mu.i0, i_last = mu.i_last;
     const KeyTiles &kt = mu.kt;
@@ -1139,15 +1173,9 @@ __global__ void __launch_bounds__(512, 1) kv_attend_many_kernel(const __grid_con
                     __syncwarp();
                 }
             }
-            // Pages that are not there, while the last softmax runs: only a replayed graph can meet one that a query sees
+            // What only a replayed graph can meet, while the last softmax runs: pages that are not there, other rows
             // (in the loop of the unpacking warps this cost the prompts 2%).
-            if (w == 1) {
-                const int step = min(a.g.P, KT), lo = a.window ? i0 + base / G - a.window + 1 : 0;
-                for (int x = lane * step; x < n * KT; x += 32 * step) {
-                    const int j = kt.tile(c0 + x / KT) * KT + x % KT;
-                    if (j <= i_last && (j + step > lo || j < a.sinks) && trow[j >> a.g.lgP] < 0) atomicCAS(a.err, 0, DEVERR_FREED);
-                }
-            }
+            if (w == 1) many_check(a, pairs);
             // every product done before TMEM is given back (also after an abort)
             if (lead) tc_commit(drain + w);
             __syncwarp();
