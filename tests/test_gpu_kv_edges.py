@@ -167,3 +167,65 @@ def test_very_many_sequences(dtype):
         kv.open()
     assert e.value.status == dtts.ERR_OOM
     kv.close()
+
+
+def grow_and_check(kv, seed, dtype, synced):
+    """A prompt, steps, a fork that grows and a compaction; synced(): waits for the cache's stream."""
+    g = rng(seed)
+    s = kv.open()
+    k, v = rand(g, 240, 2, 128), rand(g, 240, 2, 128)
+    n = 0
+    for t in (200, 1, 1, 17, 1):
+        kd, vd, q = k[n:n + t].cuda(), v[n:n + t].cuda(), rand(g, t, 12, 128)
+        qd, out = q.cuda(), torch.empty(t, 12, 128, dtype=torch.bfloat16, device="cuda")
+        torch.cuda.synchronize()
+        kv.extend([s], [t])
+        kv.write(0, kd, vd)
+        kv.attend(0, qd, out)
+        synced()
+        n += t
+        want, tol = R.attend(q, R.held(k[:n], dtype == I4), R.held(v[:n], dtype == I4), n - t, int4=dtype == I4)
+        R.assert_close(out, want, tol, f"{t} tokens at {n - t}")
+    (f,) = kv.fork(s)
+    kv.extend([f], [1])
+    keep = list(range(0, n, 3))
+    kv.compact(s, keep)
+    ko = torch.zeros(1, len(keep), 2, 128, device="cuda")
+    vo = torch.zeros_like(ko)
+    torch.cuda.synchronize()
+    kv.read(0, [s], [0], [len(keep)], ko, vo)
+    synced()
+    assert torch.equal(ko[0].cpu().double(), R.held(k[keep], dtype == I4))
+    assert torch.equal(vo[0].cpu().double(), R.held(v[keep], dtype == I4))
+    kv.close_seqs([s, f])
+
+
+@pytest.mark.parametrize("stream", [None, 1, 2])
+def test_the_caches_own_the_legacy_and_the_per_thread_stream(stream):
+    for dtype in (BF, I4):
+        kv = make(dtype=dtype, page=32)
+        kv.set_stream(stream)
+        grow_and_check(kv, 76, dtype, kv.sync)
+        kv.close()
+
+
+def test_caches_in_several_threads():
+    """Each with its own cache, on its own stream, at the same time."""
+    import threading
+    failed = []
+
+    def work(seed, dtype):
+        try:
+            kv = dtts.KVCache(1, 2, 128, 64, 4, 4096, page_tokens=32, dtype=dtype)
+            for i in range(5):
+                grow_and_check(kv, seed + i, dtype, kv.sync)
+            kv.close()
+        except BaseException as e:   # noqa: BLE001 (reported below)
+            failed.append(e)
+
+    threads = [threading.Thread(target=work, args=(80 + 10 * i, BF if i % 2 else I4)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed, failed

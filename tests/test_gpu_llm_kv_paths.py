@@ -223,3 +223,25 @@ def test_step_graphs_in_use_outlive_the_others(wide, weights):
         check(wide, np.stack([last[b], last2[b]]), dense[b], causal(6), BF, 4, f"dense sequence {b}")
     kv.close()
     llm.close()
+
+
+def test_prompts_past_32_bit_offsets(llm):
+    """64 prompts of 2000 tokens: 17920 columns of gate and up projections pass 2^31 elements.  The first and the last
+    stream come out as they do alone."""
+    n, rows = 64, 2000
+    assert n * rows * 17920 > 2 ** 31
+    g = torch.Generator(device="cuda")
+    g.manual_seed(5)
+    x = torch.randn(n * rows, 1536, device="cuda", generator=g)
+    out = torch.empty_like(x)
+    kv = llm.kv_cache(n * (rows // 64 + 1) + 40, n + 1, 64)
+    seqs = [kv.open() for _ in range(n)]
+    torch.cuda.synchronize()
+    llm.extend(kv, seqs, [rows] * n, x, out=out, mem=dtts.MEM_DEVICE)
+    kv.sync()
+    for b in (0, n - 1):
+        s = kv.open()
+        part, alone = x[b * rows:(b + 1) * rows].cpu().numpy(), out[b * rows:(b + 1) * rows].cpu().numpy()
+        assert_bf16_close(llm.extend(kv, [s], [rows], part), alone, f"stream {b}")
+        kv.close_seqs([s])
+    kv.close()
