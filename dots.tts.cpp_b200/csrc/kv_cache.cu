@@ -25,6 +25,7 @@ namespace {
 unsigned kv_pdl() { return pdl_enabled() ? kLaunchPdl : 0u; }
 
 constexpr int kWsFloats = 9 * 1024 * 1024;     // 36 MB of partial results
+static_assert(kWsFloats / (kKvFewRows * (64 + 2)) <= INT16_MAX, "KvAttendArgs::splits");
 constexpr int kMaxUnits = 1 << 16;             // split units with an arrival counter
 
 // ---------------------------------------------------------------- metadata
@@ -661,7 +662,7 @@ int dtts_kv::plan_attend(const dtts_kv_attend_args &a, KvAttendPlan *plan) const
             }
         }
         const long long splits = std::max(1ll, std::min((max_tiles + per - 1) / per, most));
-        p.splits = (int)splits;
+        p.splits = (short)splits;
         p.tiles_per_split = (int)per;
         plan->args[many] = p;
         plan->rows_or_pairs[many] = many ? rt : max_rows;

@@ -596,7 +596,7 @@ struct dtts_llm {
                 exec = used->exec;
                 std::rotate(used, used + 1, graphs.end());
             } else {
-                p.splits = splits;
+                p.splits = (short)splits;
                 p.tiles_per_split = 4;
                 auto paged = [](const Graph &g) { return g.uid != 0; };
                 if (std::count_if(graphs.begin(), graphs.end(), paged) >= kPagedGraphs) {
