@@ -539,7 +539,7 @@ def _ints(a):
     return a, a.ctypes.data, a.size
 
 
-def _rows_f32(a, shape, device, what):
+def _rows_f32(a, shape, device, what, written):
     """Checks a dense fp32 buffer: of the device with this number, or host memory (None)."""
     if tuple(a.shape) != shape:
         raise ValueError(f"{what}: {list(shape)} expected, not {list(a.shape)}")
@@ -547,7 +547,7 @@ def _rows_f32(a, shape, device, what):
         ok = str(a.dtype) == "torch.float32" and a.is_contiguous() and \
             (a.device.type == "cpu" if device is None else a.is_cuda and a.get_device() == device)
     else:
-        ok = device is None and a.dtype == np.float32 and a.flags.c_contiguous and a.flags.writeable
+        ok = device is None and a.dtype == np.float32 and a.flags.c_contiguous and (a.flags.writeable or not written)
     if not ok:
         raise ValueError(f"{what}: dense fp32 " + ("host memory" if device is None else f"on device {device}") + " expected")
 
@@ -767,7 +767,7 @@ class LLM:
             out = np.zeros_like(emb) if out is None else out
         rows = int(sum(c))
         for x, what in ((emb, "emb"), (out, "out")):
-            _rows_f32(x, (rows, 1536), self.device if mem == MEM_DEVICE else None, what)
+            _rows_f32(x, (rows, 1536), self.device if mem == MEM_DEVICE else None, what, x is out)
         kv._rows = max(kv._rows, rows)   # an error may leave either batch
         check(lib().dtts_llm_extend(self.h, kv.h, n, ps, pc, _addr(emb), window, sinks, _addr(out), mem))
         kv._rows = rows

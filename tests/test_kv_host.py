@@ -115,6 +115,8 @@ def test_decoder_buffers_of_another_kind_are_refused(dtts_mod, mem):
         for out in (None, np.zeros((3, 1536), np.float32), torch.zeros(3, 1536)):
             with pytest.raises(dtts.DttsError):        # as far as the library, which has no engine here
                 e.extend(kv, [0], [3], emb, out=out, mem=mem)
+        with pytest.raises(dtts.DttsError):            # emb is only read
+            e.extend(kv, [0], [3], frozen, mem=mem)
 
 
 @pytest.mark.parametrize("bad", [np.array([0.5]), np.array([2 ** 32 + 1]), np.array([-2 ** 31 - 1]), np.array([True]),
