@@ -497,6 +497,7 @@ int dtts_kv::extend(int n_seq, const int *sq, const int *n_new) {
         start += n_new[b];
     }
     b_rows = start;
+    last_entries = n_seq;
     // entries behind the batch hold no rows: row lookups of a graph captured for more entries stay in range, and
     // kv_batch_over tells by them that there are more entries than at a capture
     for (int b = n_seq; b < g.max_seqs; b++) {
@@ -952,6 +953,11 @@ int dtts_kv_compact(dtts_kv *kv, int seq, int n_keep, const int *keep) try {
     if (stay == (int)s.pages.size() && n_keep == s.len) return DTTS_OK;
     DTTS_CHECK(fresh <= (int)kv->free_pages.size(), DTTS_ERR_OOM, "%d pages needed, %zu free", fresh,
                kv->free_pages.size());
+    // pages are about to change hands: without a current batch, a replayed graph (which is not allowed, but cannot be seen)
+    // finds no rows any more that it could store on a page that the last batch had; extend, which also takes pages, makes
+    // a batch of its own
+    if (kv->b_seq.empty())
+        for (int b = 0; b < kv->last_entries; b++) kv->poke(2 * g.max_seqs + b, 0);
     const int j0 = stay << g.lgP, n = n_keep - j0, scratch = g.max_seqs;
     std::vector<int> pages(s.pages.begin(), s.pages.begin() + stay);
     for (int p = stay; p < total; p++) {

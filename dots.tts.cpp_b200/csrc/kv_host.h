@@ -42,6 +42,7 @@ struct dtts_kv {
     // current batch
     std::vector<int> b_seq, b_cnt, b_len;
     int b_rows = 0;
+    int last_entries = 0;                 // of the current or, where that has ended, the last batch
     long long uid = 0;                    // no two caches of a process share it
 
     ~dtts_kv();

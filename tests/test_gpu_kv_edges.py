@@ -229,3 +229,39 @@ def test_caches_in_several_threads():
     for t in threads:
         t.join()
     assert not failed, failed
+
+
+@pytest.mark.parametrize("end,rows", [("truncate", 16), ("trim", 63), ("close", 63), ("compact", 32)])
+def test_a_replay_behind_the_end_of_its_batch_spares_the_pages_of_others(end, rows):
+    """The header forbids it, and the library cannot see it: but pages that have gone to another sequence since stay as
+    that one wrote them."""
+    g = rng(91)
+    kv = make(page=16, n_pages=9, dtype=BF)
+    a, b = kv.open(), kv.open()
+    k, v = rand(g, 64, 2, 128), rand(g, 64, 2, 128)
+    fill(kv, [b], [(k, v)])
+    fill(kv, [a], [(rand(g, 48, 2, 128), rand(g, 48, 2, 128))])
+    x = torch.full((1, 2, 128), 9.0, dtype=torch.bfloat16, device="cuda")
+    kv.extend([a], [1])                                    # a row on a page of its own
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=torch.cuda.current_stream()):
+        kv.write(0, x, x)
+    graph.replay()
+    free = kv.free_pages()
+    if end == "truncate":
+        kv.truncate(a, 48)
+    elif end == "trim":
+        kv.extend([a], [15])                               # the row's page is full and out of the window
+        kv.trim(a, 1)
+    elif end == "close":
+        kv.close_seqs([a])
+    else:
+        kv.compact(a, list(range(32)))
+    assert kv.free_pages() > free
+    keep = list(range(1, 1 + rows))
+    kv.compact(b, keep)                                    # takes the freed pages, the lowest first
+    graph.replay()
+    gk, gv = read(kv, b, 0, len(keep))
+    assert torch.equal(gk[0].double(), k[keep].double()) and torch.equal(gv[0].double(), v[keep].double())
+    kv.close()
